@@ -24,3 +24,4 @@ from .decode import DecodeOutput, decode_step  # noqa: F401
 from .layer import LowRankLayerOutput, LowRankWeights, lowrank_layer_forward  # noqa: F401
 from .model import (BdhModelState, BdhModelWeights, load_model_state, model_forward_logits,  # noqa: F401
                     new_model_state, pack_model, save_model_state)
+from .streams import compact_streams, copy_streams, free_streams  # noqa: F401

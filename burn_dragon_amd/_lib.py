@@ -96,6 +96,9 @@ SIGNATURES = {
                                      ctypes.POINTER(BdhLayerStateDesc), _i32]),
     "bdh_state_record_load": (_i32, [ctypes.c_char_p, _i32, ctypes.POINTER(BdhLayerStateDesc),
                                      ctypes.POINTER(_vp), _vp]),
+    "bdh_state_copy_streams": (_i32, [_i32, ctypes.POINTER(BdhLayerStateDesc), ctypes.POINTER(_vp),
+                                      ctypes.POINTER(BdhLayerStateDesc), ctypes.POINTER(_vp), _i32,
+                                      ctypes.POINTER(_i32), ctypes.POINTER(_i32), _vp]),
     "bdh_profile_enable": (None, [_i32]),
     "bdh_profile_reset": (None, []),
     "bdh_profile_get": (None, [ctypes.POINTER(BdhProfileSnapshot)]),

@@ -8,6 +8,7 @@
 
 #include <atomic>
 #include <chrono>
+#include <exception>
 #include <map>
 #include <mutex>
 #include <string>
@@ -749,6 +750,81 @@ bdh_status bdh_lm_logits(const float* hidden, int64_t rows, int64_t embd,
   if (st != BDH_OK) return st;
   prof.done(true);
   return BDH_OK;
+}
+
+bdh_status bdh_state_copy_streams(int32_t n_layers, const bdh_layer_state_desc* layers,
+                                  float* const* rho, const bdh_layer_state_desc* src_layers,
+                                  const float* const* src_rho, int32_t n, const int32_t* dst,
+                                  const int32_t* src, void* stream) try {
+  ProfScope prof;
+  if (n_layers < 0 || n < 0) return fail(BDH_EINVAL, "negative count");
+  if ((n_layers > 0 && (!layers || !rho)) || (n > 0 && (!dst || !src))) return fail(BDH_EINVAL, "null array");
+  if (!src_layers != !src_rho) return fail(BDH_EINVAL, "src_layers and src_rho come together");
+  const bool in_place = !src_rho;
+  int64_t batch = 0, src_batch = 0;
+  std::vector<float*> to;
+  std::vector<const float*> from;
+  std::vector<int64_t> slab;
+  for (int32_t l = 0; l < n_layers; ++l) {
+    const bdh_layer_state_desc& a = layers[l];
+    const bdh_layer_state_desc& b = in_place ? a : src_layers[l];
+    if (a.batch == 0 && b.batch == 0) continue;
+    if (a.batch <= 0 || b.batch <= 0 || a.heads <= 0 || a.latent <= 0 || a.embd <= 0)
+      return fail(BDH_EINVAL, "layer without streams in one of the states, or a dimension below 1");
+    if (a.heads != b.heads || a.latent != b.latent || a.embd != b.embd)
+      return fail(BDH_EINVAL, "the states' layers have different shapes");
+    if (!to.empty() && (a.batch != batch || b.batch != src_batch))
+      return fail(BDH_EINVAL, "the layers of a state have different batches");
+    batch = a.batch;
+    src_batch = b.batch;
+    const int64_t most = (int64_t)1 << 33;  // f32 of a slot: a thread each 4 within a launch's 2^32
+    if (a.heads > most || a.latent > most / a.heads || a.embd > most / (a.heads * a.latent))
+      return fail(BDH_UNSUPPORTED, "stream too large");
+    const float* f = in_place ? rho[l] : src_rho[l];
+    if (!rho[l] || !f) return fail(BDH_EINVAL, "null tensor pointer");
+    if ((((uintptr_t)rho[l] | (uintptr_t)f) & 3) != 0)
+      return fail(BDH_EINVAL, "tensor pointers must be 4-byte aligned");
+    to.push_back(rho[l]);
+    from.push_back(f);
+    slab.push_back(a.heads * a.latent * a.embd);
+  }
+  if (batch > kMaxStreamSlots || src_batch > kMaxStreamSlots)
+    return fail(BDH_UNSUPPORTED, "more than 32767 streams");
+  if (to.empty() || n == 0) return BDH_OK;
+  // Tensors that share memory: threads of one layer would write what others read.
+  const auto apart = [](const float* p, int64_t np, const float* q, int64_t nq) {
+    return (uintptr_t)p + (uintptr_t)np * 4 <= (uintptr_t)q || (uintptr_t)q + (uintptr_t)nq * 4 <= (uintptr_t)p;
+  };
+  for (size_t l = 0; l < to.size(); ++l)
+    for (size_t k = 0; k < to.size(); ++k) {
+      if (k < l && !apart(to[l], batch * slab[l], to[k], batch * slab[k]))
+        return fail(BDH_EINVAL, "two layers' tensors share memory");
+      if (!in_place && !apart(to[l], batch * slab[l], from[k], src_batch * slab[k]))
+        return fail(BDH_EINVAL, "source and destination tensors share memory");
+    }
+  std::vector<char> taken((size_t)batch, 0);
+  for (int32_t i = 0; i < n; ++i) {
+    if (dst[i] < 0 || dst[i] >= batch || src[i] < -1 || src[i] >= src_batch)
+      return fail(BDH_EINVAL, "stream " + std::to_string(i) + " of the call lies outside its batch");
+    if (taken[dst[i]]) return fail(BDH_EINVAL, "slot " + std::to_string(dst[i]) + " is written twice");
+    taken[dst[i]] = 1;
+  }
+  StreamMoves m;
+  m.n_layers = (int)to.size();
+  m.dst_rho = to.data();
+  m.src_rho = from.data();
+  m.slab = slab.data();
+  m.dst_batch = batch;
+  m.src_batch = src_batch;
+  m.in_place = in_place;
+  m.n = n;
+  m.dst = dst;
+  m.src = src;
+  const bdh_status st = copy_streams(m, (hipStream_t)stream, &prof.launches);
+  if (st == BDH_OK) prof.done(true);
+  return st;
+} catch (const std::exception& e) {
+  return fail(BDH_EHIP, e.what());
 }
 
 void bdh_profile_enable(int32_t enabled) { g_prof_on = enabled != 0; }

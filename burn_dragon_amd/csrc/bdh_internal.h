@@ -162,6 +162,24 @@ bdh_status pack_lm_head(int64_t D, int64_t V, const float* head, bf16_t* packed,
 bdh_status lm_logits(const float* hidden, int64_t M, int64_t D, const bf16_t* head, int64_t V,
                      float* logits, hipStream_t st, uint64_t* launches);
 
+// --- streams' states (streams.hip) -------------------------------------------
+// Layer l's slot dst[i] takes the value of slot src[i] (of src_rho[l], slots
+// of the same slab[l] f32; below 0: zeros) for every i, as one assignment.
+// The destinations are distinct and every slot lies in its batch.
+struct StreamMoves {
+  int n_layers;
+  float* const* dst_rho;
+  const float* const* src_rho;  // == dst_rho's pointers when in_place
+  const int64_t* slab;
+  int64_t dst_batch, src_batch; // slots, at most kMaxStreamSlots
+  bool in_place;
+  int n;
+  const int32_t* dst;
+  const int32_t* src;
+};
+constexpr int64_t kMaxStreamSlots = 32767;
+bdh_status copy_streams(const StreamMoves& m, hipStream_t st, uint64_t* launches);
+
 // --- decode (decode.hip) ------------------------------------------------------
 // One token per stream (T = 1).  rho_in == rho (not null) and no decay:
 // the sparse step (only the active rows are read and written).  Otherwise

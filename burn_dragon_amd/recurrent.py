@@ -11,6 +11,7 @@ mismatch, plan mismatch) so that callers fall back exactly as
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from dataclasses import dataclass
 from typing import NamedTuple, Optional
@@ -92,6 +93,14 @@ def _stream_ptr(device: torch.device) -> int:
     """The current stream's handle on a CUDA tensor's device, without building
     a Stream object."""
     return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _on_current_device(device: torch.device):
+    """Makes a tensor's device current for a call where it is not: the
+    library launches on, and keeps its scratch by, the current device."""
+    if device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def _on_device(*ts) -> bool:

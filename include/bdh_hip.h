@@ -331,6 +331,27 @@ bdh_status bdh_state_record_load(const char* path, int32_t n_layers,
                                  const bdh_layer_state_desc* layers, float* const* rho,
                                  void* stream);
 
+/* Moves streams' carried states between slots: for every layer l and every
+ * i < n, slot dst[i] of rho[l] takes the value of slot src[i] of src_rho[l],
+ * or zeros where src[i] is -1 (a fresh sequence, which may begin at any
+ * position: scores depend on differences of positions).  A slot is one stream's [heads, latent, embd] of a
+ * layer's [batch, heads, latent, embd] f32 device tensor (LayerState.rho,
+ * state.rs:7-30).  One assignment: every source is read before any slot is
+ * written, whatever the pattern (forks, chains, exchanges), with no copy
+ * aside and no scratch.
+ * src_layers and src_rho NULL: within rho.  Otherwise the sources are those
+ * tensors: the same slots' shapes, any batch, no memory shared with rho.
+ * layers / src_layers give the shapes (the flags are ignored); a layer whose
+ * batch is 0 has no rho and is skipped (in both).  All layers have one batch.
+ * dst, src: host arrays, read before the call returns; dst distinct.
+ * Pointers 4-byte aligned; batches up to 32767.  No counterpart in the
+ * reference, whose batch is fixed while it generates.  May be captured into
+ * a graph on any stream. */
+bdh_status bdh_state_copy_streams(int32_t n_layers, const bdh_layer_state_desc* layers,
+                                  float* const* rho, const bdh_layer_state_desc* src_layers,
+                                  const float* const* src_rho, int32_t n, const int32_t* dst,
+                                  const int32_t* src, void* stream);
+
 /* Profiling counters with the field names of KernelProfileSnapshot
  * (crates/burn_dragon_kernel/src/profiling.rs:3-16), filled per entry-point
  * call as recurrent.rs:206-215, 344-356 fills them; collected only while

@@ -158,6 +158,11 @@ extern "C" {
     pub fn bdh_state_record_load(path: *const c_char, n_layers: i32,
                                  layers: *const bdh_layer_state_desc, rho: *const *mut f32,
                                  stream: *mut c_void) -> i32;
+    pub fn bdh_state_copy_streams(n_layers: i32, layers: *const bdh_layer_state_desc,
+                                  rho: *const *mut f32,
+                                  src_layers: *const bdh_layer_state_desc,
+                                  src_rho: *const *const f32, n: i32, dst: *const i32,
+                                  src: *const i32, stream: *mut c_void) -> i32;
     pub fn bdh_profile_enable(enabled: i32);
     pub fn bdh_profile_reset();
     pub fn bdh_profile_get(out: *mut bdh_profile_snapshot);
