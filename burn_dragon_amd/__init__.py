@@ -25,3 +25,4 @@ from .layer import LowRankLayerOutput, LowRankWeights, lowrank_layer_forward  # 
 from .model import (BdhModelState, BdhModelWeights, load_model_state, model_forward_logits,  # noqa: F401
                     new_model_state, pack_model, save_model_state)
 from .streams import compact_streams, copy_streams, free_streams  # noqa: F401
+from .sampling import SampleOutput, sample_tokens  # noqa: F401

@@ -53,6 +53,13 @@ class BdhLayerStateDesc(ctypes.Structure):
                 ("retain_terminal_sequence_state", ctypes.c_int32)]
 
 
+class BdhSampleOptions(ctypes.Structure):
+    _fields_ = [("temperature", ctypes.c_float), ("top_p", ctypes.c_float),
+                ("min_p", ctypes.c_float), ("top_k", ctypes.c_int32),
+                ("temperature_rows", ctypes.c_void_p), ("top_p_rows", ctypes.c_void_p),
+                ("min_p_rows", ctypes.c_void_p), ("top_k_rows", ctypes.c_void_p)]
+
+
 class BdhProfileSnapshot(ctypes.Structure):
     _fields_ = [(n, ctypes.c_uint64) for n in (
         "calls", "launches", "total_ns", "setup_ns", "copy_ns", "dispatch_ns",
@@ -96,6 +103,8 @@ SIGNATURES = {
                                      ctypes.POINTER(BdhLayerStateDesc), _i32]),
     "bdh_state_record_load": (_i32, [ctypes.c_char_p, _i32, ctypes.POINTER(BdhLayerStateDesc),
                                      ctypes.POINTER(_vp), _vp]),
+    "bdh_sample_tokens": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp,
+                                 ctypes.POINTER(BdhSampleOptions), _vp, _vp, _vp]),
     "bdh_state_copy_streams": (_i32, [_i32, ctypes.POINTER(BdhLayerStateDesc), ctypes.POINTER(_vp),
                                       ctypes.POINTER(BdhLayerStateDesc), ctypes.POINTER(_vp), _i32,
                                       ctypes.POINTER(_i32), ctypes.POINTER(_i32), _vp]),

@@ -752,6 +752,54 @@ bdh_status bdh_lm_logits(const float* hidden, int64_t rows, int64_t embd,
   return BDH_OK;
 }
 
+bdh_status bdh_sample_tokens(const void* logits, int32_t dtype, int64_t rows, int64_t vocab,
+                             int64_t row_stride, const float* uniform,
+                             const bdh_sample_options* options, int32_t* tokens_out,
+                             float* logprob_out, void* stream) {
+  ProfScope prof;
+  if (rows <= 0 || vocab <= 0) return fail(BDH_UNSUPPORTED, "zero-sized dimension");
+  if (!logits || !uniform || !tokens_out) return fail(BDH_EINVAL, "null tensor pointer");
+  if (dtype != BDH_F32 && dtype != BDH_BF16) return fail(BDH_EINVAL, "unknown dtype");
+  if (vocab > kMaxSampleVocab) return fail(BDH_UNSUPPORTED, "vocab must be at most 2^20");
+  if (rows > ((int64_t)1 << 22) - 1) return fail(BDH_UNSUPPORTED, "too many rows for one launch");
+  if (row_stride < 0 || row_stride > INT64_MAX / 4 / rows) return fail(BDH_EINVAL, "row_stride out of range");
+  if (((uintptr_t)logits & (dtype == BDH_F32 ? 3 : 1)) != 0)
+    return fail(BDH_EINVAL, "logits must be aligned to their elements");
+  bdh_sample_options o{1.0f, 1.0f, 0.0f, 0, nullptr, nullptr, nullptr, nullptr};
+  if (options) o = *options;
+  for (const void* t : {(const void*)uniform, (const void*)tokens_out, (const void*)logprob_out,
+                        (const void*)o.temperature_rows, (const void*)o.top_p_rows,
+                        (const void*)o.min_p_rows, (const void*)o.top_k_rows})
+    if (((uintptr_t)t & 3) != 0) return fail(BDH_EINVAL, "tensor pointers must be 4-byte aligned");
+  if (!o.temperature_rows && !(o.temperature >= 0.0f && std::isfinite(o.temperature)))
+    return fail(BDH_EINVAL, "temperature must be finite and not negative");
+  if (!o.top_p_rows && !(o.top_p >= 0.0f && o.top_p <= 1.0f))
+    return fail(BDH_EINVAL, "top_p must lie in [0, 1]");
+  if (!o.min_p_rows && !(o.min_p >= 0.0f && o.min_p <= 1.0f))
+    return fail(BDH_EINVAL, "min_p must lie in [0, 1]");
+  if (!o.top_k_rows && o.top_k < 0) return fail(BDH_EINVAL, "top_k must not be negative");
+  SampleArgs a;
+  a.logits = logits;
+  a.bf16 = dtype == BDH_BF16;
+  a.rows = rows;
+  a.vocab = vocab;
+  a.row_stride = row_stride;
+  a.uniform = uniform;
+  a.temperature = o.temperature;
+  a.top_p = o.top_p;
+  a.min_p = o.min_p;
+  a.top_k = o.top_k;
+  a.temperature_rows = o.temperature_rows;
+  a.top_p_rows = o.top_p_rows;
+  a.min_p_rows = o.min_p_rows;
+  a.top_k_rows = o.top_k_rows;
+  a.tokens = tokens_out;
+  a.logprob = logprob_out;
+  const bdh_status st = sample_tokens(a, (hipStream_t)stream, &prof.launches);
+  if (st == BDH_OK) prof.done(true);
+  return st;
+}
+
 bdh_status bdh_state_copy_streams(int32_t n_layers, const bdh_layer_state_desc* layers,
                                   float* const* rho, const bdh_layer_state_desc* src_layers,
                                   const float* const* src_rho, int32_t n, const int32_t* dst,

@@ -48,6 +48,7 @@ enum ScratchSlot {
   SLOT_VJP_RHO,      // VJP states at interval starts [n_iv - 1, S, N, D] f32
   SLOT_VJP_GAMMA,    // VJP state gradients          2 x [S, N, D] f32
   SLOT_SNAP,         // states at interval starts: bf16 path [n_iv, S, D, N] bf16, fp32 path [n_iv - 1, S, N, D] f32
+  SLOT_SAMPLE,       // sampling of long rows: chunks' histograms, candidates (sample.hip)
   SLOT_COUNT
 };
 // Scratch of the calling stream (see api.hip): grows on first use of a
@@ -179,6 +180,23 @@ struct StreamMoves {
 };
 constexpr int64_t kMaxStreamSlots = 32767;
 bdh_status copy_streams(const StreamMoves& m, hipStream_t st, uint64_t* launches);
+
+// --- sampling (sample.hip) -----------------------------------------------------
+constexpr int64_t kMaxSampleVocab = (int64_t)1 << 20;
+struct SampleArgs {
+  const void* logits;   // [rows] rows of vocab logits, row_stride elements apart
+  bool bf16;
+  int64_t rows, vocab, row_stride;
+  const float* uniform; // [rows]
+  // One value for all rows, or one a row where the pointer is set.
+  float temperature, top_p, min_p;
+  int32_t top_k;
+  const float *temperature_rows, *top_p_rows, *min_p_rows;
+  const int32_t* top_k_rows;
+  int32_t* tokens;      // [rows]
+  float* logprob;       // [rows] or null
+};
+bdh_status sample_tokens(const SampleArgs& a, hipStream_t st, uint64_t* launches);
 
 // --- decode (decode.hip) ------------------------------------------------------
 // One token per stream (T = 1).  rho_in == rho (not null) and no decay:

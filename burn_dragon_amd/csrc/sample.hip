@@ -1,0 +1,894 @@
+// The next token of every row from its logits and a given uniform number:
+// temperature, top-k, top-p and min-p.
+//
+// Of a row: x = logits (NaN as -inf, +inf as the largest finite f32), m the
+// largest, t_i = (x_i - m) log2(e) / temperature, w_i = 2^t_i where
+// t_i >= -42 and 0 below.  In the order of x descending, ties by index
+// ascending: top-k keeps the first k, top-p the ones before which the kept w
+// sum to less than top_p of all that top-k kept, min-p those of w >= min_p.
+// The token is the first in vocabulary order whose running sum of kept w
+// exceeds uniform * (their sum).
+//
+// No sort.  The weights are integers, w * 2^42 rounded, from a 64-bit 2^t:
+// sums of them are exact, so no order of atomics or of partial sums changes a
+// token, and a sum is right to 2^-42 of the largest weight where a border
+// (of top-p, of the draw) falls between two tokens.  Up to 2^20 logits, a sum
+// stays below 2^62.
+//
+//   1. A histogram over 512 bins of 1/12 octave of weight below the largest
+//      (counts for top-k, weights for top-p) finds the bin in which a cut
+//      falls; bins before it are kept whole, bins after it are not.
+//   2. The candidates of that bin go to a list.  Up to 64 are ordered in one
+//      wave, each lane counting what comes before its own; more are narrowed
+//      first by histograms of nine bits of (value, index), so equal logits
+//      are cut by index.  A list that overflows is read from the row again.
+//   3. The kept weights are summed by wave, and the draw descends into the
+//      wave, the stripe, the lane and the element that it falls in.
+//
+// Rows up to 32768 logits: one workgroup, the row in registers, read once.
+// Longer ones in chunks of 8192, four launches (sample_chunk_kernel on).
+#include "bdh_internal.h"
+
+namespace bdh {
+namespace {
+
+constexpr int kBins = 512;
+constexpr int kBinsPerOctave = 12;
+constexpr double kLeastT = -42.0;
+constexpr int kSmall = 64;       // candidates that one wave orders
+constexpr int kListMax = 4096;   // candidates that the list holds
+constexpr int kChunkThreads = 512;
+constexpr int kChunkPer = 16;    // logits a thread
+constexpr int kChunk = kChunkThreads * kChunkPer;
+constexpr int kMaxChunks = (int)(kMaxSampleVocab / kChunk);
+constexpr int kNoLimitIndex = 0x7fffffff;
+
+struct Row {
+  double c;      // log2(e) / temperature
+  double cb;     // bins per unit of x
+  double min_t;  // least t that is kept
+  double p;
+  int k;
+  bool greedy, use_k, use_p;
+  float u;
+};
+
+__device__ Row row_settings(const SampleArgs& a, int64_t r) {
+  const float tau = a.temperature_rows ? a.temperature_rows[r] : a.temperature;
+  const float p = a.top_p_rows ? a.top_p_rows[r] : a.top_p;
+  const float mp = a.min_p_rows ? a.min_p_rows[r] : a.min_p;
+  Row s;
+  s.k = a.top_k_rows ? a.top_k_rows[r] : a.top_k;
+  s.greedy = !(tau > 0.0f) || s.k == 1;
+  s.c = 1.4426950408889634074 / (double)tau;
+  s.cb = s.c * kBinsPerOctave;
+  s.use_k = s.k > 0 && s.k < a.vocab;
+  s.use_p = p < 1.0f;
+  s.p = p > 0.0f ? (double)p : 0.0;
+  s.min_t = mp > 0.0f ? fmax(log2((double)fminf(mp, 1.0f)), kLeastT) : kLeastT;
+  s.u = a.uniform[r];
+  return s;
+}
+
+// 2^t * 2^42 as an integer, t in [-42, 0]; 2^f by its series to the 11th
+// power (the rest is below 2^-47 of it), 64-bit throughout.
+__device__ __forceinline__ uint64_t weight42(double t) {
+  const double magic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer
+  const double kd = t + magic;
+  const int n = (int)(uint32_t)__double_as_longlong(kd);
+  const double f = t - (kd - magic);
+  double e = 4.45538190442164e-10;  // ln(2)^k / k!
+  e = fma(e, f, 7.054911620801123e-09);
+  e = fma(e, f, 1.0178086009239699e-07);
+  e = fma(e, f, 1.3215486790144307e-06);
+  e = fma(e, f, 1.525273380405984e-05);
+  e = fma(e, f, 0.0001540353039338161);
+  e = fma(e, f, 0.0013333558146428443);
+  e = fma(e, f, 0.009618129107628477);
+  e = fma(e, f, 0.05550410866482158);
+  e = fma(e, f, 0.2402265069591007);
+  e = fma(e, f, 0.6931471805599453);
+  e = fma(e, f, 1.0);
+  const double w = __longlong_as_double(__double_as_longlong(e) + ((int64_t)(n + 42) << 52));
+  return (uint64_t)__double_as_longlong(w + 4503599627370496.0) - 0x4330000000000000ull;
+}
+
+// Its weight where t is kept at all.
+__device__ __forceinline__ uint64_t weight_from(double t, double least) {
+  return t >= least ? weight42(t) : 0;  // (NaN: -inf logits at an infinite temperature)
+}
+
+__device__ __forceinline__ float clean(float x) {
+  x = x != x ? -INFINITY : x;
+  return fminf(x, 3.402823466e38f) + 0.0f;  // -0 as 0: equal logits are equal bits
+}
+
+// (value, index) as one number, smaller = earlier in the order.
+__device__ __forceinline__ uint64_t order_of(float x, int idx) {
+  const uint32_t b = __float_as_uint(x);
+  const uint32_t up = b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+  return ((uint64_t)~up << 32) | (uint32_t)idx;
+}
+__device__ __forceinline__ float value_of(uint64_t o) {
+  const uint32_t up = ~(uint32_t)(o >> 32);
+  return __uint_as_float((up >> 31) ? up ^ 0x80000000u : ~up);
+}
+
+// The bin of a logit in a grid that all chunks of a row share, counted from
+// the bin `top` of the largest; kBins where it is further down (weight 0).
+__device__ __forceinline__ int bin_of(float x, double top, double cb) {
+  const double d = top - floor((double)x * cb);
+  return d < (double)kBins ? (int)d : kBins;  // (-inf: +inf; NaN does not occur but at cb = 0)
+}
+__device__ __forceinline__ bool is_real(float x) { return x > -INFINITY; }
+
+template <typename T>
+__device__ __forceinline__ float load1(const T* p) { return clean((float)*p); }
+
+typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
+typedef __bf16 bf16x4_u __attribute__((ext_vector_type(4), aligned(2)));
+template <typename T> struct Vec4;
+template <> struct Vec4<float> { typedef f32x4_u type; };
+template <> struct Vec4<bf16_t> { typedef bf16x4_u type; };
+
+// A chunk's logits: each wave holds 64 * E consecutive ones in stripes of
+// 256, each lane four of a stripe.
+template <int E>
+__device__ __forceinline__ int index_of(int base, int e) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  return base + wave * (64 * E) + ((e >> 2) * 64 + lane) * 4 + (e & 3);
+}
+template <typename T, int E>
+__device__ __forceinline__ void load_chunk(const T* row, int base, int vocab, float (&x)[E]) {
+#pragma unroll
+  for (int e = 0; e < E; e += 4) {
+    const int i = index_of<E>(base, e);
+    if (i + 4 <= vocab) {
+      const typename Vec4<T>::type v = *(const typename Vec4<T>::type*)(row + i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[e + j] = clean((float)v[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[e + j] = i + j < vocab ? load1(row + i + j) : -INFINITY;
+    }
+  }
+}
+
+// Keeps the compiler from carrying what it has computed of the logits from one
+// pass over them to the next (their f64 forms alone would fill the registers).
+template <int E>
+__device__ __forceinline__ void forget(float (&x)[E]) {
+#pragma unroll
+  for (int e = 0; e < E; ++e) asm volatile("" : "+v"(x[e]));
+}
+
+template <int NT, int LIST>
+struct Shared {
+  uint64_t mass[kBins];
+  uint64_t list[LIST];
+  uint64_t small[kSmall], small_w[kSmall];
+  uint64_t wave_sum[NT / 64];
+  uint64_t lo, hi, sum;  // of a pass over the candidates
+  uint32_t cnt[kBins];
+  float wave_max[NT / 64];
+  int n_list, n_small, arg;
+  int bin;
+  uint64_t above;
+};
+
+template <int NT>
+__device__ __forceinline__ float block_max(float v, float* part) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  if (NT == 64) return v;
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = part[0];
+#pragma unroll
+  for (int w = 1; w < NT / 64; ++w) v = fmaxf(v, part[w]);
+  return v;
+}
+
+__device__ __forceinline__ uint64_t shfl_u64(uint64_t v, int lane) {
+  return (uint64_t)__shfl((unsigned long long)v, lane, 64);
+}
+__device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += (uint64_t)__shfl_xor((unsigned long long)v, o, 64);
+  return v;
+}
+__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v) {  // inclusive
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint64_t w = (uint64_t)__shfl_up((unsigned long long)v, o, 64);
+    if (lane >= o) v += w;
+  }
+  return v;
+}
+
+// One wave: the first of the kBins bins at which the running sum reaches
+// `need` (-1: it does not), and the sums before and after it, or of all.
+template <typename H>
+__device__ void cross_bins(const H* h, uint64_t need, int* bin, uint64_t* before, uint64_t* upto) {
+  const int lane = threadIdx.x & 63;
+  uint64_t v[kBins / 64], s = 0;
+#pragma unroll
+  for (int j = 0; j < kBins / 64; ++j) {
+    v[j] = h[lane * (kBins / 64) + j];
+    s += v[j];
+  }
+  const uint64_t incl = wave_scan_u64(s);
+  uint64_t run = incl - s, b = 0, up = 0;
+  int at = -1;
+#pragma unroll
+  for (int j = 0; j < kBins / 64; ++j) {
+    if (at < 0 && run + v[j] >= need) {
+      at = lane * (kBins / 64) + j;
+      b = run;
+      up = run + v[j];
+    }
+    run += v[j];
+  }
+  const uint64_t found = __ballot(at >= 0);
+  if (found == 0) {
+    *bin = -1;
+    *before = *upto = shfl_u64(incl, 63);
+    return;
+  }
+  const int first = __builtin_ctzll(found);
+  *bin = __shfl(at, first, 64);
+  *before = shfl_u64(b, first);
+  *upto = shfl_u64(up, first);
+}
+
+// What the histogram says about the cuts of a row.
+struct Cuts {
+  int k_bin;            // holds the k-th in order; kBins: top-k cuts nothing that is drawn
+  int p_first, p_last;  // bins that the top-p cut can fall in; kBins: no top-p
+  uint64_t k_above;     // logits in bins before k_bin
+  uint64_t k_mass;      // their weight (all weight: no k_bin)
+  uint64_t p_above;     // weight in bins before p_first
+};
+__device__ __forceinline__ uint64_t p_need(const Row& s, uint64_t total) {
+  const uint64_t need = (uint64_t)ceil(s.p * (double)total);
+  return need > 0 ? need : 1;  // the first in order is always kept
+}
+// One wave.
+__device__ Cuts find_cuts(const Row& s, const uint32_t* cnt, const uint64_t* mass) {
+  Cuts q;
+  q.k_bin = q.p_first = q.p_last = kBins;
+  q.k_above = q.k_mass = q.p_above = 0;
+  uint64_t upto = 0;
+  if (s.use_k) {
+    cross_bins(cnt, (uint64_t)s.k, &q.k_bin, &q.k_above, &upto);
+    if (q.k_bin < 0) q.k_bin = kBins;
+  }
+  if (s.use_p) {
+    // The weight before k_bin, and with it: between them lies what top-k keeps.
+    const int lane = threadIdx.x & 63;
+    uint64_t before = 0, at = 0;
+#pragma unroll
+    for (int j = 0; j < kBins / 64; ++j) {
+      const int b = lane * (kBins / 64) + j;
+      if (b < q.k_bin) before += mass[b];
+      if (b == q.k_bin) at = mass[b];
+    }
+    q.k_mass = wave_sum_u64(before);
+    const uint64_t most = q.k_mass + wave_sum_u64(at);
+    uint64_t unused;
+    cross_bins(mass, p_need(s, q.k_mass), &q.p_first, &q.p_above, &upto);
+    cross_bins(mass, p_need(s, most), &q.p_last, &unused, &upto);
+    // (Past k_bin the histogram may hold weights too; none is kept.)
+    if (q.p_first < 0 || q.p_first > q.k_bin) q.p_first = q.k_bin;
+    if (q.p_last < 0 || q.p_last > q.k_bin) q.p_last = q.k_bin;
+  }
+  return q;
+}
+__device__ __forceinline__ int sure_bins(const Cuts& q) { return min(q.k_bin, q.p_first); }
+__device__ __forceinline__ bool is_candidate(const Cuts& q, int bin) {
+  return bin < kBins && (bin == q.k_bin || (bin >= q.p_first && bin <= q.p_last && bin <= q.k_bin));
+}
+
+// The candidates: in the list, or where it overflowed all of the row's logits.
+template <typename T, int NT, int LIST>
+struct Candidates {
+  Shared<NT, LIST>& sh;
+  const T* row;
+  int vocab;
+  float m;
+  double top;
+  const Row& s;
+  int n;  // found; beyond LIST the list is not complete
+
+  // Calls f(order, bin) for each whose bin lies in [first, last].
+  template <typename F>
+  __device__ __forceinline__ void each(int first, int last, const F& f) {
+    if (n <= LIST) {
+      for (int i = threadIdx.x; i < n; i += NT) {
+        const uint64_t o = sh.list[i];
+        const int b = bin_of(value_of(o), top, s.cb);
+        if (b >= first && b <= last) f(o, b);
+      }
+    } else {
+      for (int i = threadIdx.x; i < vocab; i += NT) {
+        const float x = load1(row + i);
+        if (!is_real(x)) continue;
+        const int b = bin_of(x, top, s.cb);
+        if (b >= first && b <= last) f(order_of(x, i), b);
+      }
+    }
+  }
+  __device__ __forceinline__ uint64_t weight(uint64_t o, double least) const {
+    return weight_from(((double)value_of(o) - (double)m) * s.c, least);
+  }
+
+  // The last candidate in order that a cut keeps, among those of bins
+  // [first, last]: by count, the one with `need` - 1 logits before it; by
+  // weight, the last with less than `need` of weight before it.  `above`:
+  // what lies before bin `first`.
+  template <bool MASS>
+  __device__ uint64_t cut(int first, int last, uint64_t above, uint64_t need) {
+    uint64_t lo = 0, hi = ~0ull;
+    for (;;) {
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        sh.lo = ~0ull;
+        sh.hi = 0;
+        sh.n_small = 0;
+      }
+      __syncthreads();
+      each(first, last, [&](uint64_t o, int) {
+        if (o < lo || o > hi) return;
+        const int at = atomicAdd(&sh.n_small, 1);
+        if (at < kSmall) sh.small[at] = o;
+        atomicMin((unsigned long long*)&sh.lo, (unsigned long long)o);
+        atomicMax((unsigned long long*)&sh.hi, (unsigned long long)o);
+      });
+      __syncthreads();
+      const int n_in = sh.n_small;
+      if (n_in <= kSmall) {
+        if (threadIdx.x < 64) {
+          const int lane = threadIdx.x;
+          const uint64_t mine = lane < n_in ? sh.small[lane] : ~0ull;
+          if (lane < n_in) sh.small_w[lane] = MASS ? weight(mine, kLeastT) : 1;
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          uint64_t before = above;
+          for (int j = 0; j < n_in; ++j)
+            if (sh.small[j] < mine) before += sh.small_w[j];
+          const bool kept = lane < n_in && before < need;
+          uint64_t best = kept ? mine : 0;
+#pragma unroll
+          for (int o = 32; o > 0; o >>= 1) {
+            const uint64_t b = (uint64_t)__shfl_xor((unsigned long long)best, o, 64);
+            best = b > best ? b : best;
+          }
+          if (lane == 0) sh.sum = best;
+        }
+        __syncthreads();
+        return sh.sum;
+      }
+      const uint64_t from = sh.lo, to = sh.hi;
+      const int high = 63 - __builtin_clzll(from ^ to);
+      const int shift = high > 8 ? high - 8 : 0;
+      for (int b = threadIdx.x; b < kBins; b += NT) sh.mass[b] = 0;
+      __syncthreads();
+      each(first, last, [&](uint64_t o, int) {
+        if (o < lo || o > hi) return;
+        const uint64_t w = MASS ? weight(o, kLeastT) : 1;
+        atomicAdd((unsigned long long*)&sh.mass[(int)((o >> shift) - (from >> shift))], (unsigned long long)w);
+      });
+      __syncthreads();
+      if (threadIdx.x < 64) {
+        int bin;
+        uint64_t before, upto;
+        cross_bins(sh.mass, need > above ? need - above : 1, &bin, &before, &upto);
+        if (threadIdx.x == 0) {
+          // (Weights scaled from chunks may leave the sum a unit short: the last candidate.)
+          sh.bin = bin < 0 ? (int)((to >> shift) - (from >> shift)) : bin;
+          sh.above = bin < 0 ? above : above + before;
+        }
+      }
+      __syncthreads();
+      lo = ((from >> shift) + (uint64_t)sh.bin) << shift;
+      hi = lo + ((1ull << shift) - 1);
+      above = sh.above;
+    }
+  }
+
+  // The last logit in order that top-k and top-p keep.
+  __device__ uint64_t limit(const Cuts& q) {
+    uint64_t lim = ~0ull, total = q.k_mass;
+    if (q.k_bin < kBins) {
+      lim = cut<false>(q.k_bin, q.k_bin, q.k_above, (uint64_t)s.k);
+      if (s.use_p) {
+        __syncthreads();
+        if (threadIdx.x == 0) sh.sum = 0;
+        __syncthreads();
+        uint64_t w = 0;
+        each(q.k_bin, q.k_bin, [&](uint64_t o, int) { w += o <= lim ? weight(o, kLeastT) : 0; });
+        if (w) atomicAdd((unsigned long long*)&sh.sum, (unsigned long long)w);
+        __syncthreads();
+        total += sh.sum;
+      }
+    }
+    if (s.use_p && q.p_first < kBins) {
+      const uint64_t lp = cut<true>(q.p_first, q.p_last, q.p_above, p_need(s, total));
+      lim = lp < lim ? lp : lim;
+    }
+    return lim;
+  }
+};
+
+// The kept weight of a thread's logits: those up to (limit_x, limit_i) in order.
+template <int E>
+__device__ __forceinline__ uint64_t kept_weight(const Row& s, float x, int i, float m, float limit_x, int limit_i) {
+  if (!(x > limit_x || (x == limit_x && i <= limit_i))) return 0;
+  return weight_from(((double)x - (double)m) * s.c, s.min_t);
+}
+
+__device__ __forceinline__ uint64_t draw_at(float u, uint64_t total) {
+  const uint64_t at = u > 0.0f ? (uint64_t)((double)fminf(u, 0x1.fffffep-1f) * (double)total) : 0;
+  return at < total ? at : total - 1;
+}
+
+// Finds the logit of the chunk that the draw falls in: the first whose
+// running sum of kept weights exceeds `at` (at < their sum).  Returns true in
+// the one thread that holds it.
+template <int NT, int E, int LIST>
+__device__ bool locate(Shared<NT, LIST>& sh, const Row& s, const float (&x)[E], int base, float m, float limit_x,
+                       int limit_i, uint64_t at, int* token, double* t) {
+  const int wave = threadIdx.x >> 6;
+  uint64_t before = 0;
+  for (int w = 0; w < NT / 64; ++w) {
+    const uint64_t sum = sh.wave_sum[w];
+    if (at < before + sum) {
+      if (w != wave) return false;
+      break;
+    }
+    before += sum;
+  }
+  at -= before;
+  for (int e = 0; e < E; e += 4) {
+    uint64_t w[4], mine = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      // (x[e] by a select: the loop is not unrolled, one stripe at a time is few instructions.)
+      float v = 0.0f;
+#pragma unroll
+      for (int q = 0; q < E; q += 4) v = q == e ? x[q + j] : v;
+      w[j] = kept_weight<E>(s, v, index_of<E>(base, e) + j, m, limit_x, limit_i);
+      mine += w[j];
+    }
+    const uint64_t incl = wave_scan_u64(mine);
+    const uint64_t stripe = shfl_u64(incl, 63);
+    if (at >= stripe) {
+      at -= stripe;
+      continue;
+    }
+    uint64_t run = incl - mine;
+    if (at < run || at >= incl) return false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (at < run + w[j]) {
+        float v = 0.0f;
+#pragma unroll
+        for (int q = 0; q < E; q += 4) v = q == e ? x[q + j] : v;
+        *token = index_of<E>(base, e) + j;
+        *t = ((double)v - (double)m) * s.c;
+        return true;
+      }
+      run += w[j];
+    }
+  }
+  return false;
+}
+
+template <typename T, int NT, int E>
+__global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a) {
+  constexpr int LIST = NT * E < kListMax ? NT * E : kListMax;
+  __shared__ Shared<NT, LIST> sh;
+  const int64_t r = blockIdx.x;
+  const T* row = (const T*)a.logits + r * a.row_stride;
+  const Row s = row_settings(a, r);
+  const int vocab = (int)a.vocab;
+  float x[E];
+  load_chunk<T, E>(row, 0, vocab, x);
+  float best = x[0];
+#pragma unroll
+  for (int e = 1; e < E; ++e) best = fmaxf(best, x[e]);
+  const float m = block_max<NT>(best, sh.wave_max);
+  if (!is_real(m)) {
+    if (threadIdx.x == 0) {
+      a.tokens[r] = -1;
+      if (a.logprob) a.logprob[r] = -INFINITY;
+    }
+    return;
+  }
+  if (s.greedy) {
+    if (threadIdx.x == 0) sh.arg = kNoLimitIndex;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (x[e] == m) atomicMin(&sh.arg, index_of<E>(0, e));
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      a.tokens[r] = sh.arg;
+      if (a.logprob) a.logprob[r] = 0.0f;
+    }
+    return;
+  }
+  float limit_x = -INFINITY;
+  int limit_i = -1;  // (-inf itself is not kept)
+  if (s.use_k || s.use_p) {
+    const double top = floor((double)m * s.cb);
+    for (int b = threadIdx.x; b < kBins; b += NT) {
+      sh.cnt[b] = 0;
+      sh.mass[b] = 0;
+    }
+    if (threadIdx.x == 0) {
+      sh.n_list = 0;
+      sh.bin = kBins;
+    }
+    __syncthreads();
+    if (s.use_k) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int b = is_real(x[e]) ? bin_of(x[e], top, s.cb) : kBins;
+        if (b < kBins) atomicAdd(&sh.cnt[b], 1u);
+      }
+      __syncthreads();
+      if (threadIdx.x < 64) {
+        int bin;
+        uint64_t before, upto;
+        cross_bins(sh.cnt, (uint64_t)s.k, &bin, &before, &upto);
+        if (threadIdx.x == 0 && bin >= 0) sh.bin = bin;
+      }
+      __syncthreads();
+    }
+    forget<E>(x);
+    if (s.use_p) {
+      const int last = sh.bin;  // no weight past the k-th counts
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int b = is_real(x[e]) ? bin_of(x[e], top, s.cb) : kBins;
+        if (b < kBins && b <= last)
+          atomicAdd((unsigned long long*)&sh.mass[b],
+                    (unsigned long long)weight_from(((double)x[e] - (double)m) * s.c, kLeastT));
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      __syncthreads();
+    }
+    const Cuts q = find_cuts(s, sh.cnt, sh.mass);  // (every wave, the same)
+    forget<E>(x);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int b = is_real(x[e]) ? bin_of(x[e], top, s.cb) : kBins;
+      if (is_candidate(q, b)) {
+        const int at = atomicAdd(&sh.n_list, 1);
+        if (at < LIST) sh.list[at] = order_of(x[e], index_of<E>(0, e));
+      }
+    }
+    __syncthreads();
+    Candidates<T, NT, LIST> cand{sh, row, vocab, m, top, s, sh.n_list};
+    const uint64_t lim = cand.limit(q);
+    if (lim != ~0ull) {
+      limit_x = value_of(lim);
+      limit_i = (int)(uint32_t)lim;
+    }
+  }
+  forget<E>(x);
+  uint64_t mine = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    mine += kept_weight<E>(s, x[e], index_of<E>(0, e), m, limit_x, limit_i);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  mine = wave_sum_u64(mine);
+  if ((threadIdx.x & 63) == 0) sh.wave_sum[threadIdx.x >> 6] = mine;
+  __syncthreads();
+  uint64_t total = 0;
+  for (int w = 0; w < NT / 64; ++w) total += sh.wave_sum[w];
+  forget<E>(x);
+  int token;
+  double t;
+  if (locate<NT, E, LIST>(sh, s, x, 0, m, limit_x, limit_i, draw_at(s.u, total), &token, &t)) {
+    a.tokens[r] = token;
+    if (a.logprob) a.logprob[r] = (float)(t * 0.69314718055994530942 - log((double)total * 0x1p-42));
+  }
+}
+
+// --- long rows ---------------------------------------------------------------
+// What a row's launches leave for one another.
+struct RowState {
+  Cuts cuts;
+  double top;
+  float m;
+  int n_list;
+};
+struct SplitArgs {
+  SampleArgs a;
+  int64_t row0;      // of this group of rows
+  int chunks;
+  float* max;        // [rows, chunks]
+  int32_t* arg;      // [rows, chunks]: the first index of the chunk's largest
+  uint32_t* cnt;     // [rows, chunks, kBins], by the chunk's own top bin
+  uint64_t* mass;    // [rows, chunks, kBins], weights below the chunk's own largest
+  uint64_t* sure;    // [rows, chunks]: weight that is kept whatever the cuts' candidates
+  uint64_t* list;    // [rows, kListMax]
+  RowState* state;   // [rows]
+};
+
+// 1. A chunk's largest logit and its histogram, relative to that.
+template <typename T>
+__global__ __launch_bounds__(kChunkThreads) void sample_chunk_kernel(const SplitArgs p) {
+  constexpr int E = kChunkPer, NT = kChunkThreads;
+  __shared__ uint64_t mass[kBins];
+  __shared__ uint32_t cnt[kBins];
+  __shared__ float part[NT / 64];
+  __shared__ int k_bin, arg;
+  const int64_t lr = blockIdx.y, r = p.row0 + lr;
+  const int64_t slot = lr * p.chunks + blockIdx.x;
+  const T* row = (const T*)p.a.logits + r * p.a.row_stride;
+  const Row s = row_settings(p.a, r);
+  const int base = (int)blockIdx.x * kChunk;
+  float x[E];
+  load_chunk<T, E>(row, base, (int)p.a.vocab, x);
+  for (int b = threadIdx.x; b < kBins; b += NT) {
+    cnt[b] = 0;
+    mass[b] = 0;
+  }
+  if (threadIdx.x == 0) {
+    k_bin = kBins;
+    arg = kNoLimitIndex;
+  }
+  float best = x[0];
+#pragma unroll
+  for (int e = 1; e < E; ++e) best = fmaxf(best, x[e]);
+  const float m = block_max<NT>(best, part);
+  if (threadIdx.x == 0) p.max[slot] = m;
+  if (!is_real(m)) return;
+  if (s.greedy) {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (x[e] == m) atomicMin(&arg, index_of<E>(base, e));
+    __syncthreads();
+    if (threadIdx.x == 0) p.arg[slot] = arg;
+    return;
+  }
+  const double top = floor((double)m * s.cb);
+  if (s.use_k) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int b = is_real(x[e]) ? bin_of(x[e], top, s.cb) : kBins;
+      if (b < kBins) atomicAdd(&cnt[b], 1u);
+    }
+    __syncthreads();
+    // Past the chunk's own k-th no logit is among the row's first k.
+    if (threadIdx.x < 64) {
+      int bin;
+      uint64_t before, upto;
+      cross_bins(cnt, (uint64_t)s.k, &bin, &before, &upto);
+      if (threadIdx.x == 0 && bin >= 0) k_bin = bin;
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b < kBins; b += NT) p.cnt[slot * kBins + b] = cnt[b];
+  }
+  if (s.use_p) {
+    const int last = k_bin;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int b = is_real(x[e]) ? bin_of(x[e], top, s.cb) : kBins;
+      if (b < kBins && b <= last)
+        atomicAdd((unsigned long long*)&mass[b],
+                  (unsigned long long)weight_from(((double)x[e] - (double)m) * s.c, kLeastT));
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b < kBins; b += NT) p.mass[slot * kBins + b] = mass[b];
+  }
+}
+
+// 2. The row's histogram from its chunks', and the bins that its cuts fall in.
+__global__ __launch_bounds__(kBins) void sample_merge_kernel(const SplitArgs p) {
+  __shared__ uint64_t mass[kBins];
+  __shared__ uint32_t cnt[kBins];
+  const int64_t lr = blockIdx.x, r = p.row0 + lr;
+  const Row s = row_settings(p.a, r);
+  const float* max = p.max + lr * p.chunks;
+  float m = -INFINITY;
+  for (int g = 0; g < p.chunks; ++g) m = fmaxf(m, max[g]);
+  const double top = floor((double)m * s.cb);
+  Cuts q;
+  q.k_bin = q.p_first = q.p_last = kBins;
+  q.k_above = q.k_mass = q.p_above = 0;
+  if (is_real(m) && !s.greedy && (s.use_k || s.use_p)) {
+    const int b = threadIdx.x;
+    uint32_t n = 0;
+    uint64_t w = 0;
+    for (int g = 0; g < p.chunks; ++g) {
+      if (!is_real(max[g])) continue;
+      const double shift = top - floor((double)max[g] * s.cb);
+      if (!(shift <= (double)b)) continue;
+      const int64_t at = (lr * p.chunks + g) * kBins + (b - (int)shift);
+      if (s.use_k) n += p.cnt[at];
+      if (s.use_p) w += (uint64_t)rint((double)p.mass[at] * exp2(((double)max[g] - (double)m) * s.c));
+    }
+    cnt[b] = n;
+    mass[b] = w;
+    __syncthreads();
+    if (threadIdx.x < 64) q = find_cuts(s, cnt, mass);
+  }
+  if (threadIdx.x == 0) p.state[lr] = RowState{q, top, m, 0};
+}
+
+// 3. A chunk's weight that is kept for certain, and its candidates.
+template <typename T>
+__global__ __launch_bounds__(kChunkThreads) void sample_gather_kernel(const SplitArgs p) {
+  constexpr int E = kChunkPer, NT = kChunkThreads;
+  __shared__ uint64_t part[NT / 64];
+  const int64_t lr = blockIdx.y, r = p.row0 + lr;
+  const int64_t slot = lr * p.chunks + blockIdx.x;
+  const T* row = (const T*)p.a.logits + r * p.a.row_stride;
+  const Row s = row_settings(p.a, r);
+  RowState* st = p.state + lr;
+  const float m = st->m;
+  if (s.greedy || !is_real(m)) return;
+  const Cuts q = st->cuts;
+  const double top = st->top;
+  const bool cuts = s.use_k || s.use_p;
+  const int sure = sure_bins(q);
+  const int base = (int)blockIdx.x * kChunk;
+  float x[E];
+  load_chunk<T, E>(row, base, (int)p.a.vocab, x);
+  uint64_t mine = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    if (!is_real(x[e])) continue;
+    if (cuts) {
+      const int b = bin_of(x[e], top, s.cb);
+      if (is_candidate(q, b)) {
+        const int at = atomicAdd(&st->n_list, 1);
+        if (at < kListMax) p.list[lr * kListMax + at] = order_of(x[e], index_of<E>(base, e));
+        continue;
+      }
+      if (b >= sure) continue;
+    }
+    mine += weight_from(((double)x[e] - (double)m) * s.c, s.min_t);
+  }
+  mine = wave_sum_u64(mine);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = mine;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    uint64_t sum = 0;
+    for (int w = 0; w < NT / 64; ++w) sum += part[w];
+    p.sure[slot] = sum;
+  }
+}
+
+// 4. The cuts among the candidates, the chunk that the draw falls in, its token.
+template <typename T>
+__global__ __launch_bounds__(kChunkThreads) void sample_finish_kernel(const SplitArgs p) {
+  constexpr int E = kChunkPer, NT = kChunkThreads, LIST = kListMax;
+  __shared__ Shared<NT, LIST> sh;
+  __shared__ uint64_t chunk_sum[kMaxChunks];
+  const int64_t lr = blockIdx.x, r = p.row0 + lr;
+  const SampleArgs& a = p.a;
+  const T* row = (const T*)a.logits + r * a.row_stride;
+  const Row s = row_settings(a, r);
+  const RowState st = p.state[lr];
+  const float m = st.m;
+  if (!is_real(m) || s.greedy) {
+    if (threadIdx.x == 0) {
+      int token = -1;
+      for (int g = p.chunks - 1; g >= 0 && is_real(m); --g)
+        if (p.max[lr * p.chunks + g] == m) token = p.arg[lr * p.chunks + g];
+      a.tokens[r] = token;
+      if (a.logprob) a.logprob[r] = is_real(m) ? 0.0f : -INFINITY;
+    }
+    return;
+  }
+  for (int g = threadIdx.x; g < p.chunks; g += NT) chunk_sum[g] = p.sure[lr * p.chunks + g];
+  const int n = st.n_list;
+  if (n <= LIST)
+    for (int i = threadIdx.x; i < n; i += NT) sh.list[i] = p.list[lr * kListMax + i];
+  __syncthreads();
+  float limit_x = -INFINITY;
+  int limit_i = -1;
+  if (s.use_k || s.use_p) {
+    Candidates<T, NT, LIST> cand{sh, row, (int)a.vocab, m, st.top, s, n};
+    const uint64_t lim = cand.limit(st.cuts);
+    if (lim != ~0ull) {
+      limit_x = value_of(lim);
+      limit_i = (int)(uint32_t)lim;
+    }
+    const int sure = sure_bins(st.cuts);
+    cand.each(sure, kBins - 1, [&](uint64_t o, int b) {
+      if (o > lim || !is_candidate(st.cuts, b)) return;
+      const uint64_t w = cand.weight(o, s.min_t);
+      if (w) atomicAdd((unsigned long long*)&chunk_sum[(uint32_t)o / kChunk], (unsigned long long)w);
+    });
+    __syncthreads();
+  }
+  uint64_t total = 0;
+  for (int g = 0; g < p.chunks; ++g) total += chunk_sum[g];
+  uint64_t at = draw_at(s.u, total);
+  int g = 0;
+  for (; g + 1 < p.chunks && at >= chunk_sum[g]; ++g) at -= chunk_sum[g];
+  const int base = g * kChunk;
+  float x[E];
+  load_chunk<T, E>(row, base, (int)a.vocab, x);
+  uint64_t mine = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) mine += kept_weight<E>(s, x[e], index_of<E>(base, e), m, limit_x, limit_i);
+  mine = wave_sum_u64(mine);
+  if ((threadIdx.x & 63) == 0) sh.wave_sum[threadIdx.x >> 6] = mine;
+  __syncthreads();
+  int token;
+  double t;
+  if (locate<NT, E, LIST>(sh, s, x, base, m, limit_x, limit_i, at, &token, &t)) {
+    a.tokens[r] = token;
+    if (a.logprob) a.logprob[r] = (float)(t * 0.69314718055994530942 - log((double)total * 0x1p-42));
+  }
+}
+
+template <typename T, int NT, int E>
+void launch_row(const SampleArgs& a, hipStream_t st) {
+  hipLaunchKernelGGL((sample_row_kernel<T, NT, E>), dim3((uint32_t)a.rows), dim3(NT), 0, st, a);
+}
+
+size_t up(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
+
+template <typename T>
+bdh_status sample_typed(const SampleArgs& a, hipStream_t st, uint64_t* launches) {
+  if (a.vocab <= 32768) {
+    if (a.vocab <= 256) launch_row<T, 64, 4>(a, st);
+    else if (a.vocab <= 1024) launch_row<T, 256, 4>(a, st);
+    else if (a.vocab <= 4096) launch_row<T, 256, 16>(a, st);
+    else if (a.vocab <= 8192) launch_row<T, 512, 16>(a, st);
+    else if (a.vocab <= 16384) launch_row<T, 1024, 16>(a, st);
+    else launch_row<T, 1024, 32>(a, st);
+    BDH_HIP_TRY(hipGetLastError());
+    *launches += 1;
+    return BDH_OK;
+  }
+  // Groups of rows, so that the scratch stays small (64 MB at 1024 rows of 40000).
+  const int64_t group = a.rows < 1024 ? a.rows : 1024;
+  SplitArgs p;
+  p.a = a;
+  p.chunks = (int)((a.vocab + kChunk - 1) / kChunk);
+  const size_t slots = (size_t)group * (size_t)p.chunks;
+  const size_t sizes[] = {up(slots * 4), up(slots * 4), up(slots * kBins * 4), up(slots * kBins * 8),
+                          up(slots * 8), up((size_t)group * kListMax * 8), up((size_t)group * sizeof(RowState))};
+  size_t bytes = 0;
+  for (size_t s : sizes) bytes += s;
+  void* buf = nullptr;
+  const bdh_status s = scratch(st, SLOT_SAMPLE, bytes, &buf);
+  if (s != BDH_OK) return s;
+  char* at = (char*)buf;
+  p.max = (float*)at; at += sizes[0];
+  p.arg = (int32_t*)at; at += sizes[1];
+  p.cnt = (uint32_t*)at; at += sizes[2];
+  p.mass = (uint64_t*)at; at += sizes[3];
+  p.sure = (uint64_t*)at; at += sizes[4];
+  p.list = (uint64_t*)at; at += sizes[5];
+  p.state = (RowState*)at;
+  for (p.row0 = 0; p.row0 < a.rows; p.row0 += group) {
+    const uint32_t n = (uint32_t)(a.rows - p.row0 < group ? a.rows - p.row0 : group);
+    const dim3 grid((uint32_t)p.chunks, n);
+    hipLaunchKernelGGL((sample_chunk_kernel<T>), grid, dim3(kChunkThreads), 0, st, p);
+    hipLaunchKernelGGL(sample_merge_kernel, dim3(n), dim3(kBins), 0, st, p);
+    hipLaunchKernelGGL((sample_gather_kernel<T>), grid, dim3(kChunkThreads), 0, st, p);
+    hipLaunchKernelGGL((sample_finish_kernel<T>), dim3(n), dim3(kChunkThreads), 0, st, p);
+    BDH_HIP_TRY(hipGetLastError());
+    *launches += 4;
+  }
+  return BDH_OK;
+}
+
+}  // namespace
+
+bdh_status sample_tokens(const SampleArgs& a, hipStream_t st, uint64_t* launches) {
+  return a.bf16 ? sample_typed<bf16_t>(a, st, launches) : sample_typed<float>(a, st, launches);
+}
+
+}  // namespace bdh

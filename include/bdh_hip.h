@@ -299,6 +299,44 @@ bdh_status bdh_lm_logits(const float* hidden, int64_t rows, int64_t embd,
                          const void* lm_head_packed, int64_t vocab, float* logits,
                          void* stream);
 
+/* The next token of every row from its logits and a given random number:
+ * the sampling of the reference's generation loop (DragonModel::generate,
+ * dragon.rs:1749-1808) on the device, with its usual cuts.
+ * logits: `rows` rows of `vocab` (dtype BDH_F32 or BDH_BF16), row r at
+ * r * row_stride elements (0: all rows draw from the same logits);
+ * uniform [rows] f32 in [0, 1).
+ * Of a row, x = logits with NaN as -inf and +inf as the largest finite f32,
+ * m the largest; w_i = exp((x_i - m) / temperature), 0 below 2^-42.  In the
+ * order of x descending, ties by index ascending:
+ *   top_k  the first top_k are kept (0, or vocab and more: all);
+ *   top_p  of these, each before which w sums to less than top_p times
+ *          their sum (1: all; the first is always kept);
+ *   min_p  of these, each with w >= min_p (0: all).
+ * token = the first index (ascending) at which the running sum of kept w
+ * exceeds uniform times their sum; temperature 0: the first index of m.
+ * logprob_out (may be NULL): ln of its share of the kept w (0 at
+ * temperature 0).  A row without a finite or +inf logit gives -1 and -inf.
+ * Sums are exact integers (w in units of 2^-42), so a result depends on its
+ * row and settings alone.
+ * options NULL: temperature 1 and no cuts.  A *_rows pointer ([rows], device)
+ * takes the place of the scalar beside it; there, a temperature that is not
+ * above 0 counts as 0, other values outside a range as its nearest end, NaN
+ * as no cut, and a random number outside [0, 1) as the nearest inside.
+ * vocab up to 2^20; past 32768 the call uses the stream's scratch. */
+typedef struct {
+  float temperature, top_p, min_p;
+  int32_t top_k;
+  const float* temperature_rows;
+  const float* top_p_rows;
+  const float* min_p_rows;
+  const int32_t* top_k_rows;
+} bdh_sample_options;
+
+bdh_status bdh_sample_tokens(const void* logits, int32_t dtype, int64_t rows, int64_t vocab,
+                             int64_t row_stride, const float* uniform,
+                             const bdh_sample_options* options, int32_t* tokens_out,
+                             float* logprob_out, void* stream);
+
 /* Streaming-state record: the model position and each layer's carried rho
  * with its sequence-state flags, saved from / loaded into device memory.
  * Replaces, for the state this path carries, StreamingRuntimeStateRecord /

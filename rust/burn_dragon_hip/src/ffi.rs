@@ -75,6 +75,19 @@ pub struct bdh_layer_state_desc {
 }
 
 #[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct bdh_sample_options {
+    pub temperature: f32,
+    pub top_p: f32,
+    pub min_p: f32,
+    pub top_k: i32,
+    pub temperature_rows: *const f32,
+    pub top_p_rows: *const f32,
+    pub min_p_rows: *const f32,
+    pub top_k_rows: *const i32,
+}
+
+#[repr(C)]
 #[derive(Clone, Copy, Debug, Default)]
 pub struct bdh_profile_snapshot {
     pub calls: u64,
@@ -158,6 +171,10 @@ extern "C" {
     pub fn bdh_state_record_load(path: *const c_char, n_layers: i32,
                                  layers: *const bdh_layer_state_desc, rho: *const *mut f32,
                                  stream: *mut c_void) -> i32;
+    pub fn bdh_sample_tokens(logits: *const c_void, dtype: i32, rows: i64, vocab: i64,
+                             row_stride: i64, uniform: *const f32,
+                             options: *const bdh_sample_options, tokens_out: *mut i32,
+                             logprob_out: *mut f32, stream: *mut c_void) -> i32;
     pub fn bdh_state_copy_streams(n_layers: i32, layers: *const bdh_layer_state_desc,
                                   rho: *const *mut f32,
                                   src_layers: *const bdh_layer_state_desc,
