@@ -53,6 +53,11 @@ class BdhLayerStateDesc(ctypes.Structure):
                 ("retain_terminal_sequence_state", ctypes.c_int32)]
 
 
+class BdhAdapterPlan(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in
+                ("batch", "time", "in_dim", "out_dim", "rank", "adapters")]
+
+
 class BdhSampleOptions(ctypes.Structure):
     _fields_ = [("temperature", ctypes.c_float), ("top_p", ctypes.c_float),
                 ("min_p", ctypes.c_float), ("top_k", ctypes.c_int32),
@@ -103,6 +108,7 @@ SIGNATURES = {
                                      ctypes.POINTER(BdhLayerStateDesc), _i32]),
     "bdh_state_record_load": (_i32, [ctypes.c_char_p, _i32, ctypes.POINTER(BdhLayerStateDesc),
                                      ctypes.POINTER(_vp), _vp]),
+    "bdh_apply_adapters": (_i32, [ctypes.POINTER(BdhAdapterPlan), _i32] + [_vp] * 8),
     "bdh_sample_tokens": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp,
                                  ctypes.POINTER(BdhSampleOptions), _vp, _vp, _vp]),
     "bdh_state_copy_streams": (_i32, [_i32, ctypes.POINTER(BdhLayerStateDesc), ctypes.POINTER(_vp),

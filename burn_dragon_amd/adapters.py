@@ -1,0 +1,73 @@
+"""Low-rank adapters of many requests beside a shared projection
+(bdh_apply_adapters): the batch's sequences share the model's logits
+projection, and each adds its own adapter's product to it,
+
+    out[b] = base[b] + scale[id] * (hidden[b] A[id]^T) B[id]^T,   id = ids[b]
+
+with all adapters of a set in one call.  ``model_forward_logits`` applies a
+set to its logits (``adapters=``, ``adapter_ids=``).
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _lib
+from .recurrent import _dtype_code, _on_current_device, _ptr, _stream_ptr, supports_backend
+
+
+class AdapterSet(NamedTuple):
+    """n adapters of one rank (pad smaller ones with zeros)."""
+    a: torch.Tensor       # [n, R, D] bf16: into the rank (a linear layer's [out, in] weight)
+    b: torch.Tensor       # [n, V, R] bf16: out of it
+    scale: torch.Tensor   # [n] f32 (alpha / R)
+
+
+def apply_adapters(base: torch.Tensor, hidden: torch.Tensor, adapters: AdapterSet, ids: torch.Tensor,
+                   *, out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """base [B, T, V] and hidden [B, T, D] of one dtype (f32 or bf16), or [B,
+    V] and [B, D] for a token a sequence; ids [B] int32 on the device, each
+    sequence's adapter (outside [0, n): none).  Returns base plus the
+    adapters' products, in a new tensor or in ``out`` (contiguous; ``base``
+    itself for in place).  None where the library does not support the input
+    (no supported device, another dtype, an empty dimension, a rank above
+    128, a scratch that would have to grow under capture)."""
+    if not supports_backend():
+        return None
+    if base.dim() not in (2, 3) or hidden.dim() != base.dim() or not base.is_cuda:
+        return None
+    code = _dtype_code(base)
+    if code is None or hidden.dtype != base.dtype:
+        return None
+    B, T, V = base.shape if base.dim() == 3 else (base.shape[0], 1, base.shape[1])
+    D = hidden.shape[-1]
+    a, b, scale = adapters
+    if a.dim() != 3 or b.dim() != 3 or a.dtype != torch.bfloat16 or b.dtype != torch.bfloat16:
+        return None
+    n, R, _ = a.shape
+    if min(B, T, V, D, n, R) == 0:
+        return None
+    if (tuple(hidden.shape[:-1]) != tuple(base.shape[:-1]) or tuple(a.shape) != (n, R, D)
+            or tuple(b.shape) != (n, V, R) or tuple(scale.shape) != (n,) or tuple(ids.shape) != (B,)):
+        raise ValueError("base, hidden, adapters and ids do not fit together")
+    if scale.dtype != torch.float32 or ids.dtype != torch.int32:
+        raise ValueError("scale must be f32 and ids int32")
+    if any(t.device != base.device for t in (hidden, a, b, scale, ids)):
+        raise ValueError("base, hidden, adapters and ids must be on one device")
+    if out is not None and (tuple(out.shape) != tuple(base.shape) or out.dtype != base.dtype
+                            or out.device != base.device or not out.is_contiguous()):
+        raise ValueError("out must be a contiguous tensor like base")
+    base_c, hidden_c, a, b = base.contiguous(), hidden.contiguous(), a.contiguous(), b.contiguous()
+    scale, ids = scale.contiguous(), ids.contiguous()
+    if out is None:
+        out = torch.empty(base.shape, device=base.device, dtype=base.dtype)
+    plan = _lib.BdhAdapterPlan(B, T, D, V, R, n)
+    with _on_current_device(base.device):
+        st = _lib.load().bdh_apply_adapters(ctypes.byref(plan), code, _ptr(base_c), _ptr(hidden_c),
+                                            _ptr(a), _ptr(b), _ptr(scale), _ptr(ids), _ptr(out),
+                                            _stream_ptr(base.device))
+    if not _lib.check(st):
+        return None
+    return out

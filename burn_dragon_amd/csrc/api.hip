@@ -752,6 +752,58 @@ bdh_status bdh_lm_logits(const float* hidden, int64_t rows, int64_t embd,
   return BDH_OK;
 }
 
+bdh_status bdh_apply_adapters(const bdh_adapter_plan* plan, int32_t dtype, const void* base,
+                              const void* hidden, const void* a, const void* b, const float* scale,
+                              const int32_t* ids, void* out, void* stream) {
+  ProfScope prof;
+  if (!plan) return fail(BDH_EINVAL, "plan is null");
+  const bdh_adapter_plan p = *plan;
+  if (p.batch <= 0 || p.time <= 0 || p.in_dim <= 0 || p.out_dim <= 0 || p.rank <= 0 || p.adapters <= 0)
+    return fail(BDH_UNSUPPORTED, "zero-sized dimension");
+  if (!base || !hidden || !a || !b || !scale || !ids || !out) return fail(BDH_EINVAL, "null tensor pointer");
+  if (dtype != BDH_F32 && dtype != BDH_BF16) return fail(BDH_EINVAL, "unknown dtype");
+  if (p.rank > kMaxAdapterRank) return fail(BDH_UNSUPPORTED, "rank must be at most 128");
+  if (p.batch > kMaxGrid) return fail(BDH_UNSUPPORTED, "batch exceeds 65535");
+  if (p.in_dim > (int64_t)1 << 20 || p.out_dim > (int64_t)1 << 22 || p.adapters > (int64_t)1 << 20 ||
+      p.time > (int64_t)1 << 22 || p.batch * p.time > (int64_t)1 << 23)
+    return fail(BDH_UNSUPPORTED, "too large for one launch");
+  const int64_t size = dtype == BDH_F32 ? 4 : 2;
+  for (const void* t : {base, hidden, (const void*)out})
+    if (((uintptr_t)t & (size - 1)) != 0) return fail(BDH_EINVAL, "tensor pointers must be aligned to their elements");
+  for (const void* t : {a, b})
+    if (((uintptr_t)t & 1) != 0) return fail(BDH_EINVAL, "tensor pointers must be aligned to their elements");
+  for (const void* t : {(const void*)scale, (const void*)ids})
+    if (((uintptr_t)t & 3) != 0) return fail(BDH_EINVAL, "tensor pointers must be aligned to their elements");
+  // out shares no memory with an input, but for base itself.
+  const int64_t rows = p.batch * p.time, out_bytes = rows * p.out_dim * size;
+  const struct { const void* at; int64_t bytes; } in[] = {
+      {out == base ? nullptr : base, out_bytes}, {hidden, rows * p.in_dim * size},
+      {a, p.adapters * p.rank * p.in_dim * 2},   {b, p.adapters * p.out_dim * p.rank * 2},
+      {scale, p.adapters * 4},                   {ids, p.batch * 4}};
+  for (const auto& i : in)
+    if (i.at && (uintptr_t)out < (uintptr_t)i.at + (uintptr_t)i.bytes &&
+        (uintptr_t)i.at < (uintptr_t)out + (uintptr_t)out_bytes)
+      return fail(BDH_EINVAL, "out shares memory with an input");
+  AdapterArgs g{};
+  g.batch = p.batch;
+  g.time = p.time;
+  g.in_dim = p.in_dim;
+  g.out_dim = p.out_dim;
+  g.rank = p.rank;
+  g.n = p.adapters;
+  g.bf16 = dtype == BDH_BF16;
+  g.base = base;
+  g.hidden = hidden;
+  g.a = (const bf16_t*)a;
+  g.b = (const bf16_t*)b;
+  g.scale = scale;
+  g.ids = ids;
+  g.out = out;
+  const bdh_status st = apply_adapters(g, (hipStream_t)stream, &prof.launches);
+  if (st == BDH_OK) prof.done(true);
+  return st;
+}
+
 bdh_status bdh_sample_tokens(const void* logits, int32_t dtype, int64_t rows, int64_t vocab,
                              int64_t row_stride, const float* uniform,
                              const bdh_sample_options* options, int32_t* tokens_out,

@@ -49,6 +49,7 @@ enum ScratchSlot {
   SLOT_VJP_GAMMA,    // VJP state gradients          2 x [S, N, D] f32
   SLOT_SNAP,         // states at interval starts: bf16 path [n_iv, S, D, N] bf16, fp32 path [n_iv - 1, S, N, D] f32
   SLOT_SAMPLE,       // sampling of long rows: chunks' histograms, candidates (sample.hip)
+  SLOT_ADAPTER,      // adapters: hidden A^T  [rows, padded rank] f32, or as bf16 parts
   SLOT_COUNT
 };
 // Scratch of the calling stream (see api.hip): grows on first use of a
@@ -162,6 +163,25 @@ bdh_status embed_norm(const int32_t* tokens, int64_t n, const float* embed, int6
 bdh_status pack_lm_head(int64_t D, int64_t V, const float* head, bf16_t* packed, hipStream_t st);
 bdh_status lm_logits(const float* hidden, int64_t M, int64_t D, const bf16_t* head, int64_t V,
                      float* logits, hipStream_t st, uint64_t* launches);
+
+// --- adapters (adapters.hip) -----------------------------------------------------
+constexpr int64_t kMaxAdapterRank = 128;
+struct AdapterArgs {
+  int64_t batch, time, in_dim, out_dim, rank, n;
+  bool bf16;            // hidden, base and out (else f32)
+  const void* base;     // [batch, time, out_dim]
+  const void* hidden;   // [batch, time, in_dim]
+  const bf16_t* a;      // [n, rank, in_dim]
+  const bf16_t* b;      // [n, out_dim, rank]
+  const float* scale;   // [n]
+  const int32_t* ids;   // [batch]
+  void* out;            // [batch, time, out_dim], may be base
+  // Scratch, set by apply_adapters.
+  float* u;
+  bf16_t* u_parts;
+  int rp;
+};
+bdh_status apply_adapters(const AdapterArgs& a, hipStream_t st, uint64_t* launches);
 
 // --- streams' states (streams.hip) -------------------------------------------
 // Layer l's slot dst[i] takes the value of slot src[i] (of src_rho[l], slots

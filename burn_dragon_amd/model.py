@@ -27,6 +27,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
+from .adapters import AdapterSet, apply_adapters
 from .layer import LowRankWeights, lowrank_layer_forward
 from .recurrent import DEFAULT_ROPE_THETA, _ptr, _stream_ptr, supports_backend
 
@@ -82,14 +83,21 @@ def new_model_state(weights: BdhModelWeights, batch: int, device: torch.device,
 def model_forward_logits(tokens: torch.Tensor, weights: BdhModelWeights, *,
                          position: Optional[int] = 0, theta: float = DEFAULT_ROPE_THETA,
                          state: Optional[BdhModelState] = None, relu_threshold: float = 0.0,
-                         latent_mask: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+                         latent_mask: Optional[torch.Tensor] = None,
+                         adapters: Optional[AdapterSet] = None,
+                         adapter_ids: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
     """tokens [B, T] int32 on the device -> logits [B, T, vocab] f32.
     Without ``state`` every layer starts from rho = 0 at ``position``; with
     it the forward continues the state's sequence (its position wins) and
     updates the state in place.  ``relu_threshold`` and ``latent_mask`` are
-    every layer's projection options (lowrank_layer_forward)."""
+    every layer's projection options (lowrank_layer_forward).  With
+    ``adapters`` (of D into vocab) each sequence's logits gain its own
+    adapter's product, ``adapter_ids`` [B] int32 on the device
+    (apply_adapters)."""
     if not supports_backend() or weights is None:
         return None
+    if (adapters is None) != (adapter_ids is None):
+        raise ValueError("adapters and adapter_ids come together")
     if state is not None:
         if len(state.rho) != weights.n_layer:
             return None
@@ -120,6 +128,8 @@ def model_forward_logits(tokens: torch.Tensor, weights: BdhModelWeights, *,
     st = lib.bdh_lm_logits(_ptr(cur), B * T, D, _ptr(weights.lm_head), weights.vocab,
                            _ptr(logits), stream)
     if not _lib.check(st):
+        return None
+    if adapters is not None and apply_adapters(logits, cur, adapters, adapter_ids, out=logits) is None:
         return None
     if state is not None:
         state.position += T

@@ -299,6 +299,27 @@ bdh_status bdh_lm_logits(const float* hidden, int64_t rows, int64_t embd,
                          const void* lm_head_packed, int64_t vocab, float* logits,
                          void* stream);
 
+/* Low-rank adapters of many requests beside a shared projection, such as the
+ * logits of bdh_lm_logits:
+ *   out[b, t] = base[b, t] + scale[id] * (hidden[b, t] A[id]^T) B[id]^T,  id = ids[b]
+ * base, out [batch, time, out_dim] and hidden [batch, time, in_dim] of one
+ * dtype (BDH_F32 or BDH_BF16); a [adapters, rank, in_dim] and b [adapters,
+ * out_dim, rank] bf16 (a linear layer's [out, in] weights); scale [adapters]
+ * f32; ids [batch] int32 on the device, one adapter a sequence: an id outside
+ * [0, adapters) leaves out = base.  out may be base (in place), and otherwise
+ * shares no memory with the inputs.  Products and sums are f32, with BDH_F32 to
+ * f32's own precision (on the matrix cores in three bf16 parts), and out is
+ * rounded once.  rank up to 128.  Pointers aligned to their elements.  Uses the
+ * stream's scratch.  No counterpart in the reference, which adapts a model by
+ * training it. */
+typedef struct {
+  int64_t batch, time, in_dim, out_dim, rank, adapters;
+} bdh_adapter_plan;
+
+bdh_status bdh_apply_adapters(const bdh_adapter_plan* plan, int32_t dtype, const void* base,
+                              const void* hidden, const void* a, const void* b, const float* scale,
+                              const int32_t* ids, void* out, void* stream);
+
 /* The next token of every row from its logits and a given random number:
  * the sampling of the reference's generation loop (DragonModel::generate,
  * dragon.rs:1749-1808) on the device, with its usual cuts.

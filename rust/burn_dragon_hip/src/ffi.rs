@@ -75,6 +75,17 @@ pub struct bdh_layer_state_desc {
 }
 
 #[repr(C)]
+#[derive(Clone, Copy, Debug, Default)]
+pub struct bdh_adapter_plan {
+    pub batch: i64,
+    pub time: i64,
+    pub in_dim: i64,
+    pub out_dim: i64,
+    pub rank: i64,
+    pub adapters: i64,
+}
+
+#[repr(C)]
 #[derive(Clone, Copy, Debug)]
 pub struct bdh_sample_options {
     pub temperature: f32,
@@ -171,6 +182,10 @@ extern "C" {
     pub fn bdh_state_record_load(path: *const c_char, n_layers: i32,
                                  layers: *const bdh_layer_state_desc, rho: *const *mut f32,
                                  stream: *mut c_void) -> i32;
+    pub fn bdh_apply_adapters(plan: *const bdh_adapter_plan, dtype: i32, base: *const c_void,
+                              hidden: *const c_void, a: *const c_void, b: *const c_void,
+                              scale: *const f32, ids: *const i32, out: *mut c_void,
+                              stream: *mut c_void) -> i32;
     pub fn bdh_sample_tokens(logits: *const c_void, dtype: i32, rows: i64, vocab: i64,
                              row_stride: i64, uniform: *const f32,
                              options: *const bdh_sample_options, tokens_out: *mut i32,
