@@ -27,3 +27,4 @@ from .model import (BdhModelState, BdhModelWeights, load_model_state, model_forw
 from .streams import compact_streams, copy_streams, free_streams  # noqa: F401
 from .sampling import SampleOutput, sample_tokens  # noqa: F401
 from .adapters import AdapterSet, apply_adapters  # noqa: F401
+from .generation import GenerateOutput, generate_tokens  # noqa: F401
