@@ -25,7 +25,7 @@
 //   3. The kept weights are summed by wave, and the draw descends into the
 //      wave, the stripe, the lane and the element that it falls in.
 //
-// Rows up to 32768 logits: one workgroup, the row in registers, read once.
+// Rows up to 16384 logits: one workgroup, the row in registers, read once.
 // Longer ones in chunks of 8192, four launches (sample_chunk_kernel on).
 #include "bdh_internal.h"
 
@@ -33,7 +33,7 @@ namespace bdh {
 namespace {
 
 constexpr int kBins = 512;
-constexpr int kBinsPerOctave = 12;
+constexpr int kBinsPerOctave = 10;  // 420 of the bins: see bin_of
 constexpr double kLeastT = -42.0;
 constexpr int kSmall = 64;       // candidates that one wave orders
 constexpr int kListMax = 4096;   // candidates that the list holds
@@ -45,7 +45,7 @@ constexpr int kNoLimitIndex = 0x7fffffff;
 
 struct Row {
   double c;      // log2(e) / temperature
-  double cb;     // bins per unit of x
+  float cb;      // bins per unit of x
   double min_t;  // least t that is kept
   double p;
   int k;
@@ -61,7 +61,7 @@ __device__ Row row_settings(const SampleArgs& a, int64_t r) {
   s.k = a.top_k_rows ? a.top_k_rows[r] : a.top_k;
   s.greedy = !(tau > 0.0f) || s.k == 1;
   s.c = 1.4426950408889634074 / (double)tau;
-  s.cb = s.c * kBinsPerOctave;
+  s.cb = (float)fmin(s.c * kBinsPerOctave, 1e30);
   s.use_k = s.k > 0 && s.k < a.vocab;
   s.use_p = p < 1.0f;
   s.p = p > 0.0f ? (double)p : 0.0;
@@ -114,11 +114,18 @@ __device__ __forceinline__ float value_of(uint64_t o) {
   return __uint_as_float((up >> 31) ? up ^ 0x80000000u : ~up);
 }
 
-// The bin of a logit in a grid that all chunks of a row share, counted from
-// the bin `top` of the largest; kBins where it is further down (weight 0).
-__device__ __forceinline__ int bin_of(float x, double top, double cb) {
-  const double d = top - floor((double)x * cb);
-  return d < (double)kBins ? (int)d : kBins;  // (-inf: +inf; NaN does not occur but at cb = 0)
+// A grid that all chunks of a row share, of 1/10 octave of weight, and the bin
+// of a logit in it, counted down from the bin of the largest; kBins further
+// down (weight 0).  Every step is monotone in x, so the bins are ranges of the
+// order whatever is rounded.  A weight of 2^-42 lies in bin 420, so f32 leaves
+// room to be off by 92 bins together: |x| / temperature up to 2^26; past that
+// weights from about 2^-38 down may fall out too.
+__device__ __forceinline__ float grid_of(float x, float cb) {
+  return __builtin_amdgcn_fmed3f(floorf(x * cb), -3e38f, 3e38f);
+}
+__device__ __forceinline__ int bin_of(float x, float top, float cb) {
+  const float d = top - grid_of(x, cb);
+  return d < (float)kBins ? (int)d : kBins;
 }
 __device__ __forceinline__ bool is_real(float x) { return x > -INFINITY; }
 
@@ -176,10 +183,60 @@ struct Shared {
   uint64_t above;
 };
 
+// Neighbours' values by DPP: `none` where there is none.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp32(uint32_t v, uint32_t none) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp64(uint64_t v) {
+  return (uint64_t)dpp32<CTRL, ROWS>((uint32_t)(v >> 32), 0) << 32 | dpp32<CTRL, ROWS>((uint32_t)v, 0);
+}
+__device__ __forceinline__ uint64_t lane_u64(uint64_t v, int lane) {  // lane: uniform
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
+__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v) {  // inclusive
+  v += dpp64<0x111, 0xf>(v);  // the lane before, of a row of 16
+  v += dpp64<0x112, 0xf>(v);
+  v += dpp64<0x114, 0xf>(v);
+  v += dpp64<0x118, 0xf>(v);
+  v += dpp64<0x142, 0xa>(v);  // row 0's last to row 1, 2's to 3
+  v += dpp64<0x143, 0xc>(v);  // row 1's last to rows 2 and 3
+  return v;
+}
+__device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) { return lane_u64(wave_scan_u64(v), 63); }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t max_dpp(uint64_t v) {
+  const uint64_t w = dpp64<CTRL, ROWS>(v);
+  return w > v ? w : v;
+}
+__device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
+  v = max_dpp<0x111, 0xf>(v);
+  v = max_dpp<0x112, 0xf>(v);
+  v = max_dpp<0x114, 0xf>(v);
+  v = max_dpp<0x118, 0xf>(v);
+  v = max_dpp<0x142, 0xa>(v);
+  v = max_dpp<0x143, 0xc>(v);
+  return lane_u64(v, 63);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float max_dpp(float v) {
+  return fmaxf(v, __uint_as_float(dpp32<CTRL, ROWS>(__float_as_uint(v), 0xff800000u)));
+}
+__device__ __forceinline__ float wave_max_f32(float v) {
+  v = max_dpp<0x111, 0xf>(v);
+  v = max_dpp<0x112, 0xf>(v);
+  v = max_dpp<0x114, 0xf>(v);
+  v = max_dpp<0x118, 0xf>(v);
+  v = max_dpp<0x142, 0xa>(v);
+  v = max_dpp<0x143, 0xc>(v);
+  return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), 63));
+}
+
 template <int NT>
 __device__ __forceinline__ float block_max(float v, float* part) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  v = wave_max_f32(v);
   if (NT == 64) return v;
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -189,63 +246,65 @@ __device__ __forceinline__ float block_max(float v, float* part) {
   return v;
 }
 
-__device__ __forceinline__ uint64_t shfl_u64(uint64_t v, int lane) {
-  return (uint64_t)__shfl((unsigned long long)v, lane, 64);
-}
-__device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += (uint64_t)__shfl_xor((unsigned long long)v, o, 64);
-  return v;
-}
-__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v) {  // inclusive
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint64_t w = (uint64_t)__shfl_up((unsigned long long)v, o, 64);
-    if (lane >= o) v += w;
-  }
-  return v;
+// Appends to a list: one atomic a wave.
+__device__ __forceinline__ int append_at(int* n, bool mine) {
+  const uint64_t all = __ballot(mine);
+  if (all == 0) return -1;
+  int first = 0;
+  if ((threadIdx.x & 63) == (uint32_t)__builtin_ctzll(all)) first = atomicAdd(n, __popcll(all));
+  first = __builtin_amdgcn_readlane(first, __builtin_ctzll(all));
+  return mine ? first + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0)) : -1;
 }
 
-// One wave: the first of the kBins bins at which the running sum reaches
-// `need` (-1: it does not), and the sums before and after it, or of all.
-template <typename H>
-__device__ void cross_bins(const H* h, uint64_t need, int* bin, uint64_t* before, uint64_t* upto) {
-  const int lane = threadIdx.x & 63;
-  uint64_t v[kBins / 64], s = 0;
+// A histogram in one wave's registers: eight bins a lane, and the sum of what
+// lies before them.
+struct BinScan {
+  uint64_t v[kBins / 64], before, total;
+
+  template <typename H>
+  __device__ BinScan(const H* h, int last) {  // bins past `last` count as empty
+    const int first = (threadIdx.x & 63) * (kBins / 64);
+    uint64_t s = 0;
 #pragma unroll
-  for (int j = 0; j < kBins / 64; ++j) {
-    v[j] = h[lane * (kBins / 64) + j];
-    s += v[j];
-  }
-  const uint64_t incl = wave_scan_u64(s);
-  uint64_t run = incl - s, b = 0, up = 0;
-  int at = -1;
-#pragma unroll
-  for (int j = 0; j < kBins / 64; ++j) {
-    if (at < 0 && run + v[j] >= need) {
-      at = lane * (kBins / 64) + j;
-      b = run;
-      up = run + v[j];
+    for (int j = 0; j < kBins / 64; ++j) {
+      v[j] = first + j <= last ? h[first + j] : 0;
+      s += v[j];
     }
-    run += v[j];
+    before = wave_scan_u64(s) - s;
+    total = lane_u64(before + s, 63);
   }
-  const uint64_t found = __ballot(at >= 0);
-  if (found == 0) {
-    *bin = -1;
-    *before = *upto = shfl_u64(incl, 63);
-    return;
+  // The first bin at which the running sum reaches `need` (kBins: none), and
+  // the sum before it and in it.
+  __device__ int cross(uint64_t need, uint64_t* sum_before, uint64_t* in) const {
+    uint64_t run = before, b = 0, w = 0;
+    int at = -1;
+#pragma unroll
+    for (int j = 0; j < kBins / 64; ++j) {
+      if (at < 0 && run + v[j] >= need) {
+        at = j;
+        b = run;
+        w = v[j];
+      }
+      run += v[j];
+    }
+    const uint64_t found = __ballot(at >= 0);
+    if (found == 0) {
+      *sum_before = total;
+      *in = 0;
+      return kBins;
+    }
+    const int lane = __builtin_ctzll(found);
+    *sum_before = lane_u64(b, lane);
+    *in = lane_u64(w, lane);
+    return lane * (kBins / 64) + __builtin_amdgcn_readlane(at, lane);
   }
-  const int first = __builtin_ctzll(found);
-  *bin = __shfl(at, first, 64);
-  *before = shfl_u64(b, first);
-  *upto = shfl_u64(up, first);
-}
+};
 
 // What the histogram says about the cuts of a row.
 struct Cuts {
   int k_bin;            // holds the k-th in order; kBins: top-k cuts nothing that is drawn
   int p_first, p_last;  // bins that the top-p cut can fall in; kBins: no top-p
+  int m_first, m_last;  // (long rows) bins that the least kept t can fall in; kBins: none
   uint64_t k_above;     // logits in bins before k_bin
   uint64_t k_mass;      // their weight (all weight: no k_bin)
   uint64_t p_above;     // weight in bins before p_first
@@ -254,40 +313,42 @@ __device__ __forceinline__ uint64_t p_need(const Row& s, uint64_t total) {
   const uint64_t need = (uint64_t)ceil(s.p * (double)total);
   return need > 0 ? need : 1;  // the first in order is always kept
 }
-// One wave.
-__device__ Cuts find_cuts(const Row& s, const uint32_t* cnt, const uint64_t* mass) {
+__device__ __forceinline__ Cuts no_cuts() {
   Cuts q;
-  q.k_bin = q.p_first = q.p_last = kBins;
+  q.k_bin = q.p_first = q.p_last = q.m_first = q.m_last = kBins;
   q.k_above = q.k_mass = q.p_above = 0;
-  uint64_t upto = 0;
-  if (s.use_k) {
-    cross_bins(cnt, (uint64_t)s.k, &q.k_bin, &q.k_above, &upto);
-    if (q.k_bin < 0) q.k_bin = kBins;
-  }
-  if (s.use_p) {
-    // The weight before k_bin, and with it: between them lies what top-k keeps.
-    const int lane = threadIdx.x & 63;
-    uint64_t before = 0, at = 0;
-#pragma unroll
-    for (int j = 0; j < kBins / 64; ++j) {
-      const int b = lane * (kBins / 64) + j;
-      if (b < q.k_bin) before += mass[b];
-      if (b == q.k_bin) at = mass[b];
-    }
-    q.k_mass = wave_sum_u64(before);
-    const uint64_t most = q.k_mass + wave_sum_u64(at);
-    uint64_t unused;
-    cross_bins(mass, p_need(s, q.k_mass), &q.p_first, &q.p_above, &upto);
-    cross_bins(mass, p_need(s, most), &q.p_last, &unused, &upto);
-    // (Past k_bin the histogram may hold weights too; none is kept.)
-    if (q.p_first < 0 || q.p_first > q.k_bin) q.p_first = q.k_bin;
-    if (q.p_last < 0 || q.p_last > q.k_bin) q.p_last = q.k_bin;
-  }
   return q;
 }
-__device__ __forceinline__ int sure_bins(const Cuts& q) { return min(q.k_bin, q.p_first); }
+// One wave each.
+__device__ __forceinline__ void find_k(const Row& s, const uint32_t* cnt, Cuts& q) {
+  uint64_t in;
+  q.k_bin = BinScan(cnt, kBins).cross((uint64_t)s.k, &q.k_above, &in);
+}
+__device__ __forceinline__ void find_p(const Row& s, const uint64_t* mass, Cuts& q) {
+  // What top-k keeps weighs between all before k_bin, and that with k_bin.
+  const BinScan h(mass, q.k_bin);
+  uint64_t in = q.k_bin < kBins ? mass[q.k_bin] : 0;
+  q.k_mass = h.total - in;
+  q.p_first = min(h.cross(p_need(s, q.k_mass), &q.p_above, &in), q.k_bin);
+  uint64_t unused;
+  q.p_last = min(h.cross(p_need(s, h.total), &unused, &in), q.k_bin);
+}
+// (Wider than its one bin by what f32 may be off here and in bin_of.)
+__device__ __forceinline__ void find_least(const Row& s, float m, float top, Cuts& q) {
+  const float least = (float)((double)m + s.min_t / s.c);
+  if (!is_real(least)) return;  // (an infinite temperature)
+  const float bin = top - grid_of(least, s.cb);
+  const float off = 2.0f + (fabsf(m) + fabsf(least)) * s.cb * 0x1p-22f;
+  if (!(bin - off < (float)kBins)) return;
+  q.m_first = (int)fmaxf(bin - off, 0.0f);
+  q.m_last = (int)fminf(bin + off, (float)(kBins - 1));
+}
+// Bins before this are kept whole.
+__device__ __forceinline__ int sure_bins(const Cuts& q) { return min(min(q.k_bin, q.p_first), q.m_first); }
+// Bins that a cut may divide (past k_bin nothing is kept).
 __device__ __forceinline__ bool is_candidate(const Cuts& q, int bin) {
-  return bin < kBins && (bin == q.k_bin || (bin >= q.p_first && bin <= q.p_last && bin <= q.k_bin));
+  return bin < kBins && bin <= q.k_bin &&
+         (bin == q.k_bin || (bin >= q.p_first && bin <= q.p_last) || (bin >= q.m_first && bin <= q.m_last));
 }
 
 // The candidates: in the list, or where it overflowed all of the row's logits.
@@ -297,7 +358,7 @@ struct Candidates {
   const T* row;
   int vocab;
   float m;
-  double top;
+  float top;
   const Row& s;
   int n;  // found; beyond LIST the list is not complete
 
@@ -338,13 +399,22 @@ struct Candidates {
         sh.n_small = 0;
       }
       __syncthreads();
+      uint64_t low = ~0ull, high_o = 0;
       each(first, last, [&](uint64_t o, int) {
-        if (o < lo || o > hi) return;
-        const int at = atomicAdd(&sh.n_small, 1);
-        if (at < kSmall) sh.small[at] = o;
-        atomicMin((unsigned long long*)&sh.lo, (unsigned long long)o);
-        atomicMax((unsigned long long*)&sh.hi, (unsigned long long)o);
+        const bool in = o >= lo && o <= hi;
+        const int at = append_at(&sh.n_small, in);
+        if (at >= 0 && at < kSmall) sh.small[at] = o;
+        if (in) {
+          low = o < low ? o : low;
+          high_o = o > high_o ? o : high_o;
+        }
       });
+      low = ~wave_max_u64(~low);
+      high_o = wave_max_u64(high_o);
+      if ((threadIdx.x & 63) == 0 && high_o) {
+        atomicMin((unsigned long long*)&sh.lo, (unsigned long long)low);
+        atomicMax((unsigned long long*)&sh.hi, (unsigned long long)high_o);
+      }
       __syncthreads();
       const int n_in = sh.n_small;
       if (n_in <= kSmall) {
@@ -357,12 +427,7 @@ struct Candidates {
           for (int j = 0; j < n_in; ++j)
             if (sh.small[j] < mine) before += sh.small_w[j];
           const bool kept = lane < n_in && before < need;
-          uint64_t best = kept ? mine : 0;
-#pragma unroll
-          for (int o = 32; o > 0; o >>= 1) {
-            const uint64_t b = (uint64_t)__shfl_xor((unsigned long long)best, o, 64);
-            best = b > best ? b : best;
-          }
+          const uint64_t best = wave_max_u64(kept ? mine : 0);
           if (lane == 0) sh.sum = best;
         }
         __syncthreads();
@@ -380,13 +445,13 @@ struct Candidates {
       });
       __syncthreads();
       if (threadIdx.x < 64) {
-        int bin;
-        uint64_t before, upto;
-        cross_bins(sh.mass, need > above ? need - above : 1, &bin, &before, &upto);
+        uint64_t before, in;
+        const int bin = BinScan(sh.mass, kBins).cross(need > above ? need - above : 1, &before, &in);
         if (threadIdx.x == 0) {
-          // (Weights scaled from chunks may leave the sum a unit short: the last candidate.)
-          sh.bin = bin < 0 ? (int)((to >> shift) - (from >> shift)) : bin;
-          sh.above = bin < 0 ? above : above + before;
+          // (Weights scaled from chunks may leave the sum a few units short: the
+          // last candidates, of which the end keeps all.)
+          sh.bin = bin < kBins ? bin : (int)((to >> shift) - (from >> shift));
+          sh.above = bin < kBins ? above + before : above;
         }
       }
       __syncthreads();
@@ -396,8 +461,33 @@ struct Candidates {
     }
   }
 
+  // The same for up to kSmall candidates, in every wave and without a barrier:
+  // a lane compares its own with each other.  (One candidate at least is kept.)
+  __device__ uint64_t limit_small(const Cuts& q) {
+    const int lane = threadIdx.x & 63;
+    const uint64_t mine = lane < n ? sh.list[lane] : ~0ull;
+    const int bin = lane < n ? bin_of(value_of(mine), top, s.cb) : kBins;
+    const uint64_t w = s.use_p && lane < n ? weight(mine, kLeastT) : 0;
+    const bool in_k = lane < n && bin == q.k_bin, in_p = bin >= q.p_first && bin <= q.p_last;
+    const uint64_t wp = in_p ? w : 0;
+    uint64_t k_before = q.k_above, p_before = q.p_above;
+    for (int j = 0; j < n; ++j) {
+      const bool earlier = lane_u64(mine, j) < mine;
+      k_before += earlier && __builtin_amdgcn_readlane((int)in_k, j);
+      p_before += earlier ? lane_u64(wp, j) : 0;
+    }
+    bool kept = lane < n && (bin < q.k_bin || k_before < (uint64_t)s.k);
+    if (s.use_p) {
+      const uint64_t total = q.k_mass + (q.k_bin < kBins ? wave_sum_u64(in_k && kept ? w : 0) : 0);
+      kept = kept && (bin < q.p_first || (in_p && p_before < p_need(s, total)));
+    }
+    return wave_max_u64(kept ? mine : 0);
+  }
+
   // The last logit in order that top-k and top-p keep.
   __device__ uint64_t limit(const Cuts& q) {
+    if (q.k_bin == kBins && !s.use_p) return ~0ull;  // neither divides anything
+    if (n <= kSmall) return limit_small(q);
     uint64_t lim = ~0ull, total = q.k_mass;
     if (q.k_bin < kBins) {
       lim = cut<false>(q.k_bin, q.k_bin, q.k_above, (uint64_t)s.k);
@@ -461,7 +551,7 @@ __device__ bool locate(Shared<NT, LIST>& sh, const Row& s, const float (&x)[E], 
       mine += w[j];
     }
     const uint64_t incl = wave_scan_u64(mine);
-    const uint64_t stripe = shfl_u64(incl, 63);
+    const uint64_t stripe = lane_u64(incl, 63);
     if (at >= stripe) {
       at -= stripe;
       continue;
@@ -521,16 +611,14 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a) {
   float limit_x = -INFINITY;
   int limit_i = -1;  // (-inf itself is not kept)
   if (s.use_k || s.use_p) {
-    const double top = floor((double)m * s.cb);
+    const float top = grid_of(m, s.cb);
     for (int b = threadIdx.x; b < kBins; b += NT) {
       sh.cnt[b] = 0;
       sh.mass[b] = 0;
     }
-    if (threadIdx.x == 0) {
-      sh.n_list = 0;
-      sh.bin = kBins;
-    }
+    if (threadIdx.x == 0) sh.n_list = 0;
     __syncthreads();
+    Cuts q = no_cuts();
     if (s.use_k) {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
@@ -538,36 +626,27 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a) {
         if (b < kBins) atomicAdd(&sh.cnt[b], 1u);
       }
       __syncthreads();
-      if (threadIdx.x < 64) {
-        int bin;
-        uint64_t before, upto;
-        cross_bins(sh.cnt, (uint64_t)s.k, &bin, &before, &upto);
-        if (threadIdx.x == 0 && bin >= 0) sh.bin = bin;
-      }
-      __syncthreads();
+      find_k(s, sh.cnt, q);  // (every wave, the same)
+      forget<E>(x);
     }
-    forget<E>(x);
     if (s.use_p) {
-      const int last = sh.bin;  // no weight past the k-th counts
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const int b = is_real(x[e]) ? bin_of(x[e], top, s.cb) : kBins;
-        if (b < kBins && b <= last)
+        if (b < kBins && b <= q.k_bin)  // no weight past the k-th counts
           atomicAdd((unsigned long long*)&sh.mass[b],
                     (unsigned long long)weight_from(((double)x[e] - (double)m) * s.c, kLeastT));
-        __builtin_amdgcn_sched_barrier(0);
+        if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
       }
       __syncthreads();
+      find_p(s, sh.mass, q);
+      forget<E>(x);
     }
-    const Cuts q = find_cuts(s, sh.cnt, sh.mass);  // (every wave, the same)
-    forget<E>(x);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int b = is_real(x[e]) ? bin_of(x[e], top, s.cb) : kBins;
-      if (is_candidate(q, b)) {
-        const int at = atomicAdd(&sh.n_list, 1);
-        if (at < LIST) sh.list[at] = order_of(x[e], index_of<E>(0, e));
-      }
+      const int at = append_at(&sh.n_list, is_candidate(q, b));
+      if (at >= 0 && at < LIST) sh.list[at] = order_of(x[e], index_of<E>(0, e));
     }
     __syncthreads();
     Candidates<T, NT, LIST> cand{sh, row, vocab, m, top, s, sh.n_list};
@@ -582,7 +661,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a) {
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     mine += kept_weight<E>(s, x[e], index_of<E>(0, e), m, limit_x, limit_i);
-    __builtin_amdgcn_sched_barrier(0);
+    if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
   }
   mine = wave_sum_u64(mine);
   if ((threadIdx.x & 63) == 0) sh.wave_sum[threadIdx.x >> 6] = mine;
@@ -602,7 +681,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a) {
 // What a row's launches leave for one another.
 struct RowState {
   Cuts cuts;
-  double top;
+  float top;
   float m;
   int n_list;
 };
@@ -612,9 +691,10 @@ struct SplitArgs {
   int chunks;
   float* max;        // [rows, chunks]
   int32_t* arg;      // [rows, chunks]: the first index of the chunk's largest
-  uint32_t* cnt;     // [rows, chunks, kBins], by the chunk's own top bin
-  uint64_t* mass;    // [rows, chunks, kBins], weights below the chunk's own largest
-  uint64_t* sure;    // [rows, chunks]: weight that is kept whatever the cuts' candidates
+  uint32_t* cnt;     // [rows, chunks, kBins], bins counted from the chunk's own largest
+  uint64_t* mass;    // [rows, chunks, kBins], weights relative to it
+  uint64_t* sure;    // [rows, chunks]
+  int32_t* some;     // [rows, chunks]
   uint64_t* list;    // [rows, kListMax]
   RowState* state;   // [rows]
 };
@@ -626,7 +706,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_chunk_kernel(const Split
   __shared__ uint64_t mass[kBins];
   __shared__ uint32_t cnt[kBins];
   __shared__ float part[NT / 64];
-  __shared__ int k_bin, arg;
+  __shared__ int arg;
   const int64_t lr = blockIdx.y, r = p.row0 + lr;
   const int64_t slot = lr * p.chunks + blockIdx.x;
   const T* row = (const T*)p.a.logits + r * p.a.row_stride;
@@ -638,10 +718,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_chunk_kernel(const Split
     cnt[b] = 0;
     mass[b] = 0;
   }
-  if (threadIdx.x == 0) {
-    k_bin = kBins;
-    arg = kNoLimitIndex;
-  }
+  if (threadIdx.x == 0) arg = kNoLimitIndex;
   float best = x[0];
 #pragma unroll
   for (int e = 1; e < E; ++e) best = fmaxf(best, x[e]);
@@ -656,7 +733,8 @@ __global__ __launch_bounds__(kChunkThreads) void sample_chunk_kernel(const Split
     if (threadIdx.x == 0) p.arg[slot] = arg;
     return;
   }
-  const double top = floor((double)m * s.cb);
+  const float top = grid_of(m, s.cb);
+  Cuts q = no_cuts();
   if (s.use_k) {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -665,103 +743,128 @@ __global__ __launch_bounds__(kChunkThreads) void sample_chunk_kernel(const Split
     }
     __syncthreads();
     // Past the chunk's own k-th no logit is among the row's first k.
-    if (threadIdx.x < 64) {
-      int bin;
-      uint64_t before, upto;
-      cross_bins(cnt, (uint64_t)s.k, &bin, &before, &upto);
-      if (threadIdx.x == 0 && bin >= 0) k_bin = bin;
-    }
-    __syncthreads();
+    find_k(s, cnt, q);
     for (int b = threadIdx.x; b < kBins; b += NT) p.cnt[slot * kBins + b] = cnt[b];
   }
-  if (s.use_p) {
-    const int last = k_bin;
+  // What lies below the least kept t from here lies further below it from the
+  // row's largest; only top-p's total counts it.
+  const double least = s.use_p ? kLeastT : s.min_t;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int b = is_real(x[e]) ? bin_of(x[e], top, s.cb) : kBins;
-      if (b < kBins && b <= last)
-        atomicAdd((unsigned long long*)&mass[b],
-                  (unsigned long long)weight_from(((double)x[e] - (double)m) * s.c, kLeastT));
-    }
-    __syncthreads();
-    for (int b = threadIdx.x; b < kBins; b += NT) p.mass[slot * kBins + b] = mass[b];
+  for (int e = 0; e < E; ++e) {
+    const int b = is_real(x[e]) ? bin_of(x[e], top, s.cb) : kBins;
+    const double t = ((double)x[e] - (double)m) * s.c;
+    if (b < kBins && b <= q.k_bin && t >= least)
+      atomicAdd((unsigned long long*)&mass[b], (unsigned long long)weight42(t));
   }
+  __syncthreads();
+  for (int b = threadIdx.x; b < kBins; b += NT) p.mass[slot * kBins + b] = mass[b];
 }
 
-// 2. The row's histogram from its chunks', and the bins that its cuts fall in.
+// 2. The row's histogram from its chunks', the bins that its cuts fall in, and
+// of each chunk the weight that is kept whatever happens in those (`sure`) and
+// whether it holds a candidate (`some`).
 __global__ __launch_bounds__(kBins) void sample_merge_kernel(const SplitArgs p) {
   __shared__ uint64_t mass[kBins];
   __shared__ uint32_t cnt[kBins];
+  __shared__ double scale[kMaxChunks];  // of a chunk's weights to the row's
+  __shared__ int shift[kMaxChunks];     // of its bins; kBins: none of them is drawn
+  __shared__ float part[kBins / 64];
   const int64_t lr = blockIdx.x, r = p.row0 + lr;
   const Row s = row_settings(p.a, r);
-  const float* max = p.max + lr * p.chunks;
-  float m = -INFINITY;
-  for (int g = 0; g < p.chunks; ++g) m = fmaxf(m, max[g]);
-  const double top = floor((double)m * s.cb);
-  Cuts q;
-  q.k_bin = q.p_first = q.p_last = kBins;
-  q.k_above = q.k_mass = q.p_above = 0;
-  if (is_real(m) && !s.greedy && (s.use_k || s.use_p)) {
-    const int b = threadIdx.x;
-    uint32_t n = 0;
-    uint64_t w = 0;
-    for (int g = 0; g < p.chunks; ++g) {
-      if (!is_real(max[g])) continue;
-      const double shift = top - floor((double)max[g] * s.cb);
-      if (!(shift <= (double)b)) continue;
-      const int64_t at = (lr * p.chunks + g) * kBins + (b - (int)shift);
-      if (s.use_k) n += p.cnt[at];
-      if (s.use_p) w += (uint64_t)rint((double)p.mass[at] * exp2(((double)max[g] - (double)m) * s.c));
+  float mine = -INFINITY;
+  for (int g = threadIdx.x; g < p.chunks; g += kBins) mine = fmaxf(mine, p.max[lr * p.chunks + g]);
+  const float m = block_max<kBins>(mine, part);
+  const float top = grid_of(m, s.cb);
+  Cuts q = no_cuts();
+  if (is_real(m) && !s.greedy) {
+    for (int g = threadIdx.x; g < p.chunks; g += kBins) {
+      const float mg = p.max[lr * p.chunks + g], by = top - grid_of(mg, s.cb);
+      shift[g] = is_real(mg) && by < (float)kBins ? (int)by : kBins;
+      scale[g] = exp2(((double)mg - (double)m) * s.c);
     }
-    cnt[b] = n;
-    mass[b] = w;
     __syncthreads();
-    if (threadIdx.x < 64) q = find_cuts(s, cnt, mass);
+    if (s.use_k || s.use_p) {
+      const int b = threadIdx.x;
+      uint32_t n = 0;
+      uint64_t w = 0;
+#pragma unroll 4
+      for (int g = 0; g < p.chunks; ++g) {
+        if (b < shift[g]) continue;
+        const int64_t at = (lr * p.chunks + g) * kBins + (b - shift[g]);
+        if (s.use_k) n += p.cnt[at];
+        if (s.use_p) w += (uint64_t)rint((double)p.mass[at] * scale[g]);
+      }
+      cnt[b] = n;
+      mass[b] = w;
+      __syncthreads();
+      if (s.use_k) find_k(s, cnt, q);
+      if (s.use_p) find_p(s, mass, q);
+    }
+    find_least(s, m, top, q);
+    // A wave a chunk, a lane eight bins.
+    const int lane = threadIdx.x & 63, whole = sure_bins(q);
+    for (int g = threadIdx.x >> 6; g < p.chunks; g += kBins / 64) {
+      const int64_t slot = lr * p.chunks + g;
+      uint64_t sum = 0;
+      bool some = false;
+      if (shift[g] < kBins) {
+#pragma unroll
+        for (int j = 0; j < kBins / 64; ++j) {
+          const int64_t at = slot * kBins + lane + 64 * j;
+          const int b = lane + 64 * j + shift[g];
+          const uint64_t w = p.mass[at];
+          sum += b < whole ? w : 0;
+          // (Top-k counts what weighs nothing, too.)
+          some |= is_candidate(q, b) && (w > 0 || (b == q.k_bin && p.cnt[at] > 0));
+        }
+      }
+      sum = wave_sum_u64(sum);
+      some = __ballot(some) != 0;
+      if (lane == 0) {
+        p.sure[slot] = shift[g] < kBins ? (uint64_t)rint((double)sum * scale[g]) : 0;
+        p.some[slot] = some;
+      }
+    }
   }
   if (threadIdx.x == 0) p.state[lr] = RowState{q, top, m, 0};
 }
 
-// 3. A chunk's weight that is kept for certain, and its candidates.
+// 3. A chunk's candidates to the row's list: counted, a place taken for all of
+// them at once, written.
 template <typename T>
 __global__ __launch_bounds__(kChunkThreads) void sample_gather_kernel(const SplitArgs p) {
-  constexpr int E = kChunkPer, NT = kChunkThreads;
-  __shared__ uint64_t part[NT / 64];
+  constexpr int E = kChunkPer;
+  __shared__ int n_here, first;
   const int64_t lr = blockIdx.y, r = p.row0 + lr;
   const int64_t slot = lr * p.chunks + blockIdx.x;
-  const T* row = (const T*)p.a.logits + r * p.a.row_stride;
   const Row s = row_settings(p.a, r);
   RowState* st = p.state + lr;
-  const float m = st->m;
-  if (s.greedy || !is_real(m)) return;
+  if (s.greedy || !is_real(st->m) || !p.some[slot]) return;
   const Cuts q = st->cuts;
-  const double top = st->top;
-  const bool cuts = s.use_k || s.use_p;
-  const int sure = sure_bins(q);
+  const float top = st->top;
   const int base = (int)blockIdx.x * kChunk;
   float x[E];
-  load_chunk<T, E>(row, base, (int)p.a.vocab, x);
-  uint64_t mine = 0;
+  load_chunk<T, E>((const T*)p.a.logits + r * p.a.row_stride, base, (int)p.a.vocab, x);
+  if (threadIdx.x == 0) n_here = 0;
+  __syncthreads();
+  uint32_t mine = 0;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    if (!is_real(x[e])) continue;
-    if (cuts) {
-      const int b = bin_of(x[e], top, s.cb);
-      if (is_candidate(q, b)) {
-        const int at = atomicAdd(&st->n_list, 1);
-        if (at < kListMax) p.list[lr * kListMax + at] = order_of(x[e], index_of<E>(base, e));
-        continue;
-      }
-      if (b >= sure) continue;
-    }
-    mine += weight_from(((double)x[e] - (double)m) * s.c, s.min_t);
+    const int b = is_real(x[e]) ? bin_of(x[e], top, s.cb) : kBins;
+    mine |= (uint32_t)is_candidate(q, b) << e;
   }
-  mine = wave_sum_u64(mine);
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = mine;
+  const int n = (int)wave_sum_u64((uint64_t)__popc(mine));
+  int at = 0;
+  if ((threadIdx.x & 63) == 0 && n) at = atomicAdd(&n_here, n);
+  at = __builtin_amdgcn_readfirstlane(at);
   __syncthreads();
-  if (threadIdx.x == 0) {
-    uint64_t sum = 0;
-    for (int w = 0; w < NT / 64; ++w) sum += part[w];
-    p.sure[slot] = sum;
+  if (threadIdx.x == 0) first = n_here ? atomicAdd(&st->n_list, n_here) : 0;
+  __syncthreads();
+  at += first + (int)wave_scan_u64((uint64_t)__popc(mine)) - __popc(mine);
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    if ((mine >> e & 1) && at < kListMax) p.list[lr * kListMax + at] = order_of(x[e], index_of<E>(base, e));
+    at += mine >> e & 1;
   }
 }
 
@@ -792,23 +895,16 @@ __global__ __launch_bounds__(kChunkThreads) void sample_finish_kernel(const Spli
   if (n <= LIST)
     for (int i = threadIdx.x; i < n; i += NT) sh.list[i] = p.list[lr * kListMax + i];
   __syncthreads();
-  float limit_x = -INFINITY;
-  int limit_i = -1;
-  if (s.use_k || s.use_p) {
-    Candidates<T, NT, LIST> cand{sh, row, (int)a.vocab, m, st.top, s, n};
-    const uint64_t lim = cand.limit(st.cuts);
-    if (lim != ~0ull) {
-      limit_x = value_of(lim);
-      limit_i = (int)(uint32_t)lim;
-    }
-    const int sure = sure_bins(st.cuts);
-    cand.each(sure, kBins - 1, [&](uint64_t o, int b) {
-      if (o > lim || !is_candidate(st.cuts, b)) return;
-      const uint64_t w = cand.weight(o, s.min_t);
-      if (w) atomicAdd((unsigned long long*)&chunk_sum[(uint32_t)o / kChunk], (unsigned long long)w);
-    });
-    __syncthreads();
-  }
+  Candidates<T, NT, LIST> cand{sh, row, (int)a.vocab, m, st.top, s, n};
+  const uint64_t lim = cand.limit(st.cuts);
+  const float limit_x = lim != ~0ull ? value_of(lim) : -INFINITY;
+  const int limit_i = lim != ~0ull ? (int)(uint32_t)lim : -1;  // (-inf itself is not kept)
+  cand.each(0, kBins - 1, [&](uint64_t o, int b) {
+    if (o > lim || !is_candidate(st.cuts, b)) return;
+    const uint64_t w = cand.weight(o, s.min_t);
+    if (w) atomicAdd((unsigned long long*)&chunk_sum[(uint32_t)o / kChunk], (unsigned long long)w);
+  });
+  __syncthreads();
   uint64_t total = 0;
   for (int g = 0; g < p.chunks; ++g) total += chunk_sum[g];
   uint64_t at = draw_at(s.u, total);
@@ -823,6 +919,10 @@ __global__ __launch_bounds__(kChunkThreads) void sample_finish_kernel(const Spli
   mine = wave_sum_u64(mine);
   if ((threadIdx.x & 63) == 0) sh.wave_sum[threadIdx.x >> 6] = mine;
   __syncthreads();
+  // (The chunk's sum was scaled as a whole: its logits' own may be a few units less.)
+  uint64_t here = 0;
+  for (int w = 0; w < NT / 64; ++w) here += sh.wave_sum[w];
+  at = at < here ? at : here - 1;
   int token;
   double t;
   if (locate<NT, E, LIST>(sh, s, x, base, m, limit_x, limit_i, at, &token, &t)) {
@@ -840,13 +940,12 @@ size_t up(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
 
 template <typename T>
 bdh_status sample_typed(const SampleArgs& a, hipStream_t st, uint64_t* launches) {
-  if (a.vocab <= 32768) {
+  if (a.vocab <= 16384) {
     if (a.vocab <= 256) launch_row<T, 64, 4>(a, st);
     else if (a.vocab <= 1024) launch_row<T, 256, 4>(a, st);
-    else if (a.vocab <= 4096) launch_row<T, 256, 16>(a, st);
-    else if (a.vocab <= 8192) launch_row<T, 512, 16>(a, st);
-    else if (a.vocab <= 16384) launch_row<T, 1024, 16>(a, st);
-    else launch_row<T, 1024, 32>(a, st);
+    else if (a.vocab <= 4096) launch_row<T, 1024, 4>(a, st);
+    else if (a.vocab <= 8192) launch_row<T, 1024, 8>(a, st);
+    else launch_row<T, 1024, 16>(a, st);
     BDH_HIP_TRY(hipGetLastError());
     *launches += 1;
     return BDH_OK;
@@ -858,7 +957,8 @@ bdh_status sample_typed(const SampleArgs& a, hipStream_t st, uint64_t* launches)
   p.chunks = (int)((a.vocab + kChunk - 1) / kChunk);
   const size_t slots = (size_t)group * (size_t)p.chunks;
   const size_t sizes[] = {up(slots * 4), up(slots * 4), up(slots * kBins * 4), up(slots * kBins * 8),
-                          up(slots * 8), up((size_t)group * kListMax * 8), up((size_t)group * sizeof(RowState))};
+                          up(slots * 8), up(slots * 4), up((size_t)group * kListMax * 8),
+                          up((size_t)group * sizeof(RowState))};
   size_t bytes = 0;
   for (size_t s : sizes) bytes += s;
   void* buf = nullptr;
@@ -870,7 +970,8 @@ bdh_status sample_typed(const SampleArgs& a, hipStream_t st, uint64_t* launches)
   p.cnt = (uint32_t*)at; at += sizes[2];
   p.mass = (uint64_t*)at; at += sizes[3];
   p.sure = (uint64_t*)at; at += sizes[4];
-  p.list = (uint64_t*)at; at += sizes[5];
+  p.some = (int32_t*)at; at += sizes[5];
+  p.list = (uint64_t*)at; at += sizes[6];
   p.state = (RowState*)at;
   for (p.row0 = 0; p.row0 < a.rows; p.row0 += group) {
     const uint32_t n = (uint32_t)(a.rows - p.row0 < group ? a.rows - p.row0 : group);

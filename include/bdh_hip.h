@@ -343,7 +343,7 @@ bdh_status bdh_apply_adapters(const bdh_adapter_plan* plan, int32_t dtype, const
  * takes the place of the scalar beside it; there, a temperature that is not
  * above 0 counts as 0, other values outside a range as its nearest end, NaN
  * as no cut, and a random number outside [0, 1) as the nearest inside.
- * vocab up to 2^20; past 32768 the call uses the stream's scratch. */
+ * vocab up to 2^20; past 16384 the call uses the stream's scratch. */
 typedef struct {
   float temperature, top_p, min_p;
   int32_t top_k;
