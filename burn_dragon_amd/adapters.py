@@ -15,7 +15,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from .recurrent import _dtype_code, _on_current_device, _ptr, _stream_ptr, supports_backend
+from .recurrent import _call_on, _dtype_code, _ptr, _stream_ptr, _supported
 
 
 class AdapterSet(NamedTuple):
@@ -34,40 +34,35 @@ def apply_adapters(base: torch.Tensor, hidden: torch.Tensor, adapters: AdapterSe
     itself for in place).  None where the library does not support the input
     (no supported device, another dtype, an empty dimension, a rank above
     128, a scratch that would have to grow under capture)."""
-    if not supports_backend():
-        return None
-    if base.dim() not in (2, 3) or hidden.dim() != base.dim() or not base.is_cuda:
-        return None
+    dev, shape = base.device, base.shape
     code = _dtype_code(base)
-    if code is None or hidden.dtype != base.dtype:
+    if not _supported(dev) or code is None or hidden.dtype != base.dtype:
         return None
-    B, T, V = base.shape if base.dim() == 3 else (base.shape[0], 1, base.shape[1])
-    D = hidden.shape[-1]
+    if len(shape) not in (2, 3) or hidden.dim() != len(shape):
+        return None
+    B, V, D = shape[0], shape[-1], hidden.shape[-1]
+    T = shape[1] if len(shape) == 3 else 1
     a, b, scale = adapters
     if a.dim() != 3 or b.dim() != 3 or a.dtype != torch.bfloat16 or b.dtype != torch.bfloat16:
         return None
     n, R, _ = a.shape
     if min(B, T, V, D, n, R) == 0:
         return None
-    if (tuple(hidden.shape[:-1]) != tuple(base.shape[:-1]) or tuple(a.shape) != (n, R, D)
-            or tuple(b.shape) != (n, V, R) or tuple(scale.shape) != (n,) or tuple(ids.shape) != (B,)):
+    if (hidden.shape[:-1] != shape[:-1] or a.shape != (n, R, D) or b.shape != (n, V, R)
+            or scale.shape != (n,) or ids.shape != (B,)):
         raise ValueError("base, hidden, adapters and ids do not fit together")
     if scale.dtype != torch.float32 or ids.dtype != torch.int32:
         raise ValueError("scale must be f32 and ids int32")
-    if any(t.device != base.device for t in (hidden, a, b, scale, ids)):
+    if not hidden.device == a.device == b.device == scale.device == ids.device == dev:
         raise ValueError("base, hidden, adapters and ids must be on one device")
-    if out is not None and (tuple(out.shape) != tuple(base.shape) or out.dtype != base.dtype
-                            or out.device != base.device or not out.is_contiguous()):
-        raise ValueError("out must be a contiguous tensor like base")
-    base_c, hidden_c, a, b = base.contiguous(), hidden.contiguous(), a.contiguous(), b.contiguous()
-    scale, ids = scale.contiguous(), ids.contiguous()
     if out is None:
-        out = torch.empty(base.shape, device=base.device, dtype=base.dtype)
+        out = torch.empty(shape, device=dev, dtype=base.dtype)
+    elif out.shape != shape or out.dtype != base.dtype or out.device != dev or not out.is_contiguous():
+        raise ValueError("out must be a contiguous tensor like base")
+    # contiguous copies stay referenced until the launch is enqueued
+    base, hidden, a, b = base.contiguous(), hidden.contiguous(), a.contiguous(), b.contiguous()
+    scale, ids = scale.contiguous(), ids.contiguous()
     plan = _lib.BdhAdapterPlan(B, T, D, V, R, n)
-    with _on_current_device(base.device):
-        st = _lib.load().bdh_apply_adapters(ctypes.byref(plan), code, _ptr(base_c), _ptr(hidden_c),
-                                            _ptr(a), _ptr(b), _ptr(scale), _ptr(ids), _ptr(out),
-                                            _stream_ptr(base.device))
-    if not _lib.check(st):
-        return None
-    return out
+    st = _call_on(dev, _lib.load().bdh_apply_adapters, ctypes.byref(plan), code, _ptr(base), _ptr(hidden),
+                  _ptr(a), _ptr(b), _ptr(scale), _ptr(ids), _ptr(out), _stream_ptr(dev))
+    return out if _lib.check(st) else None

@@ -36,6 +36,7 @@ constexpr int kBins = 512;
 constexpr int kBinsPerOctave = 10;  // 420 of the bins: see bin_of
 constexpr double kLeastT = -42.0;
 constexpr int kSmall = 64;       // candidates that one wave orders
+constexpr int kMid = 256;        // that the workgroup compares each with each
 constexpr int kListMax = 4096;   // candidates that the list holds
 constexpr int kChunkThreads = 512;
 constexpr int kChunkPer = 16;    // logits a thread
@@ -61,7 +62,7 @@ __device__ Row row_settings(const SampleArgs& a, int64_t r) {
   s.k = a.top_k_rows ? a.top_k_rows[r] : a.top_k;
   s.greedy = !(tau > 0.0f) || s.k == 1;
   s.c = 1.4426950408889634074 / (double)tau;
-  s.cb = (float)fmin(s.c * kBinsPerOctave, 1e30);
+  s.cb = (float)fmax(fmin(s.c * kBinsPerOctave, 1e30), 1e-30);  // (finite times -inf: -inf)
   s.use_k = s.k > 0 && s.k < a.vocab;
   s.use_p = p < 1.0f;
   s.p = p > 0.0f ? (double)p : 0.0;
@@ -70,32 +71,40 @@ __device__ Row row_settings(const SampleArgs& a, int64_t r) {
   return s;
 }
 
-// 2^t * 2^42 as an integer, t in [-42, 0]; 2^f by its series to the 11th
-// power (the rest is below 2^-47 of it), 64-bit throughout.
-__device__ __forceinline__ uint64_t weight42(double t) {
+// 2^t * 2^42 as an integer, t in [-42, 0], in 64 bits: 2^f of the fraction by the
+// polynomial of degree 9 with the least largest relative error on [-1/2, 1/2]
+// (2^-46; its coefficients come out of Remez' exchange).
+//
+// The loops over a row's logits keep the coefficients in scalar registers, where
+// an FMA takes one as its addend; as literals each costs two moves, a third of
+// the instructions.
+struct Series {
+  double c[10];
+  __device__ __forceinline__ Series()
+      : c{1.0000000000000127,    0.693147180559871,     0.24022650695649653,   0.055504108668685624,
+          0.009618129192067193,  0.0013333557617602426, 0.00015403434948103528, 1.5252984839814557e-05,
+          1.3259405603573696e-06, 1.0150336495148618e-07} {}
+  __device__ __forceinline__ void keep() {
+#pragma unroll
+    for (int k = 0; k < 10; ++k) asm("" : "+s"(c[k]));
+  }
+};
+__device__ __forceinline__ uint64_t weight42(double t, const Series& series = Series()) {
   const double magic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer
   const double kd = t + magic;
-  const int n = (int)(uint32_t)__double_as_longlong(kd);
+  const int n = __double2loint(kd);
   const double f = t - (kd - magic);
-  double e = 4.45538190442164e-10;  // ln(2)^k / k!
-  e = fma(e, f, 7.054911620801123e-09);
-  e = fma(e, f, 1.0178086009239699e-07);
-  e = fma(e, f, 1.3215486790144307e-06);
-  e = fma(e, f, 1.525273380405984e-05);
-  e = fma(e, f, 0.0001540353039338161);
-  e = fma(e, f, 0.0013333558146428443);
-  e = fma(e, f, 0.009618129107628477);
-  e = fma(e, f, 0.05550410866482158);
-  e = fma(e, f, 0.2402265069591007);
-  e = fma(e, f, 0.6931471805599453);
-  e = fma(e, f, 1.0);
-  const double w = __longlong_as_double(__double_as_longlong(e) + ((int64_t)(n + 42) << 52));
-  return (uint64_t)__double_as_longlong(w + 4503599627370496.0) - 0x4330000000000000ull;
+  double e = series.c[9];
+#pragma unroll
+  for (int k = 8; k >= 0; --k) e = fma(e, f, series.c[k]);
+  const double w = __hiloint2double(__double2hiint(e) + (n << 20) + (42 << 20), __double2loint(e));
+  const double r = w + 4503599627370496.0;  // 2^52: the integer is in the low bits
+  return (uint64_t)(uint32_t)(__double2hiint(r) - 0x43300000) << 32 | (uint32_t)__double2loint(r);
 }
 
 // Its weight where t is kept at all.
-__device__ __forceinline__ uint64_t weight_from(double t, double least) {
-  return t >= least ? weight42(t) : 0;  // (NaN: -inf logits at an infinite temperature)
+__device__ __forceinline__ uint64_t weight_from(double t, double least, const Series& series = Series()) {
+  return t >= least ? weight42(t, series) : 0;  // (NaN: -inf logits at an infinite temperature)
 }
 
 __device__ __forceinline__ float clean(float x) {
@@ -173,7 +182,7 @@ template <int NT, int LIST>
 struct Shared {
   uint64_t mass[kBins];
   uint64_t list[LIST];
-  uint64_t small[kSmall], small_w[kSmall];
+  uint64_t small[kSmall], small_w[kMid];
   uint64_t wave_sum[NT / 64];
   uint64_t lo, hi, sum;  // of a pass over the candidates
   uint32_t cnt[kBins];
@@ -324,6 +333,17 @@ __device__ __forceinline__ void find_k(const Row& s, const uint32_t* cnt, Cuts& 
   uint64_t in;
   q.k_bin = BinScan(cnt, kBins).cross((uint64_t)s.k, &q.k_above, &in);
 }
+// Counts a chunk's logits by bin into cnt (cleared) and finds its k-th.
+template <int NT, int E>
+__device__ __forceinline__ void count_for_k(const Row& s, const float (&x)[E], float top, uint32_t* cnt, Cuts& q) {
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int b = bin_of(x[e], top, s.cb);
+    if (b < kBins) atomicAdd(&cnt[b], 1u);
+  }
+  __syncthreads();
+  find_k(s, cnt, q);
+}
 __device__ __forceinline__ void find_p(const Row& s, const uint64_t* mass, Cuts& q) {
   // What top-k keeps weighs between all before k_bin, and that with k_bin.
   const BinScan h(mass, q.k_bin);
@@ -374,7 +394,6 @@ struct Candidates {
     } else {
       for (int i = threadIdx.x; i < vocab; i += NT) {
         const float x = load1(row + i);
-        if (!is_real(x)) continue;
         const int b = bin_of(x, top, s.cb);
         if (b >= first && b <= last) f(order_of(x, i), b);
       }
@@ -484,10 +503,61 @@ struct Candidates {
     return wave_max_u64(kept ? mine : 0);
   }
 
+  // The same for up to kMid, a thread (or at 64 threads four) a candidate.
+  __device__ uint64_t limit_mid(const Cuts& q) {
+    constexpr int PER = kMid > NT ? kMid / NT : 1;
+    constexpr uint64_t in_k_bit = 1ull << 63;  // (weights end below)
+    uint64_t mine[PER], w[PER], k_before[PER], p_before[PER];
+    int bin[PER];
+#pragma unroll
+    for (int c = 0; c < PER; ++c) {
+      const int i = threadIdx.x + c * NT;
+      mine[c] = i < n ? sh.list[i] : ~0ull;
+      bin[c] = i < n ? bin_of(value_of(mine[c]), top, s.cb) : kBins;
+      w[c] = s.use_p && i < n ? weight(mine[c], kLeastT) : 0;
+      k_before[c] = q.k_above;
+      p_before[c] = q.p_above;
+      if (i < n)
+        sh.small_w[i] = (bin[c] >= q.p_first && bin[c] <= q.p_last ? w[c] : 0) | (bin[c] == q.k_bin ? in_k_bit : 0);
+    }
+    if (threadIdx.x == 0) sh.sum = sh.hi = 0;
+    __syncthreads();
+    if (threadIdx.x < n) {
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) {
+        const uint64_t o = sh.list[j], wj = sh.small_w[j];
+#pragma unroll
+        for (int c = 0; c < PER; ++c) {
+          k_before[c] += o < mine[c] ? wj >> 63 : 0;
+          p_before[c] += o < mine[c] ? wj & ~in_k_bit : 0;
+        }
+      }
+    }
+    uint64_t last = 0;
+#pragma unroll
+    for (int c = 0; c < PER; ++c) {
+      const bool real = threadIdx.x + c * NT < n;
+      const bool kept = real && (bin[c] < q.k_bin || k_before[c] < (uint64_t)s.k);
+      if (s.use_p && kept && bin[c] == q.k_bin) atomicAdd((unsigned long long*)&sh.sum, (unsigned long long)w[c]);
+      if (!kept) mine[c] = 0;
+    }
+    __syncthreads();
+    const uint64_t need = s.use_p ? p_need(s, q.k_mass + sh.sum) : 0;
+#pragma unroll
+    for (int c = 0; c < PER; ++c) {
+      const bool kept = !s.use_p || bin[c] < q.p_first || (bin[c] <= q.p_last && p_before[c] < need);
+      last = kept && mine[c] > last ? mine[c] : last;
+    }
+    if (last) atomicMax((unsigned long long*)&sh.hi, (unsigned long long)last);
+    __syncthreads();
+    return sh.hi;
+  }
+
   // The last logit in order that top-k and top-p keep.
   __device__ uint64_t limit(const Cuts& q) {
     if (q.k_bin == kBins && !s.use_p) return ~0ull;  // neither divides anything
     if (n <= kSmall) return limit_small(q);
+    if (n <= kMid) return limit_mid(q);
     uint64_t lim = ~0ull, total = q.k_mass;
     if (q.k_bin < kBins) {
       lim = cut<false>(q.k_bin, q.k_bin, q.k_above, (uint64_t)s.k);
@@ -512,9 +582,10 @@ struct Candidates {
 
 // The kept weight of a thread's logits: those up to (limit_x, limit_i) in order.
 template <int E>
-__device__ __forceinline__ uint64_t kept_weight(const Row& s, float x, int i, float m, float limit_x, int limit_i) {
+__device__ __forceinline__ uint64_t kept_weight(const Row& s, float x, int i, float m, float limit_x, int limit_i,
+                                                const Series& series = Series()) {
   if (!(x > limit_x || (x == limit_x && i <= limit_i))) return 0;
-  return weight_from(((double)x - (double)m) * s.c, s.min_t);
+  return weight_from(((double)x - (double)m) * s.c, s.min_t, series);
 }
 
 __device__ __forceinline__ uint64_t draw_at(float u, uint64_t total) {
@@ -608,6 +679,8 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a) {
     }
     return;
   }
+  Series series;
+  series.keep();
   float limit_x = -INFINITY;
   int limit_i = -1;  // (-inf itself is not kept)
   if (s.use_k || s.use_p) {
@@ -620,22 +693,16 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a) {
     __syncthreads();
     Cuts q = no_cuts();
     if (s.use_k) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int b = is_real(x[e]) ? bin_of(x[e], top, s.cb) : kBins;
-        if (b < kBins) atomicAdd(&sh.cnt[b], 1u);
-      }
-      __syncthreads();
-      find_k(s, sh.cnt, q);  // (every wave, the same)
+      count_for_k<NT, E>(s, x, top, sh.cnt, q);
       forget<E>(x);
     }
     if (s.use_p) {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const int b = is_real(x[e]) ? bin_of(x[e], top, s.cb) : kBins;
+        const int b = bin_of(x[e], top, s.cb);
         if (b < kBins && b <= q.k_bin)  // no weight past the k-th counts
           atomicAdd((unsigned long long*)&sh.mass[b],
-                    (unsigned long long)weight_from(((double)x[e] - (double)m) * s.c, kLeastT));
+                    (unsigned long long)weight_from(((double)x[e] - (double)m) * s.c, kLeastT, series));
         if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
       }
       __syncthreads();
@@ -644,7 +711,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a) {
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int b = is_real(x[e]) ? bin_of(x[e], top, s.cb) : kBins;
+      const int b = bin_of(x[e], top, s.cb);
       const int at = append_at(&sh.n_list, is_candidate(q, b));
       if (at >= 0 && at < LIST) sh.list[at] = order_of(x[e], index_of<E>(0, e));
     }
@@ -660,7 +727,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a) {
   uint64_t mine = 0;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    mine += kept_weight<E>(s, x[e], index_of<E>(0, e), m, limit_x, limit_i);
+    mine += kept_weight<E>(s, x[e], index_of<E>(0, e), m, limit_x, limit_i, series);
     if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
   }
   mine = wave_sum_u64(mine);
@@ -694,7 +761,6 @@ struct SplitArgs {
   uint32_t* cnt;     // [rows, chunks, kBins], bins counted from the chunk's own largest
   uint64_t* mass;    // [rows, chunks, kBins], weights relative to it
   uint64_t* sure;    // [rows, chunks]
-  int32_t* some;     // [rows, chunks]
   uint64_t* list;    // [rows, kListMax]
   RowState* state;   // [rows]
 };
@@ -736,33 +802,27 @@ __global__ __launch_bounds__(kChunkThreads) void sample_chunk_kernel(const Split
   const float top = grid_of(m, s.cb);
   Cuts q = no_cuts();
   if (s.use_k) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int b = is_real(x[e]) ? bin_of(x[e], top, s.cb) : kBins;
-      if (b < kBins) atomicAdd(&cnt[b], 1u);
-    }
-    __syncthreads();
     // Past the chunk's own k-th no logit is among the row's first k.
-    find_k(s, cnt, q);
+    count_for_k<NT, E>(s, x, top, cnt, q);
     for (int b = threadIdx.x; b < kBins; b += NT) p.cnt[slot * kBins + b] = cnt[b];
   }
   // What lies below the least kept t from here lies further below it from the
   // row's largest; only top-p's total counts it.
   const double least = s.use_p ? kLeastT : s.min_t;
+  Series series;
+  series.keep();
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const int b = is_real(x[e]) ? bin_of(x[e], top, s.cb) : kBins;
+    const int b = bin_of(x[e], top, s.cb);
     const double t = ((double)x[e] - (double)m) * s.c;
     if (b < kBins && b <= q.k_bin && t >= least)
-      atomicAdd((unsigned long long*)&mass[b], (unsigned long long)weight42(t));
+      atomicAdd((unsigned long long*)&mass[b], (unsigned long long)weight42(t, series));
   }
   __syncthreads();
   for (int b = threadIdx.x; b < kBins; b += NT) p.mass[slot * kBins + b] = mass[b];
 }
 
-// 2. The row's histogram from its chunks', the bins that its cuts fall in, and
-// of each chunk the weight that is kept whatever happens in those (`sure`) and
-// whether it holds a candidate (`some`).
+// 2. The row's histogram from its chunks' and the bins that its cuts fall in.
 __global__ __launch_bounds__(kBins) void sample_merge_kernel(const SplitArgs p) {
   __shared__ uint64_t mass[kBins];
   __shared__ uint32_t cnt[kBins];
@@ -787,7 +847,7 @@ __global__ __launch_bounds__(kBins) void sample_merge_kernel(const SplitArgs p) 
       const int b = threadIdx.x;
       uint32_t n = 0;
       uint64_t w = 0;
-#pragma unroll 4
+#pragma unroll 8
       for (int g = 0; g < p.chunks; ++g) {
         if (b < shift[g]) continue;
         const int64_t at = (lr * p.chunks + g) * kBins + (b - shift[g]);
@@ -801,56 +861,54 @@ __global__ __launch_bounds__(kBins) void sample_merge_kernel(const SplitArgs p) 
       if (s.use_p) find_p(s, mass, q);
     }
     find_least(s, m, top, q);
-    // A wave a chunk, a lane eight bins.
-    const int lane = threadIdx.x & 63, whole = sure_bins(q);
-    for (int g = threadIdx.x >> 6; g < p.chunks; g += kBins / 64) {
-      const int64_t slot = lr * p.chunks + g;
-      uint64_t sum = 0;
-      bool some = false;
-      if (shift[g] < kBins) {
-#pragma unroll
-        for (int j = 0; j < kBins / 64; ++j) {
-          const int64_t at = slot * kBins + lane + 64 * j;
-          const int b = lane + 64 * j + shift[g];
-          const uint64_t w = p.mass[at];
-          sum += b < whole ? w : 0;
-          // (Top-k counts what weighs nothing, too.)
-          some |= is_candidate(q, b) && (w > 0 || (b == q.k_bin && p.cnt[at] > 0));
-        }
-      }
-      sum = wave_sum_u64(sum);
-      some = __ballot(some) != 0;
-      if (lane == 0) {
-        p.sure[slot] = shift[g] < kBins ? (uint64_t)rint((double)sum * scale[g]) : 0;
-        p.some[slot] = some;
-      }
-    }
   }
   if (threadIdx.x == 0) p.state[lr] = RowState{q, top, m, 0};
 }
 
-// 3. A chunk's candidates to the row's list: counted, a place taken for all of
-// them at once, written.
+// 3. From a chunk's histogram the weight that is kept whatever happens in the
+// cuts' bins (`sure`), and if it has candidates those to the row's list:
+// counted, a place taken for all of them at once, written.
 template <typename T>
 __global__ __launch_bounds__(kChunkThreads) void sample_gather_kernel(const SplitArgs p) {
-  constexpr int E = kChunkPer;
-  __shared__ int n_here, first;
+  constexpr int E = kChunkPer, NT = kChunkThreads;
+  static_assert(NT == kBins, "a thread a bin");
+  __shared__ uint64_t part[NT / 64];
+  __shared__ int n_here, first, some;
   const int64_t lr = blockIdx.y, r = p.row0 + lr;
   const int64_t slot = lr * p.chunks + blockIdx.x;
   const Row s = row_settings(p.a, r);
   RowState* st = p.state + lr;
-  if (s.greedy || !is_real(st->m) || !p.some[slot]) return;
+  const float m = st->m, top = st->top, mg = p.max[slot];
+  if (s.greedy || !is_real(m)) return;
   const Cuts q = st->cuts;
-  const float top = st->top;
+  if (threadIdx.x == 0) n_here = some = 0;
+  __syncthreads();
+  const float shift = top - grid_of(mg, s.cb);  // (a chunk without a logit: beyond all bins)
+  uint64_t w = 0;
+  if (shift < (float)kBins) {
+    const int64_t at = slot * kBins + threadIdx.x;
+    const int b = threadIdx.x + (int)shift;
+    w = p.mass[at];
+    // (Top-k counts what weighs nothing, too.)
+    if (is_candidate(q, b) && (w > 0 || (b == q.k_bin && p.cnt[at] > 0))) some = 1;
+    w = b < sure_bins(q) ? w : 0;
+  }
+  w = wave_sum_u64(w);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = w;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    uint64_t sum = 0;
+    for (int i = 0; i < NT / 64; ++i) sum += part[i];
+    p.sure[slot] = sum ? (uint64_t)rint((double)sum * exp2(((double)mg - (double)m) * s.c)) : 0;
+  }
+  if (!some) return;
   const int base = (int)blockIdx.x * kChunk;
   float x[E];
   load_chunk<T, E>((const T*)p.a.logits + r * p.a.row_stride, base, (int)p.a.vocab, x);
-  if (threadIdx.x == 0) n_here = 0;
-  __syncthreads();
   uint32_t mine = 0;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const int b = is_real(x[e]) ? bin_of(x[e], top, s.cb) : kBins;
+    const int b = bin_of(x[e], top, s.cb);
     mine |= (uint32_t)is_candidate(q, b) << e;
   }
   const int n = (int)wave_sum_u64((uint64_t)__popc(mine));
@@ -957,7 +1015,7 @@ bdh_status sample_typed(const SampleArgs& a, hipStream_t st, uint64_t* launches)
   p.chunks = (int)((a.vocab + kChunk - 1) / kChunk);
   const size_t slots = (size_t)group * (size_t)p.chunks;
   const size_t sizes[] = {up(slots * 4), up(slots * 4), up(slots * kBins * 4), up(slots * kBins * 8),
-                          up(slots * 8), up(slots * 4), up((size_t)group * kListMax * 8),
+                          up(slots * 8), up((size_t)group * kListMax * 8),
                           up((size_t)group * sizeof(RowState))};
   size_t bytes = 0;
   for (size_t s : sizes) bytes += s;
@@ -970,8 +1028,7 @@ bdh_status sample_typed(const SampleArgs& a, hipStream_t st, uint64_t* launches)
   p.cnt = (uint32_t*)at; at += sizes[2];
   p.mass = (uint64_t*)at; at += sizes[3];
   p.sure = (uint64_t*)at; at += sizes[4];
-  p.some = (int32_t*)at; at += sizes[5];
-  p.list = (uint64_t*)at; at += sizes[6];
+  p.list = (uint64_t*)at; at += sizes[5];
   p.state = (RowState*)at;
   for (p.row0 = 0; p.row0 < a.rows; p.row0 += group) {
     const uint32_t n = (uint32_t)(a.rows - p.row0 < group ? a.rows - p.row0 : group);

@@ -11,7 +11,6 @@ mismatch, plan mismatch) so that callers fall back exactly as
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from dataclasses import dataclass
 from typing import NamedTuple, Optional
@@ -95,12 +94,18 @@ def _stream_ptr(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
-def _on_current_device(device: torch.device):
-    """Makes a tensor's device current for a call where it is not: the
-    library launches on, and keeps its scratch by, the current device."""
-    if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def _supported(device: torch.device) -> bool:
+    """supports_backend for a device tensor's call (torch is initialised)."""
+    return device.type == "cuda" and bool(_call_on(device, _lib.load().bdh_supports_backend))
+
+
+def _call_on(device: torch.device, fn, *args):
+    """Calls into the library with a tensor's device current: it launches on,
+    and keeps its scratch by, the current device."""
+    if torch._C._cuda_getDevice() == device.index:
+        return fn(*args)
+    with torch.cuda.device(device):
+        return fn(*args)
 
 
 def _on_device(*ts) -> bool:

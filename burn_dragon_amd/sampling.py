@@ -16,7 +16,7 @@ from typing import NamedTuple, Optional, Union
 import torch
 
 from . import _lib
-from .recurrent import _dtype_code, _on_current_device, _ptr, _stream_ptr, supports_backend
+from .recurrent import _call_on, _dtype_code, _ptr, _stream_ptr, _supported
 
 PerRow = Union[float, torch.Tensor]
 
@@ -30,7 +30,7 @@ def _per_row(value, rows: int, dtype: torch.dtype, device, name: str):
     """(scalar, tensor or None): one setting for all rows, or one a row."""
     if not isinstance(value, torch.Tensor):
         return value, None
-    if value.dtype != dtype or tuple(value.shape) != (rows,) or value.device != device:
+    if value.dtype != dtype or value.shape != (rows,) or value.device != device:
         raise ValueError(f"{name} must be a number or a {dtype} tensor of [{rows}] on the logits' device")
     return 0, value.contiguous()
 
@@ -53,18 +53,17 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: P
     not support the input (no supported device, another dtype, an empty
     dimension, V above 2^20, a scratch that would have to grow under
     capture)."""
-    if not supports_backend():
-        return None
-    if logits.dim() != 2 or not logits.is_cuda or logits.shape[0] == 0 or logits.shape[1] == 0:
-        return None
-    code = _dtype_code(logits)
-    if code is None:
+    dev = logits.device
+    if not _supported(dev) or logits.dim() != 2:
         return None
     rows, vocab = logits.shape
-    dev = logits.device
-    if vocab > 1 and logits.stride(1) != 1:
-        logits = logits.contiguous()
-    if uniform.dtype != torch.float32 or tuple(uniform.shape) != (rows,) or uniform.device != dev:
+    code = _dtype_code(logits)
+    if code is None or rows == 0 or vocab == 0:
+        return None
+    row_stride, stride = logits.stride()
+    if vocab > 1 and stride != 1:
+        logits, row_stride = logits.contiguous(), vocab
+    if uniform.dtype != torch.float32 or uniform.shape != (rows,) or uniform.device != dev:
         raise ValueError(f"uniform must be a f32 tensor of [{rows}] on the logits' device")
     uniform = uniform.contiguous()
     temp, temp_rows = _per_row(temperature, rows, torch.float32, dev, "temperature")
@@ -75,7 +74,7 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: P
         k = min(int(k), vocab) if k > 0 else int(k)
     if out is None:
         tokens = torch.empty(rows, device=dev, dtype=torch.int32)
-    elif (out.dtype != torch.int32 or tuple(out.shape) != (rows,) or out.device != dev
+    elif (out.dtype != torch.int32 or out.shape != (rows,) or out.device != dev
           or not out.is_contiguous()):
         raise ValueError(f"out must be a contiguous int32 tensor of [{rows}] on the logits' device")
     else:
@@ -83,11 +82,9 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: P
     logprob = torch.empty(rows, device=dev, dtype=torch.float32) if want_logprob else None
     opts = _lib.BdhSampleOptions(float(temp), float(p), float(mp), k, _ptr(temp_rows), _ptr(p_rows),
                                  _ptr(mp_rows), _ptr(k_rows))
-    with _on_current_device(dev):
-        st = _lib.load().bdh_sample_tokens(_ptr(logits), code, rows, vocab,
-                                           logits.stride(0) if rows > 1 else 0, _ptr(uniform),
-                                           ctypes.byref(opts), _ptr(tokens), _ptr(logprob),
-                                           _stream_ptr(dev))
+    st = _call_on(dev, _lib.load().bdh_sample_tokens, _ptr(logits), code, rows, vocab,
+                  row_stride if rows > 1 else 0, _ptr(uniform), ctypes.byref(opts), _ptr(tokens),
+                  _ptr(logprob), _stream_ptr(dev))
     if not _lib.check(st):
         return None
     return SampleOutput(tokens, logprob)

@@ -24,45 +24,40 @@ import torch
 
 from . import _lib
 from .model import BdhModelState
-from .recurrent import _on_current_device, _stream_ptr, supports_backend
+from .recurrent import _call_on, _stream_ptr, supports_backend
 
 StreamStates = Union[BdhModelState, Sequence[Optional[torch.Tensor]]]
 
 
 def _layers(state: StreamStates) -> List[Optional[torch.Tensor]]:
-    rho = list(state.rho if isinstance(state, BdhModelState) else state)
-    for r in rho:
-        if r is not None and (r.dtype != torch.float32 or not r.is_cuda or r.dim() != 4
-                              or not r.is_contiguous()):
-            raise ValueError("rho must be a contiguous f32 [B,H,N,D] device tensor")
-    if len({r.device for r in rho if r is not None}) > 1:
-        raise ValueError("the layers' rho are on different devices")
-    return rho
+    return list(state.rho if isinstance(state, BdhModelState) else state)
 
 
-def _arrays(rho):
-    n = len(rho)
-    descs = (_lib.BdhLayerStateDesc * max(n, 1))()
-    ptrs = (ctypes.c_void_p * max(n, 1))()
-    for i, r in enumerate(rho):
-        if r is not None:
-            descs[i].batch, descs[i].heads, descs[i].latent, descs[i].embd = r.shape
-            ptrs[i] = r.data_ptr()
-    return descs, ptrs
+class _Slots:
+    """The layers of a state as the library takes them."""
+
+    def __init__(self, rho):
+        n = len(rho)
+        self.descs = (_lib.BdhLayerStateDesc * n)()
+        self.ptrs = (ctypes.c_void_p * n)()
+        self.batch, self.device = 0, None
+        for i, r in enumerate(rho):
+            if r is None:
+                continue
+            if r.dtype != torch.float32 or not r.is_cuda or r.dim() != 4 or not r.is_contiguous():
+                raise ValueError("rho must be a contiguous f32 [B,H,N,D] device tensor")
+            if self.device is None:
+                self.batch, self.device = r.shape[0], r.device
+            elif r.shape[0] != self.batch or r.device != self.device:
+                raise ValueError("the layers of a state have different batches or devices")
+            d = self.descs[i]
+            d.batch, d.heads, d.latent, d.embd = r.shape
+            self.ptrs[i] = r.data_ptr()
 
 
-def _slots(slots, batch: int, what: str, least: int = 0) -> List[int]:
-    out = [int(s) for s in slots]
-    if any(s < least or s >= batch for s in out):
+def _check_slots(slots: List[int], batch: int, what: str, least: int = 0):
+    if slots and (min(slots) < least or max(slots) >= batch):
         raise ValueError(f"{what} must lie in [{least}, {batch})")
-    return out
-
-
-def _batch(rho) -> int:
-    sizes = {r.shape[0] for r in rho if r is not None}
-    if len(sizes) > 1:
-        raise ValueError("the layers of a state have different batches")
-    return sizes.pop() if sizes else 0
 
 
 def copy_streams(state: StreamStates, dst: Sequence[int], src: Sequence[int], *,
@@ -75,39 +70,36 @@ def copy_streams(state: StreamStates, dst: Sequence[int], src: Sequence[int], *,
     positions."""
     if not supports_backend():
         return None
-    rho = _layers(state)
-    from_ = None if source is None or source is state else _layers(source)
-    if from_ is not None and all(a is b for a, b in zip(rho, from_)) and len(rho) == len(from_):
-        from_ = None
-    if from_ is not None:
+    rho, dst, src = _layers(state), [int(d) for d in dst], [int(s) for s in src]
+    slots = _Slots(rho)
+    other, batch = None, slots.batch
+    if source is not None and source is not state:
+        from_ = _layers(source)
         if len(from_) != len(rho):
             raise ValueError("the states have different numbers of layers")
-        if any((a is None) != (b is None) or (a is not None and (a.shape[1:] != b.shape[1:]
-               or a.device != b.device)) for a, b in zip(rho, from_)):
-            raise ValueError("the states' layers have different shapes or devices")
-        if (isinstance(state, BdhModelState) and isinstance(source, BdhModelState)
-                and any(s >= 0 for s in src) and state.position != source.position):
-            raise ValueError(f"the states are at positions {state.position} and {source.position}")
-    batch = _batch(rho)
-    dst = _slots(dst, batch, "dst")
-    src = _slots(src, batch if from_ is None else _batch(from_), "src", -1)
+        if any(a is not b for a, b in zip(rho, from_)):
+            other = _Slots(from_)
+            batch = other.batch
+            if any((a is None) != (b is None) or (a is not None and a.shape[1:] != b.shape[1:])
+                   for a, b in zip(rho, from_)) or other.device != slots.device:
+                raise ValueError("the states' layers have different shapes or devices")
+            if (isinstance(state, BdhModelState) and isinstance(source, BdhModelState)
+                    and state.position != source.position and any(s >= 0 for s in src)):
+                raise ValueError(f"the states are at positions {state.position} and {source.position}")
     if len(dst) != len(src):
         raise ValueError("dst and src have different lengths")
-    if len(set(dst)) != len(dst):
-        raise ValueError("a slot is written twice")
-    dev = next((r.device for r in rho if r is not None), None)
-    if dev is None or not dst:
-        return state
-    descs, ptrs = _arrays(rho)
-    src_descs, src_ptrs = _arrays(from_) if from_ is not None else (None, None)
+    _check_slots(dst, slots.batch, "dst")
+    _check_slots(src, batch, "src", -1)
     n = len(dst)
-    with _on_current_device(dev):
-        st = _lib.load().bdh_state_copy_streams(len(rho), descs, ptrs, src_descs, src_ptrs, n,
-                                                (ctypes.c_int32 * n)(*dst), (ctypes.c_int32 * n)(*src),
-                                                _stream_ptr(dev))
-    if not _lib.check(st):
-        return None
-    return state
+    if len(set(dst)) != n:
+        raise ValueError("a slot is written twice")
+    dev = slots.device
+    if dev is None or n == 0:
+        return state
+    st = _call_on(dev, _lib.load().bdh_state_copy_streams, len(rho), slots.descs, slots.ptrs,
+                  other.descs if other else None, other.ptrs if other else None, n,
+                  (ctypes.c_int32 * n)(*dst), (ctypes.c_int32 * n)(*src), _stream_ptr(dev))
+    return state if _lib.check(st) else None
 
 
 def free_streams(state: StreamStates, streams: Sequence[int]) -> Optional[StreamStates]:
@@ -125,8 +117,6 @@ def compact_streams(state: StreamStates, keep: Sequence[int]) -> Optional[Stream
     keep = list(keep)
     if len(keep) == 0:
         raise ValueError("keep names no stream")
-    if len(keep) > _batch(_layers(state)):
-        raise ValueError("keep has more streams than the state has slots")
     if copy_streams(state, range(len(keep)), keep) is None:
         return None
     rho = [r if r is None else r[:len(keep)] for r in _layers(state)]
