@@ -3,35 +3,35 @@
 // with A [n, R, D] and B [n, V, R] in bf16, base the shared projection's
 // output (the logits) and out = base where ids[b] names no adapter.
 //
-// hidden A^T goes to the stream's scratch first (u, R values a row), scaled.
-// All sums in f32.  Two forms, by the tokens of a sequence:
-//
-// Few (generation): a row's products are small and its adapter its own, so
-// what counts is that each adapter's B is read once.  u by one workgroup a
-// row in f32; then a workgroup takes a block of columns and up to kShare
-// sequences of one adapter, holds the block's rows of B in registers and runs
-// over the sequences' rows.  Bound by the bytes of B, base and out.
-//
-// Many (prompts): 16-row tiles of one sequence, so of one adapter, on the
-// matrix cores.  Their f32 operands go in as bf16 parts, each the rounded rest
-// of the ones before it: three parts are an f32 to 2^-24 of it, two to 2^-16.
-// f32 hidden and its u take three; bf16 hidden is one, and its u takes two
+// On the matrix cores in tiles of 16 rows of one adapter, sums in f32.  The f32
+// operands of a product go in as bf16 parts, each the rounded rest of the ones
+// before it: three parts are an f32 to 2^-24 of it, two to 2^-16.  f32 hidden
+// and u = scale hidden A^T take three; bf16 hidden is one, and its u takes two
 // (out rounds to 2^-8).  u's parts stand side by side, as one product of two or
-// three times the depth.  Bound by base and out.
+// three times the depth with the same columns of B.
+//
+// Rows of a tile: of prompts, 16 of one sequence; with up to 16 tokens a
+// sequence (generation), gathered from the sequences of one adapter, so that B
+// is read once for up to 16 rows.
+//
+// A workgroup holds its rows' u in LDS and runs over blocks of columns, bound by
+// base, out and B.  u comes from the workgroup itself (one launch: small calls
+// are launches and latency), or, where many workgroups would compute the same
+// u, from a launch of its own through the stream's scratch.
+#include <type_traits>
+
 #include "bdh_internal.h"
 
 namespace bdh {
 namespace {
 
-constexpr int kFewTokens = 16;   // below: the rows' form; from here on: tiles of 16 rows
-constexpr int kShare = 8;        // sequences of one adapter that a workgroup serves
-constexpr int kMaxRank = 128;
+constexpr int kTile = 16;
+constexpr int kGatherTokens = 16;  // up to here tiles gather sequences
+constexpr int kRowsTokens = 2, kRowsIn = 512;  // up to here, at ranks to 16, no tiles but adapter_rows_kernel
+constexpr int kRowsShare = 8;                  // the sequences it gathers
 
 typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
-typedef float f32x2_u __attribute__((ext_vector_type(2), aligned(4)));
 typedef __bf16 bf16x8_u __attribute__((ext_vector_type(8), aligned(2)));
-typedef __bf16 bf16x4_u __attribute__((ext_vector_type(4), aligned(2)));
-typedef __bf16 bf16x2_u __attribute__((ext_vector_type(2), aligned(2)));
 
 __device__ __forceinline__ int adapter_of(const AdapterArgs& a, int64_t b) {
   const int id = a.ids[b];
@@ -46,13 +46,25 @@ __device__ __forceinline__ bf16_t next_part(float& x) {
 }
 template <typename T> constexpr int hidden_parts = sizeof(T) == 4 ? 3 : 1;
 template <typename T> constexpr int u_parts = sizeof(T) == 4 ? 3 : 2;
+// A row of u: its parts of RP, zeros up to a multiple of the product's 32.
+template <typename T, int RP> constexpr int u_row = (u_parts<T> * RP + 31) / 32 * 32;
 
-// Eight values of a row of n from index k on, zeros past its end.
-template <typename T>
-__device__ __forceinline__ void load8(const T* row, int64_t k, int64_t n, float (&x)[8]);
-template <>
-__device__ __forceinline__ void load8<float>(const float* row, int64_t k, int64_t n, float (&x)[8]) {
-  if (k + 8 <= n) {
+// Eight values of a row of n from index k on (a multiple of 8), zeros past its
+// end.  EVEN: n is a multiple of 8 too.
+template <bool EVEN>
+__device__ __forceinline__ bf16x8 load8_bf16(const bf16_t* row, int64_t k, int64_t n) {
+  bf16x8_u v = {};
+  if (EVEN ? k < n : k + 8 <= n) {
+    v = *(const bf16x8_u*)(row + k);
+  } else if (!EVEN) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = k + j < n ? row[k + j] : (bf16_t)0.0f;
+  }
+  return __builtin_bit_cast(bf16x8, v);
+}
+template <bool EVEN>
+__device__ __forceinline__ void load8_f32(const float* row, int64_t k, int64_t n, float (&x)[8]) {
+  if (EVEN ? k < n : k + 8 <= n) {
     const f32x4_u p = *(const f32x4_u*)(row + k), q = *(const f32x4_u*)(row + k + 4);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -61,329 +73,475 @@ __device__ __forceinline__ void load8<float>(const float* row, int64_t k, int64_
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = k + j < n ? row[k + j] : 0.0f;
-  }
-}
-__device__ __forceinline__ bf16x8 load8_bf16(const bf16_t* row, int64_t k, int64_t n) {
-  bf16x8 v;
-  if (k + 8 <= n) {
-    const bf16x8_u p = *(const bf16x8_u*)(row + k);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = p[j];
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = k + j < n ? row[k + j] : (bf16_t)0.0f;
-  }
-  return v;
-}
-template <>
-__device__ __forceinline__ void load8<bf16_t>(const bf16_t* row, int64_t k, int64_t n, float (&x)[8]) {
-  const bf16x8 v = load8_bf16(row, k, n);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) x[j] = (float)v[j];
-}
-
-// --- few tokens ----------------------------------------------------------------
-// u[row, k] f32, k < rp (zeros past the rank).  One workgroup a row; a wave
-// takes every fourth k, its lanes eight columns of the dot product each.
-template <typename T>
-__global__ __launch_bounds__(256) void shrink_rows_kernel(const AdapterArgs a) {
-  const int64_t row = blockIdx.x;
-  const int id = adapter_of(a, row / a.time);
-  if (id < 0) return;
-  const T* h = (const T*)a.hidden + row * a.in_dim;
-  const bf16_t* w = a.a + (int64_t)id * a.rank * a.in_dim;
-  const float scale = a.scale[id];
-  const int lane = threadIdx.x & 63;
-  for (int k = threadIdx.x >> 6; k < a.rp; k += 4) {
-    float s = 0.0f;
-    if (k < a.rank) {
-      for (int64_t d = lane * 8; d < a.in_dim; d += 512) {
-        float x[8], y[8];
-        load8<T>(h, d, a.in_dim, x);
-        load8<bf16_t>(w + k * a.in_dim, d, a.in_dim, y);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s = fmaf(x[j], y[j], s);
-      }
-      s = wave_sum(s) * scale;
-    }
-    if (lane == 0) a.u[row * a.rp + k] = s;
+    for (int j = 0; j < 8; ++j) x[j] = !EVEN && k + j < n ? row[k + j] : 0.0f;
   }
 }
 
-template <typename T, int N> struct Cols;
-template <> struct Cols<float, 4> { typedef f32x4_u type; };
-template <> struct Cols<float, 2> { typedef f32x2_u type; };
-template <> struct Cols<bf16_t, 4> { typedef bf16x4_u type; };
-template <> struct Cols<bf16_t, 2> { typedef bf16x2_u type; };
-template <typename T> struct Cols<T, 1> { typedef T type __attribute__((ext_vector_type(1))); };
+// The rows of a workgroup: 16 * MT tokens of sequence b, or gathered.
+struct Rows {
+  int id;         // adapter, -1: none
+  int n;          // rows
+  int64_t first;  // in [batch, time]; GATHER: unused
+};
 
-template <typename T, int N>
-__device__ __forceinline__ void load_cols(const T* p, int n, float (&x)[N]) {
-  if (n == N) {
-    const typename Cols<T, N>::type v = *(const typename Cols<T, N>::type*)p;
-#pragma unroll
-    for (int j = 0; j < N; ++j) x[j] = (float)v[j];
-  } else {
-#pragma unroll
-    for (int j = 0; j < N; ++j) x[j] = j < n ? (float)p[j] : 0.0f;
+// The workgroups of a sequence that is the first of its adapter, or the first
+// after `share` more of it, gather that one and the next; the others have no
+// rows.  list: their rows.  Every wave for itself, without a barrier: all
+// write the same list.
+__device__ Rows gather_rows(const AdapterArgs& a, int b, int share, int* list) {
+  const int time = (int)a.time, lane = threadIdx.x & 63;
+  Rows g{adapter_of(a, b), 0, 0};
+  if (g.id < 0 && a.out == a.base) return g;
+  int before = 0, n = 0;
+  for (int i0 = 0; i0 < (int)a.batch && n < share; i0 += 64) {
+    const int i = i0 + lane;
+    const bool is = i < (int)a.batch && adapter_of(a, i) == g.id;
+    before += __popcll(__ballot(is && i < b));
+    const uint64_t from_b = __ballot(is && i >= b);
+    if (from_b != 0 && before % share != 0) return g;
+    const int at = n + __popcll(from_b & ((1ull << lane) - 1));
+    if (is && i >= b && at < share)
+      for (int t = 0; t < time; ++t) list[at * time + t] = i * time + t;
+    n += __popcll(from_b);
   }
-}
-template <typename T, int N>
-__device__ __forceinline__ void store_cols(T* p, int n, const float (&x)[N]) {
-  if (n == N) {
-    typename Cols<T, N>::type v;
-#pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = (T)x[j];
-    *(typename Cols<T, N>::type*)p = v;
-  } else {
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (j < n) p[j] = (T)x[j];
-  }
-}
-
-// out of a block of 256 * VPT columns for the sequences of one adapter: the
-// workgroups of a sequence that is the first of its adapter, or the first
-// after kShare more of it, serve that one and the next kShare - 1; the others
-// end at once.
-template <typename T, int RP, int VPT>
-__global__ __launch_bounds__(256) void expand_rows_kernel(const AdapterArgs a) {
-  __shared__ int served[kShare];
-  __shared__ int n_before, n_served;
-  const int64_t b = blockIdx.y;
-  const int id = adapter_of(a, b);
-  if (id < 0 && a.out == a.base) return;
-  if (threadIdx.x == 0) n_before = n_served = 0;
-  __syncthreads();
-  int before = 0;
-  for (int64_t i = threadIdx.x; i < b; i += 256) before += adapter_of(a, i) == id;
-  if (before) atomicAdd(&n_before, before);
-  __syncthreads();
-  if (n_before % kShare != 0) return;
-  // The first kShare sequences of this adapter from b on, in order: one wave.
-  if (threadIdx.x < 64) {
-    int n = 0;
-    for (int64_t i0 = b; i0 < a.batch && n < kShare; i0 += 64) {
-      const int64_t i = i0 + threadIdx.x;
-      const bool is = i < a.batch && adapter_of(a, i) == id;
-      const uint64_t all = __ballot(is);
-      const int at = n + __popcll(all & ((1ull << threadIdx.x) - 1));
-      if (is && at < kShare) served[at] = (int)i;
-      n += __popcll(all);
-    }
-    if (threadIdx.x == 0) n_served = n < kShare ? n : kShare;
-  }
-  __syncthreads();
-  const int64_t v = ((int64_t)blockIdx.x * 256 + threadIdx.x) * VPT;
-  if (v >= a.out_dim) return;
-  const int cols = a.out_dim - v < VPT ? (int)(a.out_dim - v) : VPT;
-  float w[VPT][RP];
-  if (id >= 0) {
-#pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-      const bf16_t* row = a.b + ((int64_t)id * a.out_dim + v + (j < cols ? j : 0)) * a.rank;
-#pragma unroll
-      for (int k = 0; k < RP; k += 8) {
-        float x[8];
-        load8<bf16_t>(row, k, a.rank, x);
-#pragma unroll
-        for (int q = 0; q < 8; ++q) w[j][k + q] = x[q];
-      }
-    }
-  }
-  const int n = n_served * (int)a.time;
-  for (int i = 0; i < n; ++i) {
-    const int s = i / (int)a.time;
-    const int64_t row = (int64_t)__builtin_amdgcn_readfirstlane(served[s]) * a.time + (i - s * (int)a.time);
-    const T* from = (const T*)a.base + row * a.out_dim + v;
-    float x[VPT];
-    load_cols<T, VPT>(from, cols, x);
-    if (id >= 0) {
-      const float* u = a.u + row * RP;
-#pragma unroll
-      for (int j = 0; j < VPT; ++j) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int k = 0; k < RP; ++k) sum = fmaf(u[k], w[j][k], sum);
-        x[j] += sum;
-      }
-    }
-    store_cols<T, VPT>((T*)a.out + row * a.out_dim + v, cols, x);
-  }
+  g.n = (n < share ? n : share) * time;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  return g;
 }
 
-// --- many tokens ---------------------------------------------------------------
-// The parts of u, [row][part][rp].  A workgroup takes 16 rows of one sequence,
-// its waves every fourth 32-deep step of the product.
-template <typename T, int RP>
-__global__ __launch_bounds__(256) void shrink_tile_kernel(const AdapterArgs a) {
-  constexpr int NT = RP / 16, HP = hidden_parts<T>, UP = u_parts<T>;
-  __shared__ float part[4][16][RP];
-  const int64_t b = blockIdx.y;
-  const int id = adapter_of(a, b);
-  if (id < 0) return;
-  const int64_t t0 = (int64_t)blockIdx.x * 16;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t t = t0 + (lane & 15) < a.time ? t0 + (lane & 15) : a.time - 1;
-  const T* h = (const T*)a.hidden + (b * a.time + t) * a.in_dim;
-  const bf16_t* w = a.a + (int64_t)id * a.rank * a.in_dim;
-  floatx4 acc[NT];
+// u of 16 * MT rows into LDS, by the four waves of the workgroup.
+template <typename T, int RP, int MT>
+struct UTile {
+  static constexpr int KS = 4 / MT;                 // waves that share a tile's product over D
+  static constexpr int ROWS = kTile * MT, DEPTH = u_parts<T> * RP, ROW = u_row<T, RP>;
+  static constexpr int PITCH = ROW + 8;             // (bank spread)
+  union Memory {
+    float part[KS][ROWS][RP];
+    bf16_t u[ROWS][PITCH];
+  };
+
+  template <bool EVEN, typename RowAt>
+  static __device__ __forceinline__ void compute(Memory& mem, const AdapterArgs& a, int id, const RowAt& row_at) {
+    constexpr int NT = RP / 16, HP = hidden_parts<T>, UP = u_parts<T>, PER = ROWS * RP / 256;
+    const int lane = threadIdx.x & 63, low = lane & 15, high = lane >> 4;
+    const int m = wave_id() % MT, ks = wave_id() / MT;
+    const T* h = (const T*)a.hidden + row_at(kTile * m + low) * a.in_dim;
+    const bf16_t* w = a.a + (int64_t)id * a.rank * a.in_dim;
+    floatx4 acc[NT];
 #pragma unroll
-  for (int j = 0; j < NT; ++j) acc[j] = zero4();
-  for (int64_t d0 = wave * 32; d0 < a.in_dim; d0 += 128) {
-    const int64_t d = d0 + 8 * (lane >> 4);
-    bf16x8 x[HP];
-    if constexpr (HP > 1) {
-      float f[8];
-      load8<float>((const float*)h, d, a.in_dim, f);
+    for (int j = 0; j < NT; ++j) acc[j] = zero4();
+    // AHEAD steps of 32 at a time: all their loads, then their products.  (One
+    // after the other, each step waited for memory: 2.4 us a step.)
+    constexpr int AHEAD = NT <= 4 ? 4 : 2;
+    for (int d0 = ks * 32; d0 < (int)a.in_dim; d0 += 32 * KS * AHEAD) {
+      bf16x8 y[AHEAD][NT], x[AHEAD];
+      float f[AHEAD][8];
 #pragma unroll
-      for (int q = 0; q < HP; ++q)
+      for (int i = 0; i < AHEAD; ++i) {
+        const int d = d0 + 32 * KS * i + 8 * high;
+        if constexpr (HP > 1) load8_f32<EVEN>((const float*)h, d, a.in_dim, f[i]);
+        else x[i] = load8_bf16<EVEN>((const bf16_t*)h, d, a.in_dim);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[q][j] = next_part(f[j]);
-    } else {
-      x[0] = load8_bf16((const bf16_t*)h, d, a.in_dim);
-    }
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const int k = j * 16 + (lane & 15);
-      bf16x8 y;
-      if (k < a.rank) {
-        y = load8_bf16(w + k * a.in_dim, d, a.in_dim);
-      } else {
-#pragma unroll
-        for (int q = 0; q < 8; ++q) y[q] = (bf16_t)0.0f;
+        for (int j = 0; j < NT; ++j) {
+          const int k = j * 16 + low;
+          y[i][j] = load8_bf16<EVEN>(w + (k < a.rank ? k : 0) * a.in_dim, d, a.in_dim);
+        }
       }
 #pragma unroll
-      for (int q = HP - 1; q >= 0; --q) acc[j] = mfma16(x[q], y, acc[j]);
-    }
-  }
+      for (int i = 0; i < AHEAD; ++i) {
+        bf16x8 p[HP];
+        if constexpr (HP > 1) {
 #pragma unroll
-  for (int j = 0; j < NT; ++j)
+          for (int q = 0; q < HP; ++q)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) part[wave][acc16_row(lane, r)][j * 16 + acc16_col(lane)] = acc[j][r];
-  __syncthreads();
-  const float scale = a.scale[id];
-  for (int i = threadIdx.x; i < 16 * RP; i += 256) {
-    const int r = i / RP, k = i % RP;
-    if (t0 + r >= a.time) break;
-    // (Past the rank: zeros, whatever hidden holds.)
-    float s = k < a.rank ? (part[0][r][k] + part[1][r][k] + part[2][r][k] + part[3][r][k]) * scale : 0.0f;
-    bf16_t* u = a.u_parts + (b * a.time + t0 + r) * (UP * RP) + k;
-#pragma unroll
-    for (int q = 0; q < UP; ++q) u[q * RP] = next_part(s);
-  }
-}
-
-// A wave's block: 64 rows of one sequence by 16 * NC columns.  Column
-// NC * c + j of the block is column c of product tile j, so a lane's results
-// of a row are NC neighbours.
-template <typename T, int RP, int NC>
-__global__ __launch_bounds__(256) void expand_tile_kernel(const AdapterArgs a) {
-  constexpr int MT = 4, DEPTH = u_parts<T> * RP;
-  const int64_t b = blockIdx.z;
-  const int id = adapter_of(a, b);
-  if (id < 0 && a.out == a.base) return;
-  const int lane = threadIdx.x & 63;
-  const int64_t t0 = (int64_t)blockIdx.x * (16 * MT);
-  const int64_t v0 = ((int64_t)blockIdx.y * 4 + wave_id()) * (16 * NC);
-  if (v0 >= a.out_dim) return;
-  floatx4 acc[MT][NC];
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int j = 0; j < NC; ++j) acc[m][j] = zero4();
-  if (id >= 0) {
-    const bf16_t* w = a.b + (int64_t)id * a.out_dim * a.rank;
-#pragma unroll
-    for (int s = 0; s < DEPTH; s += 32) {
-      // Eight-deep slice of this lane: each of u's parts meets the same columns
-      // of B.  (A depth of 48 ends half way through the last step: zeros.)
-      const int k = s + 8 * (lane >> 4);
-      const bool in = DEPTH % 32 == 0 || k < DEPTH;
-      bf16x8 y[NC];
-#pragma unroll
-      for (int j = 0; j < NC; ++j) {
-        const int64_t v = v0 + NC * (lane & 15) + j;
-        y[j] = load8_bf16(w + (v < a.out_dim ? v : a.out_dim - 1) * a.rank, in ? k % RP : RP, a.rank);
-      }
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const int64_t t = t0 + 16 * m + (lane & 15);
-        bf16x8 x = *(const bf16x8*)(a.u_parts + (b * a.time + (t < a.time ? t : a.time - 1)) * DEPTH + (in ? k : 0));
-        if (!in) {
-#pragma unroll
-          for (int q = 0; q < 8; ++q) x[q] = (bf16_t)0.0f;
+            for (int j = 0; j < 8; ++j) p[q][j] = next_part(f[i][j]);
+        } else {
+          p[0] = x[i];
         }
 #pragma unroll
-        for (int j = 0; j < NC; ++j) acc[m][j] = mfma16(x, y[j], acc[m][j]);
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int q = HP - 1; q >= 0; --q) acc[j] = mfma16(p[q], y[i][j], acc[j]);
       }
     }
-  }
-  const int64_t v = v0 + NC * (lane & 15);
-  if (v >= a.out_dim) return;
-  const int cols = a.out_dim - v < NC ? (int)(a.out_dim - v) : NC;
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int64_t t = t0 + 16 * m + acc16_row(lane, r);
-      if (t >= a.time) continue;
-      const int64_t at = (b * a.time + t) * a.out_dim + v;
-      float x[NC];
-      load_cols<T, NC>((const T*)a.base + at, cols, x);
+      for (int r = 0; r < 4; ++r) mem.part[ks][kTile * m + acc16_row(lane, r)][j * 16 + low] = acc[j][r];
+    __syncthreads();
+    const float scale = a.scale[id];
+    float s[PER];
 #pragma unroll
-      for (int j = 0; j < NC; ++j) x[j] += acc[m][j][r];
-      store_cols<T, NC>((T*)a.out + at, cols, x);
+    for (int i = 0; i < PER; ++i) {
+      const int at = threadIdx.x + 256 * i, r = at / RP, k = at % RP;
+      s[i] = mem.part[0][r][k];
+#pragma unroll
+      for (int q = 1; q < KS; ++q) s[i] += mem.part[q][r][k];
+      // (Past the rank: zeros, whatever hidden and the rows of A there are.)
+      s[i] = k < a.rank ? s[i] * scale : 0.0f;
     }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int at = threadIdx.x + 256 * i, r = at / RP, k = at % RP;
+#pragma unroll
+      for (int q = 0; q < UP; ++q) mem.u[r][q * RP + k] = next_part(s[i]);
+      if (ROW > DEPTH) mem.u[r][DEPTH + k] = (bf16_t)0.0f;
+    }
+    static_assert(ROW == DEPTH || ROW - DEPTH == RP, "one part of zeros");
+    __syncthreads();
+  }
+};
+
+// u of a tile of 16 rows to scratch [batch * time][u_row].
+template <typename T, int RP, bool EVEN, bool GATHER>
+__global__ __launch_bounds__(256) void adapter_u_kernel(const AdapterArgs a) {
+  typedef UTile<T, RP, 1> U;
+  __shared__ __attribute__((aligned(16))) typename U::Memory mem;
+  __shared__ int list[kTile];
+  Rows g;
+  if constexpr (GATHER) {
+    g = gather_rows(a, (int)blockIdx.y, kTile / (int)a.time, list);
+  } else {
+    const int64_t t0 = (int64_t)blockIdx.x * kTile;
+    g = Rows{adapter_of(a, blockIdx.y), (int)(a.time - t0 < kTile ? a.time - t0 : kTile), blockIdx.y * a.time + t0};
+  }
+  if (g.id < 0 || g.n == 0) return;
+  const auto row_at = [&](int r) -> int64_t {
+    r = r < g.n ? r : g.n - 1;
+    return GATHER ? (int64_t)list[r] : g.first + r;
+  };
+  U::template compute<EVEN>(mem, a, g.id, row_at);
+  for (int i = threadIdx.x; i < g.n * (U::ROW / 8); i += 256) {
+    const int r = i / (U::ROW / 8), k = i % (U::ROW / 8) * 8;
+    *(bf16x8*)(a.u + row_at(r) * U::ROW + k) = *(const bf16x8*)&mem.u[r][k];
+  }
 }
 
-int padded_rank(int64_t r) { return r <= 16 ? 16 : r <= 32 ? 32 : r <= 64 ? 64 : 128; }
+template <typename T> struct Cols;  // a lane's neighbouring columns: 16 bytes at any element's address
+template <> struct Cols<float> { typedef f32x4_u type; };
+template <> struct Cols<bf16_t> { typedef bf16x8_u type; };
+template <typename T> constexpr int kCols = 16 / sizeof(T);
+template <typename T> constexpr int kWide = 4 * 16 * kCols<T>;  // columns of a workgroup's four blocks
 
-template <typename T, int RP>
-bdh_status run_typed(AdapterArgs a, hipStream_t st, uint64_t* launches) {
-  const int64_t rows = a.batch * a.time;
-  void* u = nullptr;
-  const size_t bytes = (size_t)rows * RP * (a.time < kFewTokens ? sizeof(float) : u_parts<T> * sizeof(bf16_t));
-  const bdh_status s = scratch(st, SLOT_ADAPTER, bytes, &u);
-  if (s != BDH_OK) return s;
-  a.u = (float*)u;
-  a.u_parts = (bf16_t*)u;
-  a.rp = RP;
-  if (a.time < kFewTokens) {
-    constexpr int VPT = RP <= 16 ? 4 : RP <= 32 ? 2 : 1;
-    hipLaunchKernelGGL((shrink_rows_kernel<T>), dim3((uint32_t)rows), dim3(256), 0, st, a);
-    hipLaunchKernelGGL((expand_rows_kernel<T, RP, VPT>),
-                       dim3((uint32_t)((a.out_dim + 256 * VPT - 1) / (256 * VPT)), (uint32_t)a.batch), dim3(256), 0,
-                       st, a);
+// 16 * MT rows by every gridDim.x-th run of kWide columns, the waves side by
+// side on its blocks of 16 * kCols (of a row 1 KB in one go), so that the
+// workgroups that run together cover neighbouring runs.  A wave takes a block's
+// rows of B into registers and runs over the row tiles: u from LDS, base one
+// tile ahead.  OWN: computes u itself.
+template <typename T, int RP, int MT, bool EVEN, bool GATHER, bool OWN>
+__global__ __launch_bounds__(256, RP <= 64 ? 2 : 1) void adapter_out_kernel(const AdapterArgs a) {
+  typedef UTile<T, RP, MT> U;
+  typedef typename Cols<T>::type Vec;
+  constexpr int NC = kCols<T>, BLOCK = 16 * NC;
+  constexpr int YS = RP >= 32 ? RP / 32 : 1;  // 32-deep slices of B's rows
+  __shared__ __attribute__((aligned(16))) typename U::Memory mem;
+  __shared__ int list[kTile];
+  Rows g;
+  if constexpr (GATHER) {
+    g = gather_rows(a, (int)blockIdx.z, kTile / (int)a.time, list);
   } else {
-    constexpr int NC = 4;
-    hipLaunchKernelGGL((shrink_tile_kernel<T, RP>), dim3((uint32_t)((a.time + 15) / 16), (uint32_t)a.batch),
-                       dim3(256), 0, st, a);
-    hipLaunchKernelGGL((expand_tile_kernel<T, RP, NC>),
-                       dim3((uint32_t)((a.time + 63) / 64), (uint32_t)((a.out_dim + 64 * NC - 1) / (64 * NC)),
-                            (uint32_t)a.batch),
-                       dim3(256), 0, st, a);
+    const int64_t t0 = (int64_t)blockIdx.y * U::ROWS;
+    g = Rows{adapter_of(a, blockIdx.z), (int)(a.time - t0 < U::ROWS ? a.time - t0 : U::ROWS), blockIdx.z * a.time + t0};
+    if (g.id < 0 && a.out == a.base) return;
+  }
+  if (g.n == 0) return;
+  const int id = g.id, last = g.n - 1, tiles = (g.n + kTile - 1) / kTile;
+  const auto row_at = [&](int r) -> int64_t {
+    r = r < last ? r : last;
+    return GATHER ? (int64_t)list[r] : g.first + r;
+  };
+  const int lane = threadIdx.x & 63, low = lane & 15, high = lane >> 4;
+  const int v_end = (int)a.out_dim;
+  const bf16_t* w = a.b + (int64_t)(id >= 0 ? id : 0) * a.out_dim * a.rank;
+  const auto load_base = [&](auto full, int v, int m, Vec (&x)[4]) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = kTile * m + 4 * high + r;
+      if (GATHER && row > last) continue;
+      const T* from = (const T*)a.base + row_at(row) * a.out_dim + v;
+      if (full) {
+        x[r] = *(const Vec*)from;
+      } else {
+#pragma unroll
+        for (int j = 0; j < NC; ++j) x[r][j] = v + j < v_end ? from[j] : (T)0.0f;
+      }
+    }
+  };
+  const auto load_b = [&](auto full, int v, bf16x8 (&y)[YS][NC]) {
+#pragma unroll
+    for (int s = 0; s < YS; ++s) {
+      // This lane's eight-deep slice: each of u's parts meets the same columns of B.
+      const int kb = (32 * s + 8 * high) % RP;
+#pragma unroll
+      for (int j = 0; j < NC; ++j)
+        y[s][j] = load8_bf16<EVEN>(w + (uint32_t)((full || v + j < v_end ? v + j : v_end - 1) * (int)a.rank), kb,
+                                   a.rank);
+    }
+  };
+  const auto product = [&](const bf16x8 (&y)[YS][NC], int m, floatx4 (&acc)[NC]) {
+#pragma unroll
+    for (int j = 0; j < NC; ++j) acc[j] = zero4();
+    if (id < 0) return;
+#pragma unroll
+    for (int k = U::ROW - 32; k >= 0; k -= 32) {  // the smaller parts first
+      const bf16x8 f = *(const bf16x8*)&mem.u[kTile * m + low][k + 8 * high];
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+        // (Rank 16: a step holds two parts, the last of three one and zeros,
+        // which are not to meet an infinity.)
+        const bf16x8 z = {};
+        const bool in = k + 32 <= U::DEPTH || k + 8 * high < U::DEPTH;
+        acc[j] = mfma16(f, in ? y[k / 32 % YS][j] : z, acc[j]);
+      }
+    }
+  };
+  const auto store = [&](auto full, int v, int m, const Vec (&x)[4], const floatx4 (&acc)[NC]) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = kTile * m + 4 * high + r;
+      if (row > last) continue;
+      T* to = (T*)a.out + row_at(row) * a.out_dim + v;
+      Vec o;
+#pragma unroll
+      for (int j = 0; j < NC; ++j) o[j] = (T)((float)x[r][j] + acc[j][r]);
+      if (full) {
+        *(Vec*)to = o;
+      } else {
+#pragma unroll
+        for (int j = 0; j < NC; ++j)
+          if (v + j < v_end) to[j] = o[j];
+      }
+    }
+  };
+  // Column NC * c + j of a block is column c of product tile j, so a lane's
+  // results of a row are NC neighbours: 16 bytes.  The first block's B and base
+  // are asked for ahead of u, base then comes one tile ahead.
+  const int stride = (int)gridDim.x * kWide<T>;
+  int v0 = (int)blockIdx.x * kWide<T> + wave_id() * BLOCK;
+  Vec x[2][4];
+  bf16x8 y[YS][NC];
+  if (v0 + BLOCK <= v_end) {
+    load_base(std::true_type{}, v0 + NC * low, 0, x[0]);
+    if (id >= 0) load_b(std::true_type{}, v0 + NC * low, y);
+  }
+  if (id >= 0) {
+    if constexpr (OWN) {
+      U::template compute<EVEN>(mem, a, id, row_at);
+    } else {
+      for (int i = threadIdx.x; i < tiles * kTile * (U::ROW / 8); i += 256) {
+        const int r = i / (U::ROW / 8), k = i % (U::ROW / 8) * 8;
+        *(bf16x8*)&mem.u[r][k] = *(const bf16x8*)(a.u + row_at(r) * U::ROW + k);
+      }
+      __syncthreads();
+    }
+  }
+  for (bool first = true; v0 + BLOCK <= v_end; v0 += stride, first = false) {
+    const int v = v0 + NC * low;
+    const bool more = v0 + stride + BLOCK <= v_end;
+    if (id >= 0 && !first) load_b(std::true_type{}, v, y);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      if (m >= tiles) break;
+      if (m + 1 < tiles) load_base(std::true_type{}, v, m + 1, x[(m + 1) & 1]);
+      else if (more && (m & 1)) load_base(std::true_type{}, v + stride, 0, x[0]);
+      floatx4 acc[NC];
+      product(y, m, acc);
+      store(std::true_type{}, v, m, x[m & 1], acc);
+      if (m + 1 == tiles && more && !(m & 1)) load_base(std::true_type{}, v + stride, 0, x[0]);
+    }
+  }
+  if (v0 >= v_end) return;
+  // The rows' last columns, fewer than a block.
+  const int v = v0 + NC * low;
+  if (id >= 0) load_b(std::false_type{}, v, y);
+  for (int m = 0; m < tiles; ++m) {
+    load_base(std::false_type{}, v, m, x[0]);
+    floatx4 acc[NC];
+    product(y, m, acc);
+    store(std::false_type{}, v, m, x[0], acc);
+  }
+}
+
+// --- few rows of a small model --------------------------------------------------
+// Sum over 16 neighbouring lanes, in the last of them.
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float sum16(float v) {
+  return add_dpp<0x118>(add_dpp<0x114>(add_dpp<0x112>(add_dpp<0x111>(v))));
+}
+
+// Gathered rows at ranks to 16 without matrix cores, u computed here: a thread
+// holds four columns' rows of B and runs over the rows.  A tile of the product
+// would be mostly empty, and what counts is how much a workgroup asks for at
+// once: of 64 rows with 32 adapters (D 256, V 32000, R 16) 12.5 us where the
+// tiles take 23.6 (at rank 32 and D 512 36 where they take 25).
+template <typename T>
+__global__ __launch_bounds__(256) void adapter_rows_kernel(const AdapterArgs a) {
+  constexpr int RP = 16, VPT = 4;
+  __shared__ float u[kRowsShare * kRowsTokens][RP];
+  __shared__ int list[kRowsShare * kRowsTokens];
+  const Rows g = gather_rows(a, (int)blockIdx.y, kRowsShare, list);
+  if (g.n == 0) return;
+  const int id = g.id, n = g.n, v_end = (int)a.out_dim;
+  // A thread's columns lie 256 apart: a wave's accesses are runs of neighbours.
+  const int v = (int)blockIdx.x * (256 * VPT) + threadIdx.x;
+  float w[VPT][RP];
+  if (id >= 0) {
+    // 16 lanes a rank, eight columns of the dot products each; four rows at a time.
+    const int lane = threadIdx.x & 15, k = threadIdx.x >> 4;
+    const float scale = a.scale[id];
+    const bf16_t* wa = a.a + ((int64_t)id * a.rank + (k < a.rank ? k : 0)) * a.in_dim;
+    for (int i0 = 0; i0 < n; i0 += 4) {
+      float sum[4] = {};
+      const T* h[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        h[q] = (const T*)a.hidden + (int64_t)__builtin_amdgcn_readfirstlane(list[i0 + q < n ? i0 + q : i0]) * a.in_dim;
+#pragma unroll 2
+      for (int d = lane * 8; d < (int)a.in_dim; d += 128) {
+        const bf16x8 y = load8_bf16<true>(wa, d, a.in_dim);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float x[8];
+          if constexpr (sizeof(T) == 4) {
+            load8_f32<true>((const float*)h[q], d, a.in_dim, x);
+          } else {
+            const bf16x8 p = load8_bf16<true>((const bf16_t*)h[q], d, a.in_dim);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = (float)p[j];
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) sum[q] = fmaf(x[j], (float)y[j], sum[q]);
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float s = sum16(sum[q]) * scale;
+        // (Past the rank: zeros, whatever hidden and the rows of A there are.)
+        if (lane == 15 && i0 + q < n) u[i0 + q][k] = k < a.rank ? s : 0.0f;
+      }
+    }
+    __syncthreads();
+    bf16x8 wb[VPT][RP / 8];
+    const bf16_t* from = a.b + (int64_t)id * a.out_dim * a.rank;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j)
+#pragma unroll
+      for (int k = 0; k < RP; k += 8)
+        wb[j][k / 8] = load8_bf16<true>(from + (uint32_t)((v + 256 * j < v_end ? v + 256 * j : v_end - 1) * (int)a.rank),
+                                        k, a.rank);
+#pragma unroll
+    for (int j = 0; j < VPT; ++j)
+#pragma unroll
+      for (int q = 0; q < RP; ++q) w[j][q] = (float)wb[j][q / 8][q % 8];
+  }
+  // Four rows' base values at a time, ahead of the stores.
+  for (int i0 = 0; i0 < n; i0 += 4) {
+    float x[4][VPT];
+    int64_t at[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      at[q] = (int64_t)__builtin_amdgcn_readfirstlane(list[i0 + q < n ? i0 + q : i0]) * a.out_dim + v;
+#pragma unroll
+      for (int j = 0; j < VPT; ++j) x[q][j] = v + 256 * j < v_end ? (float)((const T*)a.base)[at[q] + 256 * j] : 0.0f;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (i0 + q >= n) break;
+      if (id >= 0) {
+        float sum[VPT] = {};
+#pragma unroll
+        for (int k = 0; k < RP; ++k) {
+          const float uk = u[i0 + q][k];
+#pragma unroll
+          for (int j = 0; j < VPT; ++j) sum[j] = fmaf(uk, w[j][k], sum[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) x[q][j] += sum[j];
+      }
+#pragma unroll
+      for (int j = 0; j < VPT; ++j)
+        if (v + 256 * j < v_end) ((T*)a.out)[at[q] + 256 * j] = (T)x[q][j];
+    }
+  }
+}
+
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+template <typename T, int RP, int MT, bool EVEN, bool GATHER, bool OWN>
+void launch_out(const AdapterArgs& a, int64_t runs, hipStream_t st) {
+  const dim3 grid((uint32_t)runs, GATHER ? 1u : (uint32_t)cdiv(a.time, kTile * MT), (uint32_t)a.batch);
+  hipLaunchKernelGGL((adapter_out_kernel<T, RP, MT, EVEN, GATHER, OWN>), grid, dim3(256), 0, st, a);
+}
+
+template <typename T, int RP, bool EVEN>
+bdh_status run_typed(AdapterArgs a, hipStream_t st, uint64_t* launches) {
+  const bool gather = a.time <= kGatherTokens;
+  if constexpr (EVEN && RP == 16) {
+    if (a.time <= kRowsTokens && a.in_dim <= kRowsIn) {
+      hipLaunchKernelGGL((adapter_rows_kernel<T>), dim3((uint32_t)cdiv(a.out_dim, 1024), (uint32_t)a.batch), dim3(256),
+                         0, st, a);
+      BDH_HIP_TRY(hipGetLastError());
+      *launches += 1;
+      return BDH_OK;
+    }
+  }
+  // Workgroups along the columns: 2048 in all where there are columns enough
+  // (gathered, whose workgroups mostly end at once, 8192).  A run's remainder
+  // gets a workgroup of its own only where the chip has room: of 257 columns
+  // the last one cost a second pass over hidden (18.5 us, now 14.2, at 16
+  // prompts of 1024).
+  const auto runs_of = [&](int64_t tiles) {
+    const int64_t whole = a.out_dim / kWide<T>, want = cdiv(gather ? 8192 : 2048, tiles);
+    const int64_t wide = whole * tiles >= 256 ? whole : cdiv(a.out_dim, kWide<T>);
+    return want < wide ? want : wide;
+  };
+  // Each workgroup that computes u itself spends about D / 128 us on it, of
+  // which the chip runs some 512 at a time; a launch of its own costs about 4.
+  const int64_t own_tiles = gather ? a.batch : a.batch * cdiv(a.time, 2 * kTile);
+  if (EVEN && own_tiles * runs_of(own_tiles) * a.in_dim <= (int64_t)1 << 18) {
+    if constexpr (EVEN) {
+      if (gather) launch_out<T, RP, 1, true, true, true>(a, runs_of(own_tiles), st);
+      else launch_out<T, RP, 2, true, false, true>(a, runs_of(own_tiles), st);
+    }
+    BDH_HIP_TRY(hipGetLastError());
+    *launches += 1;
+    return BDH_OK;
+  }
+  void* u = nullptr;
+  const bdh_status s = scratch(st, SLOT_ADAPTER, (size_t)(a.batch * a.time) * u_row<T, RP> * sizeof(bf16_t), &u);
+  if (s != BDH_OK) return s;
+  a.u = (bf16_t*)u;
+  const dim3 u_grid(gather ? 1u : (uint32_t)cdiv(a.time, kTile), (uint32_t)a.batch);
+  if (gather) {
+    hipLaunchKernelGGL((adapter_u_kernel<T, RP, EVEN, true>), u_grid, dim3(256), 0, st, a);
+    launch_out<T, RP, 1, EVEN, true, false>(a, runs_of(a.batch), st);
+  } else {
+    hipLaunchKernelGGL((adapter_u_kernel<T, RP, EVEN, false>), u_grid, dim3(256), 0, st, a);
+    launch_out<T, RP, 4, EVEN, false, false>(a, runs_of(a.batch * cdiv(a.time, 4 * kTile)), st);
   }
   BDH_HIP_TRY(hipGetLastError());
   *launches += 2;
   return BDH_OK;
 }
 
-template <typename T>
+template <typename T, bool EVEN>
 bdh_status run_ranked(const AdapterArgs& a, hipStream_t st, uint64_t* launches) {
-  switch (padded_rank(a.rank)) {
-    case 16: return run_typed<T, 16>(a, st, launches);
-    case 32: return run_typed<T, 32>(a, st, launches);
-    case 64: return run_typed<T, 64>(a, st, launches);
-    default: return run_typed<T, 128>(a, st, launches);
-  }
+  if (a.rank <= 16) return run_typed<T, 16, EVEN>(a, st, launches);
+  if (a.rank <= 32) return run_typed<T, 32, EVEN>(a, st, launches);
+  if (a.rank <= 64) return run_typed<T, 64, EVEN>(a, st, launches);
+  return run_typed<T, 128, EVEN>(a, st, launches);
 }
 
 }  // namespace
 
 bdh_status apply_adapters(const AdapterArgs& a, hipStream_t st, uint64_t* launches) {
-  return a.bf16 ? run_ranked<bf16_t>(a, st, launches) : run_ranked<float>(a, st, launches);
+  if (a.rank % 8 == 0 && a.in_dim % 8 == 0)
+    return a.bf16 ? run_ranked<bf16_t, true>(a, st, launches) : run_ranked<float, true>(a, st, launches);
+  return a.bf16 ? run_ranked<bf16_t, false>(a, st, launches) : run_ranked<float, false>(a, st, launches);
 }
 
 }  // namespace bdh

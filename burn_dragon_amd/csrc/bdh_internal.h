@@ -49,7 +49,7 @@ enum ScratchSlot {
   SLOT_VJP_GAMMA,    // VJP state gradients          2 x [S, N, D] f32
   SLOT_SNAP,         // states at interval starts: bf16 path [n_iv, S, D, N] bf16, fp32 path [n_iv - 1, S, N, D] f32
   SLOT_SAMPLE,       // sampling of long rows: chunks' histograms, candidates (sample.hip)
-  SLOT_ADAPTER,      // adapters: hidden A^T  [rows, padded rank] f32, or as bf16 parts
+  SLOT_ADAPTER,      // adapters: the parts of scale hidden A^T  [rows, parts of the padded rank] bf16
   SLOT_COUNT
 };
 // Scratch of the calling stream (see api.hip): grows on first use of a
@@ -176,10 +176,7 @@ struct AdapterArgs {
   const float* scale;   // [n]
   const int32_t* ids;   // [batch]
   void* out;            // [batch, time, out_dim], may be base
-  // Scratch, set by apply_adapters.
-  float* u;
-  bf16_t* u_parts;
-  int rp;
+  bf16_t* u = nullptr;  // scratch, set by apply_adapters
 };
 bdh_status apply_adapters(const AdapterArgs& a, hipStream_t st, uint64_t* launches);
 
