@@ -26,7 +26,9 @@
 //      wave, the stripe, the lane and the element that it falls in.
 //
 // Rows up to 16384 logits: one workgroup, the row in registers, read once.
-// Longer ones in chunks of 8192, four launches (sample_chunk_kernel on).
+// Longer ones in chunks of 8192, four launches (sample_chunk_kernel on).  Where
+// top-k keeps few, the first launch already leaves all that can be drawn in
+// lists, and the last works on those alone.
 #include "bdh_internal.h"
 
 namespace bdh {
@@ -38,6 +40,7 @@ constexpr double kLeastT = -42.0;
 constexpr int kSmall = 64;       // candidates that one wave orders
 constexpr int kMid = 256;        // that the workgroup compares each with each
 constexpr int kListMax = 4096;   // candidates that the list holds
+constexpr int kNear = 256;       // logits that a chunk lists for top-k
 constexpr int kChunkThreads = 512;
 constexpr int kChunkPer = 16;    // logits a thread
 constexpr int kChunk = kChunkThreads * kChunkPer;
@@ -182,7 +185,7 @@ template <int NT, int LIST>
 struct Shared {
   uint64_t mass[kBins];
   uint64_t list[LIST];
-  uint64_t small[kSmall], small_w[kMid];
+  uint64_t small[kSmall], small_w[kMid], kept[kMid];
   uint64_t wave_sum[NT / 64];
   uint64_t lo, hi, sum;  // of a pass over the candidates
   uint32_t cnt[kBins];
@@ -329,20 +332,22 @@ __device__ __forceinline__ Cuts no_cuts() {
   return q;
 }
 // One wave each.
-__device__ __forceinline__ void find_k(const Row& s, const uint32_t* cnt, Cuts& q) {
+// (Returns the logits up to k_bin.)
+__device__ __forceinline__ uint64_t find_k(const Row& s, const uint32_t* cnt, Cuts& q) {
   uint64_t in;
   q.k_bin = BinScan(cnt, kBins).cross((uint64_t)s.k, &q.k_above, &in);
+  return q.k_above + in;
 }
 // Counts a chunk's logits by bin into cnt (cleared) and finds its k-th.
 template <int NT, int E>
-__device__ __forceinline__ void count_for_k(const Row& s, const float (&x)[E], float top, uint32_t* cnt, Cuts& q) {
+__device__ __forceinline__ uint64_t count_for_k(const Row& s, const float (&x)[E], float top, uint32_t* cnt, Cuts& q) {
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int b = bin_of(x[e], top, s.cb);
     if (b < kBins) atomicAdd(&cnt[b], 1u);
   }
   __syncthreads();
-  find_k(s, cnt, q);
+  return find_k(s, cnt, q);
 }
 __device__ __forceinline__ void find_p(const Row& s, const uint64_t* mass, Cuts& q) {
   // What top-k keeps weighs between all before k_bin, and that with k_bin.
@@ -362,6 +367,12 @@ __device__ __forceinline__ void find_least(const Row& s, float m, float top, Cut
   if (!(bin - off < (float)kBins)) return;
   q.m_first = (int)fmaxf(bin - off, 0.0f);
   q.m_last = (int)fminf(bin + off, (float)(kBins - 1));
+}
+// The cuts of a list that holds all that can be kept: each may fall anywhere.
+__device__ __forceinline__ Cuts cuts_anywhere() {
+  Cuts q = no_cuts();
+  q.k_bin = q.p_first = -1;
+  return q;
 }
 // Bins before this are kept whole.
 __device__ __forceinline__ int sure_bins(const Cuts& q) { return min(min(q.k_bin, q.p_first), q.m_first); }
@@ -487,7 +498,7 @@ struct Candidates {
     const uint64_t mine = lane < n ? sh.list[lane] : ~0ull;
     const int bin = lane < n ? bin_of(value_of(mine), top, s.cb) : kBins;
     const uint64_t w = s.use_p && lane < n ? weight(mine, kLeastT) : 0;
-    const bool in_k = lane < n && bin == q.k_bin, in_p = bin >= q.p_first && bin <= q.p_last;
+    const bool in_k = lane < n && bin >= q.k_bin, in_p = bin >= q.p_first && bin <= q.p_last;
     const uint64_t wp = in_p ? w : 0;
     uint64_t k_before = q.k_above, p_before = q.p_above;
     for (int j = 0; j < n; ++j) {
@@ -518,7 +529,7 @@ struct Candidates {
       k_before[c] = q.k_above;
       p_before[c] = q.p_above;
       if (i < n)
-        sh.small_w[i] = (bin[c] >= q.p_first && bin[c] <= q.p_last ? w[c] : 0) | (bin[c] == q.k_bin ? in_k_bit : 0);
+        sh.small_w[i] = (bin[c] >= q.p_first && bin[c] <= q.p_last ? w[c] : 0) | (bin[c] >= q.k_bin ? in_k_bit : 0);
     }
     if (threadIdx.x == 0) sh.sum = sh.hi = 0;
     __syncthreads();
@@ -538,7 +549,7 @@ struct Candidates {
     for (int c = 0; c < PER; ++c) {
       const bool real = threadIdx.x + c * NT < n;
       const bool kept = real && (bin[c] < q.k_bin || k_before[c] < (uint64_t)s.k);
-      if (s.use_p && kept && bin[c] == q.k_bin) atomicAdd((unsigned long long*)&sh.sum, (unsigned long long)w[c]);
+      if (s.use_p && kept && bin[c] >= q.k_bin) atomicAdd((unsigned long long*)&sh.sum, (unsigned long long)w[c]);
       if (!kept) mine[c] = 0;
     }
     __syncthreads();
@@ -751,6 +762,7 @@ struct RowState {
   float top;
   float m;
   int n_list;
+  bool near;  // the chunks' `near` holds all that can be drawn
 };
 struct SplitArgs {
   SampleArgs a;
@@ -760,6 +772,8 @@ struct SplitArgs {
   int32_t* arg;      // [rows, chunks]: the first index of the chunk's largest
   uint32_t* cnt;     // [rows, chunks, kBins], bins counted from the chunk's own largest
   uint64_t* mass;    // [rows, chunks, kBins], weights relative to it
+  int32_t* near_n;   // [rows, chunks]: logits in `near`, -1: they are not all there
+  uint64_t* near;    // [rows, chunks, kNear]: the logits up to the bin of the chunk's k-th
   uint64_t* sure;    // [rows, chunks]
   uint64_t* list;    // [rows, kListMax]
   RowState* state;   // [rows]
@@ -772,7 +786,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_chunk_kernel(const Split
   __shared__ uint64_t mass[kBins];
   __shared__ uint32_t cnt[kBins];
   __shared__ float part[NT / 64];
-  __shared__ int arg;
+  __shared__ int arg, n_near;
   const int64_t lr = blockIdx.y, r = p.row0 + lr;
   const int64_t slot = lr * p.chunks + blockIdx.x;
   const T* row = (const T*)p.a.logits + r * p.a.row_stride;
@@ -789,7 +803,11 @@ __global__ __launch_bounds__(kChunkThreads) void sample_chunk_kernel(const Split
 #pragma unroll
   for (int e = 1; e < E; ++e) best = fmaxf(best, x[e]);
   const float m = block_max<NT>(best, part);
-  if (threadIdx.x == 0) p.max[slot] = m;
+  if (threadIdx.x == 0) {
+    p.max[slot] = m;
+    p.near_n[slot] = s.use_k && s.k <= kNear && !is_real(m) ? 0 : -1;
+    n_near = 0;
+  }
   if (!is_real(m)) return;
   if (s.greedy) {
 #pragma unroll
@@ -803,7 +821,16 @@ __global__ __launch_bounds__(kChunkThreads) void sample_chunk_kernel(const Split
   Cuts q = no_cuts();
   if (s.use_k) {
     // Past the chunk's own k-th no logit is among the row's first k.
-    count_for_k<NT, E>(s, x, top, cnt, q);
+    const uint64_t n = count_for_k<NT, E>(s, x, top, cnt, q);
+    if (n <= kNear && s.k <= kNear) {
+      if (threadIdx.x == 0) p.near_n[slot] = (int)n;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int b = bin_of(x[e], top, s.cb);
+        const int at = append_at(&n_near, b < kBins && b <= q.k_bin);
+        if (at >= 0) p.near[slot * kNear + at] = order_of(x[e], index_of<E>(base, e));
+      }
+    }
     for (int b = threadIdx.x; b < kBins; b += NT) p.cnt[slot * kBins + b] = cnt[b];
   }
   // What lies below the least kept t from here lies further below it from the
@@ -829,14 +856,23 @@ __global__ __launch_bounds__(kBins) void sample_merge_kernel(const SplitArgs p) 
   __shared__ double scale[kMaxChunks];  // of a chunk's weights to the row's
   __shared__ int shift[kMaxChunks];     // of its bins; kBins: none of them is drawn
   __shared__ float part[kBins / 64];
+  __shared__ int n_near, away;
   const int64_t lr = blockIdx.x, r = p.row0 + lr;
   const Row s = row_settings(p.a, r);
+  if (threadIdx.x == 0) n_near = away = 0;
+  __syncthreads();
   float mine = -INFINITY;
-  for (int g = threadIdx.x; g < p.chunks; g += kBins) mine = fmaxf(mine, p.max[lr * p.chunks + g]);
-  const float m = block_max<kBins>(mine, part);
+  for (int g = threadIdx.x; g < p.chunks; g += kBins) {
+    mine = fmaxf(mine, p.max[lr * p.chunks + g]);
+    const int n = p.near_n[lr * p.chunks + g];
+    if (n < 0) away = 1;
+    else atomicAdd(&n_near, n);
+  }
+  const float m = block_max<kBins>(mine, part);  // (waits for all)
+  const bool near = !away && n_near <= kListMax;
   const float top = grid_of(m, s.cb);
   Cuts q = no_cuts();
-  if (is_real(m) && !s.greedy) {
+  if (is_real(m) && !s.greedy && !near) {
     for (int g = threadIdx.x; g < p.chunks; g += kBins) {
       const float mg = p.max[lr * p.chunks + g], by = top - grid_of(mg, s.cb);
       shift[g] = is_real(mg) && by < (float)kBins ? (int)by : kBins;
@@ -862,7 +898,7 @@ __global__ __launch_bounds__(kBins) void sample_merge_kernel(const SplitArgs p) 
     }
     find_least(s, m, top, q);
   }
-  if (threadIdx.x == 0) p.state[lr] = RowState{q, top, m, 0};
+  if (threadIdx.x == 0) p.state[lr] = RowState{q, top, m, 0, near};
 }
 
 // 3. From a chunk's histogram the weight that is kept whatever happens in the
@@ -879,7 +915,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_gather_kernel(const Spli
   const Row s = row_settings(p.a, r);
   RowState* st = p.state + lr;
   const float m = st->m, top = st->top, mg = p.max[slot];
-  if (s.greedy || !is_real(m)) return;
+  if (s.greedy || !is_real(m) || st->near) return;
   const Cuts q = st->cuts;
   if (threadIdx.x == 0) n_here = some = 0;
   __syncthreads();
@@ -926,6 +962,87 @@ __global__ __launch_bounds__(kChunkThreads) void sample_gather_kernel(const Spli
   }
 }
 
+// The draw from a list (sh.list, n of them) of all that can be kept.
+template <typename T, int NT, int LIST>
+__device__ void draw_from_list(Shared<NT, LIST>& sh, const SampleArgs& a, const Row& s, int64_t r, float m, float top,
+                               int n) {
+  static_assert(kNear <= kMid && kMid <= NT, "a thread a kept logit");
+  constexpr int PER = LIST / NT;
+  uint64_t o[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) o[j] = threadIdx.x + j * NT < n ? sh.list[threadIdx.x + j * NT] : ~0ull;
+  Cuts q = cuts_anywhere();
+  int n_cut = n;
+  if (n > kSmall) {
+    // As of a row: the bins of the cuts, and their candidates alone to the list.
+    for (int b = threadIdx.x; b < kBins; b += NT) {
+      sh.cnt[b] = 0;
+      sh.mass[b] = 0;
+    }
+    if (threadIdx.x == 0) sh.n_list = 0;
+    __syncthreads();
+    q = no_cuts();
+    int bin[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      bin[j] = o[j] != ~0ull ? bin_of(value_of(o[j]), top, s.cb) : kBins;
+      if (bin[j] < kBins) atomicAdd(&sh.cnt[bin[j]], 1u);
+    }
+    __syncthreads();
+    find_k(s, sh.cnt, q);
+    if (s.use_p) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j)
+        if (bin[j] < kBins && bin[j] <= q.k_bin)
+          atomicAdd((unsigned long long*)&sh.mass[bin[j]],
+                    (unsigned long long)weight_from(((double)value_of(o[j]) - (double)m) * s.c, kLeastT));
+      __syncthreads();
+      find_p(s, sh.mass, q);
+    }
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      if (j * NT >= n) break;
+      const int at = append_at(&sh.n_list, is_candidate(q, bin[j]));
+      if (at >= 0) sh.list[at] = o[j];
+    }
+    __syncthreads();
+    n_cut = sh.n_list;
+  }
+  const uint64_t lim = Candidates<T, NT, LIST>{sh, nullptr, 0, m, top, s, n_cut}.limit(q);
+  __syncthreads();
+  if (threadIdx.x == 0) sh.n_small = 0;
+  __syncthreads();
+  // What is kept: at most k of them, and k is at most kNear.
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    if (j * NT >= n) break;
+    const uint64_t w = o[j] != ~0ull && o[j] <= lim
+                           ? weight_from(((double)value_of(o[j]) - (double)m) * s.c, s.min_t) : 0;
+    const int at = append_at(&sh.n_small, w > 0);
+    if (at >= 0) {
+      sh.small_w[at] = w;
+      sh.kept[at] = o[j];
+    }
+  }
+  __syncthreads();
+  const int n_kept = sh.n_small;
+  if (threadIdx.x >= n_kept) return;
+  const uint64_t mine = sh.kept[threadIdx.x];
+  uint64_t before = 0, total = 0;
+#pragma unroll 4
+  for (int j = 0; j < n_kept; ++j) {
+    const uint64_t w = sh.small_w[j];
+    total += w;
+    before += (uint32_t)sh.kept[j] < (uint32_t)mine ? w : 0;
+  }
+  const uint64_t at = draw_at(s.u, total);
+  if (at < before || at >= before + sh.small_w[threadIdx.x]) return;
+  a.tokens[r] = (int)(uint32_t)mine;
+  if (a.logprob)
+    a.logprob[r] = (float)(((double)value_of(mine) - (double)m) * s.c * 0.69314718055994530942 -
+                           log((double)total * 0x1p-42));
+}
+
 // 4. The cuts among the candidates, the chunk that the draw falls in, its token.
 template <typename T>
 __global__ __launch_bounds__(kChunkThreads) void sample_finish_kernel(const SplitArgs p) {
@@ -946,6 +1063,24 @@ __global__ __launch_bounds__(kChunkThreads) void sample_finish_kernel(const Spli
       a.tokens[r] = token;
       if (a.logprob) a.logprob[r] = is_real(m) ? 0.0f : -INFINITY;
     }
+    return;
+  }
+  if (st.near) {
+    // (chunk_sum holds the lists' lengths here.)
+    for (int g = threadIdx.x; g < p.chunks; g += NT) chunk_sum[g] = (uint64_t)p.near_n[lr * p.chunks + g];
+    if (threadIdx.x == 0) sh.n_list = 0;
+    __syncthreads();
+    for (int i0 = 0; i0 < p.chunks * kNear; i0 += NT) {
+      const int i = i0 + threadIdx.x, g = i / kNear;
+      const bool is = g < p.chunks && i % kNear < (int)chunk_sum[g];
+      const uint64_t o = is ? p.near[(lr * p.chunks + g) * kNear + i % kNear] : 0;
+      const int at = append_at(&sh.n_list, is);
+      if (at >= 0) sh.list[at] = o;
+    }
+    __syncthreads();
+    const int n = sh.n_list;
+    __syncthreads();
+    draw_from_list<T, NT, LIST>(sh, a, s, r, m, st.top, n);
     return;
   }
   for (int g = threadIdx.x; g < p.chunks; g += NT) chunk_sum[g] = p.sure[lr * p.chunks + g];
@@ -1015,7 +1150,7 @@ bdh_status sample_typed(const SampleArgs& a, hipStream_t st, uint64_t* launches)
   p.chunks = (int)((a.vocab + kChunk - 1) / kChunk);
   const size_t slots = (size_t)group * (size_t)p.chunks;
   const size_t sizes[] = {up(slots * 4), up(slots * 4), up(slots * kBins * 4), up(slots * kBins * 8),
-                          up(slots * 8), up((size_t)group * kListMax * 8),
+                          up(slots * 4), up(slots * kNear * 8), up(slots * 8), up((size_t)group * kListMax * 8),
                           up((size_t)group * sizeof(RowState))};
   size_t bytes = 0;
   for (size_t s : sizes) bytes += s;
@@ -1027,8 +1162,10 @@ bdh_status sample_typed(const SampleArgs& a, hipStream_t st, uint64_t* launches)
   p.arg = (int32_t*)at; at += sizes[1];
   p.cnt = (uint32_t*)at; at += sizes[2];
   p.mass = (uint64_t*)at; at += sizes[3];
-  p.sure = (uint64_t*)at; at += sizes[4];
-  p.list = (uint64_t*)at; at += sizes[5];
+  p.near_n = (int32_t*)at; at += sizes[4];
+  p.near = (uint64_t*)at; at += sizes[5];
+  p.sure = (uint64_t*)at; at += sizes[6];
+  p.list = (uint64_t*)at; at += sizes[7];
   p.state = (RowState*)at;
   for (p.row0 = 0; p.row0 < a.rows; p.row0 += group) {
     const uint32_t n = (uint32_t)(a.rows - p.row0 < group ? a.rows - p.row0 : group);
