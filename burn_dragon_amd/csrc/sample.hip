@@ -15,13 +15,13 @@
 // (of top-p, of the draw) falls between two tokens.  Up to 2^20 logits, a sum
 // stays below 2^62.
 //
-//   1. A histogram over 512 bins of 1/12 octave of weight below the largest
+//   1. A histogram over 512 bins of 1/10 octave of weight below the largest
 //      (counts for top-k, weights for top-p) finds the bin in which a cut
 //      falls; bins before it are kept whole, bins after it are not.
-//   2. The candidates of that bin go to a list.  Up to 64 are ordered in one
-//      wave, each lane counting what comes before its own; more are narrowed
-//      first by histograms of nine bits of (value, index), so equal logits
-//      are cut by index.  A list that overflows is read from the row again.
+//   2. The candidates of that bin go to a list.  Up to 64 are compared each with
+//      each in a wave, up to 256 by the workgroup; more are narrowed first by
+//      histograms of nine bits of (value, index), so equal logits are cut by
+//      index.  A list that overflows is read from the row again.
 //   3. The kept weights are summed by wave, and the draw descends into the
 //      wave, the stripe, the lane and the element that it falls in.
 //
@@ -331,8 +331,7 @@ __device__ __forceinline__ Cuts no_cuts() {
   q.k_above = q.k_mass = q.p_above = 0;
   return q;
 }
-// One wave each.
-// (Returns the logits up to k_bin.)
+// One wave each.  (find_k returns the logits up to k_bin.)
 __device__ __forceinline__ uint64_t find_k(const Row& s, const uint32_t* cnt, Cuts& q) {
   uint64_t in;
   q.k_bin = BinScan(cnt, kBins).cross((uint64_t)s.k, &q.k_above, &in);
@@ -919,9 +918,9 @@ __global__ __launch_bounds__(kChunkThreads) void sample_gather_kernel(const Spli
   const Cuts q = st->cuts;
   if (threadIdx.x == 0) n_here = some = 0;
   __syncthreads();
-  const float shift = top - grid_of(mg, s.cb);  // (a chunk without a logit: beyond all bins)
+  const float shift = top - grid_of(mg, s.cb);
   uint64_t w = 0;
-  if (shift < (float)kBins) {
+  if (is_real(mg) && shift < (float)kBins) {  // (a chunk without a logit left no histogram)
     const int64_t at = slot * kBins + threadIdx.x;
     const int b = threadIdx.x + (int)shift;
     w = p.mass[at];

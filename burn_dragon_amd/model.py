@@ -98,6 +98,13 @@ def model_forward_logits(tokens: torch.Tensor, weights: BdhModelWeights, *,
         return None
     if (adapters is None) != (adapter_ids is None):
         raise ValueError("adapters and adapter_ids come together")
+    if adapters is not None:  # before any layer moves the state on
+        n, rank = adapters.a.shape[:2]
+        if (adapters.a.shape[2:] != (weights.layer.embd,) or adapters.b.shape != (n, weights.vocab, rank)
+                or adapter_ids.shape != tokens.shape[:1]):
+            raise ValueError("adapters and adapter_ids do not fit the model and the batch")
+        if rank > 128 or adapters.a.dtype != torch.bfloat16 or adapters.b.dtype != torch.bfloat16:
+            return None
     if state is not None:
         if len(state.rho) != weights.n_layer:
             return None

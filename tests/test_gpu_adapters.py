@@ -222,6 +222,14 @@ def test_model_logits_with_adapters():
     assert plain.position == with_.position == 22
     with pytest.raises(ValueError):
         bd.model_forward_logits(nxt, w, adapters=s)
+    # adapters that do not fit are refused before a layer moves the state on
+    kept = [r.clone() for r in with_.rho]
+    for bad, bad_ids in ((bd.AdapterSet(s.a, s.b[:, :-1], s.scale), ids), (s, ids[:2])):
+        with pytest.raises(ValueError):
+            bd.model_forward_logits(nxt, w, state=with_, adapters=bad, adapter_ids=bad_ids)
+    wide = bd.AdapterSet(s.a.repeat(1, 40, 1), s.b.repeat(1, 1, 40), s.scale)  # rank 160
+    assert bd.model_forward_logits(nxt, w, state=with_, adapters=wide, adapter_ids=ids) is None
+    assert with_.position == 22 and all(torch.equal(r, k) for r, k in zip(with_.rho, kept))
 
 
 def test_unsupported_and_refused():

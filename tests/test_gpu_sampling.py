@@ -144,6 +144,23 @@ def test_nan_infinities_zeros_and_empty_rows(V):
         check(torch, bd, x, u, **kw)
 
 
+@pytest.mark.parametrize("low", [-sampleref.F32_MAX, -3e37])
+def test_only_lowest_values_beside_masked_stretches(low):
+    # A stretch of 8192 without a logit beside others at the lowest value: it
+    # weighs nothing and is not read.
+    torch = need_gpu()
+    import burn_dragon_amd as bd
+    x = np.full((6, 40000), -np.inf, np.float32)
+    x[:, 9000:9010] = low
+    x[:, 33000] = low
+    u = np.array([0.0, 0.2, 0.4, 0.6, 0.8, 0.99], np.float32)
+    for kw in ({}, dict(top_k=3), dict(top_k=700), dict(top_p=0.5), dict(min_p=0.5), dict(top_k=8, top_p=0.6)):
+        announce("sample lowest", low, kw)
+        for _ in range(2):  # the second call finds the first's scratch
+            check(torch, bd, x, u, **kw)
+        check(torch, bd, np.where(x == -np.inf, np.float32(1.0), x), u, **kw)
+
+
 @pytest.mark.parametrize("V", [40, 2000, 60000])
 def test_settings_one_a_row(V):
     # Greedy, uncut, cut and out-of-range rows side by side.
@@ -165,6 +182,25 @@ def test_settings_one_a_row(V):
     seen["min_p"] = np.where(np.isnan(host["min_p"]), 0.0, host["min_p"]).astype(np.float32)
     announce("sample rows", V)
     check(torch, bd, x, u, settings=dev, **seen)
+
+
+@pytest.mark.parametrize("V", [20000, 131072, 300000])
+def test_top_k_around_what_the_chunks_list(V):
+    # Up to 256 a chunk go to its list: k about that, ties that overflow it,
+    # rows with fewer logits than k.
+    torch = need_gpu()
+    import burn_dragon_amd as bd
+    rng = np.random.default_rng(V)
+    for k in (2, 63, 64, 65, 200, 255, 256, 257, 600):
+        x = logits_of(rng, 4, V, "peaked").astype(np.float32)
+        x[1] = np.round(x[1])                                   # hundreds of equal logits at the k-th
+        x[2, rng.random(V) < 1 - 300 / V] = -np.inf             # about 300 logits
+        x[3] = -np.inf
+        x[3, rng.integers(0, V, 40)] = rng.standard_normal(40)  # fewer than k
+        u = rng.random(4).astype(np.float32)
+        for kw in (dict(top_k=k), dict(top_k=k, top_p=0.7), dict(top_k=k, min_p=0.05, top_p=0.99, temperature=1.5)):
+            announce("sample lists", V, kw)
+            check(torch, bd, x, u, **kw)
 
 
 def test_random_numbers_at_the_ends():
