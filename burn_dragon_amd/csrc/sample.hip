@@ -181,6 +181,17 @@ __device__ __forceinline__ void forget(float (&x)[E]) {
   for (int e = 0; e < E; ++e) asm volatile("" : "+v"(x[e]));
 }
 
+// What the histogram says about the cuts of a row.
+struct Cuts {
+  int k_bin;            // holds the k-th in order; kBins: top-k cuts nothing that is drawn
+  int p_first, p_last;  // bins that the top-p cut can fall in; kBins: no top-p
+  int m_first, m_last;  // (long rows) bins that the least kept t can fall in; kBins: none
+  uint64_t k_above;     // logits in bins before k_bin
+  uint64_t k_upto;      // and with it
+  uint64_t k_mass;      // their weight (all weight: no k_bin)
+  uint64_t p_above;     // weight in bins before p_first
+};
+
 template <int NT, int LIST>
 struct Shared {
   uint64_t mass[kBins];
@@ -193,6 +204,7 @@ struct Shared {
   int n_list, n_small, arg;
   int bin;
   uint64_t above;
+  Cuts cuts;
 };
 
 // Neighbours' values by DPP: `none` where there is none.
@@ -312,15 +324,6 @@ struct BinScan {
   }
 };
 
-// What the histogram says about the cuts of a row.
-struct Cuts {
-  int k_bin;            // holds the k-th in order; kBins: top-k cuts nothing that is drawn
-  int p_first, p_last;  // bins that the top-p cut can fall in; kBins: no top-p
-  int m_first, m_last;  // (long rows) bins that the least kept t can fall in; kBins: none
-  uint64_t k_above;     // logits in bins before k_bin
-  uint64_t k_mass;      // their weight (all weight: no k_bin)
-  uint64_t p_above;     // weight in bins before p_first
-};
 __device__ __forceinline__ uint64_t p_need(const Row& s, uint64_t total) {
   const uint64_t need = (uint64_t)ceil(s.p * (double)total);
   return need > 0 ? need : 1;  // the first in order is always kept
@@ -328,25 +331,34 @@ __device__ __forceinline__ uint64_t p_need(const Row& s, uint64_t total) {
 __device__ __forceinline__ Cuts no_cuts() {
   Cuts q;
   q.k_bin = q.p_first = q.p_last = q.m_first = q.m_last = kBins;
-  q.k_above = q.k_mass = q.p_above = 0;
+  q.k_above = q.k_upto = q.k_mass = q.p_above = 0;
   return q;
 }
-// One wave each.  (find_k returns the logits up to k_bin.)
-__device__ __forceinline__ uint64_t find_k(const Row& s, const uint32_t* cnt, Cuts& q) {
+// One wave each.
+__device__ __forceinline__ void find_k(const Row& s, const uint32_t* cnt, Cuts& q) {
   uint64_t in;
   q.k_bin = BinScan(cnt, kBins).cross((uint64_t)s.k, &q.k_above, &in);
-  return q.k_above + in;
+  q.k_upto = q.k_above + in;
 }
-// Counts a chunk's logits by bin into cnt (cleared) and finds its k-th.
+// What f does to the cuts, done by one wave for all (sixteen waves that each
+// scan the bins for themselves take 4 us of a workgroup's issue).
+template <int NT, typename F>
+__device__ __forceinline__ void by_one_wave(Cuts& q, Cuts* shared, const F& f) {
+  if (NT == 64 || threadIdx.x < 64) f();
+  if (NT == 64) return;
+  if (threadIdx.x == 0) *shared = q;
+  __syncthreads();
+  q = *shared;
+}
+// Counts a chunk's logits by bin into cnt (cleared).
 template <int NT, int E>
-__device__ __forceinline__ uint64_t count_for_k(const Row& s, const float (&x)[E], float top, uint32_t* cnt, Cuts& q) {
+__device__ __forceinline__ void count_logits(const Row& s, const float (&x)[E], float top, uint32_t* cnt) {
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int b = bin_of(x[e], top, s.cb);
     if (b < kBins) atomicAdd(&cnt[b], 1u);
   }
   __syncthreads();
-  return find_k(s, cnt, q);
 }
 __device__ __forceinline__ void find_p(const Row& s, const uint64_t* mass, Cuts& q) {
   // What top-k keeps weighs between all before k_bin, and that with k_bin.
@@ -450,11 +462,9 @@ struct Candidates {
         if (threadIdx.x < 64) {
           const int lane = threadIdx.x;
           const uint64_t mine = lane < n_in ? sh.small[lane] : ~0ull;
-          if (lane < n_in) sh.small_w[lane] = MASS ? weight(mine, kLeastT) : 1;
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          const uint64_t w = lane >= n_in ? 0 : MASS ? weight(mine, kLeastT) : 1;
           uint64_t before = above;
-          for (int j = 0; j < n_in; ++j)
-            if (sh.small[j] < mine) before += sh.small_w[j];
+          for (int j = 0; j < n_in; ++j) before += lane_u64(mine, j) < mine ? lane_u64(w, j) : 0;
           const bool kept = lane < n_in && before < need;
           const uint64_t best = wave_max_u64(kept ? mine : 0);
           if (lane == 0) sh.sum = best;
@@ -490,8 +500,8 @@ struct Candidates {
     }
   }
 
-  // The same for up to kSmall candidates, in every wave and without a barrier:
-  // a lane compares its own with each other.  (One candidate at least is kept.)
+  // The same for up to kSmall candidates, in one wave: a lane compares its own
+  // with each other.  (One candidate at least is kept.)
   __device__ uint64_t limit_small(const Cuts& q) {
     const int lane = threadIdx.x & 63;
     const uint64_t mine = lane < n ? sh.list[lane] : ~0ull;
@@ -566,7 +576,15 @@ struct Candidates {
   // The last logit in order that top-k and top-p keep.
   __device__ uint64_t limit(const Cuts& q) {
     if (q.k_bin == kBins && !s.use_p) return ~0ull;  // neither divides anything
-    if (n <= kSmall) return limit_small(q);
+    if (n <= kSmall) {
+      if (NT == 64) return limit_small(q);
+      if (threadIdx.x < 64) {
+        const uint64_t last = limit_small(q);
+        if (threadIdx.x == 0) sh.sum = last;
+      }
+      __syncthreads();
+      return sh.sum;
+    }
     if (n <= kMid) return limit_mid(q);
     uint64_t lim = ~0ull, total = q.k_mass;
     if (q.k_bin < kBins) {
@@ -703,7 +721,8 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a) {
     __syncthreads();
     Cuts q = no_cuts();
     if (s.use_k) {
-      count_for_k<NT, E>(s, x, top, sh.cnt, q);
+      count_logits<NT, E>(s, x, top, sh.cnt);
+      by_one_wave<NT>(q, &sh.cuts, [&] { find_k(s, sh.cnt, q); });
       forget<E>(x);
     }
     if (s.use_p) {
@@ -716,7 +735,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a) {
         if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
       }
       __syncthreads();
-      find_p(s, sh.mass, q);
+      by_one_wave<NT>(q, &sh.cuts, [&] { find_p(s, sh.mass, q); });
       forget<E>(x);
     }
 #pragma unroll
@@ -786,6 +805,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_chunk_kernel(const Split
   __shared__ uint32_t cnt[kBins];
   __shared__ float part[NT / 64];
   __shared__ int arg, n_near;
+  __shared__ Cuts cuts;
   const int64_t lr = blockIdx.y, r = p.row0 + lr;
   const int64_t slot = lr * p.chunks + blockIdx.x;
   const T* row = (const T*)p.a.logits + r * p.a.row_stride;
@@ -820,9 +840,10 @@ __global__ __launch_bounds__(kChunkThreads) void sample_chunk_kernel(const Split
   Cuts q = no_cuts();
   if (s.use_k) {
     // Past the chunk's own k-th no logit is among the row's first k.
-    const uint64_t n = count_for_k<NT, E>(s, x, top, cnt, q);
-    if (n <= kNear && s.k <= kNear) {
-      if (threadIdx.x == 0) p.near_n[slot] = (int)n;
+    count_logits<NT, E>(s, x, top, cnt);
+    by_one_wave<NT>(q, &cuts, [&] { find_k(s, cnt, q); });
+    if (q.k_upto <= kNear && s.k <= kNear) {
+      if (threadIdx.x == 0) p.near_n[slot] = (int)q.k_upto;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const int b = bin_of(x[e], top, s.cb);
@@ -892,8 +913,10 @@ __global__ __launch_bounds__(kBins) void sample_merge_kernel(const SplitArgs p) 
       cnt[b] = n;
       mass[b] = w;
       __syncthreads();
-      if (s.use_k) find_k(s, cnt, q);
-      if (s.use_p) find_p(s, mass, q);
+      if (threadIdx.x < 64) {
+        if (s.use_k) find_k(s, cnt, q);
+        if (s.use_p) find_p(s, mass, q);
+      }
     }
     find_least(s, m, top, q);
   }
@@ -988,7 +1011,7 @@ __device__ void draw_from_list(Shared<NT, LIST>& sh, const SampleArgs& a, const 
       if (bin[j] < kBins) atomicAdd(&sh.cnt[bin[j]], 1u);
     }
     __syncthreads();
-    find_k(s, sh.cnt, q);
+    by_one_wave<NT>(q, &sh.cuts, [&] { find_k(s, sh.cnt, q); });
     if (s.use_p) {
 #pragma unroll
       for (int j = 0; j < PER; ++j)
@@ -996,7 +1019,7 @@ __device__ void draw_from_list(Shared<NT, LIST>& sh, const SampleArgs& a, const 
           atomicAdd((unsigned long long*)&sh.mass[bin[j]],
                     (unsigned long long)weight_from(((double)value_of(o[j]) - (double)m) * s.c, kLeastT));
       __syncthreads();
-      find_p(s, sh.mass, q);
+      by_one_wave<NT>(q, &sh.cuts, [&] { find_p(s, sh.mass, q); });
     }
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
