@@ -18,6 +18,11 @@
 //
 // Bound by memory: each distinct source read once and each destination
 // written once (cycles past eight slots: two more accesses for every seven).
+// Of 6 layers of 33.5 MB slots, a slot to 8 others takes 325-345 us (5.4
+// TB/s; a large copy here 5.15), closing up 8 of 16 moved slots 574 us (5.6);
+// 3 layers of 1001 x 63 x 4 slots, 9 of 13 exchanged, 9 us; a single small
+// state 3 us, its launch.  Steps of two or four slots measured alike; eight
+// let a cycle of eight turn without a second access.
 #include <vector>
 
 #include "bdh_internal.h"
@@ -47,11 +52,25 @@ static_assert(sizeof(MoveArgs) <= 4000, "kernel arguments");
 // 16 bytes at any 4-byte address (slots of odd sizes): a dwordx4 access.
 typedef float float4_u __attribute__((ext_vector_type(4), aligned(4)));
 
-template <int K, typename V>
+enum Past { kCached, kStores, kBoth };  // which accesses pass the caches by
+
+template <Past P, typename V>
+__device__ __forceinline__ V load_slot(const float* p) {
+  if constexpr (P == kBoth) return __builtin_nontemporal_load((const V*)p);
+  else return *(const V*)p;
+}
+
+template <Past P, typename V>
+__device__ __forceinline__ void store_slot(float* p, V v) {
+  if constexpr (P == kCached) *(V*)p = v;
+  else __builtin_nontemporal_store(v, (V*)p);
+}
+
+template <int K, Past P, typename V>
 __device__ __forceinline__ int run_step(const int32_t* w, int pc, const float* src, float* dst, int64_t slab) {
   V r[K];
 #pragma unroll
-  for (int j = 0; j < K; ++j) r[j] = *(const V*)(src + (w[pc + j] & 0xffff) * slab);
+  for (int j = 0; j < K; ++j) r[j] = load_slot<P, V>(src + (w[pc + j] & 0xffff) * slab);
   // All loads are waited for here, together: a wait inside the loops below
   // would also wait for the stores before it.
 #pragma unroll
@@ -59,23 +78,24 @@ __device__ __forceinline__ int run_step(const int32_t* w, int pc, const float* s
   int at = pc + K;
 #pragma unroll
   for (int j = 0; j < K; ++j)
-    for (const int end = at + (w[pc + j] >> 16); at < end; ++at) *(V*)(dst + w[at] * slab) = r[j];
+    for (const int end = at + (w[pc + j] >> 16); at < end; ++at) store_slot<P>(dst + w[at] * slab, r[j]);
   return at;
 }
 
-template <typename V>
+template <Past P, typename V>
 __device__ __forceinline__ void run_program(const MoveArgs& a, const float* src, float* dst, int64_t slab) {
   for (int pc = 0; pc < a.n;) {
     const int k = a.words[pc];
     ++pc;
-    if (k == 8) pc = run_step<8, V>(a.words, pc, src, dst, slab);
-    else if (k == 4) pc = run_step<4, V>(a.words, pc, src, dst, slab);
-    else if (k == 2) pc = run_step<2, V>(a.words, pc, src, dst, slab);
-    else pc = run_step<1, V>(a.words, pc, src, dst, slab);
+    if (k == 8) pc = run_step<8, P, V>(a.words, pc, src, dst, slab);
+    else if (k == 4) pc = run_step<4, P, V>(a.words, pc, src, dst, slab);
+    else if (k == 2) pc = run_step<2, P, V>(a.words, pc, src, dst, slab);
+    else pc = run_step<1, P, V>(a.words, pc, src, dst, slab);
   }
-  for (int i = 0; i < a.n_zero; ++i) *(V*)(dst + a.words[a.n + i] * slab) = V{};
+  for (int i = 0; i < a.n_zero; ++i) store_slot<P>(dst + a.words[a.n + i] * slab, V{});
 }
 
+template <Past P>
 __global__ __launch_bounds__(256) void move_streams_kernel(const MoveArgs a) {
   const int64_t slab = a.slab[blockIdx.y];
   const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
@@ -83,9 +103,9 @@ __global__ __launch_bounds__(256) void move_streams_kernel(const MoveArgs a) {
   const float* src = a.src[blockIdx.y] + e;
   float* dst = a.dst[blockIdx.y] + e;
   if (e + 4 <= slab) {
-    run_program<float4_u>(a, src, dst, slab);
+    run_program<P, float4_u>(a, src, dst, slab);
   } else {
-    for (int64_t k = 0; k < slab - e; ++k) run_program<float>(a, src + k, dst + k, slab);
+    for (int64_t k = 0; k < slab - e; ++k) run_program<P, float>(a, src + k, dst + k, slab);
   }
 }
 
@@ -101,6 +121,8 @@ struct Program {
   };
   std::vector<Launch> launches{1};
   std::vector<Move> open;  // the step being filled
+  int64_t reads = 0, writes = 0;  // slots
+  bool again = false;             // a slot is read that the call has written
 
   Launch& room(size_t words) {
     if (launches.back().words.size() + launches.back().zero.size() + words > (size_t)kMaxWords)
@@ -125,6 +147,8 @@ struct Program {
     constexpr size_t kMost = 64;  // destinations of one load
     for (size_t at = 0; at < dst.size(); at += kMost) {
       const size_t end = at + kMost < dst.size() ? at + kMost : dst.size();
+      ++reads;
+      writes += (int64_t)(end - at);
       open.push_back(Move{src, std::vector<int>(dst.begin() + at, dst.begin() + end)});
       if (open.size() == (size_t)kStep) flush();
     }
@@ -188,6 +212,7 @@ void order_moves(const std::vector<int>& from_in, int src_slots, bool in_place, 
       for (size_t at = 1; at < cycle.size();) {
         std::vector<int> v{cycle[0]};
         while (v.size() < (size_t)kStep && at < cycle.size()) v.push_back(cycle[at++]);
+        p->again |= at < cycle.size();
         p->turn(v);
       }
     }
@@ -197,6 +222,21 @@ void order_moves(const std::vector<int>& from_in, int src_slots, bool in_place, 
   p->clear(cleared);
 }
 
+// What a call writes past the last-level cache's 256 MB is not there when the
+// layers read it, so it need not displace anything.  Of a state of 6 layers
+// (33.5 MB a slot and layer), us with the caches / stores past them / both:
+// 1 slot to 8: 364 / 348 / 420, 4 to 8: 491 / 433 / 414, 1 to 2: 103 / 85 / 100;
+// 8 slots to 8 others: 707 / 728 / 684, closing up 8 of 16: 637 / 650 / 574.
+// Below those sizes the caches win (1 slot to 8 of one layer: 49 / 59 / 64;
+// 8 in a cycle: 78 / 84 / 97), and so they do in a long cycle, which reads a
+// slot again (20 slots: 1776 / 1851 / 1941).
+Past past_caches(const Program& p, int64_t slot_bytes) {
+  const int64_t cache = (int64_t)256 << 20, written = p.writes * slot_bytes;
+  if (written <= cache) return kCached;
+  if (2 * p.writes >= 3 * p.reads) return kStores;
+  return written > 2 * cache && !p.again ? kBoth : kCached;
+}
+
 }  // namespace
 
 bdh_status copy_streams(const StreamMoves& m, hipStream_t st, uint64_t* launches) {
@@ -204,6 +244,9 @@ bdh_status copy_streams(const StreamMoves& m, hipStream_t st, uint64_t* launches
   for (int i = 0; i < m.n; ++i) from[m.dst[i]] = m.src[i] < 0 ? kZeros : m.src[i];
   Program p;
   order_moves(from, (int)m.src_batch, m.in_place, &p);
+  int64_t slot = 0;
+  for (int l = 0; l < m.n_layers; ++l) slot += m.slab[l];
+  const Past past = past_caches(p, slot * 4);
   for (const Program::Launch& part : p.launches) {
     if (part.words.empty() && part.zero.empty()) continue;
     for (int l0 = 0; l0 < m.n_layers; l0 += kMaxLayers) {
@@ -221,8 +264,9 @@ bdh_status copy_streams(const StreamMoves& m, hipStream_t st, uint64_t* launches
       a.n_zero = (int32_t)part.zero.size();
       for (int i = 0; i < a.n; ++i) a.words[i] = part.words[i];
       for (int i = 0; i < a.n_zero; ++i) a.words[a.n + i] = part.zero[i];
-      hipLaunchKernelGGL(move_streams_kernel, dim3((uint32_t)((most + 1023) / 1024), (uint32_t)n), dim3(256),
-                         0, st, a);
+      const auto kernel = past == kCached ? move_streams_kernel<kCached>
+                          : past == kStores ? move_streams_kernel<kStores> : move_streams_kernel<kBoth>;
+      hipLaunchKernelGGL(kernel, dim3((uint32_t)((most + 1023) / 1024), (uint32_t)n), dim3(256), 0, st, a);
       BDH_HIP_TRY(hipGetLastError());
       ++*launches;
     }

@@ -238,3 +238,24 @@ def test_captured_into_a_graph_and_on_another_stream():
             bd.copy_streams(rho, [4], [0])  # eager work between the replays
         torch.cuda.synchronize()
         assert all(torch.equal(r, w) for r, w in zip(rho, want)), i
+
+
+@pytest.mark.parametrize("name", ["fork", "close_up", "cycle", "cycle_and_forks", "from_another"])
+def test_calls_larger_than_the_caches(name):
+    # 16.8 MB a slot: 16 slots written are the last-level cache, 32 twice it.
+    torch = need_gpu()
+    import burn_dragon_amd as bd
+    B, shape = 48, (4, 4096, 256)
+    dst, src = {
+        "fork": (list(range(1, 41)), [0] * 40),
+        "close_up": (list(range(40)), list(range(8, 48))),
+        "cycle": (list(range(40)), list(range(1, 40)) + [0]),
+        "cycle_and_forks": (list(range(40)), list(range(1, 12)) + [0] + [i % 12 for i in range(28)]),
+        "from_another": (list(range(8, 48)), list(range(40))),
+    }[name]
+    announce("streams past the caches", name)
+    g = torch.Generator(device="cuda").manual_seed(12)
+    rho = [torch.randn(B, *shape, generator=g, device="cuda")]
+    source = [torch.randn(B, *shape, generator=g, device="cuda")] if name == "from_another" else None
+    for _ in range(2):
+        check(torch, bd, rho, dst, src, source)
