@@ -27,6 +27,7 @@ namespace {
 
 constexpr int kTile = 16;
 constexpr int kGatherTokens = 16;  // up to here tiles gather sequences
+constexpr int kWindow = 512;       // sequences of the batch that are gathered together
 constexpr int kRowsTokens = 2, kRowsIn = 512;  // up to here, at ranks to 16, no tiles but adapter_rows_kernel
 constexpr int kRowsShare = 8;                  // the sequences it gathers
 
@@ -87,15 +88,17 @@ struct Rows {
 // The workgroups of a sequence that is the first of its adapter, or the first
 // after `share` more of it, gather that one and the next; the others have no
 // rows.  list: their rows.  Every wave for itself, without a barrier: all
-// write the same list.
+// write the same list.  Each 512 sequences are gathered by themselves, or every
+// workgroup would go through a large batch's ids.
 __device__ Rows gather_rows(const AdapterArgs& a, int b, int share, int* list) {
   const int time = (int)a.time, lane = threadIdx.x & 63;
   Rows g{adapter_of(a, b), 0, 0};
   if (g.id < 0 && a.out == a.base) return g;
   int before = 0, n = 0;
-  for (int i0 = 0; i0 < (int)a.batch && n < share; i0 += 64) {
+  const int window = b / kWindow * kWindow, end = min(window + kWindow, (int)a.batch);
+  for (int i0 = window; i0 < end && n < share; i0 += 64) {
     const int i = i0 + lane;
-    const bool is = i < (int)a.batch && adapter_of(a, i) == g.id;
+    const bool is = i < end && adapter_of(a, i) == g.id;
     before += __popcll(__ballot(is && i < b));
     const uint64_t from_b = __ballot(is && i >= b);
     if (from_b != 0 && before % share != 0) return g;

@@ -765,7 +765,7 @@ bdh_status bdh_apply_adapters(const bdh_adapter_plan* plan, int32_t dtype, const
   if (p.rank > kMaxAdapterRank) return fail(BDH_UNSUPPORTED, "rank must be at most 128");
   if (p.batch > kMaxGrid) return fail(BDH_UNSUPPORTED, "batch exceeds 65535");
   if (p.in_dim > (int64_t)1 << 20 || p.out_dim > (int64_t)1 << 22 || p.adapters > (int64_t)1 << 20 ||
-      p.time > (int64_t)1 << 22 || p.batch * p.time > (int64_t)1 << 23)
+      p.time > kMaxGrid * 64 || p.batch * p.time > (int64_t)1 << 23)
     return fail(BDH_UNSUPPORTED, "too large for one launch");
   const int64_t size = dtype == BDH_F32 ? 4 : 2;
   for (const void* t : {base, hidden, (const void*)out})

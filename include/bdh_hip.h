@@ -309,8 +309,10 @@ bdh_status bdh_lm_logits(const float* hidden, int64_t rows, int64_t embd,
  * [0, adapters) leaves out = base.  out may be base (in place), and otherwise
  * shares no memory with the inputs.  Products and sums are f32, with BDH_F32 to
  * f32's own precision (on the matrix cores in three bf16 parts), and out is
- * rounded once.  rank up to 128.  Pointers aligned to their elements.  Uses the
- * stream's scratch.  No counterpart in the reference, which adapts a model by
+ * rounded once.  An infinity or NaN of hidden reaches its own row, one of an
+ * adapter (whose values are meant to be finite) its own sequences.  rank up to
+ * 128.  Pointers aligned to their elements.  Uses the stream's scratch, but for
+ * small calls.  No counterpart in the reference, which adapts a model by
  * training it. */
 typedef struct {
   int64_t batch, time, in_dim, out_dim, rank, adapters;

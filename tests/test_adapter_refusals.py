@@ -49,3 +49,8 @@ def test_python_surface_without_a_device():
     s = bd.AdapterSet(torch.zeros(1, 2, 4, dtype=torch.bfloat16), torch.zeros(1, 8, 2, dtype=torch.bfloat16),
                       torch.ones(1))
     assert bd.apply_adapters(torch.zeros(2, 8), torch.zeros(2, 4), s, torch.zeros(2, dtype=torch.int32)) is None
+
+
+def test_time_past_the_grid_is_refused():
+    assert call(batch=1, time=65535 * 64 + 1) == _lib.BDH_UNSUPPORTED
+    assert "large" in _lib.last_error()

@@ -253,3 +253,11 @@ def test_unsupported_and_refused():
             bd.apply_adapters(*args)
     with pytest.raises(ValueError):
         bd.apply_adapters(base, hidden, s, ids, out=base.transpose(0, 1))
+
+
+@pytest.mark.parametrize("T,D,R", [(1, 64, 16), (2, 64, 8), (3, 64, 16), (16, 20, 5)])
+def test_more_sequences_than_are_gathered_together(T, D, R):
+    # The batch is gathered 512 sequences at a time.
+    B = 1100
+    run(B, T, D, 70, R, 3, "float32", np.random.default_rng(T).integers(-1, 3, B).tolist())
+    run(B, T, D, 70, R, 3, "float32", [1] * B, in_place=True)
