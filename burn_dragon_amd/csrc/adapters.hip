@@ -15,7 +15,10 @@
 // is read once for up to 16 rows.
 //
 // A workgroup holds its rows' u in LDS and runs over blocks of columns, bound by
-// base, out and B.  u comes from the workgroup itself (one launch: small calls
+// base, out and B: 8 prompts of 512 (D 256, V 32000, R 16, f32) 212 us (4.9 TB/s),
+// 3 of 1001 (D 1024, V 50048, R 64, bf16) 184 (3.3 TB/s; at R 16 148, B being read
+// again for every 64 rows), 222 at V 50001, whose rows of odd length leave no access
+// aligned.  u comes from the workgroup itself (one launch: small calls
 // are launches and latency), or, where many workgroups would compute the same
 // u, from a launch of its own through the stream's scratch.
 #include <type_traits>

@@ -18,11 +18,11 @@
 //
 // Bound by memory: each distinct source read once and each destination
 // written once (cycles past eight slots: two more accesses for every seven).
-// Of 6 layers of 33.5 MB slots, a slot to 8 others takes 325-345 us (5.4
-// TB/s; a large copy here 5.15), closing up 8 of 16 moved slots 574 us (5.6);
-// 3 layers of 1001 x 63 x 4 slots, 9 of 13 exchanged, 9 us; a single small
-// state 3 us, its launch.  Steps of two or four slots measured alike; eight
-// let a cycle of eight turn without a second access.
+// (Steps of two or four slots measured alike; eight let a cycle of eight turn
+// without a second access.)  Of 6 layers of 33.5 MB slots, one to 8 others takes
+// 352-385 us (4.7-5.1 TB/s; a large copy here 5.15), closing up 8 of 16 slots
+// 575-590 (5.5); of 3 layers of 1 MB slots, 9 exchanged, 9 us; a single small
+// state 3 us, its launch.
 #include <vector>
 
 #include "bdh_internal.h"
@@ -52,25 +52,24 @@ static_assert(sizeof(MoveArgs) <= 4000, "kernel arguments");
 // 16 bytes at any 4-byte address (slots of odd sizes): a dwordx4 access.
 typedef float float4_u __attribute__((ext_vector_type(4), aligned(4)));
 
-enum Past { kCached, kStores, kBoth };  // which accesses pass the caches by
-
-template <Past P, typename V>
+// PAST: past the caches.
+template <bool PAST, typename V>
 __device__ __forceinline__ V load_slot(const float* p) {
-  if constexpr (P == kBoth) return __builtin_nontemporal_load((const V*)p);
+  if constexpr (PAST) return __builtin_nontemporal_load((const V*)p);
   else return *(const V*)p;
 }
 
-template <Past P, typename V>
+template <bool PAST, typename V>
 __device__ __forceinline__ void store_slot(float* p, V v) {
-  if constexpr (P == kCached) *(V*)p = v;
-  else __builtin_nontemporal_store(v, (V*)p);
+  if constexpr (PAST) __builtin_nontemporal_store(v, (V*)p);
+  else *(V*)p = v;
 }
 
-template <int K, Past P, typename V>
+template <int K, bool PAST, typename V>
 __device__ __forceinline__ int run_step(const int32_t* w, int pc, const float* src, float* dst, int64_t slab) {
   V r[K];
 #pragma unroll
-  for (int j = 0; j < K; ++j) r[j] = load_slot<P, V>(src + (w[pc + j] & 0xffff) * slab);
+  for (int j = 0; j < K; ++j) r[j] = load_slot<PAST, V>(src + (w[pc + j] & 0xffff) * slab);
   // All loads are waited for here, together: a wait inside the loops below
   // would also wait for the stores before it.
 #pragma unroll
@@ -78,24 +77,24 @@ __device__ __forceinline__ int run_step(const int32_t* w, int pc, const float* s
   int at = pc + K;
 #pragma unroll
   for (int j = 0; j < K; ++j)
-    for (const int end = at + (w[pc + j] >> 16); at < end; ++at) store_slot<P>(dst + w[at] * slab, r[j]);
+    for (const int end = at + (w[pc + j] >> 16); at < end; ++at) store_slot<PAST>(dst + w[at] * slab, r[j]);
   return at;
 }
 
-template <Past P, typename V>
+template <bool PAST, typename V>
 __device__ __forceinline__ void run_program(const MoveArgs& a, const float* src, float* dst, int64_t slab) {
   for (int pc = 0; pc < a.n;) {
     const int k = a.words[pc];
     ++pc;
-    if (k == 8) pc = run_step<8, P, V>(a.words, pc, src, dst, slab);
-    else if (k == 4) pc = run_step<4, P, V>(a.words, pc, src, dst, slab);
-    else if (k == 2) pc = run_step<2, P, V>(a.words, pc, src, dst, slab);
-    else pc = run_step<1, P, V>(a.words, pc, src, dst, slab);
+    if (k == 8) pc = run_step<8, PAST, V>(a.words, pc, src, dst, slab);
+    else if (k == 4) pc = run_step<4, PAST, V>(a.words, pc, src, dst, slab);
+    else if (k == 2) pc = run_step<2, PAST, V>(a.words, pc, src, dst, slab);
+    else pc = run_step<1, PAST, V>(a.words, pc, src, dst, slab);
   }
-  for (int i = 0; i < a.n_zero; ++i) store_slot<P>(dst + a.words[a.n + i] * slab, V{});
+  for (int i = 0; i < a.n_zero; ++i) store_slot<PAST>(dst + a.words[a.n + i] * slab, V{});
 }
 
-template <Past P>
+template <bool PAST>
 __global__ __launch_bounds__(256) void move_streams_kernel(const MoveArgs a) {
   const int64_t slab = a.slab[blockIdx.y];
   const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
@@ -103,9 +102,9 @@ __global__ __launch_bounds__(256) void move_streams_kernel(const MoveArgs a) {
   const float* src = a.src[blockIdx.y] + e;
   float* dst = a.dst[blockIdx.y] + e;
   if (e + 4 <= slab) {
-    run_program<P, float4_u>(a, src, dst, slab);
+    run_program<PAST, float4_u>(a, src, dst, slab);
   } else {
-    for (int64_t k = 0; k < slab - e; ++k) run_program<P, float>(a, src + k, dst + k, slab);
+    for (int64_t k = 0; k < slab - e; ++k) run_program<PAST, float>(a, src + k, dst + k, slab);
   }
 }
 
@@ -222,19 +221,16 @@ void order_moves(const std::vector<int>& from_in, int src_slots, bool in_place, 
   p->clear(cleared);
 }
 
-// What a call writes past the last-level cache's 256 MB is not there when the
-// layers read it, so it need not displace anything.  Of a state of 6 layers
-// (33.5 MB a slot and layer), us with the caches / stores past them / both:
-// 1 slot to 8: 364 / 348 / 420, 4 to 8: 491 / 433 / 414, 1 to 2: 103 / 85 / 100;
-// 8 slots to 8 others: 707 / 728 / 684, closing up 8 of 16: 637 / 650 / 574.
-// Below those sizes the caches win (1 slot to 8 of one layer: 49 / 59 / 64;
-// 8 in a cycle: 78 / 84 / 97), and so they do in a long cycle, which reads a
-// slot again (20 slots: 1776 / 1851 / 1941).
-Past past_caches(const Program& p, int64_t slot_bytes) {
-  const int64_t cache = (int64_t)256 << 20, written = p.writes * slot_bytes;
-  if (written <= cache) return kCached;
-  if (2 * p.writes >= 3 * p.reads) return kStores;
-  return written > 2 * cache && !p.again ? kBoth : kCached;
+// Whether a call passes the caches by: what it moves is more than the last
+// level's 256 MB, so neither finds its slots there nor leaves them for the
+// layers.  Of a state of 6 layers (33.5 MB a slot and layer), us through the
+// caches / past them, after a call that filled them with other data: 1 slot to
+// another 97 / 76, 8 to 8 others 740 / 715, closing up 11 of 16 837 / 768, 4 to 8
+// 503 / 426, 1 to 2 126 / 112; but 1 to 8 385 / 434 (2 to 8 422 / 427), and 20 in
+// a cycle, which reads a slot again, 1835 / 2007.  Smaller calls whose slots the
+// caches hold win by them (2 to 2 others of two layers 39 / 47).
+bool past_caches(const Program& p, int64_t slot_bytes) {
+  return (p.reads + p.writes) * slot_bytes > (int64_t)256 << 20 && p.writes <= 3 * p.reads && !p.again;
 }
 
 }  // namespace
@@ -246,7 +242,7 @@ bdh_status copy_streams(const StreamMoves& m, hipStream_t st, uint64_t* launches
   order_moves(from, (int)m.src_batch, m.in_place, &p);
   int64_t slot = 0;
   for (int l = 0; l < m.n_layers; ++l) slot += m.slab[l];
-  const Past past = past_caches(p, slot * 4);
+  const bool past = past_caches(p, slot * 4);
   for (const Program::Launch& part : p.launches) {
     if (part.words.empty() && part.zero.empty()) continue;
     for (int l0 = 0; l0 < m.n_layers; l0 += kMaxLayers) {
@@ -264,8 +260,7 @@ bdh_status copy_streams(const StreamMoves& m, hipStream_t st, uint64_t* launches
       a.n_zero = (int32_t)part.zero.size();
       for (int i = 0; i < a.n; ++i) a.words[i] = part.words[i];
       for (int i = 0; i < a.n_zero; ++i) a.words[a.n + i] = part.zero[i];
-      const auto kernel = past == kCached ? move_streams_kernel<kCached>
-                          : past == kStores ? move_streams_kernel<kStores> : move_streams_kernel<kBoth>;
+      const auto kernel = past ? move_streams_kernel<true> : move_streams_kernel<false>;
       hipLaunchKernelGGL(kernel, dim3((uint32_t)((most + 1023) / 1024), (uint32_t)n), dim3(256), 0, st, a);
       BDH_HIP_TRY(hipGetLastError());
       ++*launches;

@@ -242,7 +242,7 @@ def test_captured_into_a_graph_and_on_another_stream():
 
 @pytest.mark.parametrize("name", ["fork", "close_up", "cycle", "cycle_and_forks", "from_another"])
 def test_calls_larger_than_the_caches(name):
-    # 16.8 MB a slot: 16 slots written are the last-level cache, 32 twice it.
+    # 16.8 MB a slot: each of these moves more than the last-level cache holds.
     torch = need_gpu()
     import burn_dragon_amd as bd
     B, shape = 48, (4, 4096, 256)
