@@ -1180,11 +1180,13 @@ bdh_status sample_typed(const SampleArgs& a, hipStream_t st, uint64_t* launches)
     *launches += 1;
     return BDH_OK;
   }
-  // Groups of rows, so that the scratch stays small (64 MB at 1024 rows of 40000).
-  const int64_t group = a.rows < 1024 ? a.rows : 1024;
   SplitArgs p;
   p.a = a;
   p.chunks = (int)((a.vocab + kChunk - 1) / kChunk);
+  // Groups of rows, so that the scratch stays below 170 MB (8 KB a chunk, 32 a
+  // row).  16384 chunks fill the chip many times over.
+  const int64_t most = 16384 / p.chunks < 1024 ? 16384 / p.chunks : 1024;
+  const int64_t group = a.rows < most ? a.rows : most;
   const size_t slots = (size_t)group * (size_t)p.chunks;
   const size_t sizes[] = {up(slots * 4), up(slots * 4), up(slots * kBins * 4), up(slots * kBins * 8),
                           up(slots * 4), up(slots * kNear * 8), up(slots * 8), up((size_t)group * kListMax * 8),

@@ -371,3 +371,21 @@ def test_unsupported_and_refused():
                 dict(min_p=2.0), dict(top_k=-1), dict(temperature=math.inf)):
         with pytest.raises(_lib.BdhError):
             bd.sample_tokens(x, u, **bad)
+
+
+@pytest.mark.parametrize("V,rows", [(1 << 20, 300), (400000, 700), (20000, 2100)])
+def test_rows_in_groups(V, rows):
+    # Long rows go through the scratch some at a time: one row of logits, shared.
+    torch = need_gpu()
+    import burn_dragon_amd as bd
+    rng = np.random.default_rng(V)
+    x = (rng.standard_normal((1, V)) * 3).astype(np.float32)
+    u = rng.random(rows).astype(np.float32)
+    announce("sampling in groups", V, rows)
+    t = torch.from_numpy(x).cuda().expand(rows, V)
+    got = bd.sample_tokens(t, torch.from_numpy(u).cuda(), top_p=0.9).tokens.cpu().numpy()
+    some = np.r_[0:3, 127:130, 255:258, rows - 2:rows]
+    want, _ = sampleref.sample(np.repeat(x, len(some), 0), u[some], top_p=0.9)
+    assert np.array_equal(got[some], want)
+    one = bd.sample_tokens(t[:1].expand(100, V), torch.from_numpy(u[-100:]).cuda(), top_p=0.9).tokens
+    assert np.array_equal(got[-100:], one.cpu().numpy())
