@@ -21,7 +21,8 @@
 //   2. The candidates of that bin go to a list.  Up to 64 are compared each with
 //      each in a wave, up to 256 by the workgroup; more are narrowed first by
 //      histograms of nine bits of (value, index), so equal logits are cut by
-//      index.  A list that overflows is read from the row again.
+//      index.  What a workgroup's list does not hold is read from a longer one in
+//      the scratch (long rows), or from the row again.
 //   3. The kept weights are summed by wave, and the draw descends into the
 //      wave, the stripe, the lane and the element that it falls in.
 //
@@ -35,6 +36,10 @@
 // rows are bound by the chain of block-wide steps, long ones by the launches in
 // turn up to some 50 rows; past that by the 64-bit 2^t and the histogram's atomics
 // of the first launch (2.8 TB/s), and by the second read.
+// Flat rows have many candidates in a cut's bin: 256 of 131072 normal logits of
+// deviation 0.2 with top-p 0.9 144 (803 where the workgroup went through the row
+// for what its list of 4096 could not hold; equal logits, which the scratch's list
+// cannot hold either, 971).
 #include "bdh_internal.h"
 
 namespace bdh {
@@ -45,7 +50,8 @@ constexpr int kBinsPerOctave = 10;  // 420 of the bins: see bin_of
 constexpr double kLeastT = -42.0;
 constexpr int kSmall = 64;       // candidates that one wave orders
 constexpr int kMid = 256;        // that the workgroup compares each with each
-constexpr int kListMax = 4096;   // candidates that the list holds
+constexpr int kListMax = 4096;   // candidates that a workgroup's list holds
+constexpr int kFarMax = 32768;   // that a long row's list in the scratch holds
 constexpr int kNear = 256;       // logits that a chunk lists for top-k
 constexpr int kChunkThreads = 512;
 constexpr int kChunkPer = 16;    // logits a thread
@@ -399,7 +405,8 @@ __device__ __forceinline__ bool is_candidate(const Cuts& q, int bin) {
          (bin == q.k_bin || (bin >= q.p_first && bin <= q.p_last) || (bin >= q.m_first && bin <= q.m_last));
 }
 
-// The candidates: in the list, or where it overflowed all of the row's logits.
+// The candidates: in the workgroup's list, in the scratch's where they are more,
+// or where that overflowed, too, all of the row's logits.
 template <typename T, int NT, int LIST>
 struct Candidates {
   Shared<NT, LIST>& sh;
@@ -408,7 +415,8 @@ struct Candidates {
   float m;
   float top;
   const Row& s;
-  int n;  // found; beyond LIST the list is not complete
+  int n;  // found; beyond LIST the workgroup's list is not complete, beyond kFarMax the scratch's
+  const uint64_t* far;  // the scratch's, or null
 
   // Calls f(order, bin) for each whose bin lies in [first, last].
   template <typename F>
@@ -416,6 +424,12 @@ struct Candidates {
     if (n <= LIST) {
       for (int i = threadIdx.x; i < n; i += NT) {
         const uint64_t o = sh.list[i];
+        const int b = bin_of(value_of(o), top, s.cb);
+        if (b >= first && b <= last) f(o, b);
+      }
+    } else if (far && n <= kFarMax) {
+      for (int i = threadIdx.x; i < n; i += NT) {
+        const uint64_t o = far[i];
         const int b = bin_of(value_of(o), top, s.cb);
         if (b >= first && b <= last) f(o, b);
       }
@@ -447,24 +461,32 @@ struct Candidates {
       }
       __syncthreads();
       uint64_t low = ~0ull, high_o = 0;
+      int count = 0;
       each(first, last, [&](uint64_t o, int) {
-        const bool in = o >= lo && o <= hi;
-        const int at = append_at(&sh.n_small, in);
-        if (at >= 0 && at < kSmall) sh.small[at] = o;
-        if (in) {
-          low = o < low ? o : low;
-          high_o = o > high_o ? o : high_o;
-        }
+        if (o < lo || o > hi) return;
+        ++count;
+        low = o < low ? o : low;
+        high_o = o > high_o ? o : high_o;
       });
       low = ~wave_max_u64(~low);
       high_o = wave_max_u64(high_o);
-      if ((threadIdx.x & 63) == 0 && high_o) {
+      count = (int)wave_sum_u64((uint64_t)count);
+      if ((threadIdx.x & 63) == 0 && count) {
+        atomicAdd(&sh.n_small, count);
         atomicMin((unsigned long long*)&sh.lo, (unsigned long long)low);
         atomicMax((unsigned long long*)&sh.hi, (unsigned long long)high_o);
       }
       __syncthreads();
       const int n_in = sh.n_small;
       if (n_in <= kSmall) {
+        __syncthreads();
+        if (threadIdx.x == 0) sh.n_small = 0;
+        __syncthreads();
+        each(first, last, [&](uint64_t o, int) {
+          const int at = append_at(&sh.n_small, o >= lo && o <= hi);
+          if (at >= 0) sh.small[at] = o;
+        });
+        __syncthreads();
         if (threadIdx.x < 64) {
           const int lane = threadIdx.x;
           const uint64_t mine = lane < n_in ? sh.small[lane] : ~0ull;
@@ -751,7 +773,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a) {
       if (at >= 0 && at < LIST) sh.list[at] = order_of(x[e], index_of<E>(0, e));
     }
     __syncthreads();
-    Candidates<T, NT, LIST> cand{sh, row, vocab, m, top, s, sh.n_list};
+    Candidates<T, NT, LIST> cand{sh, row, vocab, m, top, s, sh.n_list, nullptr};
     const uint64_t lim = cand.limit(q);
     if (lim != ~0ull) {
       limit_x = value_of(lim);
@@ -799,7 +821,7 @@ struct SplitArgs {
   int32_t* near_n;   // [rows, chunks]: logits in `near`, -1: they are not all there
   uint64_t* near;    // [rows, chunks, kNear]: the logits up to the bin of the chunk's k-th
   uint64_t* sure;    // [rows, chunks]
-  uint64_t* list;    // [rows, kListMax]
+  uint64_t* list;    // [rows, kFarMax]
   RowState* state;   // [rows]
 };
 
@@ -988,7 +1010,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_gather_kernel(const Spli
   at += first + (int)wave_scan_u64((uint64_t)__popc(mine)) - __popc(mine);
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    if ((mine >> e & 1) && at < kListMax) p.list[lr * kListMax + at] = order_of(x[e], index_of<E>(base, e));
+    if ((mine >> e & 1) && at < kFarMax) p.list[lr * kFarMax + at] = order_of(x[e], index_of<E>(base, e));
     at += mine >> e & 1;
   }
 }
@@ -1039,7 +1061,7 @@ __device__ void draw_from_list(Shared<NT, LIST>& sh, const SampleArgs& a, const 
     __syncthreads();
     n_cut = sh.n_list;
   }
-  const uint64_t lim = Candidates<T, NT, LIST>{sh, nullptr, 0, m, top, s, n_cut}.limit(q);
+  const uint64_t lim = Candidates<T, NT, LIST>{sh, nullptr, 0, m, top, s, n_cut, nullptr}.limit(q);
   __syncthreads();
   if (threadIdx.x == 0) sh.n_small = 0;
   __syncthreads();
@@ -1118,9 +1140,9 @@ __global__ __launch_bounds__(kChunkThreads) void sample_finish_kernel(const Spli
   for (int g = threadIdx.x; g < p.chunks; g += NT) chunk_sum[g] = p.sure[lr * p.chunks + g];
   const int n = st.n_list;
   if (n <= LIST)
-    for (int i = threadIdx.x; i < n; i += NT) sh.list[i] = p.list[lr * kListMax + i];
+    for (int i = threadIdx.x; i < n; i += NT) sh.list[i] = p.list[lr * kFarMax + i];
   __syncthreads();
-  Candidates<T, NT, LIST> cand{sh, row, (int)a.vocab, m, st.top, s, n};
+  Candidates<T, NT, LIST> cand{sh, row, (int)a.vocab, m, st.top, s, n, p.list + lr * kFarMax};
   const uint64_t lim = cand.limit(st.cuts);
   const float limit_x = lim != ~0ull ? value_of(lim) : -INFINITY;
   const int limit_i = lim != ~0ull ? (int)(uint32_t)lim : -1;  // (-inf itself is not kept)
@@ -1183,13 +1205,13 @@ bdh_status sample_typed(const SampleArgs& a, hipStream_t st, uint64_t* launches)
   SplitArgs p;
   p.a = a;
   p.chunks = (int)((a.vocab + kChunk - 1) / kChunk);
-  // Groups of rows, so that the scratch stays below 170 MB (8 KB a chunk, 32 a
-  // row).  16384 chunks fill the chip many times over.
-  const int64_t most = 16384 / p.chunks < 1024 ? 16384 / p.chunks : 1024;
+  // Groups of rows, so that the scratch stays below 270 MB (8 KB a chunk, 256 a
+  // row).  16384 chunks, or 512 rows, fill the chip many times over.
+  const int64_t most = 16384 / p.chunks < 512 ? 16384 / p.chunks : 512;
   const int64_t group = a.rows < most ? a.rows : most;
   const size_t slots = (size_t)group * (size_t)p.chunks;
   const size_t sizes[] = {up(slots * 4), up(slots * 4), up(slots * kBins * 4), up(slots * kBins * 8),
-                          up(slots * 4), up(slots * kNear * 8), up(slots * 8), up((size_t)group * kListMax * 8),
+                          up(slots * 4), up(slots * kNear * 8), up(slots * 8), up((size_t)group * kFarMax * 8),
                           up((size_t)group * sizeof(RowState))};
   size_t bytes = 0;
   for (size_t s : sizes) bytes += s;

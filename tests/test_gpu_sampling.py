@@ -389,3 +389,15 @@ def test_rows_in_groups(V, rows):
     assert np.array_equal(got[some], want)
     one = bd.sample_tokens(t[:1].expand(100, V), torch.from_numpy(u[-100:]).cuda(), top_p=0.9).tokens
     assert np.array_equal(got[-100:], one.cpu().numpy())
+
+
+@pytest.mark.parametrize("V,spread", [(60000, 0.02), (131072, 0.2), (131072, 0.02), (200000, 0.7)])
+def test_flat_rows_with_many_candidates(V, spread):
+    # A cut's bin holds more than a workgroup's list, or than the scratch's.
+    torch = need_gpu()
+    import burn_dragon_amd as bd
+    rng = np.random.default_rng(V)
+    for kw in (dict(top_p=0.9), dict(min_p=0.05 if spread > 0.5 else 0.98), dict(top_k=2000),
+               dict(top_k=20000, top_p=0.5), dict(top_k=V - 5, top_p=0.3, min_p=0.5)):
+        announce("flat rows", V, spread, kw)
+        check(torch, bd, rng.standard_normal((3, V)) * spread, rng.random(3), **kw)
