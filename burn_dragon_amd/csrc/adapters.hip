@@ -31,7 +31,7 @@ namespace {
 constexpr int kTile = 16;
 constexpr int kGatherTokens = 16;  // up to here tiles gather sequences
 constexpr int kWindow = 512;       // sequences of the batch that are gathered together
-constexpr int kRowsTokens = 2, kRowsIn = 512;  // up to here, at ranks to 16, no tiles but adapter_rows_kernel
+constexpr int kRowsTokens = 2, kRowsIn = 512;  // up to here, at ranks to 16, adapter_rows_kernel may do without tiles
 constexpr int kRowsShare = 8;                  // the sequences it gathers
 
 typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
@@ -380,10 +380,10 @@ __device__ __forceinline__ float sum16(float v) {
 }
 
 // Gathered rows at ranks to 16 without matrix cores, u computed here: a thread
-// holds four columns' rows of B and runs over the rows.  A tile of the product
-// would be mostly empty, and what counts is how much a workgroup asks for at
-// once: of 64 rows with 32 adapters (D 256, V 32000, R 16) 12.5 us where the
-// tiles take 23.6 (at rank 32 and D 512 36 where they take 25).
+// holds four columns' rows of B and runs over the rows.  Where a tile of the
+// product would be mostly empty, what counts is how much a workgroup asks for at
+// once: of 64 rows with 32 adapters (D 256, V 32000, R 16) 12.2 us where the
+// tiles take 23.7 (at rank 32 and D 512 36 where they take 25).
 template <typename T>
 __global__ __launch_bounds__(256) void adapter_rows_kernel(const AdapterArgs a) {
   constexpr int RP = 16, VPT = 4;
@@ -487,7 +487,15 @@ template <typename T, int RP, bool EVEN>
 bdh_status run_typed(AdapterArgs a, hipStream_t st, uint64_t* launches) {
   const bool gather = a.time <= kGatherTokens;
   if constexpr (EVEN && RP == 16) {
-    if (a.time <= kRowsTokens && a.in_dim <= kRowsIn) {
+    // Without tiles where those would be mostly empty (few rows an adapter of the
+    // set) in a call large enough.  us, this / tiles, D 256, V 32000, R 16:
+    //   f32   64 rows of 32 adapters 12.2 / 23.7, of 8 12.8 / 15.3; 256 of 16 28.9 / 27.1
+    //   bf16  64 rows of 32 adapters 12.7 / 18.6, of 8 11.9 / 11.3; one 5.9 / 4.9
+    //   two tokens, f32  64 sequences of 32 adapters 15.5 / 25.5, of 8 22.6 / 17.5;
+    //   at V 256 16 of 4 8.5 / 5.9
+    const bool one_f32 = sizeof(T) == 4 && a.time == 1;
+    if (a.time <= kRowsTokens && a.in_dim <= kRowsIn && a.batch * a.time <= (one_f32 ? 8 : 4) * a.n &&
+        (one_f32 || a.batch * a.out_dim >= (int64_t)1 << 20)) {
       hipLaunchKernelGGL((adapter_rows_kernel<T>), dim3((uint32_t)cdiv(a.out_dim, 1024), (uint32_t)a.batch), dim3(256),
                          0, st, a);
       BDH_HIP_TRY(hipGetLastError());

@@ -261,3 +261,10 @@ def test_more_sequences_than_are_gathered_together(T, D, R):
     B = 1100
     run(B, T, D, 70, R, 3, "float32", np.random.default_rng(T).integers(-1, 3, B).tolist())
     run(B, T, D, 70, R, 3, "float32", [1] * B, in_place=True)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("T,D,R,n", [(1, 24, 8, 16), (2, 24, 8, 20), (1, 512, 16, 10), (2, 512, 16, 30), (2, 64, 16, 2)])
+def test_few_rows_of_an_adapter_in_a_large_call(T, D, R, n, dtype):
+    # 40 x 30001: with and without tiles by the number of adapters.
+    run(40, T, D, 30001, R, n, dtype, np.random.default_rng(n).integers(-1, n, 40).tolist())
