@@ -27,7 +27,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from .adapters import AdapterSet, apply_adapters
+from .adapters import AdapterSet, adapter_plan, apply_adapters
 from .layer import LowRankWeights, lowrank_layer_forward
 from .recurrent import DEFAULT_ROPE_THETA, _ptr, _stream_ptr, supports_backend
 
@@ -93,18 +93,14 @@ def model_forward_logits(tokens: torch.Tensor, weights: BdhModelWeights, *,
     every layer's projection options (lowrank_layer_forward).  With
     ``adapters`` (of D into vocab) each sequence's logits gain its own
     adapter's product, ``adapter_ids`` [B] int32 on the device
-    (apply_adapters)."""
+    (apply_adapters); what does not fit or is not supported of them is refused
+    (ValueError or None) before a layer runs.  A call that fails later, for
+    want of device memory or of scratch under capture, may leave layers moved
+    on at the old position: the state is then to be restored."""
     if not supports_backend() or weights is None:
         return None
     if (adapters is None) != (adapter_ids is None):
         raise ValueError("adapters and adapter_ids come together")
-    if adapters is not None:  # before any layer moves the state on
-        n, rank = adapters.a.shape[:2]
-        if (adapters.a.shape[2:] != (weights.layer.embd,) or adapters.b.shape != (n, weights.vocab, rank)
-                or adapter_ids.shape != tokens.shape[:1]):
-            raise ValueError("adapters and adapter_ids do not fit the model and the batch")
-        if rank > 128 or adapters.a.dtype != torch.bfloat16 or adapters.b.dtype != torch.bfloat16:
-            return None
     if state is not None:
         if len(state.rho) != weights.n_layer:
             return None
@@ -114,6 +110,9 @@ def model_forward_logits(tokens: torch.Tensor, weights: BdhModelWeights, *,
     B, T = tokens.shape
     D = weights.layer.embd
     dev = tokens.device
+    # Before any layer moves the state on.
+    if adapters is not None and adapter_plan((B, T, weights.vocab), (B, T, D), dev, adapters, adapter_ids) is None:
+        return None
     stream = _stream_ptr(dev)
     lib = _lib.load()
     tok = tokens.contiguous()

@@ -54,3 +54,30 @@ def test_python_surface_without_a_device():
 def test_time_past_the_grid_is_refused():
     assert call(batch=1, time=65535 * 64 + 1) == _lib.BDH_UNSUPPORTED
     assert "large" in _lib.last_error()
+
+
+def test_the_plan_s_limits_are_the_library_s():
+    # The largest of each size that the plan takes passes the library's check of
+    # sizes too (and ends at the misaligned base); one more is refused by both.
+    torch = pytest.importorskip("torch")
+    from burn_dragon_amd import AdapterSet
+    from burn_dragon_amd import adapters as ad
+
+    def plan(batch, time, in_dim, out_dim, rank, adapters):
+        one = torch.zeros(1, dtype=torch.bfloat16)
+        s = AdapterSet(one.expand(adapters, rank, in_dim), one.expand(adapters, out_dim, rank),
+                       torch.ones(1).expand(adapters))
+        return ad.adapter_plan((batch, time, out_dim), (batch, time, in_dim), torch.device("cpu"), s,
+                               torch.zeros(1, dtype=torch.int32).expand(batch))
+    for size, most in (("batch", 65535), ("time", 65535 * 64), ("in_dim", 1 << 20), ("out_dim", 1 << 22),
+                       ("rank", 128), ("adapters", 1 << 20)):
+        small = dict(batch=1, time=1, in_dim=1, out_dim=1, rank=1, adapters=1)
+        p = plan(**{**small, size: most})
+        assert [getattr(p, k) for k in SIZES] == [{**small, size: most}[k] for k in SIZES]
+        assert call(base=MB + 2, **{**small, size: most}) == _lib.BDH_EINVAL and "aligned" in _lib.last_error()
+        assert plan(**{**small, size: most + 1}) is None
+        assert call(base=MB + 2, **{**small, size: most + 1}) == _lib.BDH_UNSUPPORTED
+    rows = dict(batch=4, in_dim=1, out_dim=1, rank=1, adapters=1)
+    assert plan(time=1 << 21, **rows) is not None and plan(time=(1 << 21) + 1, **rows) is None
+    assert call(base=MB + 2, **rows, time=1 << 21) == _lib.BDH_EINVAL
+    assert call(base=MB + 2, **rows, time=(1 << 21) + 1) == _lib.BDH_UNSUPPORTED
