@@ -13,7 +13,7 @@ import torch
 from .adapters import AdapterSet
 from .model import BdhModelState, BdhModelWeights, model_forward_logits, new_model_state
 from .recurrent import DEFAULT_ROPE_THETA
-from .sampling import PerRow, sample_tokens
+from .sampling import PerRow, check_settings, sample_tokens
 
 
 class GenerateOutput(NamedTuple):
@@ -34,14 +34,21 @@ def generate_tokens(prompt: torch.Tensor, weights: BdhModelWeights, uniform: tor
     numbers.  ``state`` (default: a new one) is continued in place and holds
     the prompt and all drawn tokens but the last, which the next call's
     prompt begins with.  The cuts are sample_tokens', the other options
-    model_forward_logits'.  Returns None where the library does not support a
-    call; the state then holds what ran."""
+    model_forward_logits'.  Settings, random numbers and adapters that do not
+    fit are refused with those calls' errors before the prompt runs.  Returns
+    None where the library does not support a call: for the arguments' types
+    and sizes, before the prompt runs; for want of scratch under capture, with
+    what ran in the state."""
     if weights is None or prompt.dim() != 2 or not prompt.is_cuda:
         return None
     B = prompt.shape[0]
     if uniform.dim() != 2 or uniform.shape[0] == 0 or uniform.shape[1] != B:
         raise ValueError(f"uniform must be [steps, {B}]")
     steps = uniform.shape[0]
+    if uniform.device != prompt.device:
+        raise ValueError("uniform must be on the prompt's device")
+    if not check_settings(B, weights.vocab, uniform[0], temperature, top_k, top_p, min_p):
+        return None
     if state is None:
         state = new_model_state(weights, B, prompt.device)
     tokens = torch.empty((steps, B), device=prompt.device, dtype=torch.int32)

@@ -11,6 +11,7 @@ whatever the batch around a row.
 from __future__ import annotations
 
 import ctypes
+import math
 from typing import NamedTuple, Optional, Union
 
 import torch
@@ -33,6 +34,42 @@ def _per_row(value, rows: int, dtype: torch.dtype, device, name: str):
     if value.dtype != dtype or value.shape != (rows,) or value.device != device:
         raise ValueError(f"{name} must be a number or a {dtype} tensor of [{rows}] on the logits' device")
     return 0, value.contiguous()
+
+
+def _options(rows: int, vocab: int, dev: torch.device, uniform: torch.Tensor, temperature: PerRow,
+             top_k: Union[int, torch.Tensor], top_p: PerRow, min_p: PerRow):
+    """The library's options and the tensors that they point to; raises
+    ValueError where the random numbers or a setting a row do not fit."""
+    if uniform.dtype != torch.float32 or uniform.shape != (rows,) or uniform.device != dev:
+        raise ValueError(f"uniform must be a f32 tensor of [{rows}] on the logits' device")
+    temp, temp_rows = _per_row(temperature, rows, torch.float32, dev, "temperature")
+    p, p_rows = _per_row(top_p, rows, torch.float32, dev, "top_p")
+    mp, mp_rows = _per_row(min_p, rows, torch.float32, dev, "min_p")
+    k, k_rows = _per_row(top_k, rows, torch.int32, dev, "top_k")
+    if k_rows is None:
+        k = min(int(k), vocab) if k > 0 else int(k)
+    opts = _lib.BdhSampleOptions(float(temp), float(p), float(mp), k, _ptr(temp_rows), _ptr(p_rows),
+                                 _ptr(mp_rows), _ptr(k_rows))
+    return opts, (temp_rows, p_rows, mp_rows, k_rows)
+
+
+def check_settings(rows: int, vocab: int, uniform: torch.Tensor, temperature: PerRow,
+                   top_k: Union[int, torch.Tensor], top_p: PerRow, min_p: PerRow) -> bool:
+    """What sample_tokens would say to [rows, vocab] logits on uniform's device
+    with these arguments, before there are any: False where it returns None
+    for their size, its errors where it raises."""
+    o, _ = _options(rows, vocab, uniform.device, uniform, temperature, top_k, top_p, min_p)
+    if not 0 < rows < 1 << 22 or not 0 < vocab <= 1 << 20:
+        return False
+    if not o.temperature_rows and not 0.0 <= o.temperature < math.inf:
+        raise _lib.BdhError("temperature must be finite and not negative")
+    if not o.top_p_rows and not 0.0 <= o.top_p <= 1.0:
+        raise _lib.BdhError("top_p must lie in [0, 1]")
+    if not o.min_p_rows and not 0.0 <= o.min_p <= 1.0:
+        raise _lib.BdhError("min_p must lie in [0, 1]")
+    if not o.top_k_rows and o.top_k < 0:
+        raise _lib.BdhError("top_k must not be negative")
+    return True
 
 
 def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: PerRow = 1.0,
@@ -63,15 +100,8 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: P
     row_stride, stride = logits.stride()
     if vocab > 1 and stride != 1:
         logits, row_stride = logits.contiguous(), vocab
-    if uniform.dtype != torch.float32 or uniform.shape != (rows,) or uniform.device != dev:
-        raise ValueError(f"uniform must be a f32 tensor of [{rows}] on the logits' device")
+    opts, rows_of = _options(rows, vocab, dev, uniform, temperature, top_k, top_p, min_p)
     uniform = uniform.contiguous()
-    temp, temp_rows = _per_row(temperature, rows, torch.float32, dev, "temperature")
-    p, p_rows = _per_row(top_p, rows, torch.float32, dev, "top_p")
-    mp, mp_rows = _per_row(min_p, rows, torch.float32, dev, "min_p")
-    k, k_rows = _per_row(top_k, rows, torch.int32, dev, "top_k")
-    if k_rows is None:
-        k = min(int(k), vocab) if k > 0 else int(k)
     if out is None:
         tokens = torch.empty(rows, device=dev, dtype=torch.int32)
     elif (out.dtype != torch.int32 or out.shape != (rows,) or out.device != dev
@@ -80,8 +110,7 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: P
     else:
         tokens = out
     logprob = torch.empty(rows, device=dev, dtype=torch.float32) if want_logprob else None
-    opts = _lib.BdhSampleOptions(float(temp), float(p), float(mp), k, _ptr(temp_rows), _ptr(p_rows),
-                                 _ptr(mp_rows), _ptr(k_rows))
+    # (rows_of holds what opts points to until the launch is enqueued.)
     st = _call_on(dev, _lib.load().bdh_sample_tokens, _ptr(logits), code, rows, vocab,
                   row_stride if rows > 1 else 0, _ptr(uniform), ctypes.byref(opts), _ptr(tokens),
                   _ptr(logprob), _stream_ptr(dev))

@@ -76,3 +76,62 @@ def test_adapters_that_a_forward_refuses(name):
     want = bd.model_forward_logits(tokens, w, state=again, adapters=s, adapter_ids=ids)
     torch.cuda.synchronize()
     assert torch.equal(got, want) and state.position == again.position == 12
+
+
+def per_row(torch, v, dtype, n=B):
+    return torch.full((n,), v, dtype=getattr(torch, dtype), device="cuda")
+
+
+# How each changes generate_tokens' arguments, given torch and uniform, and the error.
+BAD_DRAWS = {
+    "uniform_f64": (lambda t, u: dict(uniform=u.double()), ValueError),
+    "uniform_on_the_host": (lambda t, u: dict(uniform=u.cpu()), ValueError),
+    "uniform_of_another_batch": (lambda t, u: dict(uniform=u[:, :2]), ValueError),
+    "top_k_int64": (lambda t, u: dict(top_k=per_row(t, 5, "int64")), ValueError),
+    "top_k_of_another_batch": (lambda t, u: dict(top_k=per_row(t, 5, "int32", 2)), ValueError),
+    "temperature_f64": (lambda t, u: dict(temperature=per_row(t, 1, "float64")), ValueError),
+    "top_p_on_the_host": (lambda t, u: dict(top_p=per_row(t, 1, "float32").cpu()), ValueError),
+    "min_p_int": (lambda t, u: dict(min_p=per_row(t, 0, "int32")), ValueError),
+    "temperature_negative": (lambda t, u: dict(temperature=-1.0), "BdhError"),
+    "temperature_nan": (lambda t, u: dict(temperature=float("nan")), "BdhError"),
+    "temperature_past_f32": (lambda t, u: dict(temperature=1e39), "BdhError"),
+    "top_p_above_1": (lambda t, u: dict(top_p=1.5), "BdhError"),
+    "min_p_negative": (lambda t, u: dict(min_p=-0.1), "BdhError"),
+    "top_k_negative": (lambda t, u: dict(top_k=-1), "BdhError"),
+}
+
+
+@pytest.mark.parametrize("name", sorted(BAD_DRAWS))
+def test_draws_that_generation_refuses(name):
+    torch = need_gpu()
+    import burn_dragon_amd as bd
+    from burn_dragon_amd import _lib
+    g, w, _, state, tokens, _ = build(torch, bd)
+    u = torch.rand(3, B, generator=g, device="cuda")
+    change, error = BAD_DRAWS[name]
+    error = _lib.BdhError if error == "BdhError" else error
+    bad = {**dict(uniform=u), **change(torch, u)}
+    kept = [r.clone() for r in state.rho]
+    announce("generation refuses", name)
+    refused(torch, state, kept,
+            lambda: bd.generate_tokens(tokens, w, bad["uniform"], state=state,
+                                       **{k: v for k, v in bad.items() if k != "uniform"}), error)
+    # sample_tokens says the same of these arguments
+    logits = torch.zeros(B, V, device="cuda")
+    with pytest.raises(error):
+        bd.sample_tokens(logits, bad["uniform"][0], **{k: v for k, v in bad.items() if k != "uniform"})
+
+
+def test_adapters_and_prompts_that_generation_refuses():
+    torch = need_gpu()
+    import burn_dragon_amd as bd
+    g, w, s, state, tokens, ids = build(torch, bd)
+    u = torch.rand(2, B, generator=g, device="cuda")
+    kept = [r.clone() for r in state.rho]
+    announce("generation refuses adapters, prompts")
+    for kw, error in ((dict(adapters=s, adapter_ids=ids.long()), ValueError), (dict(adapters=s), ValueError),
+                      (dict(adapters=s._replace(scale=s.scale.double()), adapter_ids=ids), ValueError)):
+        refused(torch, state, kept, lambda: bd.generate_tokens(tokens, w, u, state=state, **kw), error)
+    refused(torch, state, kept, lambda: bd.generate_tokens(tokens.long(), w, u, state=state), None)
+    refused(torch, state, kept, lambda: bd.generate_tokens(tokens[:, :0], w, u, state=state), None)
+    refused(torch, state, kept, lambda: bd.generate_tokens(tokens, w, u[:0], state=state), ValueError)
