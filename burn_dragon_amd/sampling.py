@@ -47,7 +47,7 @@ def _options(rows: int, vocab: int, dev: torch.device, uniform: torch.Tensor, te
     mp, mp_rows = _per_row(min_p, rows, torch.float32, dev, "min_p")
     k, k_rows = _per_row(top_k, rows, torch.int32, dev, "top_k")
     if k_rows is None:
-        k = min(int(k), vocab) if k > 0 else int(k)
+        k = min(max(int(k), -1), vocab)  # (an int32 to the library)
     opts = _lib.BdhSampleOptions(float(temp), float(p), float(mp), k, _ptr(temp_rows), _ptr(p_rows),
                                  _ptr(mp_rows), _ptr(k_rows))
     return opts, (temp_rows, p_rows, mp_rows, k_rows)

@@ -98,6 +98,7 @@ BAD_DRAWS = {
     "top_p_above_1": (lambda t, u: dict(top_p=1.5), "BdhError"),
     "min_p_negative": (lambda t, u: dict(min_p=-0.1), "BdhError"),
     "top_k_negative": (lambda t, u: dict(top_k=-1), "BdhError"),
+    "top_k_0_mod_2_32": (lambda t, u: dict(top_k=-2 ** 32), "BdhError"),
 }
 
 
