@@ -77,7 +77,9 @@ __device__ Row row_settings(const SampleArgs& a, int64_t r) {
   s.k = a.top_k_rows ? a.top_k_rows[r] : a.top_k;
   s.greedy = !(tau > 0.0f) || s.k == 1;
   s.c = 1.4426950408889634074 / (double)tau;
-  s.cb = (float)fmax(fmin(s.c * kBinsPerOctave, 1e30), 1e-30);  // (finite times -inf: -inf)
+  // Above 0, so that -inf stays -inf; below the least that a finite temperature
+  // gives (4e-38), so that bins are as wide as the weights' at any of them.
+  s.cb = (float)fmax(fmin(s.c * kBinsPerOctave, 1e30), 0x1p-126);
   s.use_k = s.k > 0 && s.k < a.vocab;
   s.use_p = p < 1.0f;
   s.p = p > 0.0f ? (double)p : 0.0;

@@ -401,3 +401,20 @@ def test_flat_rows_with_many_candidates(V, spread):
                dict(top_k=20000, top_p=0.5), dict(top_k=V - 5, top_p=0.3, min_p=0.5)):
         announce("flat rows", V, spread, kw)
         check(torch, bd, rng.standard_normal((3, V)) * spread, rng.random(3), **kw)
+
+
+@pytest.mark.parametrize("V", [40, 3000, 40000])
+@pytest.mark.parametrize("temperature,scale", [(1e31, 1e31), (1e33, 2e33), (1e37, 2e37), (3e38, 6e37),
+                                               (math.inf, 6e37), (1e-28, 2e-28), (1e-33, 3e-33), (1e-37, 3e-37),
+                                               (1e-42, 2e-42), (1e-45, 6e-45)])
+def test_temperatures_from_the_least_to_the_largest(V, temperature, scale):
+    # Logits as large as the temperature: their weights are those of ordinary rows.
+    torch = need_gpu()
+    import burn_dragon_amd as bd
+    rng = np.random.default_rng(V + 17)
+    x = np.clip(rng.standard_normal((4, V)) * scale, -sampleref.F32_MAX, sampleref.F32_MAX).astype(np.float32)
+    u = rng.random(4).astype(np.float32)
+    rows = np.full(4, temperature, np.float32)
+    for cut in ({}, dict(top_k=20), dict(top_k=V // 2), dict(top_p=0.7), dict(top_k=V // 3, top_p=0.8, min_p=0.05)):
+        announce("sample hot", V, temperature, cut)
+        check(torch, bd, x, u, settings=dict(temperature=torch.from_numpy(rows).cuda(), **cut), temperature=rows, **cut)
