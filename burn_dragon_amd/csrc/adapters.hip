@@ -7,8 +7,10 @@
 // operands of a product go in as bf16 parts, each the rounded rest of the ones
 // before it: three parts are an f32 to 2^-24 of it, two to 2^-16.  f32 hidden
 // and u = scale hidden A^T take three; bf16 hidden is one, and its u takes two
-// (out rounds to 2^-8).  u's parts stand side by side, as one product of two or
-// three times the depth with the same columns of B.
+// (out rounds to 2^-8).  Parts below 2^-126 are subnormal bf16, which the matrix
+// cores keep: nothing is held closer than half the least of them, 2^-134, so f32
+// values below 2^-110 lose their last bits.  u's parts stand side by side, as one
+// product of two or three times the depth with the same columns of B.
 //
 // Rows of a tile: of prompts, 16 of one sequence; with up to 16 tokens a
 // sequence (generation), gathered from the sequences of one adapter, so that B
@@ -43,8 +45,10 @@ __device__ __forceinline__ int adapter_of(const AdapterArgs& a, int64_t b) {
 }
 
 // The next bf16 part of an f32 whose rest is x.  (An infinity is one part.)
-__device__ __forceinline__ bf16_t next_part(float& x) {
-  const bf16_t p = (bf16_t)x;
+// first: what would round past bf16's largest is cut there, and its rest goes on.
+__device__ __forceinline__ bf16_t next_part(float& x, bool first) {
+  bf16_t p = (bf16_t)x;
+  if (first && fabsf((float)p) == INFINITY) p = __builtin_bit_cast(bf16_t, (uint16_t)(__float_as_uint(x) >> 16));
   x = fabsf((float)p) < INFINITY ? x - (float)p : 0.0f;
   return p;
 }
@@ -160,7 +164,7 @@ struct UTile {
 #pragma unroll
           for (int q = 0; q < HP; ++q)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) p[q][j] = next_part(f[i][j]);
+            for (int j = 0; j < 8; ++j) p[q][j] = next_part(f[i][j], q == 0);
         } else {
           p[0] = x[i];
         }
@@ -191,7 +195,7 @@ struct UTile {
     for (int i = 0; i < PER; ++i) {
       const int at = threadIdx.x + 256 * i, r = at / RP, k = at % RP;
 #pragma unroll
-      for (int q = 0; q < UP; ++q) mem.u[r][q * RP + k] = next_part(s[i]);
+      for (int q = 0; q < UP; ++q) mem.u[r][q * RP + k] = next_part(s[i], q == 0);
       if (ROW > DEPTH) mem.u[r][DEPTH + k] = (bf16_t)0.0f;
     }
     static_assert(ROW == DEPTH || ROW - DEPTH == RP, "one part of zeros");

@@ -307,9 +307,10 @@ bdh_status bdh_lm_logits(const float* hidden, int64_t rows, int64_t embd,
  * out_dim, rank] bf16 (a linear layer's [out, in] weights); scale [adapters]
  * f32; ids [batch] int32 on the device, one adapter a sequence: an id outside
  * [0, adapters) leaves out = base.  out may be base (in place), and otherwise
- * shares no memory with the inputs.  Products and sums are f32, with BDH_F32 to
- * f32's own precision (on the matrix cores in three bf16 parts), and out is
- * rounded once.  An infinity or NaN of hidden reaches its own row, one of an
+ * shares no memory with the inputs.  Sums are f32.  hidden and u = scale
+ * hidden A^T enter the matrix cores in bf16 parts: with BDH_F32 three, so a value
+ * is held to 2^-24 of it (or to 2^-134, below 2^-110); with BDH_BF16 hidden is
+ * exact and u is held to 2^-16 of it.  out is rounded once.  An infinity or NaN of hidden reaches its own row, one of an
  * adapter (whose values are meant to be finite) its own sequences.  rank up to
  * 128.  Pointers aligned to their elements.  Uses the stream's scratch, but for
  * small calls.  No counterpart in the reference, which adapts a model by

@@ -268,3 +268,61 @@ def test_more_sequences_than_are_gathered_together(T, D, R):
 def test_few_rows_of_an_adapter_in_a_large_call(T, D, R, n, dtype):
     # 40 x 30001: with and without tiles by the number of adapters.
     run(40, T, D, 30001, R, n, dtype, np.random.default_rng(n).integers(-1, n, 40).tolist())
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("T,D,R", [(1, 64, 16), (1, 64, 32), (40, 64, 16), (40, 64, 64), (20, 33, 5), (1, 33, 5),
+                                   (40, 2048, 8)])
+def test_values_up_to_f32_s_largest(T, D, R, dtype):
+    # hidden, and scale hidden A^T, between bf16's largest finite value and f32's.
+    torch = need_gpu()
+    import burn_dragon_amd as bd
+    dtype = getattr(torch, dtype)
+    V = 300
+    base, hidden, a, b, scale = make(torch, 2, T, D, V, R, 2, dtype)
+    top = float(torch.finfo(dtype).max)
+    hidden.zero_()
+    hidden[0, :, 0] = top                      # f32: 2^128 (1 - 2^-24)
+    hidden[1, :, 1] = -top
+    a.zero_()
+    a[0, :, 0] = 0.5
+    a[1, :, 1] = 1.0
+    b.mul_(2.0 ** -100)
+    # f32: 0.5 top * 1.99 and -top; bf16, whose largest is 2^128 (1 - 2^-8): beyond that again
+    scale = torch.tensor([1.99, 1.0 if dtype == torch.float32 else 1.003], device="cuda")
+    ids = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    base.mul_(2.0 ** 28)
+    announce("adapters near the largest", T, D, R, dtype)
+    out = bd.apply_adapters(base, hidden, bd.AdapterSet(a, b, scale), ids)
+    torch.cuda.synchronize()
+    assert bool(out.isfinite().all())
+    check(torch, out, base, hidden, a, b, scale, ids)
+
+
+@pytest.mark.parametrize("T,D,R", [(1, 64, 32), (40, 64, 16), (20, 33, 5)])
+def test_small_values_hold_to_2_134(T, D, R):
+    # Parts below 2^-126 are subnormal: an operand is held to half the least of
+    # them, 2^-134, where that is more than 2^-24 of it.  Of a row each operand
+    # meets one value of the other here, so that what it lost is seen alone.
+    torch = need_gpu()
+    import burn_dragon_amd as bd
+    V = 300
+    base, hidden, a, b, scale = make(torch, 1, T, D, V, R, 1, torch.float32)
+    g = torch.Generator(device="cuda").manual_seed(T + D)
+    a.zero_()
+    b.zero_()
+    for k in range(R):
+        a[0, k, k] = 1.0
+        b[0, k, k] = 2.0 ** 90
+    ids = torch.zeros(1, dtype=torch.int32, device="cuda")
+    m = 1 + torch.rand(1, T, D, generator=g, device="cuda")
+    announce("adapters small", T, D, R)
+    for e in (-100, -110, -114, -120, -126):
+        for h, s in ((m * 2.0 ** e, 2.0 ** 20), (m, 2.0 ** e)):
+            out = bd.apply_adapters(torch.zeros_like(base), h, bd.AdapterSet(a, b, torch.tensor([s], device="cuda")), ids)
+            u = h[..., :R].double() * s
+            off = (out[..., :R].double() / 2.0 ** 90 - u).abs()
+            lost = 2.0 ** -134 * (s if s > 1 else 1.0)
+            # three roundings to f32 beside the parts' (u, its product, the sum with base)
+            assert bool((off <= u * (2.0 ** -24 + 3 * 2.0 ** -24) + lost).all()), (e, s)
+            assert not out[..., R:].any()
