@@ -418,3 +418,18 @@ def test_temperatures_from_the_least_to_the_largest(V, temperature, scale):
     for cut in ({}, dict(top_k=20), dict(top_k=V // 2), dict(top_p=0.7), dict(top_k=V // 3, top_p=0.8, min_p=0.05)):
         announce("sample hot", V, temperature, cut)
         check(torch, bd, x, u, settings=dict(temperature=torch.from_numpy(rows).cuda(), **cut), temperature=rows, **cut)
+
+
+@pytest.mark.parametrize("V", [40, 3000, 40000])
+@pytest.mark.parametrize("offset,temperature", [(1e5, 0.1), (-1e5, 1.0), (3e7, 1.0), (-3e7, 0.3), (2e8, 1.0), (1e9, 9.0)])
+def test_logits_far_from_zero(V, offset, temperature):
+    # Neighbouring values of f32 are up to 42 octaves of weight apart: bins are off
+    # by more than their width there, and have to hold what is drawn all the same.
+    torch = need_gpu()
+    import burn_dragon_amd as bd
+    rng = np.random.default_rng(V + 23)
+    x = (offset + rng.standard_normal((4, V)) * temperature * 6).astype(np.float32)
+    u = rng.random(4).astype(np.float32)
+    for cut in ({}, dict(top_k=20), dict(top_k=V // 2), dict(top_p=0.7), dict(top_k=V // 3, top_p=0.8, min_p=1e-4)):
+        announce("sample far from zero", V, offset, cut)
+        check(torch, bd, x, u, temperature=temperature, **cut)
