@@ -57,6 +57,7 @@ constexpr int kChunkThreads = 512;
 constexpr int kChunkPer = 16;    // logits a thread
 constexpr int kChunk = kChunkThreads * kChunkPer;
 constexpr int kMaxChunks = (int)(kMaxSampleVocab / kChunk);
+constexpr int64_t kGroupBytes = (int64_t)256 << 20;  // of scratch that rows go through at a time
 constexpr int kNoLimitIndex = 0x7fffffff;
 
 struct Row {
@@ -417,8 +418,9 @@ struct Candidates {
   float m;
   float top;
   const Row& s;
-  int n;  // found; beyond LIST the workgroup's list is not complete, beyond kFarMax the scratch's
-  const uint64_t* far;  // the scratch's, or null
+  int n;  // found; beyond LIST the workgroup's list is not complete, beyond far_max the scratch's
+  const uint64_t* far;  // the scratch's
+  int far_max;          // (0: none)
 
   // Calls f(order, bin) for each whose bin lies in [first, last].
   template <typename F>
@@ -429,7 +431,7 @@ struct Candidates {
         const int b = bin_of(value_of(o), top, s.cb);
         if (b >= first && b <= last) f(o, b);
       }
-    } else if (far && n <= kFarMax) {
+    } else if (n <= far_max) {
       for (int i = threadIdx.x; i < n; i += NT) {
         const uint64_t o = far[i];
         const int b = bin_of(value_of(o), top, s.cb);
@@ -775,7 +777,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a) {
       if (at >= 0 && at < LIST) sh.list[at] = order_of(x[e], index_of<E>(0, e));
     }
     __syncthreads();
-    Candidates<T, NT, LIST> cand{sh, row, vocab, m, top, s, sh.n_list, nullptr};
+    Candidates<T, NT, LIST> cand{sh, row, vocab, m, top, s, sh.n_list, nullptr, 0};
     const uint64_t lim = cand.limit(q);
     if (lim != ~0ull) {
       limit_x = value_of(lim);
@@ -823,7 +825,8 @@ struct SplitArgs {
   int32_t* near_n;   // [rows, chunks]: logits in `near`, -1: they are not all there
   uint64_t* near;    // [rows, chunks, kNear]: the logits up to the bin of the chunk's k-th
   uint64_t* sure;    // [rows, chunks]
-  uint64_t* list;    // [rows, kFarMax]
+  int far;           // what a row's list holds: its logits, up to kFarMax
+  uint64_t* list;    // [rows, far]
   RowState* state;   // [rows]
 };
 
@@ -1012,7 +1015,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_gather_kernel(const Spli
   at += first + (int)wave_scan_u64((uint64_t)__popc(mine)) - __popc(mine);
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    if ((mine >> e & 1) && at < kFarMax) p.list[lr * kFarMax + at] = order_of(x[e], index_of<E>(base, e));
+    if ((mine >> e & 1) && at < p.far) p.list[lr * p.far + at] = order_of(x[e], index_of<E>(base, e));
     at += mine >> e & 1;
   }
 }
@@ -1063,7 +1066,7 @@ __device__ void draw_from_list(Shared<NT, LIST>& sh, const SampleArgs& a, const 
     __syncthreads();
     n_cut = sh.n_list;
   }
-  const uint64_t lim = Candidates<T, NT, LIST>{sh, nullptr, 0, m, top, s, n_cut, nullptr}.limit(q);
+  const uint64_t lim = Candidates<T, NT, LIST>{sh, nullptr, 0, m, top, s, n_cut, nullptr, 0}.limit(q);
   __syncthreads();
   if (threadIdx.x == 0) sh.n_small = 0;
   __syncthreads();
@@ -1142,9 +1145,9 @@ __global__ __launch_bounds__(kChunkThreads) void sample_finish_kernel(const Spli
   for (int g = threadIdx.x; g < p.chunks; g += NT) chunk_sum[g] = p.sure[lr * p.chunks + g];
   const int n = st.n_list;
   if (n <= LIST)
-    for (int i = threadIdx.x; i < n; i += NT) sh.list[i] = p.list[lr * kFarMax + i];
+    for (int i = threadIdx.x; i < n; i += NT) sh.list[i] = p.list[lr * p.far + i];
   __syncthreads();
-  Candidates<T, NT, LIST> cand{sh, row, (int)a.vocab, m, st.top, s, n, p.list + lr * kFarMax};
+  Candidates<T, NT, LIST> cand{sh, row, (int)a.vocab, m, st.top, s, n, p.list + lr * p.far, p.far};
   const uint64_t lim = cand.limit(st.cuts);
   const float limit_x = lim != ~0ull ? value_of(lim) : -INFINITY;
   const int limit_i = lim != ~0ull ? (int)(uint32_t)lim : -1;  // (-inf itself is not kept)
@@ -1207,19 +1210,28 @@ bdh_status sample_typed(const SampleArgs& a, hipStream_t st, uint64_t* launches)
   SplitArgs p;
   p.a = a;
   p.chunks = (int)((a.vocab + kChunk - 1) / kChunk);
-  // Groups of rows, so that the scratch stays below 270 MB (8 KB a chunk, 256 a
-  // row).  16384 chunks, or 512 rows, fill the chip many times over.
-  const int64_t most = 16384 / p.chunks < 512 ? 16384 / p.chunks : 512;
-  const int64_t group = a.rows < most ? a.rows : most;
-  const size_t slots = (size_t)group * (size_t)p.chunks;
-  const size_t sizes[] = {up(slots * 4), up(slots * 4), up(slots * kBins * 4), up(slots * kBins * 8),
-                          up(slots * 4), up(slots * kNear * 8), up(slots * 8), up((size_t)group * kFarMax * 8),
-                          up((size_t)group * sizeof(RowState))};
-  size_t bytes = 0;
-  for (size_t s : sizes) bytes += s;
+  p.far = a.vocab < kFarMax ? (int)a.vocab : kFarMax;
+  // Groups of rows that kGroupBytes of scratch hold (8.2 KB a chunk, up to 256 KB a
+  // row; the stream keeps up to a quarter more), as many in each, and smaller ones
+  // where there is less to be had.  1024 rows of 20000 in one group 113 us, in two
+  // of 512 130; of 131072, which fill the chip many times over, 403 in two or three.
+  const int64_t row_bytes = p.chunks * (int64_t)(4 + 4 + kBins * 4 + kBins * 8 + 4 + kNear * 8 + 8) +
+                            (int64_t)p.far * 8 + (int64_t)sizeof(RowState);
+  const int64_t most = kGroupBytes / row_bytes, groups = (a.rows + most - 1) / most;
+  int64_t group = (a.rows + groups - 1) / groups;
+  size_t sizes[9];
   void* buf = nullptr;
-  const bdh_status s = scratch(st, SLOT_SAMPLE, bytes, &buf);
-  if (s != BDH_OK) return s;
+  for (;; group = (group + 1) / 2) {
+    const size_t slots = (size_t)group * (size_t)p.chunks;
+    const size_t need[9] = {up(slots * 4), up(slots * 4), up(slots * kBins * 4), up(slots * kBins * 8), up(slots * 4),
+                            up(slots * kNear * 8), up(slots * 8), up((size_t)group * (size_t)p.far * 8),
+                            up((size_t)group * sizeof(RowState))};
+    size_t bytes = 0;
+    for (int i = 0; i < 9; ++i) bytes += sizes[i] = need[i];
+    const bdh_status s = scratch(st, SLOT_SAMPLE, bytes, &buf);
+    if (s == BDH_OK) break;
+    if (group == 1 || !scratch_short(s)) return s;
+  }
   char* at = (char*)buf;
   p.max = (float*)at; at += sizes[0];
   p.arg = (int32_t*)at; at += sizes[1];

@@ -117,3 +117,65 @@ def test_backward_without_room_for_partials():
         torch.cuda.empty_cache()
     for t, w in zip(out, want):
         assert rel_l2(host(t), host(w)) <= TOL_F32
+
+
+@pytest.mark.parametrize("rows,V", [(300, 60000), (200, 20000), (3, 1 << 20)])
+def test_sampling_captured_in_a_smaller_calls_scratch(rows, V):
+    # Rows that do not fit go through it in groups.
+    torch = need_gpu()
+    import burn_dragon_amd as bd
+    announce("sampling, captured in a smaller call's scratch", rows, V)
+    g = torch.Generator(device="cuda").manual_seed(V)
+    x = torch.randn(rows, V, generator=g, device="cuda") * 2
+    u = torch.rand(rows, generator=g, device="cuda")
+    kw = dict(top_p=0.9, temperature=0.9, want_logprob=True)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        bd.sample_tokens(x[:rows // 8 + 1], u[:rows // 8 + 1], **kw)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        out = bd.sample_tokens(x, u, **kw)
+    assert out is not None
+    for _ in range(3):
+        x.normal_(generator=g).mul_(2)
+        u.uniform_(generator=g)
+        want = bd.sample_tokens(x, u, **kw)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out.tokens, want.tokens) and torch.equal(out.logprob, want.logprob)
+    del graph
+    bd.release_stream_scratch(st)
+
+
+def test_sampling_without_room_for_all_rows():
+    # 700 rows of 131072 take some 270 MB at once: with less than 100 MB left on
+    # the device they go through it a few at a time.
+    torch = need_gpu()
+    import burn_dragon_amd as bd
+    announce("sampling, memory short")
+    rows, V = 700, 131072
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = (torch.randn(1, V, generator=g, device="cuda") * 2).expand(rows, V)
+    u = torch.rand(rows, generator=g, device="cuda")
+    want = bd.sample_tokens(x, u, top_p=0.9, want_logprob=True)
+    spare = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")  # for the call's own outputs
+    torch.cuda.synchronize()
+    bd.release_stream_scratch()
+    torch.cuda.empty_cache()
+    hold = []
+    try:
+        free = torch.cuda.mem_get_info()[0]
+        while free > 96 << 20:
+            hold.append(torch.empty(min(free - (64 << 20), 32 << 30), dtype=torch.uint8, device="cuda"))
+            free = torch.cuda.mem_get_info()[0]
+        del spare
+        out = bd.sample_tokens(x, u, top_p=0.9, want_logprob=True)
+        torch.cuda.synchronize()
+    finally:
+        del hold
+        bd.release_stream_scratch()
+        torch.cuda.empty_cache()
+    assert torch.equal(out.tokens, want.tokens) and torch.equal(out.logprob, want.logprob)
