@@ -120,6 +120,14 @@ __device__ __forceinline__ uint64_t weight42(double t, const Series& series = Se
   return (uint64_t)(uint32_t)(__double2hiint(r) - 0x43300000) << 32 | (uint32_t)__double2loint(r);
 }
 
+// t of a logit.  It is computed again wherever a weight is needed, and all of
+// them have to agree to the unit, or a draw falls behind the last weight: its
+// product is never fused into what follows it.
+__device__ __forceinline__ double t_of(float x, float m, double c) {
+#pragma clang fp contract(off)
+  return ((double)x - (double)m) * c;
+}
+
 // Its weight where t is kept at all.
 __device__ __forceinline__ uint64_t weight_from(double t, double least, const Series& series = Series()) {
   return t >= least ? weight42(t, series) : 0;  // (NaN: -inf logits at an infinite temperature)
@@ -446,7 +454,7 @@ struct Candidates {
     }
   }
   __device__ __forceinline__ uint64_t weight(uint64_t o, double least) const {
-    return weight_from(((double)value_of(o) - (double)m) * s.c, least);
+    return weight_from(t_of(value_of(o), m, s.c), least);
   }
 
   // The last candidate in order that a cut keeps, among those of bins
@@ -645,7 +653,7 @@ template <int E>
 __device__ __forceinline__ uint64_t kept_weight(const Row& s, float x, int i, float m, float limit_x, int limit_i,
                                                 const Series& series = Series()) {
   if (!(x > limit_x || (x == limit_x && i <= limit_i))) return 0;
-  return weight_from(((double)x - (double)m) * s.c, s.min_t, series);
+  return weight_from(t_of(x, m, s.c), s.min_t, series);
 }
 
 __device__ __forceinline__ uint64_t draw_at(float u, uint64_t total) {
@@ -696,7 +704,7 @@ __device__ bool locate(Shared<NT, LIST>& sh, const Row& s, const float (&x)[E], 
 #pragma unroll
         for (int q = 0; q < E; q += 4) v = q == e ? x[q + j] : v;
         *token = index_of<E>(base, e) + j;
-        *t = ((double)v - (double)m) * s.c;
+        *t = t_of(v, m, s.c);
         return true;
       }
       run += w[j];
@@ -763,7 +771,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a) {
         const int b = bin_of(x[e], top, s.cb);
         if (b < kBins && b <= q.k_bin)  // no weight past the k-th counts
           atomicAdd((unsigned long long*)&sh.mass[b],
-                    (unsigned long long)weight_from(((double)x[e] - (double)m) * s.c, kLeastT, series));
+                    (unsigned long long)weight_from(t_of(x[e], m, s.c), kLeastT, series));
         if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
       }
       __syncthreads();
@@ -895,7 +903,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_chunk_kernel(const Split
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int b = bin_of(x[e], top, s.cb);
-    const double t = ((double)x[e] - (double)m) * s.c;
+    const double t = t_of(x[e], m, s.c);
     if (b < kBins && b <= q.k_bin && t >= least)
       atomicAdd((unsigned long long*)&mass[b], (unsigned long long)weight42(t, series));
   }
@@ -931,7 +939,7 @@ __global__ __launch_bounds__(kBins) void sample_merge_kernel(const SplitArgs p) 
     for (int g = threadIdx.x; g < p.chunks; g += kBins) {
       const float mg = p.max[lr * p.chunks + g], by = top - grid_of(mg, s.cb);
       shift[g] = is_real(mg) && by < (float)kBins ? (int)by : kBins;
-      scale[g] = exp2(((double)mg - (double)m) * s.c);
+      scale[g] = exp2(t_of(mg, m, s.c));
     }
     __syncthreads();
     if (s.use_k || s.use_p) {
@@ -993,7 +1001,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_gather_kernel(const Spli
   if (threadIdx.x == 0) {
     uint64_t sum = 0;
     for (int i = 0; i < NT / 64; ++i) sum += part[i];
-    p.sure[slot] = sum ? (uint64_t)rint((double)sum * exp2(((double)mg - (double)m) * s.c)) : 0;
+    p.sure[slot] = sum ? (uint64_t)rint((double)sum * exp2(t_of(mg, m, s.c))) : 0;
   }
   if (!some) return;
   const int base = (int)blockIdx.x * kChunk;
@@ -1053,7 +1061,7 @@ __device__ void draw_from_list(Shared<NT, LIST>& sh, const SampleArgs& a, const 
       for (int j = 0; j < PER; ++j)
         if (bin[j] < kBins && bin[j] <= q.k_bin)
           atomicAdd((unsigned long long*)&sh.mass[bin[j]],
-                    (unsigned long long)weight_from(((double)value_of(o[j]) - (double)m) * s.c, kLeastT));
+                    (unsigned long long)weight_from(t_of(value_of(o[j]), m, s.c), kLeastT));
       __syncthreads();
       by_one_wave<NT>(q, &sh.cuts, [&] { find_p(s, sh.mass, q); });
     }
@@ -1075,7 +1083,7 @@ __device__ void draw_from_list(Shared<NT, LIST>& sh, const SampleArgs& a, const 
   for (int j = 0; j < PER; ++j) {
     if (j * NT >= n) break;
     const uint64_t w = o[j] != ~0ull && o[j] <= lim
-                           ? weight_from(((double)value_of(o[j]) - (double)m) * s.c, s.min_t) : 0;
+                           ? weight_from(t_of(value_of(o[j]), m, s.c), s.min_t) : 0;
     const int at = append_at(&sh.n_small, w > 0);
     if (at >= 0) {
       sh.small_w[at] = w;
@@ -1097,7 +1105,7 @@ __device__ void draw_from_list(Shared<NT, LIST>& sh, const SampleArgs& a, const 
   if (at < before || at >= before + sh.small_w[threadIdx.x]) return;
   a.tokens[r] = (int)(uint32_t)mine;
   if (a.logprob)
-    a.logprob[r] = (float)(((double)value_of(mine) - (double)m) * s.c * 0.69314718055994530942 -
+    a.logprob[r] = (float)(t_of(value_of(mine), m, s.c) * 0.69314718055994530942 -
                            log((double)total * 0x1p-42));
 }
 
@@ -1214,7 +1222,7 @@ bdh_status sample_typed(const SampleArgs& a, hipStream_t st, uint64_t* launches)
   // Groups of rows that kGroupBytes of scratch hold (8.2 KB a chunk, up to 256 KB a
   // row; the stream keeps up to a quarter more), as many in each, and smaller ones
   // where there is less to be had.  1024 rows of 20000 in one group 113 us, in two
-  // of 512 130; of 131072, which fill the chip many times over, 403 in two or three.
+  // of 512 130; 300 of 2^20 in two groups 1017, in three 1133.
   const int64_t row_bytes = p.chunks * (int64_t)(4 + 4 + kBins * 4 + kBins * 8 + 4 + kNear * 8 + 8) +
                             (int64_t)p.far * 8 + (int64_t)sizeof(RowState);
   const int64_t most = kGroupBytes / row_bytes, groups = (a.rows + most - 1) / most;

@@ -433,3 +433,28 @@ def test_logits_far_from_zero(V, offset, temperature):
     for cut in ({}, dict(top_k=20), dict(top_k=V // 2), dict(top_p=0.7), dict(top_k=V // 3, top_p=0.8, min_p=1e-4)):
         announce("sample far from zero", V, offset, cut)
         check(torch, bd, x, u, temperature=temperature, **cut)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("rows,V", [(20000, 260), (4000, 1500), (1500, 16384), (600, 40001)])
+def test_every_draw_finds_its_token(rows, V, dtype):
+    # A weight is computed at several places, which have to agree to the unit: a
+    # draw at the far end of the sum still ends in a token that is kept.
+    torch = need_gpu()
+    import burn_dragon_amd as bd
+    g = torch.Generator(device="cuda").manual_seed(V)
+    x = (torch.randn(rows, V, generator=g, device="cuda") * 5).to(getattr(torch, dtype))
+    u = torch.rand(rows, generator=g, device="cuda")
+    u[::2] = 1 - 2.0 ** -24
+    temperature = 0.3 + torch.rand(rows, generator=g, device="cuda")
+    out = torch.full((rows,), -9, dtype=torch.int32, device="cuda")
+    for cut in ({}, dict(top_k=37), dict(top_k=700), dict(top_p=0.8), dict(min_p=0.01), dict(top_k=90, top_p=0.9)):
+        announce("sample every draw", rows, V, dtype, cut)
+        out.fill_(-9)
+        got = bd.sample_tokens(x, u, temperature=temperature, out=out, want_logprob=True, **cut)
+        torch.cuda.synchronize()
+        assert int(out.min()) >= 0 and int(out.max()) < V
+        t = (x.gather(1, out[:, None].long())[:, 0].double() - x.amax(1).double()) / temperature.double()
+        # kept: by min-p from its threshold up (half a step of f32 off at most), else from 2^-42 up
+        least = math.log(0.01) if "min_p" in cut else -42 * math.log(2)
+        assert bool((t >= least - 1e-6).all()) and bool((got.logprob >= t - 20).all()) and bool((got.logprob <= 0).all())
