@@ -326,3 +326,58 @@ def test_small_values_hold_to_2_134(T, D, R):
             # three roundings to f32 beside the parts' (u, its product, the sum with base)
             assert bool((off <= u * (2.0 ** -24 + 3 * 2.0 ** -24) + lost).all()), (e, s)
             assert not out[..., R:].any()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("T,D,V,R", [(1, 64, 300, 16), (1, 64, 300, 8), (1, 64, 300, 32), (1, 2048, 9000, 64),
+                                     (2, 64, 300000, 16), (3, 64, 300, 16), (40, 64, 300, 16), (40, 64, 300, 24),
+                                     (300, 512, 2000, 64), (70, 64, 300, 128)])
+def test_what_is_masked_does_not_spread_from_aligned_rows(T, D, V, R, dtype):
+    # Ranks and widths that are multiples of 8: without tiles, gathered tiles and
+    # tiles of one sequence, u in the workgroup and from its own launch.  The first
+    # and the last sequence share their adapter, and so their tile where gathered.
+    torch = need_gpu()
+    import burn_dragon_amd as bd
+    base, hidden, a, b, scale = make(torch, 4, T, D, V, R, 3, getattr(torch, dtype))
+    ids = torch.tensor([0, 2, -1, 0], dtype=torch.int32, device="cuda")
+    announce("adapters masked, aligned", T, D, V, R, dtype)
+    want = bd.apply_adapters(base, hidden, bd.AdapterSet(a, b, scale), ids)
+    h = hidden.clone()
+    h[0, -1] = float("nan")
+    h[2] = float("nan")
+    a2, b2, s2 = a.clone(), b.clone(), scale.clone()
+    a2[1], b2[1], s2[1] = float("nan"), float("inf"), float("nan")
+    s = bd.AdapterSet(a2, b2, s2)
+    got = bd.apply_adapters(base, h, s, ids)
+    torch.cuda.synchronize()
+    assert torch.equal(got[1], want[1]) and torch.equal(got[2], base[2]) and torch.equal(got[3], want[3])
+    assert torch.equal(got[0, :-1], want[0, :-1]) and bool(got[0, -1].isnan().all())
+    h[0, -1] = hidden[0, -1]
+    h[3, 0, 3] = float("inf")
+    got = bd.apply_adapters(base, h, s, ids)
+    torch.cuda.synchronize()
+    assert torch.equal(got[:2], want[:2]) and torch.equal(got[3, 1:], want[3, 1:])
+    assert not bool(got[3, 0].isfinite().any())
+
+
+@pytest.mark.parametrize("T,D,V,R,n,B", [(1, 128, 600, 16, 2, 40), (1, 64, 4000, 16, 2, 300), (50, 128, 600, 16, 2, 400),
+                                         (2, 64, 30000, 8, 20, 64), (40, 1024, 300, 64, 2, 30)])
+def test_a_sequence_in_small_and_large_batches(T, D, V, R, n, B):
+    # A call's kernels go by its batch (without tiles or with, u computed in place or
+    # by its own launch), which sum in different orders: a sequence's results in
+    # different batches are the same within the bound of each, not bit for bit.
+    torch = need_gpu()
+    import burn_dragon_amd as bd
+    for dtype in (torch.float32, torch.bfloat16):
+        base, hidden, a, b, scale = make(torch, B, T, D, V, R, n, dtype)
+        ids = (torch.arange(B, device="cuda") % n).to(torch.int32)
+        s = bd.AdapterSet(a, b, scale)
+        announce("adapters small and large", T, D, V, R, n, B, dtype)
+        whole = bd.apply_adapters(base, hidden, s, ids)
+        assert torch.equal(whole, bd.apply_adapters(base, hidden, s, ids))  # the same call: bit for bit
+        for i in (0, B // 2, B - 1):
+            at = slice(i, i + 1)
+            one = bd.apply_adapters(base[at], hidden[at], s, ids[at])
+            torch.cuda.synchronize()
+            check(torch, one, base[at], hidden[at], a, b, scale, ids[at])
+            check(torch, whole[at], base[at], hidden[at], a, b, scale, ids[at])

@@ -259,3 +259,37 @@ def test_calls_larger_than_the_caches(name):
     source = [torch.randn(B, *shape, generator=g, device="cuda")] if name == "from_another" else None
     for _ in range(2):
         check(torch, bd, rho, dst, src, source)
+
+
+@pytest.mark.parametrize("name", ["swaps", "cycles_of_3", "cycles_of_8", "last_step_of_1", "last_step_of_2",
+                                  "last_step_of_3", "clears_and_moves", "clears_alone", "from_another_and_clears"])
+def test_calls_larger_than_the_caches_at_odd_sizes(name):
+    # 16.7 MB a slot, not a multiple of 16 bytes, at addresses that are not one
+    # either.  All but clears_alone pass the caches by: 33 slots or more are read and
+    # written, at most three written for one read, none in a cycle past eight.
+    torch = need_gpu()
+    import burn_dragon_amd as bd
+    B, shape = 40, (3, 1367, 1021)
+    turn = lambda n, k: (list(range(n * k)), [i // k * k + (i + 1) % k for i in range(n * k)])  # noqa: E731
+    chain = lambda n: (list(range(n)), list(range(1, n + 1)))  # noqa: E731
+    dst, src = {
+        "swaps": turn(10, 2), "cycles_of_3": turn(7, 3), "cycles_of_8": turn(4, 8),
+        "last_step_of_1": chain(17), "last_step_of_2": chain(18), "last_step_of_3": chain(35),
+        "clears_and_moves": (list(range(30)), [-1 if i % 3 == 0 else i + 10 for i in range(30)]),
+        "clears_alone": (list(range(0, 40, 2)), [-1] * 20),
+        "from_another_and_clears": (list(range(40)), [-1 if i % 4 == 0 else i for i in range(40)]),
+    }[name]
+    announce("streams past the caches, odd", name)
+    g = torch.Generator(device="cuda").manual_seed(15)
+    slot = shape[0] * shape[1] * shape[2]
+
+    def odd(first):
+        flat = torch.empty(B * slot + 8, device="cuda")
+        flat.normal_(generator=g)
+        return flat, [flat[first:first + B * slot].view(B, *shape)]
+    flat, rho = odd(1)
+    source = odd(3)[1] if name == "from_another_and_clears" else None
+    around = flat[:1].clone(), flat[1 + B * slot:].clone()
+    for _ in range(2):
+        check(torch, bd, rho, dst, src, source)
+    assert torch.equal(flat[:1], around[0]) and torch.equal(flat[1 + B * slot:], around[1])
