@@ -44,11 +44,16 @@ __device__ __forceinline__ int adapter_of(const AdapterArgs& a, int64_t b) {
   return id >= 0 && id < a.n ? id : -1;
 }
 
-// The next bf16 part of an f32 whose rest is x.  (An infinity is one part.)
-// first: what would round past bf16's largest is cut there, and its rest goes on.
+// The next bf16 part of an f32 whose rest is x.  first: rounded to a finite value,
+// so that nothing finite grows past bf16's largest; an infinity or a NaN is what
+// then remains of one, and is the second part.
 __device__ __forceinline__ bf16_t next_part(float& x, bool first) {
-  bf16_t p = (bf16_t)x;
-  if (first && fabsf((float)p) == INFINITY) p = __builtin_bit_cast(bf16_t, (uint16_t)(__float_as_uint(x) >> 16));
+  if (first) {
+    const bf16_t p = (bf16_t)__builtin_amdgcn_fmed3f(x, -0x1.fep127f, 0x1.fep127f);
+    x -= (float)p;
+    return p;
+  }
+  const bf16_t p = (bf16_t)x;
   x = fabsf((float)p) < INFINITY ? x - (float)p : 0.0f;
   return p;
 }
