@@ -426,9 +426,8 @@ struct Candidates {
   float m;
   float top;
   const Row& s;
-  int n;  // found; beyond LIST the workgroup's list is not complete, beyond far_max the scratch's
-  const uint64_t* far;  // the scratch's
-  int far_max;          // (0: none)
+  int n;  // found; beyond LIST the workgroup's list is not complete, beyond kFarMax the scratch's
+  const uint64_t* far;  // the scratch's, or null
 
   // Calls f(order, bin) for each whose bin lies in [first, last].
   template <typename F>
@@ -439,7 +438,7 @@ struct Candidates {
         const int b = bin_of(value_of(o), top, s.cb);
         if (b >= first && b <= last) f(o, b);
       }
-    } else if (n <= far_max) {
+    } else if (far && n <= kFarMax) {
       for (int i = threadIdx.x; i < n; i += NT) {
         const uint64_t o = far[i];
         const int b = bin_of(value_of(o), top, s.cb);
@@ -785,7 +784,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a) {
       if (at >= 0 && at < LIST) sh.list[at] = order_of(x[e], index_of<E>(0, e));
     }
     __syncthreads();
-    Candidates<T, NT, LIST> cand{sh, row, vocab, m, top, s, sh.n_list, nullptr, 0};
+    Candidates<T, NT, LIST> cand{sh, row, vocab, m, top, s, sh.n_list, nullptr};
     const uint64_t lim = cand.limit(q);
     if (lim != ~0ull) {
       limit_x = value_of(lim);
@@ -826,6 +825,7 @@ struct SplitArgs {
   SampleArgs a;
   int64_t row0;      // of this group of rows
   int chunks;
+  int far;           // what a row's list holds: kFarMax, or its logits where they are fewer
   float* max;        // [rows, chunks]
   int32_t* arg;      // [rows, chunks]: the first index of the chunk's largest
   uint32_t* cnt;     // [rows, chunks, kBins], bins counted from the chunk's own largest
@@ -833,7 +833,6 @@ struct SplitArgs {
   int32_t* near_n;   // [rows, chunks]: logits in `near`, -1: they are not all there
   uint64_t* near;    // [rows, chunks, kNear]: the logits up to the bin of the chunk's k-th
   uint64_t* sure;    // [rows, chunks]
-  int far;           // what a row's list holds: its logits, up to kFarMax
   uint64_t* list;    // [rows, far]
   RowState* state;   // [rows]
 };
@@ -1023,7 +1022,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_gather_kernel(const Spli
   at += first + (int)wave_scan_u64((uint64_t)__popc(mine)) - __popc(mine);
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    if ((mine >> e & 1) && at < p.far) p.list[lr * p.far + at] = order_of(x[e], index_of<E>(base, e));
+    if ((mine >> e & 1) && at < kFarMax) p.list[lr * p.far + at] = order_of(x[e], index_of<E>(base, e));
     at += mine >> e & 1;
   }
 }
@@ -1074,7 +1073,7 @@ __device__ void draw_from_list(Shared<NT, LIST>& sh, const SampleArgs& a, const 
     __syncthreads();
     n_cut = sh.n_list;
   }
-  const uint64_t lim = Candidates<T, NT, LIST>{sh, nullptr, 0, m, top, s, n_cut, nullptr, 0}.limit(q);
+  const uint64_t lim = Candidates<T, NT, LIST>{sh, nullptr, 0, m, top, s, n_cut, nullptr}.limit(q);
   __syncthreads();
   if (threadIdx.x == 0) sh.n_small = 0;
   __syncthreads();
@@ -1155,7 +1154,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_finish_kernel(const Spli
   if (n <= LIST)
     for (int i = threadIdx.x; i < n; i += NT) sh.list[i] = p.list[lr * p.far + i];
   __syncthreads();
-  Candidates<T, NT, LIST> cand{sh, row, (int)a.vocab, m, st.top, s, n, p.list + lr * p.far, p.far};
+  Candidates<T, NT, LIST> cand{sh, row, (int)a.vocab, m, st.top, s, n, p.list + lr * p.far};
   const uint64_t lim = cand.limit(st.cuts);
   const float limit_x = lim != ~0ull ? value_of(lim) : -INFINITY;
   const int limit_i = lim != ~0ull ? (int)(uint32_t)lim : -1;  // (-inf itself is not kept)
