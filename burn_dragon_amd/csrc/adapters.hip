@@ -497,14 +497,21 @@ bdh_status run_typed(AdapterArgs a, hipStream_t st, uint64_t* launches) {
   const bool gather = a.time <= kGatherTokens;
   if constexpr (EVEN && RP == 16) {
     // Without tiles where those would be mostly empty (few rows an adapter of the
-    // set) in a call large enough.  us, this / tiles, D 256, V 32000, R 16:
-    //   f32   64 rows of 32 adapters 12.2 / 23.7, of 8 12.8 / 15.3; 256 of 16 28.9 / 27.1
-    //   bf16  64 rows of 32 adapters 12.7 / 18.6, of 8 11.9 / 11.3; one 5.9 / 4.9
-    //   two tokens, f32  64 sequences of 32 adapters 15.5 / 25.5, of 8 22.6 / 17.5;
-    //   at V 256 16 of 4 8.5 / 5.9
-    const bool one_f32 = sizeof(T) == 4 && a.time == 1;
-    if (a.time <= kRowsTokens && a.in_dim <= kRowsIn && a.batch * a.time <= (one_f32 ? 8 : 4) * a.n &&
-        (one_f32 || a.batch * a.out_dim >= (int64_t)1 << 20)) {
+    // set) in a call with columns enough.  us in a graph, this / tiles, R 16, by rows,
+    // adapters and columns; the ranges are over D of 64 to 512:
+    //   f32    64 of 32: V 128000 35-41 / 49-52, 32000 11-16 / 23-24, 4096 9-12 / 8-10
+    //          16 of 16: 32000 6.7-8.3 / 11-12;  4 of 4: 128000 6.0-7.7 / 11-12, 32000 5.7-6.8 / 5.6-7.1
+    //          64 of 8: 128000 27-32 / 26-29, 32000 12-16 / 15-16, 4096 11-13 / 5.6-8.9
+    //          256 of 16: 32000 30-37 / 35-36;  1: 32000 5.1-6.1 / 5.0-5.4
+    //   two tokens, D 256: 64 sequences of 32: 128000 47 / 59, 32000 20 / 25;  64 of 8: 32000 24 / 20
+    //   bf16, D 256: 64 of 32: 128000 43 / 46, 32000 18.6 / 18.9;  256 of 64: 128000 181 / 138
+    // (At D 1024 64 of 32 20 / 25 and 16 of 2 16 / 11; at rank 32 and D 512 36 / 25.)
+    const int64_t rows = a.batch * a.time, columns = a.batch * a.out_dim;
+    const bool sparse = sizeof(T) == 4
+                            ? (rows <= 4 * a.n && columns > (int64_t)1 << 18) ||
+                                  (a.time == 1 && rows <= 8 * a.n && columns >= (int64_t)1 << 20)
+                            : rows <= 2 * a.n && columns >= (int64_t)1 << 20;
+    if (a.time <= kRowsTokens && a.in_dim <= kRowsIn && sparse) {
       hipLaunchKernelGGL((adapter_rows_kernel<T>), dim3((uint32_t)cdiv(a.out_dim, 1024), (uint32_t)a.batch), dim3(256),
                          0, st, a);
       BDH_HIP_TRY(hipGetLastError());

@@ -329,7 +329,8 @@ def test_small_values_hold_to_2_134(T, D, R):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
-@pytest.mark.parametrize("T,D,V,R", [(1, 64, 300, 16), (1, 64, 300, 8), (1, 64, 300, 32), (1, 2048, 9000, 64),
+@pytest.mark.parametrize("T,D,V,R", [(1, 64, 300, 16), (1, 64, 300, 8), (1, 64, 300, 32), (1, 64, 300000, 16), (1, 64, 70000, 8),
+                                     (1, 2048, 9000, 64),
                                      (2, 64, 300000, 16), (3, 64, 300, 16), (40, 64, 300, 16), (40, 64, 300, 24),
                                      (300, 512, 2000, 64), (70, 64, 300, 128)])
 def test_what_is_masked_does_not_spread_from_aligned_rows(T, D, V, R, dtype):
@@ -361,7 +362,7 @@ def test_what_is_masked_does_not_spread_from_aligned_rows(T, D, V, R, dtype):
 
 
 @pytest.mark.parametrize("T,D,V,R,n,B", [(1, 128, 600, 16, 2, 40), (1, 64, 4000, 16, 2, 300), (50, 128, 600, 16, 2, 400),
-                                         (2, 64, 30000, 8, 20, 64), (40, 1024, 300, 64, 2, 30)])
+                                         (2, 64, 30000, 8, 20, 64), (40, 1024, 300, 64, 2, 30), (1, 64, 70000, 8, 40, 64)])
 def test_a_sequence_in_small_and_large_batches(T, D, V, R, n, B):
     # A call's kernels go by its batch (without tiles or with, u computed in place or
     # by its own launch), which sum in different orders: a sequence's results in
@@ -381,3 +382,12 @@ def test_a_sequence_in_small_and_large_batches(T, D, V, R, n, B):
             torch.cuda.synchronize()
             check(torch, one, base[at], hidden[at], a, b, scale, ids[at])
             check(torch, whole[at], base[at], hidden[at], a, b, scale, ids[at])
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("B,T,D,V,R,n", [(40, 1, 24, 30001, 8, 20), (40, 2, 512, 30001, 16, 40), (9, 1, 64, 130000, 16, 5),
+                                         (5, 1, 256, 70000, 16, 2), (5, 2, 256, 53000, 8, 2), (64, 1, 64, 4096, 16, 32),
+                                         (64, 1, 64, 4097, 16, 32), (64, 1, 64, 17000, 16, 8), (64, 1, 64, 16000, 16, 8)])
+def test_few_rows_of_an_adapter_around_the_choice(B, T, D, V, R, n, dtype):
+    # With and without tiles by rows an adapter, columns and type.
+    run(B, T, D, V, R, n, dtype, np.random.default_rng(V).integers(-1, n, B).tolist())
