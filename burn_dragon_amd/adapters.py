@@ -30,30 +30,39 @@ _MOST_IN, _MOST_OUT, _MOST_ADAPTERS = 1 << 20, 1 << 22, 1 << 20
 _MOST_BATCH, _MOST_TIME, _MOST_ROWS, _MOST_RANK = 65535, 65535 * 64, 1 << 23, 128
 
 
-def adapter_plan(base_shape, hidden_shape, device: torch.device, adapters: AdapterSet,
-                 ids: torch.Tensor) -> Optional[_lib.BdhAdapterPlan]:
-    """The plan of a call on a base [B, T, V] and a hidden [B, T, D] of these
-    shapes on ``device``: every check of the adapters and ids, before anything
-    is computed.  None where the library does not support them; raises
-    ValueError where they do not fit."""
-    (B, T, V), D = base_shape, hidden_shape[-1]
+def _plan(base_shape, hidden_shape, device: torch.device, adapters: AdapterSet,
+          ids: torch.Tensor) -> Optional[_lib.BdhAdapterPlan]:
+    """adapter_plan without the limits of sizes, which the library checks."""
+    B, T, V = base_shape
+    Bh, Th, D = hidden_shape
     a, b, scale = adapters
     if a.dim() != 3 or b.dim() != 3 or a.dtype != torch.bfloat16 or b.dtype != torch.bfloat16:
         return None
     n, R, _ = a.shape
     if min(B, T, V, D, n, R) == 0:
         return None
-    if (tuple(hidden_shape) != (B, T, D) or a.shape != (n, R, D) or b.shape != (n, V, R)
+    if (Bh != B or Th != T or a.shape != (n, R, D) or b.shape != (n, V, R)
             or scale.shape != (n,) or ids.shape != (B,)):
         raise ValueError("base, hidden, adapters and ids do not fit together")
     if scale.dtype != torch.float32 or ids.dtype != torch.int32:
         raise ValueError("scale must be f32 and ids int32")
     if not a.device == b.device == scale.device == ids.device == device:
         raise ValueError("base, hidden, adapters and ids must be on one device")
-    if (R > _MOST_RANK or D > _MOST_IN or V > _MOST_OUT or n > _MOST_ADAPTERS or B > _MOST_BATCH
-            or T > _MOST_TIME or B * T > _MOST_ROWS):
-        return None
     return _lib.BdhAdapterPlan(B, T, D, V, R, n)
+
+
+def adapter_plan(base_shape, hidden_shape, device: torch.device, adapters: AdapterSet,
+                 ids: torch.Tensor) -> Optional[_lib.BdhAdapterPlan]:
+    """The plan of a call on a base [B, T, V] and a hidden [B, T, D] of these
+    shapes on ``device``: every check of the adapters and ids, before anything
+    is computed.  None where the library does not support them; raises
+    ValueError where they do not fit."""
+    p = _plan(base_shape, hidden_shape, device, adapters, ids)
+    if p is None or (p.rank > _MOST_RANK or p.in_dim > _MOST_IN or p.out_dim > _MOST_OUT
+                     or p.adapters > _MOST_ADAPTERS or p.batch > _MOST_BATCH or p.time > _MOST_TIME
+                     or p.batch * p.time > _MOST_ROWS):
+        return None
+    return p
 
 
 def apply_adapters(base: torch.Tensor, hidden: torch.Tensor, adapters: AdapterSet, ids: torch.Tensor,
@@ -72,8 +81,11 @@ def apply_adapters(base: torch.Tensor, hidden: torch.Tensor, adapters: AdapterSe
         return None
     if len(shape) not in (2, 3) or hidden.dim() != len(shape):
         return None
-    tokens = [t.shape if len(shape) == 3 else (t.shape[0], 1, t.shape[1]) for t in (base, hidden)]
-    plan = adapter_plan(*tokens, dev, adapters, ids)
+    hidden_shape = hidden.shape
+    if len(shape) == 2:
+        plan = _plan((shape[0], 1, shape[1]), (hidden_shape[0], 1, hidden_shape[1]), dev, adapters, ids)
+    else:
+        plan = _plan(shape, hidden_shape, dev, adapters, ids)
     if plan is None:
         return None
     if hidden.device != dev:
@@ -84,7 +96,7 @@ def apply_adapters(base: torch.Tensor, hidden: torch.Tensor, adapters: AdapterSe
         raise ValueError("out must be a contiguous tensor like base")
     # contiguous copies stay referenced until the launch is enqueued
     base, hidden, ids = base.contiguous(), hidden.contiguous(), ids.contiguous()
-    a, b, scale = (t.contiguous() for t in adapters)
+    a, b, scale = adapters.a.contiguous(), adapters.b.contiguous(), adapters.scale.contiguous()
     st = _call_on(dev, _lib.load().bdh_apply_adapters, ctypes.byref(plan), code, _ptr(base), _ptr(hidden),
                   _ptr(a), _ptr(b), _ptr(scale), _ptr(ids), _ptr(out), _stream_ptr(dev))
     return out if _lib.check(st) else None
