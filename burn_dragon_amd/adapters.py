@@ -72,9 +72,12 @@ def apply_adapters(base: torch.Tensor, hidden: torch.Tensor, adapters: AdapterSe
     sequence's adapter (outside [0, n): none).  Returns base plus the
     adapters' products, in a new tensor or in ``out`` (contiguous; ``base``
     itself for in place).  Sums are f32; scale * hidden A^T is held to 2^-24 of
-    it in f32 calls, to 2^-16 in bf16 calls, and the result is rounded once.  None where the library does not support the input
-    (no supported device, another dtype, an empty dimension, a rank above
-    128, a scratch that would have to grow under capture)."""
+    it in f32 calls, to 2^-16 in bf16 calls, and the result is rounded once.
+    The form of a call goes by its sizes: the same call repeats bit for bit, a
+    sequence in another batch within these bounds.  None where the library does
+    not support the input (no supported device, another dtype, an empty
+    dimension, a rank above 128, a scratch that would have to grow under
+    capture)."""
     dev, shape = base.device, base.shape
     code = _dtype_code(base)
     if not _supported(dev) or code is None or hidden.dtype != base.dtype:

@@ -9,11 +9,17 @@
 // The token is the first in vocabulary order whose running sum of kept w
 // exceeds uniform * (their sum).
 //
-// No sort.  The weights are integers, w * 2^42 rounded, from a 64-bit 2^t:
-// sums of them are exact, so no order of atomics or of partial sums changes a
-// token, and a sum is right to 2^-42 of the largest weight where a border
-// (of top-p, of the draw) falls between two tokens.  Up to 2^20 logits, a sum
-// stays below 2^62.
+// No sort.  The weights are integers, w * 2^42 rounded, from a 64-bit 2^t: sums
+// of them are exact, so no order of atomics or of partial sums changes a token.
+// Up to 2^20 logits, a sum stays below 2^62.
+// Long rows sum in chunks, each in units of 2^-42 of its own largest weight, and
+// the chunks' sums are scaled to the row's units and rounded (a bin's for the cuts,
+// what is kept whole for the draw).  Such a sum is off from the one of the row's
+// own integers by up to half a unit a logit, and top-p's total also counts weights
+// below 2^-42 of the row's largest that are not below that of their chunk's, up to a
+// unit each: a border is right to about V units, 2^-42 V of the largest weight
+// (2^-22 at 2^20 logits).  Where a chunk's sum is more than its logits' own, its last kept
+// logit has the rest.  Chunks lie by index, so none of it depends on the batch.
 //
 //   1. A histogram over 512 bins of 1/10 octave of weight below the largest
 //      (counts for top-k, weights for top-p) finds the bin in which a cut
@@ -526,8 +532,8 @@ struct Candidates {
         uint64_t before, in;
         const int bin = BinScan(sh.mass, kBins).cross(need > above ? need - above : 1, &before, &in);
         if (threadIdx.x == 0) {
-          // (Weights scaled from chunks may leave the sum a few units short: the
-          // last candidates, of which the end keeps all.)
+          // (Weights scaled from chunks may leave the sum short, by up to a unit a
+          // logit: the last candidates, of which the end keeps all.)
           sh.bin = bin < kBins ? bin : (int)((to >> shift) - (from >> shift));
           sh.above = bin < kBins ? above + before : above;
         }
@@ -1178,7 +1184,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_finish_kernel(const Spli
   mine = wave_sum_u64(mine);
   if ((threadIdx.x & 63) == 0) sh.wave_sum[threadIdx.x >> 6] = mine;
   __syncthreads();
-  // (The chunk's sum was scaled as a whole: its logits' own may be a few units less.)
+  // (The chunk's sum was scaled as a whole: its logits' own may be less, by half a unit each.)
   uint64_t here = 0;
   for (int w = 0; w < NT / 64; ++w) here += sh.wave_sum[w];
   at = at < here ? at : here - 1;

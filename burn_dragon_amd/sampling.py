@@ -88,7 +88,7 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: P
     number or a tensor of [rows] (f32; top_k int32).  ``logprob`` is the log
     of the token's share of the kept w.  Returns None where the library does
     not support the input (no supported device, another dtype, an empty
-    dimension, V above 2^20, a scratch that would have to grow under
+    dimension, V above 2^20, a scratch too small for a single row under
     capture)."""
     dev = logits.device
     if not _supported(dev) or logits.dim() != 2:

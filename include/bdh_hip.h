@@ -310,11 +310,13 @@ bdh_status bdh_lm_logits(const float* hidden, int64_t rows, int64_t embd,
  * shares no memory with the inputs.  Sums are f32.  hidden and u = scale
  * hidden A^T enter the matrix cores in bf16 parts: with BDH_F32 three, so a value
  * is held to 2^-24 of it (or to 2^-134, below 2^-110); with BDH_BF16 hidden is
- * exact and u is held to 2^-16 of it.  out is rounded once.  An infinity or NaN of hidden reaches its own row, one of an
- * adapter (whose values are meant to be finite) its own sequences.  rank up to
- * 128.  Pointers aligned to their elements.  Uses the stream's scratch, but for
- * small calls.  No counterpart in the reference, which adapts a model by
- * training it. */
+ * exact and u is held to 2^-16 of it.  out is rounded once.  The form of a call
+ * goes by its sizes: the same call repeats bit for bit, a sequence in another
+ * batch within these bounds.  An infinity or NaN of hidden reaches its own row,
+ * one of an adapter (whose values are meant to be finite) its own sequences.
+ * rank up to 128.  Pointers aligned to their elements.  Uses the stream's
+ * scratch, but for small calls.  No counterpart in the reference, which adapts a
+ * model by training it. */
 typedef struct {
   int64_t batch, time, in_dim, out_dim, rank, adapters;
 } bdh_adapter_plan;
@@ -340,13 +342,17 @@ bdh_status bdh_apply_adapters(const bdh_adapter_plan* plan, int32_t dtype, const
  * exceeds uniform times their sum; temperature 0: the first index of m.
  * logprob_out (may be NULL): ln of its share of the kept w (0 at
  * temperature 0).  A row without a finite or +inf logit gives -1 and -inf.
- * Sums are exact integers (w in units of 2^-42), so a result depends on its
- * row and settings alone.
+ * Sums are of integers (w in units of 2^-42), whose order does not matter: a
+ * result depends on its row and settings alone.  Past 16384 logits they are
+ * taken in stretches of 8192 whose sums are rounded, so that a border lies within
+ * about vocab units of where it should (2^-22 of the largest weight at 2^20
+ * logits).
  * options NULL: temperature 1 and no cuts.  A *_rows pointer ([rows], device)
  * takes the place of the scalar beside it; there, a temperature that is not
  * above 0 counts as 0, other values outside a range as its nearest end, NaN
  * as no cut, and a random number outside [0, 1) as the nearest inside.
- * vocab up to 2^20; past 16384 the call uses the stream's scratch. */
+ * vocab up to 2^20; past 16384 the call uses the stream's scratch (256 MB and a
+ * quarter at most; rows go through less of it in smaller groups). */
 typedef struct {
   float temperature, top_p, min_p;
   int32_t top_k;
