@@ -98,8 +98,9 @@ def apply_adapters(base: torch.Tensor, hidden: torch.Tensor, adapters: AdapterSe
     elif out.shape != shape or out.dtype != base.dtype or out.device != dev or not out.is_contiguous():
         raise ValueError("out must be a contiguous tensor like base")
     # contiguous copies stay referenced until the launch is enqueued
-    base, hidden, ids = base.contiguous(), hidden.contiguous(), ids.contiguous()
-    a, b, scale = adapters.a.contiguous(), adapters.b.contiguous(), adapters.scale.contiguous()
+    a, b, scale = adapters
+    base, hidden, a, b = base.contiguous(), hidden.contiguous(), a.contiguous(), b.contiguous()
+    scale, ids = scale.contiguous(), ids.contiguous()
     st = _call_on(dev, _lib.load().bdh_apply_adapters, ctypes.byref(plan), code, _ptr(base), _ptr(hidden),
                   _ptr(a), _ptr(b), _ptr(scale), _ptr(ids), _ptr(out), _stream_ptr(dev))
     return out if _lib.check(st) else None

@@ -391,3 +391,13 @@ def test_a_sequence_in_small_and_large_batches(T, D, V, R, n, B):
 def test_few_rows_of_an_adapter_around_the_choice(B, T, D, V, R, n, dtype):
     # With and without tiles by rows an adapter, columns and type.
     run(B, T, D, V, R, n, dtype, np.random.default_rng(V).integers(-1, n, B).tolist())
+
+
+def test_a_set_given_as_a_tuple():
+    torch = need_gpu()
+    import burn_dragon_amd as bd
+    base, hidden, a, b, scale = make(torch, 3, 2, 64, 100, 8, 2, torch.float32)
+    ids = torch.tensor([1, 0, -1], dtype=torch.int32, device="cuda")
+    announce("adapters tuple")
+    assert torch.equal(bd.apply_adapters(base, hidden, (a, b, scale), ids),
+                       bd.apply_adapters(base, hidden, bd.AdapterSet(a, b, scale), ids))
