@@ -28,3 +28,8 @@ from .streams import compact_streams, copy_streams, free_streams  # noqa: F401
 from .sampling import SampleOutput, sample_tokens  # noqa: F401
 from .adapters import AdapterSet, apply_adapters  # noqa: F401
 from .generation import GenerateOutput, generate_tokens  # noqa: F401
+from .embedding import embed_tokens, embed_tokens_vjp  # noqa: F401
+from .activations import (ActivationCheckpoint, checkpoint_activations,  # noqa: F401
+                          restore_activations)
+from .gated import (GatedGrads, GatedOutput, GatedSaved, GatedWeights, gated_block,  # noqa: F401
+                    gated_block_vjp)

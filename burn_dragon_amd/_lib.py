@@ -21,6 +21,8 @@ BDH_EHIP = -2
 BDH_F32 = 0
 BDH_BF16 = 1
 
+BDH_RELU, BDH_SILU, BDH_GELU = 0, 1, 2
+
 BDH_KERNEL_PREFILL, BDH_KERNEL_DECODE = 0, 1
 BDH_CALIB_READ, BDH_CALIB_COPY, BDH_CALIB_RMW, BDH_CALIB_RMW_ROWS = 0, 1, 2, 3
 BDH_CALIB_MFMA_16X16X32_BF16, BDH_CALIB_MFMA_32X32X16_BF16, BDH_CALIB_MFMA_32X32X2_F32 = 0, 1, 2
@@ -63,6 +65,11 @@ class BdhSampleOptions(ctypes.Structure):
                 ("min_p", ctypes.c_float), ("top_k", ctypes.c_int32),
                 ("temperature_rows", ctypes.c_void_p), ("top_p_rows", ctypes.c_void_p),
                 ("min_p_rows", ctypes.c_void_p), ("top_k_rows", ctypes.c_void_p)]
+
+
+class BdhGatedOptions(ctypes.Structure):
+    _fields_ = [("activation", ctypes.c_int32), ("relu_threshold", ctypes.c_float),
+                ("latent_mask", ctypes.c_void_p)]
 
 
 class BdhProfileSnapshot(ctypes.Structure):
@@ -111,6 +118,15 @@ SIGNATURES = {
     "bdh_apply_adapters": (_i32, [ctypes.POINTER(BdhAdapterPlan), _i32] + [_vp] * 8),
     "bdh_sample_tokens": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp,
                                  ctypes.POINTER(BdhSampleOptions), _vp, _vp, _vp]),
+    "bdh_embed_tokens": (_i32, [_vp, _i64, _vp, _i32, _i64, _i64, ctypes.c_float, _i32, _vp, _vp]),
+    "bdh_embed_tokens_vjp": (_i32, [_vp, _i64, _vp, _i32, _i64, _i64, ctypes.c_float, _i32, _vp, _vp,
+                                    _i32, _vp]),
+    "bdh_activations_save": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _vp]),
+    "bdh_activations_restore": (_i32, [_vp, _vp, _i64, _i64, _i32, _vp, _vp]),
+    "bdh_gated_block_fwd": (_i32, [ctypes.POINTER(BdhLayerPlan)] + [_vp] * 4 +
+                            [ctypes.POINTER(BdhGatedOptions)] + [_vp] * 6),
+    "bdh_gated_block_vjp": (_i32, [ctypes.POINTER(BdhLayerPlan)] + [_vp] * 4 +
+                            [ctypes.POINTER(BdhGatedOptions)] + [_vp] * 10),
     "bdh_state_copy_streams": (_i32, [_i32, ctypes.POINTER(BdhLayerStateDesc), ctypes.POINTER(_vp),
                                       ctypes.POINTER(BdhLayerStateDesc), ctypes.POINTER(_vp), _i32,
                                       ctypes.POINTER(_i32), ctypes.POINTER(_i32), _vp]),

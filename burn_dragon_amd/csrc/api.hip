@@ -852,6 +852,232 @@ bdh_status bdh_sample_tokens(const void* logits, int32_t dtype, int64_t rows, in
   return st;
 }
 
+static bool overlap(const void* p, int64_t np, const void* q, int64_t nq) {
+  return p && q && (uintptr_t)p < (uintptr_t)q + (uintptr_t)nq && (uintptr_t)q < (uintptr_t)p + (uintptr_t)np;
+}
+
+// What both embedding calls check.
+static bdh_status embed_checks(const int32_t* tokens, int64_t n, int32_t dtype, int64_t vocab, int64_t embd, float scale,
+                               const void* table, const void* a, const void* b) {
+  if (n <= 0 || vocab <= 0 || embd <= 0) return fail(BDH_UNSUPPORTED, "zero-sized dimension");
+  if (dtype != BDH_F32 && dtype != BDH_BF16) return fail(BDH_EINVAL, "unknown dtype");
+  if (!std::isfinite(scale)) return fail(BDH_EINVAL, "scale must be finite");
+  if (embd > kMaxEmbedDim) return fail(BDH_UNSUPPORTED, "embd must be at most 2048");
+  if (vocab > kMaxEmbedVocab || n > kMaxEmbedTokens)
+    return fail(BDH_UNSUPPORTED, "vocab and tokens must be at most 2^24");
+  const uintptr_t size = dtype == BDH_F32 ? 4 : 2;
+  if (((uintptr_t)tokens & 3) != 0) return fail(BDH_EINVAL, "tensor pointers must be aligned to their elements");
+  for (const void* t : {table, a, b})
+    if (((uintptr_t)t & (size - 1)) != 0) return fail(BDH_EINVAL, "tensor pointers must be aligned to their elements");
+  return BDH_OK;
+}
+
+bdh_status bdh_embed_tokens(const int32_t* tokens, int64_t n_tokens, const void* table, int32_t dtype,
+                            int64_t vocab, int64_t embd, float scale, int32_t norm, void* out,
+                            void* stream) {
+  ProfScope prof;
+  bdh_status st = embed_checks(tokens, n_tokens, dtype, vocab, embd, scale, table, out, nullptr);
+  if (st != BDH_OK) return st;
+  if (!tokens || !table || !out) return fail(BDH_EINVAL, "null tensor pointer");
+  const int64_t size = dtype == BDH_F32 ? 4 : 2, bytes = n_tokens * embd * size;
+  if (overlap(out, bytes, table, vocab * embd * size) || overlap(out, bytes, tokens, n_tokens * 4))
+    return fail(BDH_EINVAL, "out shares memory with an input");
+  EmbedArgs a{};
+  a.tokens = tokens;
+  a.n = n_tokens;
+  a.vocab = vocab;
+  a.embd = embd;
+  a.table = table;
+  a.bf16 = dtype == BDH_BF16;
+  a.norm = norm != 0;
+  a.scale = scale;
+  a.out = out;
+  st = embed_tokens(a, (hipStream_t)stream);
+  if (st != BDH_OK) return st;
+  prof.launches = 1;
+  prof.done(true);
+  return BDH_OK;
+}
+
+bdh_status bdh_embed_tokens_vjp(const int32_t* tokens, int64_t n_tokens, const void* table,
+                                int32_t dtype, int64_t vocab, int64_t embd, float scale,
+                                int32_t norm, const void* grad_out, void* grad_table,
+                                int32_t accumulate, void* stream) {
+  ProfScope prof;
+  bdh_status st = embed_checks(tokens, n_tokens, dtype, vocab, embd, scale, table, grad_out, grad_table);
+  if (st != BDH_OK) return st;
+  if (!tokens || !grad_out || !grad_table || (norm && !table)) return fail(BDH_EINVAL, "null tensor pointer");
+  const int64_t size = dtype == BDH_F32 ? 4 : 2, bytes = vocab * embd * size;
+  if (overlap(grad_table, bytes, table, bytes) || overlap(grad_table, bytes, tokens, n_tokens * 4) ||
+      overlap(grad_table, bytes, grad_out, n_tokens * embd * size))
+    return fail(BDH_EINVAL, "grad_table shares memory with an input");
+  EmbedArgs a{};
+  a.tokens = tokens;
+  a.n = n_tokens;
+  a.vocab = vocab;
+  a.embd = embd;
+  a.table = table;
+  a.bf16 = dtype == BDH_BF16;
+  a.norm = norm != 0;
+  a.scale = scale;
+  a.out = grad_table;
+  a.grad = grad_out;
+  a.accumulate = accumulate != 0;
+  st = embed_tokens_vjp(a, (hipStream_t)stream, &prof.launches);
+  if (st == BDH_OK) prof.done(true);
+  return st;
+}
+
+static bdh_status activations_checks(const void* x, int32_t dtype, int64_t rows, int64_t cols, const void* codes,
+                                     const void* scales) {
+  if (rows <= 0 || cols <= 0) return fail(BDH_UNSUPPORTED, "zero-sized dimension");
+  if (!x || !codes || !scales) return fail(BDH_EINVAL, "null tensor pointer");
+  if (dtype != BDH_F32 && dtype != BDH_BF16) return fail(BDH_EINVAL, "unknown dtype");
+  const int64_t blocks = (cols + 31) / 32, size = dtype == BDH_F32 ? 4 : 2;
+  if (cols > (int64_t)1 << 30 || rows > ((int64_t)1 << 40) / blocks) return fail(BDH_UNSUPPORTED, "too large for one launch");
+  if (((uintptr_t)x & (size - 1)) != 0) return fail(BDH_EINVAL, "tensor pointers must be aligned to their elements");
+  if (overlap(x, rows * cols * size, codes, rows * cols) || overlap(x, rows * cols * size, scales, rows * blocks) ||
+      overlap(codes, rows * cols, scales, rows * blocks))
+    return fail(BDH_EINVAL, "the tensors share memory");
+  return BDH_OK;
+}
+
+bdh_status bdh_activations_save(const void* x, int32_t dtype, int64_t rows, int64_t cols,
+                                void* codes, void* scales, void* stream) {
+  ProfScope prof;
+  bdh_status st = activations_checks(x, dtype, rows, cols, codes, scales);
+  if (st != BDH_OK) return st;
+  st = save_activations(x, dtype == BDH_BF16, rows, cols, (uint8_t*)codes, (uint8_t*)scales, (hipStream_t)stream);
+  if (st != BDH_OK) return st;
+  prof.launches = 1;
+  prof.done(true);
+  return BDH_OK;
+}
+
+bdh_status bdh_activations_restore(const void* codes, const void* scales, int64_t rows,
+                                   int64_t cols, int32_t dtype, void* out, void* stream) {
+  ProfScope prof;
+  bdh_status st = activations_checks(out, dtype, rows, cols, codes, scales);
+  if (st != BDH_OK) return st;
+  st = restore_activations((const uint8_t*)codes, (const uint8_t*)scales, rows, cols, dtype == BDH_BF16, out,
+                           (hipStream_t)stream);
+  if (st != BDH_OK) return st;
+  prof.launches = 1;
+  prof.done(true);
+  return BDH_OK;
+}
+
+// A gated block's plan, options and inputs; fills the call.
+static bdh_status gated_checks(const bdh_layer_plan* plan, const void* current, const void* context, const void* up,
+                               const void* gate, const bdh_gated_options* options,
+                               std::initializer_list<const void*> more, GatedCall* g) {
+  if (!plan) return fail(BDH_EINVAL, "plan is null");
+  const bdh_layer_plan p = *plan;
+  if (p.batch <= 0 || p.heads <= 0 || p.time <= 0 || p.latent <= 0 || p.embd <= 0)
+    return fail(BDH_UNSUPPORTED, "zero-sized dimension");
+  if (!current || !up || !gate) return fail(BDH_EINVAL, "null tensor pointer");
+  if (p.latent % 8 != 0 || p.embd % 8 != 0) return fail(BDH_UNSUPPORTED, "latent and embd must be multiples of 8");
+  const int64_t most = (int64_t)1 << 22;
+  if (p.batch > most || p.time > most || p.batch * p.time > most || p.heads > 512 || p.latent > (int64_t)1 << 20 ||
+      p.embd > (int64_t)1 << 16 || p.batch * p.time > (((int64_t)1 << 35) - 1) / (p.heads * p.latent))
+    return fail(BDH_UNSUPPORTED, "too large for one launch");
+  bdh_gated_options o{BDH_RELU, 0.0f, nullptr};
+  if (options) o = *options;
+  if (o.activation != BDH_RELU && o.activation != BDH_SILU && o.activation != BDH_GELU)
+    return fail(BDH_EINVAL, "unknown activation");
+  if (!std::isfinite(o.relu_threshold)) return fail(BDH_EINVAL, "relu_threshold must be finite");
+  if (o.activation != BDH_RELU && (o.relu_threshold != 0.0f || o.latent_mask))
+    return fail(BDH_EINVAL, "a threshold and a mask go with BDH_RELU");
+  for (const void* t : {current, context, up, gate, (const void*)o.latent_mask})
+    if (((uintptr_t)t & 15) != 0) return fail(BDH_EINVAL, "tensor pointers must be 16-byte aligned");
+  for (const void* t : more)
+    if (((uintptr_t)t & 15) != 0) return fail(BDH_EINVAL, "tensor pointers must be 16-byte aligned");
+  g->B = p.batch;
+  g->H = p.heads;
+  g->T = p.time;
+  g->N = p.latent;
+  g->D = p.embd;
+  g->x = (const bf16_t*)current;
+  g->c = (const bf16_t*)context;
+  g->up = (const bf16_t*)up;
+  g->gate = (const bf16_t*)gate;
+  g->act = o.activation;
+  g->th = o.relu_threshold;
+  g->mask = o.latent_mask;
+  return BDH_OK;
+}
+
+// Whether one of the outputs shares memory with an input or another output.
+static bool outputs_overlap(std::initializer_list<std::pair<const void*, int64_t>> in,
+                            std::initializer_list<std::pair<const void*, int64_t>> out) {
+  for (auto o = out.begin(); o != out.end(); ++o) {
+    for (const auto& i : in)
+      if (overlap(o->first, o->second, i.first, i.second)) return true;
+    for (auto q = out.begin(); q != o; ++q)
+      if (overlap(o->first, o->second, q->first, q->second)) return true;
+  }
+  return false;
+}
+
+bdh_status bdh_gated_block_fwd(const bdh_layer_plan* plan, const void* current, const void* context,
+                               const void* up, const void* gate, const bdh_gated_options* options,
+                               void* out, void* up_codes, void* up_scales, void* gate_codes,
+                               void* gate_scales, void* stream) {
+  ProfScope prof;
+  GatedCall g{};
+  bdh_status st = gated_checks(plan, current, context, up, gate, options, {out, up_codes, gate_codes}, &g);
+  if (st != BDH_OK) return st;
+  if (!out) return fail(BDH_EINVAL, "null tensor pointer");
+  const int saved = !!up_codes + !!up_scales + !!gate_codes + !!gate_scales;
+  if (saved != 0 && saved != 4) return fail(BDH_EINVAL, "the codes and scales of both projections come together");
+  const int64_t M = g.B * g.T, L = M * g.H * g.N, S = M * g.H * ((g.N + 31) / 32), W = g.H * g.D * g.N * 2;
+  if (outputs_overlap({{current, M * g.D * 2}, {context, M * g.H * g.D * 2}, {up, W}, {gate, W}, {g.mask, g.N * 4}},
+                      {{out, L * 2}, {up_codes, L}, {gate_codes, L}, {up_scales, S}, {gate_scales, S}}))
+    return fail(BDH_EINVAL, "an output shares memory with an input or another output");
+  g.out = (bf16_t*)out;
+  g.up_codes = (uint8_t*)up_codes;
+  g.up_scales = (uint8_t*)up_scales;
+  g.gate_codes = (uint8_t*)gate_codes;
+  g.gate_scales = (uint8_t*)gate_scales;
+  st = gated_block(g, (hipStream_t)stream, &prof.launches);
+  if (st == BDH_OK) prof.done(true);
+  return st;
+}
+
+bdh_status bdh_gated_block_vjp(const bdh_layer_plan* plan, const void* current, const void* context,
+                               const void* up, const void* gate, const bdh_gated_options* options,
+                               const void* grad_out, const void* up_codes, const void* up_scales,
+                               const void* gate_codes, const void* gate_scales, void* grad_current,
+                               void* grad_context, void* grad_up, void* grad_gate, void* stream) {
+  ProfScope prof;
+  GatedCall g{};
+  bdh_status st = gated_checks(plan, current, context, up, gate, options,
+                               {grad_out, up_codes, gate_codes, grad_current, grad_context, grad_up, grad_gate}, &g);
+  if (st != BDH_OK) return st;
+  if (!grad_out || !grad_current || !grad_up || !grad_gate) return fail(BDH_EINVAL, "null tensor pointer");
+  if (!context != !grad_context) return fail(BDH_EINVAL, "context and grad_context come together");
+  const int saved = !!up_codes + !!up_scales + !!gate_codes + !!gate_scales;
+  if (saved != 0 && saved != 4) return fail(BDH_EINVAL, "the codes and scales of both projections come together");
+  const int64_t M = g.B * g.T, L = M * g.H * g.N, S = M * g.H * ((g.N + 31) / 32), W = g.H * g.D * g.N * 2;
+  const int64_t X = M * g.D * 2, C = M * g.H * g.D * 2;
+  if (outputs_overlap({{current, X}, {context, C}, {up, W}, {gate, W}, {g.mask, g.N * 4}, {grad_out, L * 2},
+                       {up_codes, L}, {gate_codes, L}, {up_scales, S}, {gate_scales, S}},
+                      {{grad_current, X}, {grad_context, C}, {grad_up, W}, {grad_gate, W}}))
+    return fail(BDH_EINVAL, "an output shares memory with an input or another output");
+  g.g = (const bf16_t*)grad_out;
+  g.up_codes = (uint8_t*)const_cast<void*>(up_codes);
+  g.up_scales = (uint8_t*)const_cast<void*>(up_scales);
+  g.gate_codes = (uint8_t*)const_cast<void*>(gate_codes);
+  g.gate_scales = (uint8_t*)const_cast<void*>(gate_scales);
+  g.d_x = (bf16_t*)grad_current;
+  g.d_c = (bf16_t*)grad_context;
+  g.d_up = (bf16_t*)grad_up;
+  g.d_gate = (bf16_t*)grad_gate;
+  st = gated_block_vjp(g, (hipStream_t)stream, &prof.launches);
+  if (st == BDH_OK) prof.done(true);
+  return st;
+}
+
 bdh_status bdh_state_copy_streams(int32_t n_layers, const bdh_layer_state_desc* layers,
                                   float* const* rho, const bdh_layer_state_desc* src_layers,
                                   const float* const* src_rho, int32_t n, const int32_t* dst,

@@ -50,6 +50,9 @@ enum ScratchSlot {
   SLOT_SNAP,         // states at interval starts: bf16 path [n_iv, S, D, N] bf16, fp32 path [n_iv - 1, S, N, D] f32
   SLOT_SAMPLE,       // sampling of long rows: chunks' histograms, candidates (sample.hip)
   SLOT_ADAPTER,      // adapters: the parts of scale hidden A^T  [rows, parts of the padded rank] bf16
+  SLOT_EMBED,        // embedding gradient: keys and order twice, digit counts, partial sums  (embed.hip)
+  SLOT_GATED_GRADS,  // gated block: gradients of both projections  2 x [tokens, H, N] bf16
+  SLOT_GATED_SUMS,   // gated block: partial sums of its gradients  f32
   SLOT_COUNT
 };
 // Scratch of the calling stream (see api.hip): grows on first use of a
@@ -179,6 +182,56 @@ struct AdapterArgs {
   bf16_t* u = nullptr;  // scratch, set by apply_adapters
 };
 bdh_status apply_adapters(const AdapterArgs& a, hipStream_t st, uint64_t* launches);
+
+// --- token embedding (embed.hip) -----------------------------------------------
+constexpr int64_t kMaxEmbedTokens = (int64_t)1 << 24, kMaxEmbedVocab = (int64_t)1 << 24, kMaxEmbedDim = 2048;
+struct EmbedArgs {
+  const int32_t* tokens;  // [n]
+  int64_t n, vocab, embd;
+  const void* table;      // [vocab, embd]
+  bool bf16;              // table, out and grad (else f32)
+  bool norm;
+  float scale;
+  void* out;              // [n, embd], or the table's gradient
+  const void* grad;       // [n, embd] (gradient)
+  bool accumulate;        // add to the table's gradient
+  // Scratch, set by embed_tokens_vjp.
+  const uint32_t *keys = nullptr, *order = nullptr;  // [n] ids in order, their positions
+  int run = 0;                                       // positions that a wave sums
+  float* part = nullptr;                             // [runs, 2, embd]
+};
+struct SortArgs {
+  const int32_t* tokens;
+  int64_t n, vocab;
+  const uint32_t *keys, *order;  // null: tokens in their order
+  uint32_t *keys_out, *order_out, *counts;
+  int shift, bins;
+};
+bdh_status embed_tokens(const EmbedArgs& a, hipStream_t st);
+bdh_status embed_tokens_vjp(EmbedArgs a, hipStream_t st, uint64_t* launches);
+
+// --- activations in 8 bits (activations.hip) -----------------------------------------
+bdh_status save_activations(const void* x, bool bf16, int64_t rows, int64_t cols, uint8_t* codes, uint8_t* scales,
+                            hipStream_t st);
+bdh_status restore_activations(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t cols, bool bf16,
+                               void* out, hipStream_t st);
+
+// --- gated block (gated.hip) -----------------------------------------------------------
+struct GatedCall {
+  int64_t B, H, T, N, D;
+  const bf16_t *x, *c;      // [B, T, D], [B, H, T, D] or null
+  const bf16_t *up, *gate;  // [H, D, N]
+  int act;                  // bdh_activation
+  float th;
+  const float* mask;        // [N] or null
+  bf16_t* out;              // [B, T, H, N] (forward)
+  const bf16_t* g;          // its gradient (backward)
+  // What the forward saves: [B, T, H, N] and [B, T, H, ceil(N / 32)], or null.
+  uint8_t *up_codes, *up_scales, *gate_codes, *gate_scales;
+  bf16_t *d_x, *d_c, *d_up, *d_gate;
+};
+bdh_status gated_block(const GatedCall& g, hipStream_t st, uint64_t* launches);
+bdh_status gated_block_vjp(const GatedCall& g, hipStream_t st, uint64_t* launches);
 
 // --- streams' states (streams.hip) -------------------------------------------
 // Layer l's slot dst[i] takes the value of slot src[i] (of src_rho[l], slots

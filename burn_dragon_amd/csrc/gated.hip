@@ -1,0 +1,699 @@
+// The gated block of latents and its backward pass, bf16 with f32 sums:
+//   p = x U_h - th, q = c_h G_h - th                 per head h, [tokens, N]
+//   out = up(p) m * act(q) m                         [tokens, H, N]
+// with relu: up = act = ReLU (y of the layer, residual_stream.rs:440-505), m the latent
+// mask; silu, gelu: up linear, th 0 and no mask.  c = x where there is no context.
+// Backward, with g the gradient of out:
+//   dp = g act(q) up'(p) m^2,  dq = g up(p) act'(q) m^2
+//   dx = sum_h dp_h U_h^T,  dc_h = dq_h G_h^T,  dU_h = x^T dp_h,  dG_h = c_h^T dq_h.
+//
+// All products run on v_mfma_f32_32x32x16_bf16 from LDS tiles of 32 k's that direct
+// loads fill one or two steps ahead.  A tile holds an operand as it lies in memory:
+// rows along k (KC), or rows of k (MC), whose fragments ds_read_b64_tr_b16 transposes
+// on the way to the registers; so no operand is ever laid out anew, U and G
+// [H, D, N] serve the forward (MC) and dx, dc (KC) alike, dp and dq serve dx (KC) and
+// dU (MC).  The first factor of a product is the one whose rows lie along the
+// result's rows in memory: a lane's sums are then neighbours there.
+#include <type_traits>
+
+#include "bdh_fp8.h"
+#include "bdh_internal.h"
+
+namespace bdh {
+namespace {
+
+constexpr int BK = 32;
+enum { KC, MC };
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+__device__ __forceinline__ uint32_t lds_addr(const void* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
+}
+// 16 bytes from p to LDS at m0 + 16 * lane (M0 needs a wait state before it).
+__device__ __forceinline__ void load_lds16(const char* p, uint32_t m0) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "{m0}"(m0) : "memory");
+}
+// At most n of this wave's loads are in flight and all its LDS accesses are done, in every wave.
+template <int N>
+__device__ __forceinline__ void wait_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// An operand's tile of 32 k's by W rows (KC) or columns (MC), 64 W bytes of LDS.
+//   KC  [W][32]: the 16-byte chunk c of row r lies at c ^ (r >> 1 & 3)
+//   MC  [32][W]: the 32-byte piece q of row k lies at q ^ 2 (k & 3)
+// which leaves both the fragments' reads without bank conflicts.  A direct load fills
+// 1 KB; of the W / 16 that a tile takes the four waves issue every fourth.
+template <int MODE, int W>
+struct Tile {
+  static constexpr int BYTES = 64 * W, LOADS = W / 64;
+  static constexpr int PER = 512 / W;  // MC: rows of k in 1 KB
+  // The lane's row (KC) or k (MC) of load j, and its chunk along the row.
+  static __device__ __forceinline__ int row(int j, int w, int lane) {
+    const int block = w + 4 * j;
+    return MODE == KC ? 16 * block + (lane >> 2) : PER * block + lane / (W / 8);
+  }
+  static __device__ __forceinline__ int chunk(int w, int lane) {
+    if (MODE == KC) return (lane & 3) ^ ((lane >> 3) & 3);
+    const int slot = lane % (W / 8), k = row(0, w, lane);
+    return slot ^ ((k & 3) << 2);
+  }
+  // Fragment of 32 rows / columns from at (a multiple of 32), k's 16 kk ..+15.
+  static __device__ __forceinline__ bf16x8 frag(const char* tile, int at, int kk, int lane) {
+    if constexpr (MODE == KC) {
+      const int r = at + (lane & 31), c = 2 * kk + (lane >> 5);
+      return *(const bf16x8*)(tile + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+    } else {
+      const int k = 8 * (lane >> 5) + ((lane & 15) >> 2);  // of the lane's first row; the second is 4 on
+      const int piece = at / 16 + ((lane >> 4) & 1);
+      const char* p = tile + (16 * kk + k) * (2 * W) + ((piece ^ ((k & 3) << 1)) << 5) + ((lane & 3) << 3);
+      const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+      const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 8 * W));
+      return __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  }
+};
+
+// Fills a tile from per-lane addresses; lanes that are not in write zeros.
+template <class Tl, class At, class In>
+__device__ __forceinline__ void fill(char* lds, uint32_t tile, int w, int lane, bool whole, At&& at, In&& in) {
+#pragma unroll
+  for (int j = 0; j < Tl::LOADS; ++j) {
+    const uint32_t to = tile + (uint32_t)((w + 4 * j) * 1024);
+    if (whole || in(j)) load_lds16(at(j), lds_addr(lds) + to);
+    else *(u32x4*)(lds + to + 16 * lane) = u32x4{0, 0, 0, 0};
+  }
+}
+
+// Rows of tokens: token i = (b, t) lies at b * batch + t * step elements.
+struct TokenRows {
+  int64_t batch, step;
+  uint32_t time;
+  float inverse;  // 1 / time
+  __device__ __forceinline__ int64_t at(uint32_t i) const {
+    // (i < 2^24 is exact in f32, so the quotient is off by one at most.)
+    int32_t b = (int32_t)((float)i * inverse);
+    int32_t t = (int32_t)(i - (uint32_t)b * time);
+    if (t < 0) {
+      --b;
+      t += (int32_t)time;
+    } else if (t >= (int32_t)time) {
+      ++b;
+      t -= (int32_t)time;
+    }
+    return b * batch + t * step;
+  }
+};
+
+// --- activations ---------------------------------------------------------------------
+enum { RELU = BDH_RELU, SILU = BDH_SILU, GELU = BDH_GELU };
+
+// (A NaN stays one.)
+__device__ __forceinline__ float relu(float x) { return x <= 0.0f ? 0.0f : x; }
+__device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
+__device__ __forceinline__ float normal_cdf(float x) { return 0.5f * (1.0f + erff(x * 0.70710678f)); }
+
+// up(p) act(q) with relu's taken already.
+template <int ACT>
+__device__ __forceinline__ float value_of(float p, float q) {
+  if (ACT == RELU) return p * q;
+  return p * (q * (ACT == SILU ? sigmoid(q) : normal_cdf(q)));
+}
+// g act(q) up'(p) and g up(p) act'(q), likewise.
+template <int ACT>
+__device__ __forceinline__ void grads_of(float g, float p, float q, float& dp, float& dq) {
+  if (ACT == RELU) {
+    dp = p <= 0.0f ? 0.0f : g * q;
+    dq = q <= 0.0f ? 0.0f : g * p;
+    return;
+  }
+  const float z = ACT == SILU ? sigmoid(q) : normal_cdf(q);
+  const float slope = ACT == SILU ? z + q * z * (1.0f - z) : z + q * __expf(-0.5f * q * q) * 0.39894228f;
+  dp = g * (q * z);
+  dq = g * p * slope;
+}
+
+struct GatedArgs {
+  const bf16_t *x, *c;      // [M, D]; c (or null) by heads and tokens
+  const bf16_t *up, *gate;  // [H, D, N]
+  int64_t M, N, D;
+  int H;
+  int64_t c_head;           // elements from a head of c to the next
+  TokenRows c_rows;
+  float th;
+  const float* mask;        // [N] or null
+  bf16_t* out;              // [M, H, N]
+  const bf16_t* g;          // [M, H, N]
+  uint8_t *up_codes, *up_scales, *gate_codes, *gate_scales;
+  bf16_t *dp, *dq;          // [M, H, N]
+};
+
+// --- both projections, and what is made of them ------------------------------------------
+enum { OUT, SAVE, BACK };
+
+// Two sums that lanes l and l + 32 hold four neighbours each of, to eight neighbours a lane.
+__device__ __forceinline__ void join_halves(u32x2 a, u32x2 b, u32x4& v) {
+  const auto x = __builtin_amdgcn_permlane32_swap(a.x, b.x, false, false);
+  const auto y = __builtin_amdgcn_permlane32_swap(a.y, b.y, false, false);
+  v = u32x4{x[0], y[0], x[1], y[1]};
+}
+__device__ __forceinline__ u32x2 join_halves(uint32_t a, uint32_t b) {
+  const auto x = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  return u32x2{x[0], x[1]};
+}
+
+// A workgroup: 128 latents (n) of a head by 128 tokens (m), a wave 64 by 64 of both
+// products.
+template <int ACT, int EPI, bool CTX>
+__global__ __launch_bounds__(256, 2) void gated_kernel(const GatedArgs a) {
+  typedef Tile<MC, 128> W;
+  typedef Tile<KC, 128> X;
+  constexpr int STAGE = 2 * W::BYTES + (CTX ? 2 : 1) * X::BYTES;
+  __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
+  const int lane = threadIdx.x & 63, w = wave_id();
+  const int D = (int)a.D, N = (int)a.N, M = (int)a.M;
+  const int n_tiles = (N + 127) / 128, per = n_tiles * a.H;
+  const int at = (int)(blockIdx.x % per), m0 = (int)(blockIdx.x / per) * 128;
+  const int n0 = at % n_tiles * 128, h = at / n_tiles;
+  const char* wp[2][2];
+  {
+    const int c = W::chunk(w, lane) * 8;
+    const int col = n0 + c < N ? n0 + c : 0;  // (past the end: any, never stored)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int64_t off = ((int64_t)h * D + W::row(j, w, lane)) * N + col;
+      wp[0][j] = (const char*)(a.up + off);
+      wp[1][j] = (const char*)(a.gate + off);
+    }
+  }
+  const char* xp[2][2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int m = m0 + X::row(j, w, lane);
+    const uint32_t i = (uint32_t)(m < M ? m : M - 1);
+    xp[0][j] = (const char*)(a.x + (int64_t)i * D + X::chunk(w, lane) * 8);
+    if (CTX) xp[1][j] = (const char*)(a.c + (int64_t)h * a.c_head + a.c_rows.at(i) + X::chunk(w, lane) * 8);
+  }
+  const int steps = (D + BK - 1) / BK;
+  const auto issue = [&](int s, int stage) {
+    const int k0 = s * BK;
+    const bool whole = k0 + BK <= D;
+    const uint32_t base = (uint32_t)(stage * STAGE);
+    const auto w_ok = [&](int j) { return k0 + W::row(j, w, lane) < D; };
+    const auto x_ok = [&](int) { return k0 + X::chunk(w, lane) * 8 < D; };
+    const int64_t wo = (int64_t)k0 * N * 2;
+    fill<W>(lds, base, w, lane, whole, [&](int j) { return wp[0][j] + wo; }, w_ok);
+    fill<W>(lds, base + W::BYTES, w, lane, whole, [&](int j) { return wp[1][j] + wo; }, w_ok);
+    fill<X>(lds, base + 2 * W::BYTES, w, lane, whole, [&](int j) { return xp[0][j] + 2 * k0; }, x_ok);
+    if (CTX)
+      fill<X>(lds, base + 2 * W::BYTES + X::BYTES, w, lane, whole, [&](int j) { return xp[1][j] + 2 * k0; }, x_ok);
+  };
+  floatx16 p[2][2], q[2][2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) p[i][j] = q[i][j] = zero16();
+  const int nw = 64 * (w & 1), mw = 64 * (w >> 1);
+  issue(0, 0);
+  for (int s = 0; s < steps; ++s) {
+    wait_barrier<0>();
+    if (s + 1 < steps) issue(s + 1, (s + 1) & 1);
+    const char* t = lds + (s & 1) * STAGE;
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      bf16x8 u[2], g[2], x[2], c[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        u[i] = W::frag(t, nw + 32 * i, kk, lane);
+        x[i] = X::frag(t + 2 * W::BYTES, mw + 32 * i, kk, lane);
+        g[i] = W::frag(t + W::BYTES, nw + 32 * i, kk, lane);
+        c[i] = CTX ? X::frag(t + 2 * W::BYTES + X::BYTES, mw + 32 * i, kk, lane) : x[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) p[i][j] = mfma32(u[i], x[j], p[i][j]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) q[i][j] = mfma32(g[i], c[j], q[i][j]);
+    }
+  }
+  // A lane has token mw + 32 j + (lane & 31) and, of 32 latents, 8 r + 4 (lane >> 5)
+  // ..+3 for r of 0..3.
+  const int high = lane >> 5;
+  const int nb = (N + kFp8Block - 1) / kFp8Block;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int m = m0 + mw + 32 * j + (lane & 31);
+    const int64_t row = (int64_t)m * a.H + h;  // of [tokens, H]
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int nt = n0 + nw + 32 * i;
+      float mask[16];
+      if (ACT == RELU && a.mask) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int n = nt + 8 * (r >> 2) + 4 * high + (r & 3);
+          mask[r] = n < N ? a.mask[n] : 0.0f;
+          mask[r] *= mask[r];
+        }
+      }
+      if (ACT == RELU) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          p[i][j][r] = relu(p[i][j][r] - a.th);
+          q[i][j][r] = relu(q[i][j][r] - a.th);
+        }
+      }
+      if (EPI == SAVE) {
+        // The same 32 latents in 8 bits.  (Past N: zeros, as the weights' columns are not.)
+        const auto keep = [&](const floatx16& v, uint8_t* codes, uint8_t* scales) {
+          uint32_t top = 0;
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (nt + 8 * (r >> 2) < N) top = max(top, finite_bits(v[r]));
+          const auto both = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+          top = max((uint32_t)both[0], (uint32_t)both[1]);
+          const int scale = fp8_scale(top);
+          const float inverse = fp8_inverse(scale);
+          uint32_t c[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float f[4] = {v[4 * r], v[4 * r + 1], v[4 * r + 2], v[4 * r + 3]};
+            fp8_keep_finite(f, scale);
+            c[r] = fp8_pack4(f[0], f[1], f[2], f[3], inverse);
+          }
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const u32x2 o = join_halves(c[2 * r], c[2 * r + 1]);
+            const int n = nt + 16 * r + 8 * high;
+            if (m < M && n < N) *(u32x2*)(codes + row * N + n) = o;
+          }
+          if (m < M && nt < N && high == 0) scales[row * nb + nt / kFp8Block] = (uint8_t)scale;
+        };
+        keep(p[i][j], a.up_codes, a.up_scales);
+        keep(q[i][j], a.gate_codes, a.gate_scales);
+      }
+      if (EPI != BACK) {
+        u32x2 o[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float f[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int k = 4 * r + e;
+            f[e] = value_of<ACT>(p[i][j][k], q[i][j][k]);
+            if (ACT == RELU && a.mask) f[e] *= mask[k];
+          }
+          o[r] = u32x2{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3])};
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          u32x4 v;
+          join_halves(o[2 * r], o[2 * r + 1], v);
+          const int n = nt + 16 * r + 8 * high;
+          if (m < M && n < N) *(u32x4*)(a.out + row * N + n) = v;
+        }
+      } else {
+        // (Each lane's own four neighbours of the gradient at a time.)
+#pragma unroll
+        for (int r = 0; r < 4; r += 2) {
+          u32x2 op[2], oq[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int n = nt + 8 * (r + e) + 4 * high;
+            bf16x4 g = {};
+            if (m < M && n < N) g = *(const bf16x4*)(a.g + row * N + n);
+            float fp[4], fq[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int at = 4 * (r + e) + k;
+              float gv = (float)g[k];
+              if (ACT == RELU && a.mask) gv *= mask[at];
+              grads_of<ACT>(gv, p[i][j][at], q[i][j][at], fp[k], fq[k]);
+            }
+            op[e] = u32x2{pack_bf16x2(fp[0], fp[1]), pack_bf16x2(fp[2], fp[3])};
+            oq[e] = u32x2{pack_bf16x2(fq[0], fq[1]), pack_bf16x2(fq[2], fq[3])};
+          }
+          u32x4 vp, vq;
+          join_halves(op[0], op[1], vp);
+          join_halves(oq[0], oq[1], vq);
+          const int n = nt + 8 * r + 8 * high;
+          if (m < M && n < N) {
+            *(u32x4*)(a.dp + row * N + n) = vp;
+            *(u32x4*)(a.dq + row * N + n) = vq;
+          }
+        }
+      }
+    }
+  }
+}
+
+// dp and dq from what the forward saved: eight neighbours a thread.
+template <int ACT>
+__global__ __launch_bounds__(256) void gated_grads_kernel(const GatedArgs a) {
+  const int N = (int)a.N, per = N / 8, nb = (N + kFp8Block - 1) / kFp8Block;
+  const int64_t total = a.M * a.H * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const uint32_t row = (uint32_t)i / (uint32_t)per;  // (total < 2^32)
+    const int n = (int)((uint32_t)i - row * (uint32_t)per) * 8;
+    const int64_t at = (int64_t)row * N + n, block = (int64_t)row * nb + n / kFp8Block;
+    const bf16x8 g = *(const bf16x8*)(a.g + at);
+    const u32x2 cp = *(const u32x2*)(a.up_codes + at), cq = *(const u32x2*)(a.gate_codes + at);
+    const float sp = fp8_power(a.up_scales[block]), sq = fp8_power(a.gate_scales[block]);
+    bf16x8 dp, dq;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      float p[4], q[4];
+      fp8_unpack4(cp[half], sp, p);
+      fp8_unpack4(cq[half], sq, q);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float gv = (float)g[4 * half + k], fp, fq;
+        if (ACT == RELU && a.mask) {
+          const float m = a.mask[n + 4 * half + k];
+          gv *= m * m;
+        }
+        grads_of<ACT>(gv, p[k], q[k], fp, fq);
+        dp[4 * half + k] = (bf16_t)fp;
+        dq[4 * half + k] = (bf16_t)fq;
+      }
+    }
+    *(bf16x8*)(a.dp + at) = dp;
+    *(bf16x8*)(a.dq + at) = dq;
+  }
+}
+
+// --- the four products of the backward pass -----------------------------------------------
+// A workgroup: 256 of the result's columns (first factor) by 128 of its rows, a wave
+// 128 by 64.  blockIdx.z: job and part of k.
+enum { INPUTS, WEIGHTS };
+struct ProductArgs {
+  const bf16_t *dp, *dq, *x, *c, *up, *gate;  // as GatedArgs
+  int64_t M, N, D;
+  int H;
+  int64_t c_head;
+  TokenRows c_rows;
+  int parts;                // of this launch's k
+  int x_parts;              // sums that make up d_x
+  int64_t x_size, c_size;   // elements of d_x, d_c
+  bf16_t *d_x, *d_c, *d_up, *d_gate;
+  float *x_sums, *c_sums, *w_sums;
+};
+
+template <int WHAT>
+__global__ __launch_bounds__(256, 2) void product_kernel(const ProductArgs a) {
+  typedef Tile<WHAT == INPUTS ? KC : MC, 256> A;  // U, G rows d / dp, dq columns n
+  typedef Tile<WHAT == INPUTS ? KC : MC, 128> B;  // dp, dq rows m / x, c columns d
+  constexpr int STAGE = A::BYTES + B::BYTES, LOADS = A::LOADS + B::LOADS;
+  __shared__ __attribute__((aligned(16))) char lds[3 * STAGE];
+  const int lane = threadIdx.x & 63, w = wave_id();
+  const int D = (int)a.D, N = (int)a.N, M = (int)a.M;
+  const int part = (int)blockIdx.z % a.parts, job = (int)blockIdx.z / a.parts;
+  const int h = job % a.H, which = job / a.H;  // which: 0 up, 1 gate
+  const int a0 = (int)blockIdx.x * 256, b0 = (int)blockIdx.y * 128;
+  const int K = WHAT == INPUTS ? N : M;
+  const int a_end = WHAT == INPUTS ? D : N, b_end = WHAT == INPUTS ? M : D;
+  const bf16_t* dv = which ? a.dq : a.dp;        // [M, H, N]
+  const int64_t d_row = (int64_t)a.H * N;
+  const bool ctx = which && a.c;
+  const char* ap[A::LOADS];
+  const char* bp[B::LOADS];
+  const int ac = A::chunk(w, lane) * 8, bc = B::chunk(w, lane) * 8;
+#pragma unroll
+  for (int j = 0; j < A::LOADS; ++j) {
+    const int r = A::row(j, w, lane);
+    if (WHAT == INPUTS) {
+      const int d = a0 + r < D ? a0 + r : D - 1;
+      ap[j] = (const char*)((which ? a.gate : a.up) + ((int64_t)h * D + d) * N + ac);
+    } else {
+      const int n = a0 + ac < N ? a0 + ac : 0;
+      ap[j] = (const char*)(dv + (int64_t)r * d_row + (int64_t)h * N + n);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < B::LOADS; ++j) {
+    const int r = B::row(j, w, lane);
+    if (WHAT == INPUTS) {
+      const int m = b0 + r < M ? b0 + r : M - 1;
+      bp[j] = (const char*)(dv + (int64_t)m * d_row + (int64_t)h * N + bc);
+    } else {
+      const int d = b0 + bc < D ? b0 + bc : 0;
+      bp[j] = (const char*)((ctx ? a.c + (int64_t)h * a.c_head : a.x + (int64_t)r * D) + d);
+    }
+  }
+  const int steps = (K + BK - 1) / BK;
+  const int s0 = (int)((int64_t)steps * part / a.parts), s1 = (int)((int64_t)steps * (part + 1) / a.parts);
+  const auto issue = [&](int s, int stage) {
+    const int k0 = s * BK;
+    const bool whole = k0 + BK <= K;
+    const uint32_t base = (uint32_t)(stage * STAGE);
+    const auto a_in = [&](int j) { return k0 + (WHAT == INPUTS ? ac : A::row(j, w, lane)) < K; };
+    const auto b_in = [&](int j) { return k0 + (WHAT == INPUTS ? bc : B::row(j, w, lane)) < K; };
+    fill<A>(lds, base, w, lane, whole,
+            [&](int j) { return ap[j] + 2 * (WHAT == INPUTS ? (int64_t)k0 : k0 * d_row); }, a_in);
+    fill<B>(lds, base + A::BYTES, w, lane, whole,
+            [&](int j) {
+              if (WHAT == INPUTS) return bp[j] + 2 * (int64_t)k0;
+              if (ctx) return bp[j] + 2 * a.c_rows.at((uint32_t)(k0 + B::row(j, w, lane)));
+              return bp[j] + 2 * (int64_t)k0 * D;
+            },
+            b_in);
+  };
+  floatx16 acc[4][2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) acc[i][j] = zero16();
+  const int aw = 128 * (w & 1), bw = 64 * (w >> 1);
+  // Ring of three stages.  A step's loads may be in flight while the one before it is
+  // multiplied, but only whole steps' are counted: a last one leaves out some.
+  if (s0 < s1) issue(s0, 0);
+  if (s0 + 1 < s1) issue(s0 + 1, 1);
+  for (int s = s0, stage = 0; s < s1; ++s) {
+    if (s + 1 < s1 && (s + 2) * BK <= K) wait_barrier<LOADS>();
+    else wait_barrier<0>();
+    if (s + 2 < s1) issue(s + 2, stage == 0 ? 2 : stage - 1);
+    const char* t = lds + stage * STAGE;
+    stage = stage == 2 ? 0 : stage + 1;
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      bf16x8 fa[4], fb[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) fb[j] = B::frag(t + A::BYTES, bw + 32 * j, kk, lane);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) fa[i] = A::frag(t, aw + 32 * i, kk, lane);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = mfma32(fa[i], fb[j], acc[i][j]);
+    }
+  }
+  const int high = lane >> 5;
+  bf16_t* out = nullptr;
+  float* sums = nullptr;
+  int64_t out_at = 0;
+  if (WHAT == INPUTS) {
+    if (ctx) {
+      out_at = (int64_t)h * a.c_head;
+      out = a.d_c;
+      sums = a.c_sums + part * a.c_size;
+    } else {
+      out = a.d_x;
+      sums = a.x_sums + ((int64_t)(which * a.H + h) * a.parts + part) * a.x_size;
+    }
+  } else {
+    out_at = (int64_t)h * D * N;
+    out = which ? a.d_gate : a.d_up;
+    sums = a.w_sums + ((int64_t)part * 2 + which) * a.H * D * N;
+  }
+  const bool direct = WHAT == INPUTS ? (ctx ? a.parts == 1 : a.x_parts == 1) : a.parts == 1;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int b = b0 + bw + 32 * j + (lane & 31);
+    if (b >= b_end) continue;
+    const int64_t row = out_at + (WHAT == INPUTS ? (ctx ? a.c_rows.at((uint32_t)b) : (int64_t)b * D) : (int64_t)b * N);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[i][j][8 * r + e]),
+                                                          __float_as_uint(acc[i][j][8 * r + 4 + e]), false, false);
+          v[e] = __uint_as_float(x[0]);
+          v[4 + e] = __uint_as_float(x[1]);
+        }
+        const int at = a0 + aw + 32 * i + 16 * r + 8 * high;
+        if (at >= a_end) continue;
+        if (direct) {
+          *(u32x4*)(out + row + at) = u32x4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
+                                            pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
+        } else {
+          *(floatx4*)(sums + row + at) = floatx4{v[0], v[1], v[2], v[3]};
+          *(floatx4*)(sums + row + at + 4) = floatx4{v[4], v[5], v[6], v[7]};
+        }
+      }
+    }
+  }
+}
+
+// out[i] = the sum of n parts, in their order; eight neighbours a thread.
+__global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ sums, int n, int64_t stride,
+                                                   bf16_t* __restrict__ out, int64_t size) {
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; i < size; i += (int64_t)gridDim.x * 2048) {
+    floatx4 a = *(const floatx4*)(sums + i), b = *(const floatx4*)(sums + i + 4);
+    for (int k = 1; k < n; ++k) {
+      a += *(const floatx4*)(sums + k * stride + i);
+      b += *(const floatx4*)(sums + k * stride + i + 4);
+    }
+    *(u32x4*)(out + i) = u32x4{pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(b[0], b[1]),
+                               pack_bf16x2(b[2], b[3])};
+  }
+}
+
+unsigned cdiv(int64_t a, int64_t b) { return (unsigned)((a + b - 1) / b); }
+int64_t capped(int64_t grid) { return grid < 8192 ? grid : 8192; }
+
+TokenRows token_rows(int64_t time, int64_t batch_stride, int64_t step) {
+  return TokenRows{batch_stride, step, (uint32_t)time, 1.0f / (float)time};
+}
+
+template <int ACT, int EPI>
+void launch_projections(const GatedArgs& a, hipStream_t st) {
+  const dim3 grid(cdiv(a.N, 128) * (unsigned)a.H * cdiv(a.M, 128));
+  if (a.c) hipLaunchKernelGGL((gated_kernel<ACT, EPI, true>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((gated_kernel<ACT, EPI, false>), grid, dim3(256), 0, st, a);
+}
+template <int EPI>
+void launch_projections(const GatedArgs& a, int act, hipStream_t st) {
+  if (act == RELU) launch_projections<RELU, EPI>(a, st);
+  else if (act == SILU) launch_projections<SILU, EPI>(a, st);
+  else launch_projections<GELU, EPI>(a, st);
+}
+
+GatedArgs args_of(const GatedCall& g) {
+  GatedArgs a{};
+  a.x = g.x;
+  a.c = g.c;
+  a.up = g.up;
+  a.gate = g.gate;
+  a.M = g.B * g.T;
+  a.H = (int)g.H;
+  a.N = g.N;
+  a.D = g.D;
+  a.c_head = g.T * g.D;
+  a.c_rows = token_rows(g.T, g.H * g.T * g.D, g.D);
+  a.th = g.th;
+  a.mask = g.mask;
+  a.out = g.out;
+  a.g = g.g;
+  a.up_codes = g.up_codes;
+  a.up_scales = g.up_scales;
+  a.gate_codes = g.gate_codes;
+  a.gate_scales = g.gate_scales;
+  return a;
+}
+
+}  // namespace
+
+bdh_status gated_block(const GatedCall& g, hipStream_t st, uint64_t* launches) {
+  const GatedArgs a = args_of(g);
+  if (g.up_codes) launch_projections<SAVE>(a, g.act, st);
+  else launch_projections<OUT>(a, g.act, st);
+  BDH_HIP_TRY(hipGetLastError());
+  *launches += 1;
+  return BDH_OK;
+}
+
+bdh_status gated_block_vjp(const GatedCall& g, hipStream_t st, uint64_t* launches) {
+  GatedArgs a = args_of(g);
+  const int64_t M = a.M, H = g.H, N = g.N, D = g.D;
+  // Parts of k: enough workgroups to fill the chip twice.
+  const int64_t want = 2 * (int64_t)device_cus();
+  const auto parts_of = [&](int64_t tiles, int64_t K) {
+    int64_t p = (want + tiles - 1) / tiles;
+    const int64_t most = K / 256 > 1 ? K / 256 : 1;
+    p = p < most ? p : most;
+    return (int)(p < 32 ? p : 32);
+  };
+  const int in_parts = parts_of((int64_t)cdiv(D, 256) * cdiv(M, 128) * 2 * H, N);
+  const int w_parts = parts_of((int64_t)cdiv(N, 256) * cdiv(D, 128) * 2 * H, M);
+  ProductArgs p{};
+  p.x_parts = (int)((g.c ? 1 : 2) * H * in_parts);
+  p.x_size = M * D;
+  p.c_size = M * H * D;
+  const int64_t w_size = H * D * N;
+  const size_t x_bytes = p.x_parts > 1 ? (size_t)p.x_parts * p.x_size * 4 : 0;
+  const size_t c_bytes = g.c && in_parts > 1 ? (size_t)in_parts * p.c_size * 4 : 0;
+  const size_t w_bytes = w_parts > 1 ? (size_t)w_parts * 2 * w_size * 4 : 0;
+  void* buf = nullptr;
+  bdh_status s = scratch(st, SLOT_GATED_GRADS, (size_t)(2 * M * H * N) * sizeof(bf16_t), &buf);
+  if (s != BDH_OK) return s;
+  a.dp = (bf16_t*)buf;
+  a.dq = a.dp + M * H * N;
+  // (The inputs' sums are joined before the weights' are made.)
+  const size_t sums = x_bytes + c_bytes > w_bytes ? x_bytes + c_bytes : w_bytes;
+  void* part = nullptr;
+  if (sums > 0) {
+    s = scratch(st, SLOT_GATED_SUMS, sums, &part);
+    if (s != BDH_OK) return s;
+  }
+  if (g.up_codes) {
+    const dim3 grid((unsigned)capped(cdiv(M * H * (N / 8), 256)));
+    if (g.act == RELU) hipLaunchKernelGGL((gated_grads_kernel<RELU>), grid, dim3(256), 0, st, a);
+    else if (g.act == SILU) hipLaunchKernelGGL((gated_grads_kernel<SILU>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((gated_grads_kernel<GELU>), grid, dim3(256), 0, st, a);
+  } else {
+    launch_projections<BACK>(a, g.act, st);
+  }
+  p.dp = a.dp;
+  p.dq = a.dq;
+  p.x = a.x;
+  p.c = a.c;
+  p.up = a.up;
+  p.gate = a.gate;
+  p.M = M;
+  p.N = N;
+  p.D = D;
+  p.H = (int)H;
+  p.c_head = a.c_head;
+  p.c_rows = a.c_rows;
+  p.d_x = g.d_x;
+  p.d_c = g.d_c;
+  p.d_up = g.d_up;
+  p.d_gate = g.d_gate;
+  p.x_sums = (float*)part;
+  p.c_sums = (float*)((char*)part + x_bytes);
+  p.w_sums = (float*)part;
+  p.parts = in_parts;
+  hipLaunchKernelGGL((product_kernel<INPUTS>), dim3(cdiv(D, 256), cdiv(M, 128), (unsigned)(2 * H * in_parts)),
+                     dim3(256), 0, st, p);
+  *launches += 2;
+  const auto join = [&](const float* from, int n, int64_t size, bf16_t* out) {
+    hipLaunchKernelGGL(join_kernel, dim3((unsigned)capped(cdiv(size, 2048))), dim3(256), 0, st, from, n, size, out,
+                       size);
+    *launches += 1;
+  };
+  if (x_bytes) join(p.x_sums, p.x_parts, p.x_size, g.d_x);
+  if (c_bytes) join(p.c_sums, in_parts, p.c_size, g.d_c);
+  p.parts = w_parts;
+  hipLaunchKernelGGL((product_kernel<WEIGHTS>), dim3(cdiv(N, 256), cdiv(D, 128), (unsigned)(2 * H * w_parts)),
+                     dim3(256), 0, st, p);
+  *launches += 1;
+  if (w_bytes) {
+    hipLaunchKernelGGL(join_kernel, dim3((unsigned)capped(cdiv(w_size, 2048))), dim3(256), 0, st, p.w_sums, w_parts,
+                       2 * w_size, g.d_up, w_size);
+    hipLaunchKernelGGL(join_kernel, dim3((unsigned)capped(cdiv(w_size, 2048))), dim3(256), 0, st, p.w_sums + w_size,
+                       w_parts, 2 * w_size, g.d_gate, w_size);
+    *launches += 2;
+  }
+  BDH_HIP_TRY(hipGetLastError());
+  return BDH_OK;
+}
+
+}  // namespace bdh

@@ -367,6 +367,85 @@ bdh_status bdh_sample_tokens(const void* logits, int32_t dtype, int64_t rows, in
                              const bdh_sample_options* options, int32_t* tokens_out,
                              float* logprob_out, void* stream);
 
+/* Token embedding: out[i] = scale * table[tokens[i]] or, with norm, scale *
+ * LN(table[tokens[i]]) (eps 1e-5, no weights: the model's input norm,
+ * dragon.rs:3352, norm.rs:302-328).  tokens [n_tokens] int32; table [vocab, embd] and
+ * out [n_tokens, embd] of one dtype (BDH_F32 or BDH_BF16), computed in f32, rounded
+ * once.  An id outside [0, vocab) gives a zero row (padding).  embd up to 2048, vocab
+ * and n_tokens up to 2^24.  Pointers aligned to their elements. */
+bdh_status bdh_embed_tokens(const int32_t* tokens, int64_t n_tokens, const void* table, int32_t dtype,
+                            int64_t vocab, int64_t embd, float scale, int32_t norm, void* out,
+                            void* stream);
+
+/* The table's gradient from out's, grad_out [n_tokens, embd]:
+ *   grad_table[v] = scale * sum over i with tokens[i] = v of grad_out[i]
+ * and with norm the transposed Jacobian of LN at table[v] times that sum (table
+ * may be NULL without).  Written whole, rows without a token as zeros, or with
+ * accumulate added to what is there (rows without a token stay untouched).  Sums are
+ * f32 over the tokens sorted by id, in an order that depends on the tokens alone:
+ * the same call repeats bit for bit.  grad_table shares no memory with the inputs.
+ * Uses the stream's scratch.  No counterpart in the reference, whose tensor library
+ * differentiates the lookup. */
+bdh_status bdh_embed_tokens_vjp(const int32_t* tokens, int64_t n_tokens, const void* table,
+                                int32_t dtype, int64_t vocab, int64_t embd, float scale,
+                                int32_t norm, const void* grad_out, void* grad_table,
+                                int32_t accumulate, void* stream);
+
+/* Activations kept between forward and backward in 8 bits: x [rows, cols]
+ * (BDH_F32 or BDH_BF16) as e4m3 codes [rows, cols] and a power of two for 32
+ * neighbours of a row, scales [rows, ceil(cols / 32)] (a row's last may be fewer).
+ * The power is the least 2^e, e >= -117, with which the block's largest finite
+ * magnitude is at most 448; its byte is e + 127.  Values round to nearest, ties to
+ * even: by at most 2^-4 of their magnitude, or 2^-10 * 2^e below 2^-6 * 2^e.
+ * (With the largest power, 2^120, finite values past 240 * 2^120 are held as that.)
+ * Infinities and NaN are held as NaN.  restore gives the values in dtype (exact but for
+ * that rounding).  codes and scales are bytes; x and out aligned to their elements.
+ * rows * ceil(cols / 32) up to 2^40, cols up to 2^30. */
+bdh_status bdh_activations_save(const void* x, int32_t dtype, int64_t rows, int64_t cols,
+                                void* codes, void* scales, void* stream);
+bdh_status bdh_activations_restore(const void* codes, const void* scales, int64_t rows,
+                                   int64_t cols, int32_t dtype, void* out, void* stream);
+
+/* The gated block of latents, bf16 with f32 sums: with plan (batch, heads, time,
+ * latent N, embd D), both projections, the activation and the product at once,
+ *   p = current up_h - th,  q = context_h gate_h - th            per head h
+ *   out[b, t, h] = u(p) mask * act(q) mask
+ * BDH_RELU: u = act = ReLU, the layer's y = (ReLU(a Ev - th) mask) * (ReLU(cur E - th)
+ * mask) (residual_stream.rs:440-505) with up = encoder, gate = encoder_v and context the
+ * normalised attention output; BDH_SILU, BDH_GELU (by erf): u(p) = p, an ordinary gated
+ * feed-forward block (th 0, no mask).
+ * current [B,T,D], context [B,H,T,D] or NULL (current), up and gate [H,D,N] (the
+ * reference's parameter layout), out [B,T,H,N], all bf16; out rounds once.
+ * up_codes .. gate_scales (all four or none): p and q (with BDH_RELU after the ReLU, before
+ * the mask) in 8 bits for the backward, as bdh_activations_save lays out [B*T*H, N].
+ * D and N multiples of 8, up to 2^16 and 2^20; B*T up to 2^22, heads up to 512, B*T*H*N
+ * below 2^35.  Tensors 16-byte aligned.  Outputs share no memory with inputs. */
+typedef enum { BDH_RELU = 0, BDH_SILU = 1, BDH_GELU = 2 } bdh_activation;
+typedef struct {
+  int32_t activation;        /* bdh_activation */
+  float relu_threshold;      /* th */
+  const float* latent_mask;  /* [N] f32 device pointer, or NULL */
+} bdh_gated_options;
+
+bdh_status bdh_gated_block_fwd(const bdh_layer_plan* plan, const void* current, const void* context,
+                               const void* up, const void* gate, const bdh_gated_options* options,
+                               void* out, void* up_codes, void* up_scales, void* gate_codes,
+                               void* gate_scales, void* stream);
+
+/* The gradients of current, context, up and gate from out's, grad_out [B,T,H,N],
+ * in their layouts, bf16: from what the forward saved (all four, read in place of p and
+ * q: the gradient of the block at the saved values), or with all four NULL from p and q
+ * computed again.  grad_context is NULL with context NULL; grad_current then has both
+ * parts.  The gradients of p and q are rounded to bf16 once before the four products
+ * over them, which sum in f32 (heads and parts of a sum in a fixed order: a call
+ * repeats bit for bit) and round once.  Uses the stream's scratch: 4 bytes for each of
+ * the B*T*H*N latents, and partial sums. */
+bdh_status bdh_gated_block_vjp(const bdh_layer_plan* plan, const void* current, const void* context,
+                               const void* up, const void* gate, const bdh_gated_options* options,
+                               const void* grad_out, const void* up_codes, const void* up_scales,
+                               const void* gate_codes, const void* gate_scales, void* grad_current,
+                               void* grad_context, void* grad_up, void* grad_gate, void* stream);
+
 /* Streaming-state record: the model position and each layer's carried rho
  * with its sequence-state flags, saved from / loaded into device memory.
  * Replaces, for the state this path carries, StreamingRuntimeStateRecord /

@@ -99,6 +99,14 @@ pub struct bdh_sample_options {
 }
 
 #[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct bdh_gated_options {
+    pub activation: i32,
+    pub relu_threshold: f32,
+    pub latent_mask: *const f32,
+}
+
+#[repr(C)]
 #[derive(Clone, Copy, Debug, Default)]
 pub struct bdh_profile_snapshot {
     pub calls: u64,
@@ -190,6 +198,33 @@ extern "C" {
                              row_stride: i64, uniform: *const f32,
                              options: *const bdh_sample_options, tokens_out: *mut i32,
                              logprob_out: *mut f32, stream: *mut c_void) -> i32;
+    pub fn bdh_embed_tokens(tokens: *const i32, n_tokens: i64, table: *const c_void, dtype: i32,
+                            vocab: i64, embd: i64, scale: f32, norm: i32, out: *mut c_void,
+                            stream: *mut c_void) -> i32;
+    pub fn bdh_embed_tokens_vjp(tokens: *const i32, n_tokens: i64, table: *const c_void, dtype: i32,
+                                vocab: i64, embd: i64, scale: f32, norm: i32,
+                                grad_out: *const c_void, grad_table: *mut c_void, accumulate: i32,
+                                stream: *mut c_void) -> i32;
+    pub fn bdh_activations_save(x: *const c_void, dtype: i32, rows: i64, cols: i64,
+                                codes: *mut c_void, scales: *mut c_void,
+                                stream: *mut c_void) -> i32;
+    pub fn bdh_activations_restore(codes: *const c_void, scales: *const c_void, rows: i64,
+                                   cols: i64, dtype: i32, out: *mut c_void,
+                                   stream: *mut c_void) -> i32;
+    pub fn bdh_gated_block_fwd(plan: *const bdh_layer_plan, current: *const c_void,
+                               context: *const c_void, up: *const c_void, gate: *const c_void,
+                               options: *const bdh_gated_options, out: *mut c_void,
+                               up_codes: *mut c_void, up_scales: *mut c_void,
+                               gate_codes: *mut c_void, gate_scales: *mut c_void,
+                               stream: *mut c_void) -> i32;
+    pub fn bdh_gated_block_vjp(plan: *const bdh_layer_plan, current: *const c_void,
+                               context: *const c_void, up: *const c_void, gate: *const c_void,
+                               options: *const bdh_gated_options, grad_out: *const c_void,
+                               up_codes: *const c_void, up_scales: *const c_void,
+                               gate_codes: *const c_void, gate_scales: *const c_void,
+                               grad_current: *mut c_void, grad_context: *mut c_void,
+                               grad_up: *mut c_void, grad_gate: *mut c_void,
+                               stream: *mut c_void) -> i32;
     pub fn bdh_state_copy_streams(n_layers: i32, layers: *const bdh_layer_state_desc,
                                   rho: *const *mut f32,
                                   src_layers: *const bdh_layer_state_desc,
