@@ -48,12 +48,14 @@ __device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d
   int w = __builtin_amdgcn_cvt_pk_fp8_f32(a * inverse, b * inverse, 0, false);
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c * inverse, d * inverse, w, true);
 }
+// (The conversion takes the power's exponent.)
 __device__ __forceinline__ void fp8_unpack4(uint32_t w, float power, float (&x)[4]) {
-  const floatx2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
-  x[0] = lo.x * power;
-  x[1] = lo.y * power;
-  x[2] = hi.x * power;
-  x[3] = hi.y * power;
+  const floatx2 lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, power, false);
+  const floatx2 hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, power, true);
+  x[0] = lo.x;
+  x[1] = lo.y;
+  x[2] = hi.x;
+  x[3] = hi.y;
 }
 
 }  // namespace bdh

@@ -26,6 +26,8 @@ constexpr int BK = 32;
 enum { KC, MC };
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x4_8 __attribute__((ext_vector_type(4), aligned(8)));
+typedef unsigned int u32_1 __attribute__((aligned(1)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 __device__ __forceinline__ uint32_t lds_addr(const void* p) {
@@ -45,14 +47,15 @@ __device__ __forceinline__ void wait_barrier() {
 //   KC  [W][32]: the 16-byte chunk c of row r lies at c ^ (r >> 1 & 3)
 //   MC  [32][W]: the 32-byte piece q of row k lies at q ^ 2 (k & 3)
 // which leaves both the fragments' reads without bank conflicts.  A direct load fills
-// 1 KB; of the W / 16 that a tile takes the four waves issue every fourth.
-template <int MODE, int W>
+// 1 KB; of the W / 16 that a tile takes each wave issues its share.
+template <int MODE, int W, int WAVES = 4>
 struct Tile {
-  static constexpr int BYTES = 64 * W, LOADS = W / 64;
+  static constexpr int BYTES = 64 * W, LOADS = W / 16 / WAVES;
   static constexpr int PER = 512 / W;  // MC: rows of k in 1 KB
+  static constexpr int WAVE_STEP = WAVES;
   // The lane's row (KC) or k (MC) of load j, and its chunk along the row.
   static __device__ __forceinline__ int row(int j, int w, int lane) {
-    const int block = w + 4 * j;
+    const int block = w + WAVES * j;
     return MODE == KC ? 16 * block + (lane >> 2) : PER * block + lane / (W / 8);
   }
   static __device__ __forceinline__ int chunk(int w, int lane) {
@@ -81,7 +84,7 @@ template <class Tl, class At, class In>
 __device__ __forceinline__ void fill(char* lds, uint32_t tile, int w, int lane, bool whole, At&& at, In&& in) {
 #pragma unroll
   for (int j = 0; j < Tl::LOADS; ++j) {
-    const uint32_t to = tile + (uint32_t)((w + 4 * j) * 1024);
+    const uint32_t to = tile + (uint32_t)((w + Tl::WAVE_STEP * j) * 1024);
     if (whole || in(j)) load_lds16(at(j), lds_addr(lds) + to);
     else *(u32x4*)(lds + to + 16 * lane) = u32x4{0, 0, 0, 0};
   }
@@ -106,6 +109,41 @@ struct TokenRows {
     return b * batch + t * step;
   }
 };
+
+// Which tile a workgroup has.  Workgroup i runs on XCD i % 8, which has an L2 of its own:
+// an XCD takes blocks of up to 8 by 8 tiles (what it runs at a time), along b first, so
+// that its a-tiles' operand (8 of the weights' tiles, say) stays in its L2 while the other
+// one streams.
+struct TileOrder {
+  int a_tiles, b_tiles;    // in all
+  int a_block, b_block;    // of a block
+  int b_blocks, blocks, per_xcd;
+  __device__ __forceinline__ bool at(int id, int& a, int& b) const {
+    const int k = id >> 3, size = a_block * b_block, local = k / size, r = k - local * size;
+    const int block = (id & 7) * per_xcd + local;
+    const int ga = block / b_blocks, gb = block - ga * b_blocks;
+    a = ga * a_block + r % a_block;
+    b = gb * b_block + r / a_block;
+    return local < per_xcd && block < blocks && a < a_tiles && b < b_tiles;
+  }
+};
+TileOrder tile_order(int64_t a_tiles, int64_t b_tiles) {
+  TileOrder t{};
+  t.a_tiles = (int)a_tiles;
+  t.b_tiles = (int)b_tiles;
+  t.a_block = a_tiles < 8 ? (int)a_tiles : 8;
+  t.b_block = b_tiles < 8 ? (int)b_tiles : 8;
+  const auto count = [&] {
+    t.b_blocks = (t.b_tiles + t.b_block - 1) / t.b_block;
+    t.blocks = (t.a_tiles + t.a_block - 1) / t.a_block * t.b_blocks;
+    t.per_xcd = (t.blocks + 7) / 8;
+    return t.blocks;
+  };
+  // Smaller blocks where there are too few for the eight XCDs.
+  while (count() < 16 && (t.a_block > 1 || t.b_block > 1)) (t.b_block >= t.a_block ? t.b_block : t.a_block) /= 2;
+  return t;
+}
+unsigned grid_of(const TileOrder& t) { return (unsigned)(8 * t.per_xcd * t.a_block * t.b_block); }
 
 // --- activations ---------------------------------------------------------------------
 enum { RELU = BDH_RELU, SILU = BDH_SILU, GELU = BDH_GELU };
@@ -148,6 +186,7 @@ struct GatedArgs {
   const bf16_t* g;          // [M, H, N]
   uint8_t *up_codes, *up_scales, *gate_codes, *gate_scales;
   bf16_t *dp, *dq;          // [M, H, N]
+  TileOrder order;          // tiles of latents (of all heads) and of tokens
 };
 
 // --- both projections, and what is made of them ------------------------------------------
@@ -170,13 +209,14 @@ template <int ACT, int EPI, bool CTX>
 __global__ __launch_bounds__(256, 2) void gated_kernel(const GatedArgs a) {
   typedef Tile<MC, 128> W;
   typedef Tile<KC, 128> X;
-  constexpr int STAGE = 2 * W::BYTES + (CTX ? 2 : 1) * X::BYTES;
-  __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
+  constexpr int STAGE = 2 * W::BYTES + (CTX ? 2 : 1) * X::BYTES, STAGES = CTX ? 2 : 3;
+  __shared__ __attribute__((aligned(16))) char lds[STAGES * STAGE];
   const int lane = threadIdx.x & 63, w = wave_id();
   const int D = (int)a.D, N = (int)a.N, M = (int)a.M;
-  const int n_tiles = (N + 127) / 128, per = n_tiles * a.H;
-  const int at = (int)(blockIdx.x % per), m0 = (int)(blockIdx.x / per) * 128;
-  const int n0 = at % n_tiles * 128, h = at / n_tiles;
+  int an, am;
+  if (!a.order.at((int)blockIdx.x, an, am)) return;
+  const int n_tiles = (N + 127) / 128;
+  const int n0 = an % n_tiles * 128, h = an / n_tiles, m0 = am * 128;
   const char* wp[2][2];
   {
     const int c = W::chunk(w, lane) * 8;
@@ -217,10 +257,13 @@ __global__ __launch_bounds__(256, 2) void gated_kernel(const GatedArgs a) {
     for (int j = 0; j < 2; ++j) p[i][j] = q[i][j] = zero16();
   const int nw = 64 * (w & 1), mw = 64 * (w >> 1);
   issue(0, 0);
-  for (int s = 0; s < steps; ++s) {
-    wait_barrier<0>();
-    if (s + 1 < steps) issue(s + 1, (s + 1) & 1);
-    const char* t = lds + (s & 1) * STAGE;
+  if (STAGES == 3 && steps > 1) issue(1, 1);
+  for (int s = 0, stage = 0; s < steps; ++s) {
+    if (STAGES == 3 && s + 1 < steps && (s + 2) * BK <= D) wait_barrier<6>();
+    else wait_barrier<0>();
+    if (s + STAGES - 1 < steps) issue(s + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
+    const char* t = lds + stage * STAGE;
+    stage = stage == STAGES - 1 ? 0 : stage + 1;
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
       bf16x8 u[2], g[2], x[2], c[2];
@@ -242,22 +285,41 @@ __global__ __launch_bounds__(256, 2) void gated_kernel(const GatedArgs a) {
     }
   }
   // A lane has token mw + 32 j + (lane & 31) and, of 32 latents, 8 r + 4 (lane >> 5)
-  // ..+3 for r of 0..3.
-  const int high = lane >> 5;
-  const int nb = (N + kFp8Block - 1) / kFp8Block;
+  // ..+3 for r of 0..3.  Half of the tile's tokens at a time (j) go through LDS, so that
+  // memory sees whole rows of 128 latents, stored past the caches, which they would only
+  // empty (16384 tokens, 4 heads of 8192, D 256, saved: 1400 -> 1200 us).
+  constexpr int VP = 272, CP = 144;  // row pitches in bytes (bank spread)
+  char* const vals = lds;            // [64][VP]: out; the gradient, then dp
+  char* const more = lds + 64 * VP;  // [64][VP]: dq; or [2][64][CP] codes, [2][64][4] scales
+  char* const bytes = more + 128 * CP;
+  static_assert(64 * VP + 128 * CP + 512 <= 2 * STAGE && 128 * VP <= 2 * STAGE, "the stages' memory");
+  const int high = lane >> 5, nb = (N + kFp8Block - 1) / kFp8Block;
+  const int mine = 32 * (w >> 1) + (lane & 31);  // the lane's row of the half
+  // Row r of half j, and its place in [tokens, H].
+  const auto token = [&](int r, int j) { return m0 + 64 * (r >> 5) + 32 * j + (r & 31); };
+  const auto place = [&](int m) { return (int64_t)m * a.H + h; };
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    const int m = m0 + mw + 32 * j + (lane & 31);
-    const int64_t row = (int64_t)m * a.H + h;  // of [tokens, H]
+    wait_barrier<0>();
+    if (EPI == BACK) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = (int)threadIdx.x / 16 + 16 * e, c = (int)threadIdx.x % 16, m = token(r, j);
+        u32x4 g = {0, 0, 0, 0};
+        if (m < M && n0 + 8 * c < N) g = *(const u32x4*)(a.g + place(m) * N + n0 + 8 * c);
+        *(u32x4*)(vals + r * VP + 16 * c) = g;
+      }
+      __syncthreads();
+    }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int nt = n0 + nw + 32 * i;
-      float mask[16];
+      const int nt = nw + 32 * i;  // in the tile
+      floatx4 mask[4];
       if (ACT == RELU && a.mask) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int n = nt + 8 * (r >> 2) + 4 * high + (r & 3);
-          mask[r] = n < N ? a.mask[n] : 0.0f;
+        for (int r = 0; r < 4; ++r) {
+          const int n = n0 + nt + 8 * r + 4 * high;
+          mask[r] = *(const floatx4*)(a.mask + (n < N ? n : 0));
           mask[r] *= mask[r];
         }
       }
@@ -269,12 +331,12 @@ __global__ __launch_bounds__(256, 2) void gated_kernel(const GatedArgs a) {
         }
       }
       if (EPI == SAVE) {
-        // The same 32 latents in 8 bits.  (Past N: zeros, as the weights' columns are not.)
-        const auto keep = [&](const floatx16& v, uint8_t* codes, uint8_t* scales) {
+        // The same 32 latents in 8 bits (those past N do not count).
+        const auto keep = [&](const floatx16& v, int which) {
           uint32_t top = 0;
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            if (nt + 8 * (r >> 2) < N) top = max(top, finite_bits(v[r]));
+            if (n0 + nt + 8 * (r >> 2) < N) top = max(top, finite_bits(v[r]));
           const auto both = __builtin_amdgcn_permlane32_swap(top, top, false, false);
           top = max((uint32_t)both[0], (uint32_t)both[1]);
           const int scale = fp8_scale(top);
@@ -287,64 +349,76 @@ __global__ __launch_bounds__(256, 2) void gated_kernel(const GatedArgs a) {
             c[r] = fp8_pack4(f[0], f[1], f[2], f[3], inverse);
           }
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const u32x2 o = join_halves(c[2 * r], c[2 * r + 1]);
-            const int n = nt + 16 * r + 8 * high;
-            if (m < M && n < N) *(u32x2*)(codes + row * N + n) = o;
-          }
-          if (m < M && nt < N && high == 0) scales[row * nb + nt / kFp8Block] = (uint8_t)scale;
+          for (int r = 0; r < 2; ++r)
+            *(u32x2*)(more + (64 * which + mine) * CP + nt + 16 * r + 8 * high) = join_halves(c[2 * r], c[2 * r + 1]);
+          if (high == 0) bytes[(64 * which + mine) * 4 + nt / kFp8Block] = (char)scale;
         };
-        keep(p[i][j], a.up_codes, a.up_scales);
-        keep(q[i][j], a.gate_codes, a.gate_scales);
+        keep(p[i][j], 0);
+        keep(q[i][j], 1);
       }
-      if (EPI != BACK) {
-        u32x2 o[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float f[4];
+      for (int r = 0; r < 4; r += 2) {  // two groups of four neighbours, then eight a lane
+        char* const at = vals + mine * VP + 2 * (nt + 8 * r + 8 * high);
+        u32x2 o[2], oq[2];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int k = 4 * r + e;
-            f[e] = value_of<ACT>(p[i][j][k], q[i][j][k]);
-            if (ACT == RELU && a.mask) f[e] *= mask[k];
-          }
-          o[r] = u32x2{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3])};
-        }
+        for (int e = 0; e < 2; ++e) {
+          float f[4], fq[4];
+          bf16x4 g;
+          if (EPI == BACK) g = *(const bf16x4*)(vals + mine * VP + 2 * (nt + 8 * (r + e) + 4 * high));
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          u32x4 v;
-          join_halves(o[2 * r], o[2 * r + 1], v);
-          const int n = nt + 16 * r + 8 * high;
-          if (m < M && n < N) *(u32x4*)(a.out + row * N + n) = v;
-        }
-      } else {
-        // (Each lane's own four neighbours of the gradient at a time.)
-#pragma unroll
-        for (int r = 0; r < 4; r += 2) {
-          u32x2 op[2], oq[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int n = nt + 8 * (r + e) + 4 * high;
-            bf16x4 g = {};
-            if (m < M && n < N) g = *(const bf16x4*)(a.g + row * N + n);
-            float fp[4], fq[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int at = 4 * (r + e) + k;
+          for (int k = 0; k < 4; ++k) {
+            const int v = 4 * (r + e) + k;
+            if (EPI == BACK) {
               float gv = (float)g[k];
-              if (ACT == RELU && a.mask) gv *= mask[at];
-              grads_of<ACT>(gv, p[i][j][at], q[i][j][at], fp[k], fq[k]);
+              if (ACT == RELU && a.mask) gv *= mask[r + e][k];
+              grads_of<ACT>(gv, p[i][j][v], q[i][j][v], f[k], fq[k]);
+            } else {
+              f[k] = value_of<ACT>(p[i][j][v], q[i][j][v]);
+              if (ACT == RELU && a.mask) f[k] *= mask[r + e][k];
             }
-            op[e] = u32x2{pack_bf16x2(fp[0], fp[1]), pack_bf16x2(fp[2], fp[3])};
-            oq[e] = u32x2{pack_bf16x2(fq[0], fq[1]), pack_bf16x2(fq[2], fq[3])};
           }
-          u32x4 vp, vq;
-          join_halves(op[0], op[1], vp);
-          join_halves(oq[0], oq[1], vq);
-          const int n = nt + 8 * r + 8 * high;
-          if (m < M && n < N) {
-            *(u32x4*)(a.dp + row * N + n) = vp;
-            *(u32x4*)(a.dq + row * N + n) = vq;
+          o[e] = u32x2{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3])};
+          if (EPI == BACK) oq[e] = u32x2{pack_bf16x2(fq[0], fq[1]), pack_bf16x2(fq[2], fq[3])};
+        }
+        // (BACK: the two lanes of a row have read its gradients before either writes over them.)
+        u32x4 v;
+        join_halves(o[0], o[1], v);
+        *(u32x4*)at = v;
+        if (EPI == BACK) {
+          join_halves(oq[0], oq[1], v);
+          *(u32x4*)(at + 64 * VP) = v;
+        }
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int r = (int)threadIdx.x / 16 + 16 * e, c = (int)threadIdx.x % 16, m = token(r, j);
+      if (m >= M || n0 + 8 * c >= N) continue;
+      const int64_t to = place(m) * N + n0 + 8 * c;
+      const u32x4 v = *(const u32x4*)(vals + r * VP + 16 * c);
+      __builtin_nontemporal_store(v, (u32x4*)((EPI == BACK ? a.dp : a.out) + to));
+      if (EPI == BACK) *(u32x4*)(a.dq + to) = *(const u32x4*)(more + r * VP + 16 * c);
+    }
+    if (EPI == SAVE) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int which = e >> 1, r = (int)threadIdx.x / 8 + 32 * (e & 1), c = (int)threadIdx.x % 8, m = token(r, j);
+        if (m >= M || n0 + 16 * c >= N) continue;
+        uint8_t* to = (which ? a.gate_codes : a.up_codes) + place(m) * N + n0 + 16 * c;
+        const u32x4 v = *(const u32x4*)(more + (64 * which + r) * CP + 16 * c);
+        if (n0 + 16 * c + 16 <= N) __builtin_nontemporal_store(v, (u32x4_8*)to);
+        else *(u32x2*)to = u32x2{v[0], v[1]};
+      }
+      if (threadIdx.x < 128) {
+        const int which = (int)threadIdx.x >> 6, r = (int)threadIdx.x & 63, m = token(r, j);
+        if (m < M) {
+          uint8_t* to = (which ? a.gate_scales : a.up_scales) + place(m) * nb + n0 / kFp8Block;
+          const uint32_t v = *(const uint32_t*)(bytes + threadIdx.x * 4);
+          if (n0 + 96 < N) {
+            *(u32_1*)to = v;
+          } else {
+            for (int k = 0; n0 + kFp8Block * k < N; ++k) to[k] = (uint8_t)(v >> (8 * k));
           }
         }
       }
@@ -365,6 +439,14 @@ __global__ __launch_bounds__(256) void gated_grads_kernel(const GatedArgs a) {
     const u32x2 cp = *(const u32x2*)(a.up_codes + at), cq = *(const u32x2*)(a.gate_codes + at);
     const float sp = fp8_power(a.up_scales[block]), sq = fp8_power(a.gate_scales[block]);
     bf16x8 dp, dq;
+    floatx4 m2[2];
+    if (ACT == RELU && a.mask) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        m2[half] = *(const floatx4*)(a.mask + n + 4 * half);
+        m2[half] *= m2[half];
+      }
+    }
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       float p[4], q[4];
@@ -373,10 +455,7 @@ __global__ __launch_bounds__(256) void gated_grads_kernel(const GatedArgs a) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         float gv = (float)g[4 * half + k], fp, fq;
-        if (ACT == RELU && a.mask) {
-          const float m = a.mask[n + 4 * half + k];
-          gv *= m * m;
-        }
+        if (ACT == RELU && a.mask) gv *= m2[half][k];
         grads_of<ACT>(gv, p[k], q[k], fp, fq);
         dp[4 * half + k] = (bf16_t)fp;
         dq[4 * half + k] = (bf16_t)fq;
@@ -398,11 +477,70 @@ struct ProductArgs {
   int64_t c_head;
   TokenRows c_rows;
   int parts;                // of this launch's k
+  int fused_tiles;          // fused_kernel: tiles of 128 tokens or latents
   int x_parts;              // sums that make up d_x
   int64_t x_size, c_size;   // elements of d_x, d_c
   bf16_t *d_x, *d_c, *d_up, *d_gate;
   float *x_sums, *c_sums, *w_sums;
 };
+
+// A wave's sums of a product, 32 NA of the result's columns from a0 by 32 NB of its rows
+// from b0: to the gradient in bf16, or as one of the parts that join_kernel adds.
+template <int WHAT, int NA, int NB>
+__device__ __forceinline__ void store_product(const ProductArgs& a, const floatx16 (&acc)[NA][NB], int h, int which,
+                                              int part, int a0, int b0, int lane) {
+  const int high = lane >> 5;
+  const bool ctx = which && a.c;
+  const int a_end = (int)(WHAT == INPUTS ? a.D : a.N), b_end = (int)(WHAT == INPUTS ? a.M : a.D);
+  bf16_t* out;
+  float* sums;
+  int64_t out_at = 0;
+  bool direct;
+  if (WHAT == INPUTS && ctx) {
+    out_at = (int64_t)h * a.c_head;
+    out = a.d_c;
+    sums = a.c_sums + part * a.c_size;
+    direct = a.parts == 1;
+  } else if (WHAT == INPUTS) {
+    out = a.d_x;
+    sums = a.x_sums + ((int64_t)(which * a.H + h) * a.parts + part) * a.x_size;
+    direct = a.x_parts == 1;
+  } else {
+    out_at = (int64_t)h * a.D * a.N;
+    out = which ? a.d_gate : a.d_up;
+    sums = a.w_sums + ((int64_t)part * 2 + which) * a.H * a.D * a.N;
+    direct = a.parts == 1;
+  }
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    const int b = b0 + 32 * j + (lane & 31);
+    if (b >= b_end) continue;
+    const int64_t row = out_at + (WHAT == WEIGHTS ? b * a.N : ctx ? a.c_rows.at((uint32_t)b) : b * a.D);
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[i][j][8 * r + e]),
+                                                          __float_as_uint(acc[i][j][8 * r + 4 + e]), false, false);
+          v[e] = __uint_as_float(x[0]);
+          v[4 + e] = __uint_as_float(x[1]);
+        }
+        const int at = a0 + 32 * i + 16 * r + 8 * high;
+        if (at >= a_end) continue;
+        if (direct) {
+          *(u32x4*)(out + row + at) = u32x4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
+                                            pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
+        } else {
+          *(floatx4*)(sums + row + at) = floatx4{v[0], v[1], v[2], v[3]};
+          *(floatx4*)(sums + row + at + 4) = floatx4{v[4], v[5], v[6], v[7]};
+        }
+      }
+    }
+  }
+}
 
 template <int WHAT>
 __global__ __launch_bounds__(256, 2) void product_kernel(const ProductArgs a) {
@@ -416,7 +554,6 @@ __global__ __launch_bounds__(256, 2) void product_kernel(const ProductArgs a) {
   const int h = job % a.H, which = job / a.H;  // which: 0 up, 1 gate
   const int a0 = (int)blockIdx.x * 256, b0 = (int)blockIdx.y * 128;
   const int K = WHAT == INPUTS ? N : M;
-  const int a_end = WHAT == INPUTS ? D : N, b_end = WHAT == INPUTS ? M : D;
   const bf16_t* dv = which ? a.dq : a.dp;        // [M, H, N]
   const int64_t d_row = (int64_t)a.H * N;
   const bool ctx = which && a.c;
@@ -492,54 +629,245 @@ __global__ __launch_bounds__(256, 2) void product_kernel(const ProductArgs a) {
         for (int j = 0; j < 2; ++j) acc[i][j] = mfma32(fa[i], fb[j], acc[i][j]);
     }
   }
-  const int high = lane >> 5;
-  bf16_t* out = nullptr;
-  float* sums = nullptr;
-  int64_t out_at = 0;
-  if (WHAT == INPUTS) {
-    if (ctx) {
-      out_at = (int64_t)h * a.c_head;
-      out = a.d_c;
-      sums = a.c_sums + part * a.c_size;
+  store_product<WHAT>(a, acc, h, which, part, a0 + aw, b0 + bw, lane);
+}
+
+// Both products of a kind straight from what the forward saved, D up to 256: dp and dq are
+// made a step or two ahead, between memory and LDS, and never written.  A workgroup has
+// eight waves, four for each product: INPUTS  128 tokens of a head by all columns, dx by
+// four waves and dc by four; WEIGHTS  128 latents by all columns of dU and of dG.  Beside
+// the tiles' direct loads a thread asks for eight neighbours of the gradient and of both
+// codes a step, four steps ahead: WEIGHTS of 32 tokens by 128 latents; INPUTS of 64 tokens
+// by the 64 latents of two steps, so that memory sees 128 (64) bytes of a row.
+template <int WHAT, int ACT, bool MASK>
+__global__ __launch_bounds__(512, 1) void fused_kernel(const ProductArgs a, const GatedArgs g) {
+  constexpr bool IN = WHAT == INPUTS;
+  typedef Tile<IN ? KC : MC, 256, 8> F;  // U, G rows d / x, c columns d
+  typedef Tile<MC, 128, 8> P;            // WEIGHTS: dp, dq columns n
+  constexpr int TILES = 2 * F::BYTES, LOADS = 2 * F::LOADS;
+  // dp and dq: INPUTS [128 tokens][64 latents], chunk c of row r at c ^ (r & 7), twice;
+  // WEIGHTS a tile of a step, three times.
+  constexpr int GRAD = IN ? 128 * 128 : P::BYTES, GRADS = IN ? 2 : 3;
+  constexpr int NA = IN ? 4 : 2, NB = 6 - NA;
+  __shared__ __attribute__((aligned(16))) char lds[3 * TILES + GRADS * 2 * GRAD];
+  char* const grads = lds + 3 * TILES;
+  const int lane = threadIdx.x & 63, w = wave_id(), which = w >> 2;
+  const int D = (int)a.D, N = (int)a.N, M = (int)a.M;
+  // An XCD (every eighth workgroup) takes neighbours of a head, which share its tiles.
+  const int tiles = a.fused_tiles, per_xcd = (tiles * a.H * a.parts + 7) / 8;
+  const int id = ((int)blockIdx.x & 7) * per_xcd + ((int)blockIdx.x >> 3);
+  if ((int)blockIdx.x >> 3 >= per_xcd || id >= tiles * a.H * a.parts) return;
+  const int at0 = id % tiles * 128, part = id / tiles % a.parts, h = id / tiles / a.parts;
+  const int K = IN ? N : M;
+  const int nb = (N + kFp8Block - 1) / kFp8Block;
+  // The tiles' sources.
+  const int fc = F::chunk(w, lane) * 8;
+  const char* fp[2][F::LOADS];
+#pragma unroll
+  for (int j = 0; j < F::LOADS; ++j) {
+    const int r = F::row(j, w, lane);
+    if (IN) {
+      const int64_t off = ((int64_t)h * D + (r < D ? r : D - 1)) * N + fc;
+      fp[0][j] = (const char*)(a.up + off);
+      fp[1][j] = (const char*)(a.gate + off);
     } else {
-      out = a.d_x;
-      sums = a.x_sums + ((int64_t)(which * a.H + h) * a.parts + part) * a.x_size;
+      const int d = fc < D ? fc : 0;
+      fp[0][j] = (const char*)(a.x + (int64_t)r * D + d);
+      fp[1][j] = (const char*)(a.c + (int64_t)h * a.c_head + d);
     }
-  } else {
-    out_at = (int64_t)h * D * N;
-    out = which ? a.d_gate : a.d_up;
-    sums = a.w_sums + ((int64_t)part * 2 + which) * a.H * D * N;
   }
-  const bool direct = WHAT == INPUTS ? (ctx ? a.parts == 1 : a.x_parts == 1) : a.parts == 1;
+  const bool two = IN || a.c;  // WEIGHTS without a context: x for both
+  // Steps of this part: an even number before it.
+  const int steps = (K + BK - 1) / BK, pairs = (steps + 1) / 2;
+  const int s0 = 2 * (int)((int64_t)pairs * part / a.parts);
+  const int s1 = min(steps, 2 * (int)((int64_t)pairs * (part + 1) / a.parts));
+  const auto issue = [&](auto inside, int s, int stage) {
+    const int k0 = s * BK;
+    const bool whole = decltype(inside)::value || (s < s1 && k0 + BK <= K);
+    const uint32_t base = (uint32_t)(stage * TILES);
+    const auto in = [&](int j) { return s < s1 && k0 + (IN ? fc : F::row(j, w, lane)) < K; };
+    fill<F>(lds, base, w, lane, whole, [&](int j) { return fp[0][j] + 2 * (IN ? (int64_t)k0 : (int64_t)k0 * D); }, in);
+    if (two)
+      fill<F>(lds, base + F::BYTES, w, lane, whole,
+              [&](int j) { return fp[1][j] + 2 * (IN ? (int64_t)k0 : a.c_rows.at((uint32_t)(k0 + F::row(j, w, lane)))); },
+              in);
+  };
+  // A thread's eight neighbours of step s (their k: where the step's begin, and theirs
+  // beyond that).  odd: s & 1.  Where they lie: a base that moves with the step, and the
+  // thread's place (rows and latents past the end: the last ones').
+  const int row = (int)threadIdx.x / (IN ? 8 : 16), col = 8 * ((int)threadIdx.x % (IN ? 8 : 16));
+  const int64_t d_row = (int64_t)a.H * N, b_row = (int64_t)a.H * nb;
+  const int64_t d_base = (int64_t)h * N + (IN ? at0 * d_row : 0), b_base = (int64_t)h * nb + (IN ? at0 * b_row : 0);
+  const auto k_of = [&](int s) { return IN ? (s >> 1) * 2 * BK + col : s * BK + row; };
+  const auto place = [&](int odd, uint32_t& d, uint32_t& b) {
+    const int r = IN ? row + 64 * odd : row;
+    const int m = IN && at0 + r >= M ? M - 1 - at0 : r, n = IN ? col : (at0 + col < N ? at0 + col : N - 8);
+    d = (uint32_t)(m * d_row + n);
+    b = (uint32_t)(m * b_row + n / kFp8Block);
+  };
+  uint32_t d_own[2], b_own[2];
+  place(0, d_own[0], b_own[0]);
+  place(1, d_own[1], b_own[1]);
+  struct Raw {
+    u32x4 g;
+    u32x2 p, q;
+    int sp, sq;
+  };
+  // Always RAW loads, which the waits below count.
+  constexpr int RAW = 5;
+  const auto load_at = [&](int64_t d, int64_t b, uint32_t d_off, uint32_t b_off, Raw& r) {
+    r.g = *(const u32x4*)((const char*)(g.g + d) + 2 * d_off);
+    r.p = *(const u32x2*)(g.up_codes + d + d_off);
+    r.q = *(const u32x2*)(g.gate_codes + d + d_off);
+    r.sp = (g.up_scales + b)[b_off];
+    r.sq = (g.gate_scales + b)[b_off];
+  };
+  // inside: all of a step's k lies within K.
+  const auto load = [&](auto inside, int s, int odd, Raw& r) {
+    const auto d_at = [&](int s) { return d_base + (IN ? (int64_t)(s >> 1) * 2 * BK : s * BK * d_row); };
+    const auto b_at = [&](int s) { return b_base + (IN ? (int64_t)(s >> 1) * 2 : s * BK * b_row); };
+    if constexpr (decltype(inside)::value) {
+      load_at(d_at(s), b_at(s), d_own[odd], b_own[odd], r);
+      return;
+    }
+    // Past the end: INPUTS the last eight latents, WEIGHTS the last token.
+    const int k = k_of(s), last = IN ? K - 8 : K - 1;
+    if (k <= last) {
+      load_at(d_at(s), b_at(s), d_own[odd], b_own[odd], r);
+    } else if (IN) {
+      load_at(d_base + last - col, b_base + last / kFp8Block - col / kFp8Block, d_own[odd], b_own[odd], r);
+    } else {
+      load_at(d_base + (last - row) * d_row, b_base + (last - row) * b_row, d_own[odd], b_own[odd], r);
+    }
+  };
+  // MASK: relu's mask, squared, of the thread's latents.
+  const auto mask_of = [&](int n, floatx4 (&m2)[2]) {
+    const float* at = g.mask + (n < N ? n : N - 8);
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int b = b0 + bw + 32 * j + (lane & 31);
-    if (b >= b_end) continue;
-    const int64_t row = out_at + (WHAT == INPUTS ? (ctx ? a.c_rows.at((uint32_t)b) : (int64_t)b * D) : (int64_t)b * N);
+    for (int half = 0; half < 2; ++half) {
+      m2[half] = *(const floatx4*)(at + 4 * half);
+      m2[half] *= m2[half];
+    }
+  };
+  floatx4 m2[2];
+  if (MASK && !IN) mask_of(at0 + col, m2);
+  u32x4 dp, dq;
+  const auto make = [&](auto inside, int s, const Raw& r) {
+    const float sp = fp8_power(r.sp), sq = fp8_power(r.sq);
+    const bf16x8 gv = __builtin_bit_cast(bf16x8, r.g);
+    if (MASK && IN) mask_of(k_of(s), m2);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int half = 0; half < 2; ++half) {
+      float p[4], q[4], fp_[4], fq[4];
+      fp8_unpack4(r.p[half], sp, p);
+      fp8_unpack4(r.q[half], sq, q);
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        float v[8];
+      for (int k = 0; k < 4; ++k) {
+        float v = (float)gv[4 * half + k];
+        if (MASK) v *= m2[half][k];
+        grads_of<ACT>(v, p[k], q[k], fp_[k], fq[k]);
+      }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[i][j][8 * r + e]),
-                                                          __float_as_uint(acc[i][j][8 * r + 4 + e]), false, false);
-          v[e] = __uint_as_float(x[0]);
-          v[4 + e] = __uint_as_float(x[1]);
-        }
-        const int at = a0 + aw + 32 * i + 16 * r + 8 * high;
-        if (at >= a_end) continue;
-        if (direct) {
-          *(u32x4*)(out + row + at) = u32x4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
-                                            pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
-        } else {
-          *(floatx4*)(sums + row + at) = floatx4{v[0], v[1], v[2], v[3]};
-          *(floatx4*)(sums + row + at + 4) = floatx4{v[4], v[5], v[6], v[7]};
-        }
+      for (int k = 0; k < 2; ++k) {
+        dp[2 * half + k] = pack_bf16x2(fp_[2 * k], fp_[2 * k + 1]);
+        dq[2 * half + k] = pack_bf16x2(fq[2 * k], fq[2 * k + 1]);
       }
     }
+    if constexpr (!decltype(inside)::value)
+      if ((IN ? s & ~1 : s) >= s1 || k_of(s) >= K) dp = dq = u32x4{0, 0, 0, 0};
+  };
+  // In LDS: WEIGHTS as a tile of 32 k's; buffer: of the step or pair.
+  const uint32_t to = IN ? (uint32_t)(row * 128 + (((col >> 3) ^ (row & 7)) << 4))
+                         : (uint32_t)(row * 256 + (((col >> 3) ^ ((row & 3) << 2)) << 4));
+  const auto put = [&](int buffer, int odd) {
+    char* t = grads + buffer * 2 * GRAD + to + (IN ? odd * 64 * 128 : 0);
+    *(u32x4*)t = dp;
+    *(u32x4*)(t + GRAD) = dq;
+  };
+  floatx16 acc[NA][NB];
+#pragma unroll
+  for (int i = 0; i < NA; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) acc[i][j] = zero16();
+  const int w4 = w & 3;
+  const int aw = 32 * NA * (w4 & 1), bw = 32 * NB * (w4 >> 1);
+  const uint32_t f_at = which && two ? F::BYTES : 0, p_at = (uint32_t)(which * GRAD);
+  const auto grad_frag = [&](const char* t, int at, int odd, int kk) -> bf16x8 {
+    if constexpr (!IN) return P::frag(t, at, kk, lane);
+    const int r = at + (lane & 31), c = 4 * odd + 2 * kk + (lane >> 5);
+    return *(const bf16x8*)(t + r * 128 + ((c ^ (r & 7)) << 4));
+  };
+  // Fragments of 16 k's, read in the order in which the products take them.
+  struct Frags {
+    bf16x8 a[NA], b[NB];
+  };
+  const auto frag_of = [&](Frags& f, int i, const char* t, const char* d, int odd, int kk) {
+    if (i < NB) {
+      f.b[i] = IN ? grad_frag(d + p_at, bw + 32 * i, odd, kk) : F::frag(t + f_at, bw + 32 * i, kk, lane);
+    } else {
+      const int j = i - NB;
+      f.a[j] = IN ? F::frag(t + f_at, aw + 32 * j, kk, lane) : grad_frag(d + p_at, aw + 32 * j, odd, kk);
+    }
+  };
+  const auto product = [&](const Frags& f, int i) {
+    acc[i / NB][i % NB] = mfma32(f.a[i / NB], f.b[i % NB], acc[i / NB][i % NB]);
+  };
+  // Step s: the tile of step s + 2 is asked for, the gradients of step s + AHEAD are made
+  // from what was asked for four steps ago, step s is multiplied.  (INPUTS: a pair's
+  // gradients are made while the pair before it is multiplied.)  Groups of four steps, in
+  // which the raw values keep their registers; inside: all that a group asks for lies
+  // within k, and nothing in it branches.  The last groups end with steps of zeros.
+  constexpr int AHEAD = IN ? 2 : 1;
+  const std::false_type no{};
+  Raw raw[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) load(no, s0 + u, u & 1, raw[u]);
+  issue(no, s0, 0);
+  issue(no, s0 + 1, 1);
+#pragma unroll
+  for (int u = 0; u < AHEAD; ++u) {
+    make(no, s0 + u, raw[u]);
+    put(0, u);
+    load(no, s0 + 4 + u, u, raw[u]);
   }
+  int stage = 0, s = s0;
+  const auto group = [&](auto inside) {
+    constexpr bool INSIDE = decltype(inside)::value;
+#pragma unroll
+    for (int u = 0; u < 4; ++u, ++s) {
+      // Since this step's tiles were asked for: two steps' raw values, the next step's tiles.
+      if (INSIDE || (s > s0 && s + 1 < s1 && (s + 2) * BK <= K)) {
+        if (two) wait_barrier<LOADS + 2 * RAW>();
+        else wait_barrier<F::LOADS + 2 * RAW>();
+      } else {
+        wait_barrier<0>();
+      }
+      const int next = stage == 2 ? 0 : stage + 1, after = next == 2 ? 0 : next + 1;
+      const char* t = lds + stage * TILES;
+      const char* d = grads + (IN ? u >> 1 : stage) * 2 * GRAD;
+      const int to_buffer = IN ? (u >> 1) ^ 1 : next;
+      Raw& r = raw[(u + AHEAD) & 3];
+      issue(inside, s + 2, after);
+      Frags f;
+#pragma unroll
+      for (int i = 0; i < NA + NB; ++i) frag_of(f, i, t, d, u & 1, 0);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) product(f, i);
+#pragma unroll
+      for (int i = 0; i < NA + NB; ++i) frag_of(f, i, t, d, u & 1, 1);
+      make(inside, s + AHEAD, r);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) product(f, i);
+      put(to_buffer, u & 1);
+      load(inside, s + AHEAD + 4, (u + AHEAD) & 1, r);
+      stage = next;
+    }
+  };
+  const int last = min(s1, K / BK) - 1;  // whole step
+  if (s < s1) group(no);
+  while (s + 10 <= last) group(std::true_type{});
+  while (s < s1) group(no);
+  store_product<WHAT>(a, acc, h, which, part, (IN ? 0 : at0) + aw, (IN ? at0 : 0) + bw, lane);
 }
 
 // out[i] = the sum of n parts, in their order; eight neighbours a thread.
@@ -565,7 +893,7 @@ TokenRows token_rows(int64_t time, int64_t batch_stride, int64_t step) {
 
 template <int ACT, int EPI>
 void launch_projections(const GatedArgs& a, hipStream_t st) {
-  const dim3 grid(cdiv(a.N, 128) * (unsigned)a.H * cdiv(a.M, 128));
+  const dim3 grid(grid_of(a.order));
   if (a.c) hipLaunchKernelGGL((gated_kernel<ACT, EPI, true>), grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL((gated_kernel<ACT, EPI, false>), grid, dim3(256), 0, st, a);
 }
@@ -574,6 +902,16 @@ void launch_projections(const GatedArgs& a, int act, hipStream_t st) {
   if (act == RELU) launch_projections<RELU, EPI>(a, st);
   else if (act == SILU) launch_projections<SILU, EPI>(a, st);
   else launch_projections<GELU, EPI>(a, st);
+}
+
+template <int WHAT>
+void launch_fused(ProductArgs p, const GatedArgs& a, int act, hipStream_t st) {
+  p.fused_tiles = (int)cdiv(WHAT == INPUTS ? p.M : p.N, 128);
+  const dim3 grid(cdiv((int64_t)p.fused_tiles * p.H * p.parts, 8) * 8);
+  if (act == RELU && a.mask) hipLaunchKernelGGL((fused_kernel<WHAT, RELU, true>), grid, dim3(512), 0, st, p, a);
+  else if (act == RELU) hipLaunchKernelGGL((fused_kernel<WHAT, RELU, false>), grid, dim3(512), 0, st, p, a);
+  else if (act == SILU) hipLaunchKernelGGL((fused_kernel<WHAT, SILU, false>), grid, dim3(512), 0, st, p, a);
+  else hipLaunchKernelGGL((fused_kernel<WHAT, GELU, false>), grid, dim3(512), 0, st, p, a);
 }
 
 GatedArgs args_of(const GatedCall& g) {
@@ -596,6 +934,7 @@ GatedArgs args_of(const GatedCall& g) {
   a.up_scales = g.up_scales;
   a.gate_codes = g.gate_codes;
   a.gate_scales = g.gate_scales;
+  a.order = tile_order((int64_t)cdiv(g.N, 128) * g.H, cdiv(a.M, 128));
   return a;
 }
 
@@ -613,16 +952,20 @@ bdh_status gated_block(const GatedCall& g, hipStream_t st, uint64_t* launches) {
 bdh_status gated_block_vjp(const GatedCall& g, hipStream_t st, uint64_t* launches) {
   GatedArgs a = args_of(g);
   const int64_t M = a.M, H = g.H, N = g.N, D = g.D;
-  // Parts of k: enough workgroups to fill the chip twice.
-  const int64_t want = 2 * (int64_t)device_cus();
-  const auto parts_of = [&](int64_t tiles, int64_t K) {
+  // (The fused kernels hold a step of 128 tokens' places in 32 bits.)
+  const bool fused = g.up_codes && D <= 256 && H * N <= (int64_t)1 << 23;
+  // Parts of k: enough workgroups to fill the chip.
+  const int64_t cus = device_cus();
+  const auto parts_of = [&](int64_t tiles, int64_t want, int64_t K) {
     int64_t p = (want + tiles - 1) / tiles;
     const int64_t most = K / 256 > 1 ? K / 256 : 1;
     p = p < most ? p : most;
     return (int)(p < 32 ? p : 32);
   };
-  const int in_parts = parts_of((int64_t)cdiv(D, 256) * cdiv(M, 128) * 2 * H, N);
-  const int w_parts = parts_of((int64_t)cdiv(N, 256) * cdiv(D, 128) * 2 * H, M);
+  const int in_parts = fused ? parts_of(cdiv(M, 128) * H, cus, N)
+                             : parts_of((int64_t)cdiv(D, 256) * cdiv(M, 128) * 2 * H, 2 * cus, N);
+  const int w_parts = fused ? parts_of(cdiv(N, 128) * H, cus, M)
+                            : parts_of((int64_t)cdiv(N, 256) * cdiv(D, 128) * 2 * H, 2 * cus, M);
   ProductArgs p{};
   p.x_parts = (int)((g.c ? 1 : 2) * H * in_parts);
   p.x_size = M * D;
@@ -631,11 +974,14 @@ bdh_status gated_block_vjp(const GatedCall& g, hipStream_t st, uint64_t* launche
   const size_t x_bytes = p.x_parts > 1 ? (size_t)p.x_parts * p.x_size * 4 : 0;
   const size_t c_bytes = g.c && in_parts > 1 ? (size_t)in_parts * p.c_size * 4 : 0;
   const size_t w_bytes = w_parts > 1 ? (size_t)w_parts * 2 * w_size * 4 : 0;
-  void* buf = nullptr;
-  bdh_status s = scratch(st, SLOT_GATED_GRADS, (size_t)(2 * M * H * N) * sizeof(bf16_t), &buf);
-  if (s != BDH_OK) return s;
-  a.dp = (bf16_t*)buf;
-  a.dq = a.dp + M * H * N;
+  bdh_status s;
+  if (!fused) {
+    void* buf = nullptr;
+    s = scratch(st, SLOT_GATED_GRADS, (size_t)(2 * M * H * N) * sizeof(bf16_t), &buf);
+    if (s != BDH_OK) return s;
+    a.dp = (bf16_t*)buf;
+    a.dq = a.dp + M * H * N;
+  }
   // (The inputs' sums are joined before the weights' are made.)
   const size_t sums = x_bytes + c_bytes > w_bytes ? x_bytes + c_bytes : w_bytes;
   void* part = nullptr;
@@ -643,13 +989,16 @@ bdh_status gated_block_vjp(const GatedCall& g, hipStream_t st, uint64_t* launche
     s = scratch(st, SLOT_GATED_SUMS, sums, &part);
     if (s != BDH_OK) return s;
   }
-  if (g.up_codes) {
-    const dim3 grid((unsigned)capped(cdiv(M * H * (N / 8), 256)));
-    if (g.act == RELU) hipLaunchKernelGGL((gated_grads_kernel<RELU>), grid, dim3(256), 0, st, a);
-    else if (g.act == SILU) hipLaunchKernelGGL((gated_grads_kernel<SILU>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((gated_grads_kernel<GELU>), grid, dim3(256), 0, st, a);
-  } else {
-    launch_projections<BACK>(a, g.act, st);
+  if (!fused) {
+    if (g.up_codes) {
+      const dim3 grid((unsigned)capped(cdiv(M * H * (N / 8), 256)));
+      if (g.act == RELU) hipLaunchKernelGGL((gated_grads_kernel<RELU>), grid, dim3(256), 0, st, a);
+      else if (g.act == SILU) hipLaunchKernelGGL((gated_grads_kernel<SILU>), grid, dim3(256), 0, st, a);
+      else hipLaunchKernelGGL((gated_grads_kernel<GELU>), grid, dim3(256), 0, st, a);
+    } else {
+      launch_projections<BACK>(a, g.act, st);
+    }
+    *launches += 1;
   }
   p.dp = a.dp;
   p.dq = a.dq;
@@ -671,26 +1020,26 @@ bdh_status gated_block_vjp(const GatedCall& g, hipStream_t st, uint64_t* launche
   p.c_sums = (float*)((char*)part + x_bytes);
   p.w_sums = (float*)part;
   p.parts = in_parts;
-  hipLaunchKernelGGL((product_kernel<INPUTS>), dim3(cdiv(D, 256), cdiv(M, 128), (unsigned)(2 * H * in_parts)),
-                     dim3(256), 0, st, p);
-  *launches += 2;
-  const auto join = [&](const float* from, int n, int64_t size, bf16_t* out) {
-    hipLaunchKernelGGL(join_kernel, dim3((unsigned)capped(cdiv(size, 2048))), dim3(256), 0, st, from, n, size, out,
+  if (fused) launch_fused<INPUTS>(p, a, g.act, st);
+  else
+    hipLaunchKernelGGL((product_kernel<INPUTS>), dim3(cdiv(D, 256), cdiv(M, 128), (unsigned)(2 * H * in_parts)),
+                       dim3(256), 0, st, p);
+  const auto join = [&](const float* from, int n, int64_t stride, bf16_t* out, int64_t size) {
+    hipLaunchKernelGGL(join_kernel, dim3((unsigned)capped(cdiv(size, 2048))), dim3(256), 0, st, from, n, stride, out,
                        size);
     *launches += 1;
   };
-  if (x_bytes) join(p.x_sums, p.x_parts, p.x_size, g.d_x);
-  if (c_bytes) join(p.c_sums, in_parts, p.c_size, g.d_c);
+  if (x_bytes) join(p.x_sums, p.x_parts, p.x_size, g.d_x, p.x_size);
+  if (c_bytes) join(p.c_sums, in_parts, p.c_size, g.d_c, p.c_size);
   p.parts = w_parts;
-  hipLaunchKernelGGL((product_kernel<WEIGHTS>), dim3(cdiv(N, 256), cdiv(D, 128), (unsigned)(2 * H * w_parts)),
-                     dim3(256), 0, st, p);
-  *launches += 1;
+  if (fused) launch_fused<WEIGHTS>(p, a, g.act, st);
+  else
+    hipLaunchKernelGGL((product_kernel<WEIGHTS>), dim3(cdiv(N, 256), cdiv(D, 128), (unsigned)(2 * H * w_parts)),
+                       dim3(256), 0, st, p);
+  *launches += 2;
   if (w_bytes) {
-    hipLaunchKernelGGL(join_kernel, dim3((unsigned)capped(cdiv(w_size, 2048))), dim3(256), 0, st, p.w_sums, w_parts,
-                       2 * w_size, g.d_up, w_size);
-    hipLaunchKernelGGL(join_kernel, dim3((unsigned)capped(cdiv(w_size, 2048))), dim3(256), 0, st, p.w_sums + w_size,
-                       w_parts, 2 * w_size, g.d_gate, w_size);
-    *launches += 2;
+    join(p.w_sums, w_parts, 2 * w_size, g.d_up, w_size);
+    join(p.w_sums + w_size, w_parts, 2 * w_size, g.d_gate, w_size);
   }
   BDH_HIP_TRY(hipGetLastError());
   return BDH_OK;
