@@ -205,7 +205,10 @@ struct SortArgs {
   int64_t n, vocab;
   const uint32_t *keys, *order;  // null: tokens in their order
   uint32_t *keys_out, *order_out, *counts;
-  int shift, bins;
+  int shift, bins;               // of this pass (or bits a pass: all in one launch)
+  int passes, blocks;            // workgroups of the sort
+  char* clear;                   // the table's gradient, and the bytes of it that the
+  int64_t clear_from, clear_to;  // workgroups past the sort's own set to 0
 };
 bdh_status embed_tokens(const EmbedArgs& a, hipStream_t st);
 bdh_status embed_tokens_vjp(EmbedArgs a, hipStream_t st, uint64_t* launches);

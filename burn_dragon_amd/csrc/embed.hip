@@ -7,9 +7,13 @@
 //
 // The gradient goes by sorted tokens, without atomics on values, so a call repeats
 // bit for bit: the positions are sorted by id (a stable radix sort of up to 9 bits
-// a pass: one pass for up to 511 rows of E, two for 2^18 - 1), then each wave sums the rows of a
-// run of positions, and writes the ids that lie within it.  An id that runs on into
-// the next runs leaves partial sums, which a second launch joins in their order.
+// a pass: one pass for up to 511 rows of E, two for 2^18 - 1; in one launch up to
+// 4096 tokens), then each wave sums the rows of a run of positions, and writes the ids
+// that lie within it.  An id that runs on into the next runs leaves partial sums,
+// which a second launch joins in their order.  The rows without a token are cleared
+// by the sort's launches beside their own work.
+#include <type_traits>
+
 #include "bdh_internal.h"
 
 namespace bdh {
@@ -17,104 +21,129 @@ namespace {
 
 typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
 typedef __bf16 bf16x4_u __attribute__((ext_vector_type(4), aligned(2)));
+typedef __bf16 bf16x8_u __attribute__((ext_vector_type(8), aligned(2)));
+template <typename T, int VEC> struct Vec;
+template <> struct Vec<float, 4> { typedef f32x4_u type; };
+template <> struct Vec<bf16_t, 4> { typedef bf16x4_u type; };
+template <> struct Vec<bf16_t, 8> { typedef bf16x8_u type; };
 
-// Four neighbouring values of a row of n from c on, zeros past its end.
-__device__ __forceinline__ floatx4 load4(const float* row, int c, int n) {
-  if (c + 4 <= n) return *(const f32x4_u*)(row + c);
-  floatx4 v = zero4();
-#pragma unroll
-  for (int j = 0; j < 3; ++j)
-    if (c + j < n) v[j] = row[c + j];
-  return v;
-}
-__device__ __forceinline__ floatx4 load4(const bf16_t* row, int c, int n) {
-  floatx4 v = zero4();
-  if (c + 4 <= n) {
-    const bf16x4_u p = *(const bf16x4_u*)(row + c);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = (float)p[j];
-  } else {
-#pragma unroll
-    for (int j = 0; j < 3; ++j)
-      if (c + j < n) v[j] = (float)row[c + j];
-  }
-  return v;
-}
-__device__ __forceinline__ void store4(float* row, int c, int n, const floatx4& v) {
-  if (c + 4 <= n) {
-    *(f32x4_u*)(row + c) = v;
-  } else {
-#pragma unroll
-    for (int j = 0; j < 3; ++j)
-      if (c + j < n) row[c + j] = v[j];
-  }
-}
-__device__ __forceinline__ void store4(bf16_t* row, int c, int n, const floatx4& v) {
-  if (c + 4 <= n) {
-    bf16x4_u p;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) p[j] = (bf16_t)v[j];
-    *(bf16x4_u*)(row + c) = p;
-  } else {
-#pragma unroll
-    for (int j = 0; j < 3; ++j)
-      if (c + j < n) row[c + j] = (bf16_t)v[j];
-  }
-}
+// A row of n columns held by a wave: lane l has columns VEC (l + 64 k) ..+VEC-1, zeros
+// past the end.
+template <typename T, int VEC, int PER>
+struct Row {
+  float v[PER][VEC];
 
-// A row held by a wave: lane l has columns 4 l + 256 k ..+3.  Sums over the row.
-template <int PER>
-__device__ __forceinline__ float row_sum(const floatx4 (&v)[PER]) {
-  float s = 0.0f;
-#pragma unroll
-  for (int k = 0; k < PER; ++k) s += (v[k][0] + v[k][1]) + (v[k][2] + v[k][3]);
-  return wave_sum(s);
-}
-template <int PER>
-__device__ __forceinline__ float row_dot(const floatx4 (&v)[PER], const floatx4 (&u)[PER]) {
-  float s = 0.0f;
-#pragma unroll
-  for (int k = 0; k < PER; ++k)
-    s += (v[k][0] * u[k][0] + v[k][1] * u[k][1]) + (v[k][2] * u[k][2] + v[k][3] * u[k][3]);
-  return wave_sum(s);
-}
-// Less its mean, zeros past column n; returns 1 / sqrt(var + eps).  The mean is taken
-// twice: the first one's rounding is large beside the values of a row that lies far
-// from zero.
-template <int PER>
-__device__ __forceinline__ float center(floatx4 (&v)[PER], int n, int lane) {
-#pragma unroll
-  for (int pass = 0; pass < 2; ++pass) {
-    const float mean = row_sum(v) / (float)n;
+  template <typename F>
+  __device__ __forceinline__ void each(F&& f) {
 #pragma unroll
     for (int k = 0; k < PER; ++k)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[k][j] = 256 * k + 4 * lane + j < n ? v[k][j] - mean : 0.0f;
+      for (int j = 0; j < VEC; ++j) f(v[k][j], VEC * 64 * k + j);
   }
-  return 1.0f / sqrtf(row_dot(v, v) / (float)n + 1e-5f);
-}
+  __device__ __forceinline__ void clear() {
+    each([](float& x, int) { x = 0.0f; });
+  }
+  template <typename S>  // of T, or partial sums of f32
+  __device__ __forceinline__ void load(const S* row, int n, int lane) {
+    constexpr int W = sizeof(S) == 4 ? 4 : VEC;
+    typedef typename Vec<S, W>::type V;
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+#pragma unroll
+      for (int q = 0; q < VEC; q += W) {
+        const int c = VEC * (lane + 64 * k) + q;
+        if (c + W <= n) {
+          const V x = *(const V*)(row + c);
+#pragma unroll
+          for (int j = 0; j < W; ++j) v[k][q + j] = (float)x[j];
+        } else {
+#pragma unroll
+          for (int j = 0; j < W; ++j) v[k][q + j] = c + j < n ? (float)row[c + j] : 0.0f;
+        }
+      }
+  }
+  template <typename S>
+  __device__ __forceinline__ void store(S* row, int n, int lane) const {
+    constexpr int W = sizeof(S) == 4 ? 4 : VEC;
+    typedef typename Vec<S, W>::type V;
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+#pragma unroll
+      for (int q = 0; q < VEC; q += W) {
+        const int c = VEC * (lane + 64 * k) + q;
+        if (c + W <= n) {
+          V x;
+#pragma unroll
+          for (int j = 0; j < W; ++j) x[j] = (S)v[k][q + j];
+          *(V*)(row + c) = x;
+        } else {
+#pragma unroll
+          for (int j = 0; j < W - 1; ++j)
+            if (c + j < n) row[c + j] = (S)v[k][q + j];
+        }
+      }
+  }
+  __device__ __forceinline__ float sum() const {
+    float s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+#pragma unroll
+      for (int j = 0; j < VEC; j += 4) s += (v[k][j] + v[k][j + 1]) + (v[k][j + 2] + v[k][j + 3]);
+    return wave_sum(s);
+  }
+  __device__ __forceinline__ float dot(const Row& u) const {
+    float s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+#pragma unroll
+      for (int j = 0; j < VEC; j += 4)
+        s += (v[k][j] * u.v[k][j] + v[k][j + 1] * u.v[k][j + 1]) +
+             (v[k][j + 2] * u.v[k][j + 2] + v[k][j + 3] * u.v[k][j + 3]);
+    return wave_sum(s);
+  }
+  // Less its mean, zeros past column n; returns 1 / sqrt(var + eps).  The mean is taken
+  // twice: the first one's rounding is large beside the values of a row that lies far
+  // from zero.
+  __device__ __forceinline__ float center(int n, int lane) {
+#pragma unroll
+    for (int pass = 0; pass < 2; ++pass) {
+      const float mean = sum() / (float)n;
+      each([&](float& x, int c) { x = c + VEC * lane < n ? x - mean : 0.0f; });
+    }
+    return 1.0f / sqrtf(dot(*this) / (float)n + 1e-5f);
+  }
+};
 
-// One wave a token.
-template <typename T, int PER, bool NORM>
+// A wave takes `each` neighbouring tokens, their rows asked for together: with one token a
+// wave, what counted was the wait for its id, then for its row (65536 tokens, D 1024, bf16).
+template <typename T, int VEC, int PER, int EACH, bool NORM>
 __global__ __launch_bounds__(256) void embed_kernel(const EmbedArgs a) {
-  const int64_t i = (int64_t)blockIdx.x * 4 + wave_id();
-  if (i >= a.n) return;
+  const int64_t i0 = ((int64_t)blockIdx.x * 4 + wave_id()) * EACH;
+  if (i0 >= a.n) return;
   const int lane = threadIdx.x & 63, D = (int)a.embd;
-  const int id = a.tokens[i];
-  const bool there = id >= 0 && id < a.vocab;
-  const T* row = (const T*)a.table + (int64_t)(there ? id : 0) * D;
-  T* out = (T*)a.out + i * D;
-  floatx4 v[PER];
+  Row<T, VEC, PER> v[EACH];
+  bool there[EACH];
+  int id[EACH];
 #pragma unroll
-  for (int k = 0; k < PER; ++k) v[k] = there ? load4(row, 256 * k + 4 * lane, D) : zero4();
-  float f = a.scale;
-  if constexpr (NORM) f = there ? f * center(v, D, lane) : 0.0f;
+  for (int q = 0; q < EACH; ++q) id[q] = a.tokens[i0 + q < a.n ? i0 + q : a.n - 1];
 #pragma unroll
-  for (int k = 0; k < PER; ++k) store4(out, 256 * k + 4 * lane, D, v[k] * f);
+  for (int q = 0; q < EACH; ++q) {
+    there[q] = id[q] >= 0 && id[q] < a.vocab;
+    v[q].load((const T*)a.table + (int64_t)(there[q] ? id[q] : 0) * D, D, lane);
+  }
+#pragma unroll
+  for (int q = 0; q < EACH; ++q) {
+    if (i0 + q >= a.n) break;
+    float f = a.scale;
+    if (NORM) f *= v[q].center(D, lane);
+    v[q].each([&](float& x, int) { x = there[q] ? x * f : 0.0f; });
+    v[q].store((T*)a.out + (i0 + q) * D, D, lane);
+  }
 }
 
 // --- the order of the positions by id -----------------------------------------------
-constexpr int kMostBins = 512, kItems = 2048;  // a pass's digits; a workgroup's positions
+constexpr int kMostBins = 512;                              // a pass's digits
+constexpr int kWaves = 16, kOwn = 256, kItems = kWaves * kOwn;  // a workgroup's positions, 256 a wave
 
 // The key of position i: its id, or vocab (past all ids) where it is none.
 __device__ __forceinline__ uint32_t key_of(const SortArgs& s, int64_t i) {
@@ -123,240 +152,365 @@ __device__ __forceinline__ uint32_t key_of(const SortArgs& s, int64_t i) {
   return id >= 0 && id < (int)s.vocab ? (uint32_t)id : (uint32_t)s.vocab;
 }
 
-// counts[workgroup][digit].
-__global__ __launch_bounds__(256) void digit_counts_kernel(const SortArgs s) {
-  __shared__ uint32_t bins[kMostBins];
-  for (int d = threadIdx.x; d < s.bins; d += 256) bins[d] = 0;
-  __syncthreads();
-  const int64_t i0 = (int64_t)blockIdx.x * kItems;
-  for (int j = threadIdx.x; j < kItems; j += 256)
-    if (i0 + j < s.n) atomicAdd(&bins[(key_of(s, i0 + j) >> s.shift) & (s.bins - 1)], 1u);
-  __syncthreads();
-  for (int d = threadIdx.x; d < s.bins; d += 256) s.counts[(int64_t)blockIdx.x * s.bins + d] = bins[d];
-}
-
-// Stable: within a digit by position.  A wave takes 512 neighbours in rounds of 64.
-__global__ __launch_bounds__(256) void digit_scatter_kernel(const SortArgs s) {
-  __shared__ uint32_t at[4][kMostBins];  // next place of a wave's digit
-  __shared__ uint32_t sums[256];
-  const int lane = threadIdx.x & 63, w = wave_id(), blocks = (int)gridDim.x, mine = (int)blockIdx.x;
-  // Places before this workgroup's: smaller digits anywhere, this digit in earlier workgroups.
-  uint32_t total[2] = {}, before[2] = {};  // of digits 2 t and 2 t + 1
-  for (int d = 0; d < 2; ++d) {
-    const int digit = 2 * threadIdx.x + d;
-    if (digit >= s.bins) break;
-    for (int b = 0; b < blocks; ++b) {
-      const uint32_t c = s.counts[(int64_t)b * s.bins + digit];
-      total[d] += c;
-      if (b < mine) before[d] += c;
+// The workgroups past the sort's own clear a share of the table's gradient.
+__device__ void clear_share(const SortArgs& s, int block, int blocks) {
+  typedef unsigned int u32x4_2 __attribute__((ext_vector_type(4), aligned(2)));
+  const int64_t stride = (int64_t)blocks * 16384;
+  for (int64_t i = s.clear_from + ((int64_t)block * 1024 + threadIdx.x) * 16; i < s.clear_to; i += stride) {
+    if (i + 16 <= s.clear_to) {
+      *(u32x4_2*)(s.clear + i) = u32x4_2{0, 0, 0, 0};
+    } else {
+      for (int64_t j = i; j < s.clear_to; j += 2) *(uint16_t*)(s.clear + j) = 0;
     }
   }
-  sums[threadIdx.x] = total[0] + total[1];
-  for (int d = threadIdx.x; d < s.bins; d += 256)
-    for (int q = 0; q < 4; ++q) at[q][d] = 0;
+}
+
+// counts[workgroup][digit].
+__global__ __launch_bounds__(1024) void digit_counts_kernel(const SortArgs s) {
+  if ((int)blockIdx.x >= s.blocks) return clear_share(s, (int)blockIdx.x - s.blocks, (int)gridDim.x - s.blocks);
+  __shared__ uint32_t bins[kMostBins];
+  for (int d = threadIdx.x; d < s.bins; d += 1024) bins[d] = 0;
   __syncthreads();
-  for (int o = 1; o < 256; o <<= 1) {
-    const uint32_t v = (int)threadIdx.x >= o ? sums[threadIdx.x - o] : 0;
-    __syncthreads();
-    sums[threadIdx.x] += v;
-    __syncthreads();
+  const int64_t i0 = (int64_t)blockIdx.x * kItems;
+#pragma unroll
+  for (int j = 0; j < kItems; j += 1024) {
+    const int64_t i = i0 + j + threadIdx.x;
+    if (i < s.n) atomicAdd(&bins[(key_of(s, i) >> s.shift) & (s.bins - 1)], 1u);
   }
-  // Each wave's counts, then their places.
-  const int64_t i0 = (int64_t)mine * kItems + w * (kItems / 4);
-  for (int j = lane; j < kItems / 4; j += 64)
-    if (i0 + j < s.n) atomicAdd(&at[w][(key_of(s, i0 + j) >> s.shift) & (s.bins - 1)], 1u);
   __syncthreads();
-  for (int d = 0; d < 2; ++d) {
-    const int digit = 2 * threadIdx.x + d;
-    if (digit >= s.bins) break;
-    uint32_t place = (threadIdx.x ? sums[threadIdx.x - 1] : 0) + (d ? total[0] : 0) + before[d];
-    for (int q = 0; q < 4; ++q) {
-      const uint32_t c = at[q][digit];
-      at[q][digit] = place;
+  for (int d = threadIdx.x; d < s.bins; d += 1024) s.counts[(int64_t)blockIdx.x * s.bins + d] = bins[d];
+}
+
+// The places of a workgroup's positions, stable: wave w has 256 neighbours, four rounds
+// of 64.  key(j), 0 <= j < 256 of the lane's wave: -1 where there is none.  first(digit):
+// the place of the workgroup's first one.  put(j, key, place).
+struct SortMemory {
+  uint32_t at[kWaves][kMostBins];  // counts, then next places
+  uint32_t total[kMostBins];
+  uint32_t sums[8];
+};
+template <typename Key, typename First, typename Put>
+__device__ __forceinline__ void sort_step(SortMemory& mem, int shift, int bins, const Key& key, const First& first,
+                                          const Put& put) {
+  const int lane = threadIdx.x & 63, w = wave_id();
+  for (int d = threadIdx.x; d < kWaves * kMostBins; d += 1024) (&mem.at[0][0])[d] = 0;
+  __syncthreads();
+  int64_t keys[kOwn / 64];
+  uint32_t rank[kOwn / 64];
+  // Each round's ranks within its digit; the digit's last lane moves the count on.
+#pragma unroll
+  for (int q = 0; q < kOwn / 64; ++q) {
+    keys[q] = key(64 * q + lane);
+    const int digit = (int)(keys[q] >> shift) & (bins - 1);
+    uint64_t same = __ballot(keys[q] >= 0);
+    for (int b = 1; b < bins; b <<= 1) {
+      const uint64_t set = __ballot((digit & b) != 0);
+      same &= (digit & b) ? set : ~set;
+    }
+    if (keys[q] >= 0) {
+      rank[q] = mem.at[w][digit] + __popcll(same & ((1ull << lane) - 1));
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      if ((same >> lane) == 1) mem.at[w][digit] = rank[q] + 1;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+  __syncthreads();
+  // Counts to places: waves in order after the digit's first place.
+  first(mem);
+  if ((int)threadIdx.x < bins) {
+    uint32_t place = mem.total[threadIdx.x];
+#pragma unroll
+    for (int q = 0; q < kWaves; ++q) {
+      const uint32_t c = mem.at[q][threadIdx.x];
+      mem.at[q][threadIdx.x] = place;
       place += c;
     }
   }
   __syncthreads();
-  for (int j = lane; j < kItems / 4; j += 64) {
-    const int64_t i = i0 + j;
-    const bool is = i < s.n;
-    const uint32_t key = is ? key_of(s, i) : 0;
-    const int digit = (int)(key >> s.shift) & (s.bins - 1);
-    uint64_t same = __ballot(is);
-    for (int b = 1; b < s.bins; b <<= 1) {
-      const uint64_t set = __ballot((digit & b) != 0);
-      same &= (digit & b) ? set : ~set;
+#pragma unroll
+  for (int q = 0; q < kOwn / 64; ++q)
+    if (keys[q] >= 0)
+      put(64 * q + lane, (uint32_t)keys[q], mem.at[w][(int)(keys[q] >> shift) & (bins - 1)] + rank[q]);
+  __syncthreads();
+}
+// mem.total[d]: the sum over the digits before d, from its own; plus[d] added.  512 threads.
+__device__ __forceinline__ void scan_digits(SortMemory& mem, uint32_t own, uint32_t plus, int bins) {
+  const int lane = threadIdx.x & 63, w = wave_id();
+  uint32_t s = own;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t v = (uint32_t)__shfl_up((int)s, o, 64);
+    if (lane >= o) s += v;
+  }
+  if (lane == 63 && w < 8) mem.sums[w] = s;
+  __syncthreads();
+  if (w < 8) {
+    for (int q = 0; q < w; ++q) s += mem.sums[q];
+    if ((int)threadIdx.x < bins) mem.total[threadIdx.x] = s - own + plus;
+  }
+  __syncthreads();
+}
+
+__global__ __launch_bounds__(1024) void digit_scatter_kernel(const SortArgs s) {
+  if ((int)blockIdx.x >= s.blocks) return clear_share(s, (int)blockIdx.x - s.blocks, (int)gridDim.x - s.blocks);
+  __shared__ SortMemory mem;
+  __shared__ uint32_t half[2][kMostBins];
+  const int mine = (int)blockIdx.x;
+  const int64_t i0 = (int64_t)mine * kItems + wave_id() * kOwn;
+  // Of a digit: all its positions, and those of earlier workgroups, by two threads.
+  uint32_t total = 0, before = 0;
+  {
+    const int digit = (int)threadIdx.x & (kMostBins - 1);
+    if (digit < s.bins) {
+#pragma unroll 8
+      for (int b = (int)threadIdx.x >> 9; b < s.blocks; b += 2) {
+        const uint32_t c = s.counts[(int64_t)b * s.bins + digit];
+        total += c;
+        before += b < mine ? c : 0;
+      }
     }
-    if (is) {
-      const uint32_t place = at[w][digit] + __popcll(same & ((1ull << lane) - 1));
-      // (The last lane of a digit moves its place on, after every lane has read it.)
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      if ((same >> lane) == 1) at[w][digit] = place + 1;
-      s.keys_out[place] = key;
-      s.order_out[place] = s.order ? s.order[i] : (uint32_t)i;
+  }
+  sort_step(
+      mem, s.shift, s.bins, [&](int j) { return i0 + j < s.n ? (int64_t)key_of(s, i0 + j) : (int64_t)-1; },
+      [&](SortMemory& m) {
+        if (threadIdx.x >= kMostBins) {
+          half[0][threadIdx.x - kMostBins] = total;
+          half[1][threadIdx.x - kMostBins] = before;
+        }
+        __syncthreads();
+        if (threadIdx.x < kMostBins) {
+          total += half[0][threadIdx.x];
+          before += half[1][threadIdx.x];
+        }
+        scan_digits(m, threadIdx.x < kMostBins ? total : 0, before, s.bins);
+      },
+      [&](int j, uint32_t key, uint32_t place) {
+        s.keys_out[place] = key;
+        s.order_out[place] = s.order ? s.order[i0 + j] : (uint32_t)(i0 + j);
+      });
+}
+
+// All passes of up to 4096 positions.
+__global__ __launch_bounds__(1024) void sort_small_kernel(const SortArgs s) {
+  if (blockIdx.x >= 1) return clear_share(s, (int)blockIdx.x - 1, (int)gridDim.x - 1);
+  __shared__ SortMemory mem;
+  __shared__ uint32_t keys[kItems], order[kItems];
+  const int i0 = wave_id() * kOwn, n = (int)s.n;
+  for (int pass = 0; pass < s.passes; ++pass) {
+    const bool last = pass + 1 == s.passes;
+    uint32_t from[kOwn / 64];
+#pragma unroll
+    for (int q = 0; q < kOwn / 64; ++q) {
+      const int i = i0 + 64 * q + ((int)threadIdx.x & 63);
+      from[q] = pass > 0 && i < n ? order[i] : (uint32_t)i;
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    sort_step(
+        mem, pass * s.shift, s.bins,
+        [&](int j) {
+          if (i0 + j >= n) return (int64_t)-1;
+          return (int64_t)(pass > 0 ? keys[i0 + j] : key_of(s, i0 + j));
+        },
+        [&](SortMemory& m) {
+          uint32_t own = 0;
+          if ((int)threadIdx.x < s.bins)
+            for (int q = 0; q < kWaves; ++q) own += m.at[q][threadIdx.x];
+          scan_digits(m, own, 0, s.bins);
+        },
+        [&](int j, uint32_t key, uint32_t place) {
+          (last ? s.keys_out : keys)[place] = key;
+          (last ? s.order_out : order)[place] = from[j >> 6];
+        });
   }
 }
 
 // --- the sums ---------------------------------------------------------------------------
-// Rows of absent ids: zeros everywhere, before the sums.
-__global__ __launch_bounds__(256) void zero_rows_kernel(uint32_t* out, int64_t words, bool last_half) {
-  const int64_t stride = (int64_t)gridDim.x * 1024;
-  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < words; i += stride) {
-    if (i + 4 <= words) {
-      typedef unsigned int u32x4_w __attribute__((ext_vector_type(4), aligned(4)));
-      *(u32x4_w*)(out + i) = u32x4_w{0, 0, 0, 0};
-    } else {
-      for (int64_t j = i; j < words; ++j) out[j] = 0;
-    }
-  }
-  if (last_half && blockIdx.x == 0 && threadIdx.x == 0) ((uint16_t*)(out + words))[0] = 0;
-}
-
 // The sum of id's rows, scaled and through the norm, to its row of the gradient.
-template <typename T, int PER>
-__device__ __forceinline__ void write_row(const EmbedArgs& a, uint32_t id, floatx4 (&s)[PER], int lane) {
+template <typename T, int VEC, int PER>
+__device__ __forceinline__ void write_row(const EmbedArgs& a, uint32_t id, Row<T, VEC, PER>& s, int lane) {
   const int D = (int)a.embd;
-#pragma unroll
-  for (int k = 0; k < PER; ++k) s[k] *= a.scale;
+  s.each([&](float& x, int) { x *= a.scale; });
   if (a.norm) {
-    floatx4 x[PER];
+    Row<T, VEC, PER> x;
+    x.load((const T*)a.table + (int64_t)id * D, D, lane);
+    const float r = x.center(D, lane);
+    x.each([&](float& v, int) { v *= r; });
+    const float mean = s.sum() / (float)D, along = s.dot(x) / (float)D;
 #pragma unroll
-    for (int k = 0; k < PER; ++k) x[k] = load4((const T*)a.table + (int64_t)id * D, 256 * k + 4 * lane, D);
-    const float r = center(x, D, lane);
+    for (int k = 0; k < PER; ++k)
 #pragma unroll
-    for (int k = 0; k < PER; ++k) x[k] *= r;
-    const float mean = row_sum(s) / (float)D, along = row_dot(s, x) / (float)D;
-#pragma unroll
-    for (int k = 0; k < PER; ++k) s[k] = (s[k] - mean - x[k] * along) * r;
+      for (int j = 0; j < VEC; ++j) s.v[k][j] = (s.v[k][j] - mean - x.v[k][j] * along) * r;
   }
   T* out = (T*)a.out + (int64_t)id * D;
+  if (a.accumulate) {
+    Row<T, VEC, PER> old;
+    old.load(out, D, lane);
 #pragma unroll
-  for (int k = 0; k < PER; ++k) {
-    const int c = 256 * k + 4 * lane;
-    if (a.accumulate) s[k] += load4(out, c, D);
-    store4(out, c, D, s[k]);
+    for (int k = 0; k < PER; ++k)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) s.v[k][j] += old.v[k][j];
   }
+  s.store(out, D, lane);
 }
 
-// A wave sums the rows of positions [run * a.run, ..).  part [runs][2][D]: the sum of
-// the run's first id where that id began before it, of its last where it goes on
-// after it; an id that does both is in the first.
-template <typename T, int PER>
+template <typename T, int VEC, int PER>
+__device__ __forceinline__ void add(Row<T, VEC, PER>& s, const Row<T, VEC, PER>& g) {
+#pragma unroll
+  for (int k = 0; k < PER; ++k)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) s.v[k][j] += g.v[k][j];
+}
+
+// A wave sums the rows of positions [run * a.run, ..), whose ids and places one load each
+// takes.  part [runs][2][D]: the sum of the run's first id where that id began before it,
+// of its last where it goes on after it; an id that does both is in the first.
+template <typename T, int VEC, int PER>
 __global__ __launch_bounds__(256) void embed_sums_kernel(const EmbedArgs a) {
   const int run = (int)blockIdx.x * 4 + wave_id(), lane = threadIdx.x & 63, D = (int)a.embd;
-  const int64_t p0 = (int64_t)run * a.run, p1 = p0 + a.run < a.n ? p0 + a.run : a.n;
+  const int64_t p0 = (int64_t)run * a.run;
   if (p0 >= a.n) return;
-  uint32_t id = a.keys[p0];
+  const int n = (int)(a.n - p0 < a.run ? a.n - p0 : a.run);
+  // Lane l: position p0 + l - 1 (a.run + 2 <= 64 of them).
+  const int64_t at = p0 + lane - 1;
+  const bool in = at >= 0 && at < a.n && lane <= a.run + 1;
+  const uint32_t none = ~0u;
+  const uint32_t key = in ? a.keys[at] : none, place = in ? a.order[at] : 0;
+  const auto id_at = [&](int p) { return (uint32_t)__builtin_amdgcn_readlane((int)key, p + 1); };
+  uint32_t id = id_at(0);
   if (id >= (uint32_t)a.vocab) return;
-  bool begun = p0 > 0 && a.keys[p0 - 1] == id;  // before this run
-  floatx4 s[PER];
-#pragma unroll
-  for (int k = 0; k < PER; ++k) s[k] = zero4();
-  const auto to_part = [&](int which) {
-    float* part = a.part + ((int64_t)run * 2 + which) * D;
-#pragma unroll
-    for (int k = 0; k < PER; ++k) store4(part, 256 * k + 4 * lane, D, s[k]);
-  };
-  constexpr int AHEAD = PER <= 2 ? 8 : PER <= 4 ? 4 : 2;  // rows asked for together
-  for (int64_t p = p0; p < p1; p += AHEAD) {
-    floatx4 g[AHEAD][PER];
-    uint32_t ids[AHEAD];
+  bool begun = id_at(-1) == id;  // before this run
+  Row<T, VEC, PER> s;
+  s.clear();
+  const auto to_part = [&](int which) { s.store(a.part + ((int64_t)run * 2 + which) * D, D, lane); };
+  constexpr int AHEAD = 64 / (VEC * PER);  // rows asked for together
+  for (int p = 0; p < n; p += AHEAD) {
+    Row<T, VEC, PER> g[AHEAD];
 #pragma unroll
     for (int q = 0; q < AHEAD; ++q) {
-      const int64_t at = p + q < p1 ? p + q : p1 - 1;
-      ids[q] = __builtin_amdgcn_readfirstlane(a.keys[at]);
-      const T* row = (const T*)a.grad + (int64_t)__builtin_amdgcn_readfirstlane(a.order[at]) * D;
-#pragma unroll
-      for (int k = 0; k < PER; ++k) g[q][k] = load4(row, 256 * k + 4 * lane, D);
+      const uint32_t i = (uint32_t)__builtin_amdgcn_readlane((int)place, (p + q < n ? p + q : n - 1) + 1);
+      g[q].load((const T*)a.grad + (int64_t)i * D, D, lane);
     }
 #pragma unroll
     for (int q = 0; q < AHEAD; ++q) {
-      if (p + q >= p1) break;
-      if (ids[q] != id) {
+      if (p + q >= n) break;
+      if (id_at(p + q) != id) {
         if (begun) to_part(0);
-        else write_row<T, PER>(a, id, s, lane);
-        id = ids[q];
+        else write_row(a, id, s, lane);
+        id = id_at(p + q);
         begun = false;
         if (id >= (uint32_t)a.vocab) return;
-#pragma unroll
-        for (int k = 0; k < PER; ++k) s[k] = zero4();
+        s.clear();
       }
-#pragma unroll
-      for (int k = 0; k < PER; ++k) s[k] += g[q][k];
+      add(s, g[q]);
     }
   }
   if (begun) to_part(0);
-  else if (p1 < a.n && a.keys[p1] == id) to_part(1);
-  else write_row<T, PER>(a, id, s, lane);
+  else if (id_at(n) == id) to_part(1);
+  else write_row(a, id, s, lane);
 }
 
 // A workgroup for each run: joins the id that begins in it and goes on past it.
-template <typename T, int PER>
-__global__ __launch_bounds__(256) void embed_join_kernel(const EmbedArgs a) {
-  __shared__ float sums[3][PER * 256];
+constexpr int kJoinWaves = 8;
+template <typename T, int VEC, int PER>
+__global__ __launch_bounds__(64 * kJoinWaves) void embed_join_kernel(const EmbedArgs a) {
+  __shared__ float sums[kJoinWaves][VEC * PER * 64];
   const int run = (int)blockIdx.x, lane = threadIdx.x & 63, w = wave_id(), D = (int)a.embd;
-  const int64_t end = ((int64_t)run + 1) * a.run;
+  const int64_t p0 = (int64_t)run * a.run, end = p0 + a.run;
   if (end >= a.n) return;
-  const uint32_t id = a.keys[end];
-  if (id >= (uint32_t)a.vocab || a.keys[end - 1] != id) return;
-  const int64_t p0 = (int64_t)run * a.run;
-  if (a.keys[p0] == id && p0 > 0 && a.keys[p0 - 1] == id) return;  // began earlier
-  // The last run that begins with this id.
+  const uint32_t id = a.keys[end], before = a.keys[end - 1], first = a.keys[p0], last = p0 > 0 ? a.keys[p0 - 1] : ~0u;
+  if (id >= (uint32_t)a.vocab || before != id) return;
+  if (first == id && last == id) return;  // began earlier
+  // The runs from the next one on that begin with this id too, 64 at a time.
   const int runs = (int)((a.n + a.run - 1) / a.run);
-  int low = run + 1, high = runs - 1;
-  while (low < high) {
-    const int mid = (low + high + 1) / 2;
-    if (a.keys[(int64_t)mid * a.run] == id) low = mid;
-    else high = mid - 1;
+  int n = 1;
+  for (;; n += 64) {
+    const int r = run + n + lane;
+    const uint64_t is = __ballot(r < runs && a.keys[(int64_t)(r < runs ? r : run) * a.run] == id);
+    if (is != ~0ull) {
+      n += __builtin_ctzll(~is);
+      break;
+    }
   }
-  // This run's second sum, then the first of each run up to there, a quarter a wave.
-  const int n = low - run + 1, q0 = (int)((int64_t)n * w / 4), q1 = (int)((int64_t)n * (w + 1) / 4);
-  floatx4 s[PER];
+  // This run's second sum, then the first of each of those, a share a wave.
+  const int q0 = (int)((int64_t)n * w / kJoinWaves), q1 = (int)((int64_t)n * (w + 1) / kJoinWaves);
+  Row<T, VEC, PER> s;
+  s.clear();
+  constexpr int AHEAD = 64 / (VEC * PER);
+  for (int q = q0; q < q1; q += AHEAD) {
+    Row<T, VEC, PER> g[AHEAD];
 #pragma unroll
-  for (int k = 0; k < PER; ++k) s[k] = zero4();
-#pragma unroll 4
-  for (int q = q0; q < q1; ++q) {
-    const float* part = a.part + ((int64_t)(run + q) * 2 + (q == 0 ? 1 : 0)) * D;
+    for (int k = 0; k < AHEAD; ++k) {
+      const int r = q + k < q1 ? q + k : q1 - 1;
+      g[k].load(a.part + ((int64_t)(run + r) * 2 + (r == 0 ? 1 : 0)) * D, D, lane);
+    }
 #pragma unroll
-    for (int k = 0; k < PER; ++k) s[k] += load4(part, 256 * k + 4 * lane, D);
+    for (int k = 0; k < AHEAD; ++k)
+      if (q + k < q1) add(s, g[k]);
   }
-  if (w > 0) {
-#pragma unroll
-    for (int k = 0; k < PER; ++k) *(floatx4*)&sums[w - 1][256 * k + 4 * lane] = s[k];
-  }
+  s.store(sums[w], VEC * PER * 64, lane);
   __syncthreads();
   if (w > 0) return;
-#pragma unroll
-  for (int q = 0; q < 3; ++q)
-#pragma unroll
-    for (int k = 0; k < PER; ++k) s[k] += *(const floatx4*)&sums[q][256 * k + 4 * lane];
-  write_row<T, PER>(a, id, s, lane);
+  for (int q = 1; q < kJoinWaves; ++q) {
+    Row<T, VEC, PER> g;
+    g.load(sums[q], VEC * PER * 64, lane);
+    add(s, g);
+  }
+  write_row(a, id, s, lane);
 }
 
 unsigned cdiv(int64_t a, int64_t b) { return (unsigned)((a + b - 1) / b); }
 
-// f(std::integral_constant PER) for rows of D columns.
-template <typename F>
+// f(VEC, PER) for rows of D columns.
+template <typename T, typename F>
 void by_columns(int64_t D, F&& f) {
-  if (D <= 256) f(std::integral_constant<int, 1>{});
-  else if (D <= 512) f(std::integral_constant<int, 2>{});
-  else if (D <= 1024) f(std::integral_constant<int, 4>{});
-  else f(std::integral_constant<int, 8>{});
+  const auto call = [&](auto vec, auto per) { f(vec, per); };
+  typedef std::integral_constant<int, 1> one;
+  typedef std::integral_constant<int, 2> two;
+  typedef std::integral_constant<int, 4> four;
+  typedef std::integral_constant<int, 8> eight;
+  if (D <= 256) return call(four{}, one{});
+  if constexpr (sizeof(T) == 4) {
+    if (D <= 512) return call(four{}, two{});
+    if (D <= 1024) return call(four{}, four{});
+    return call(four{}, eight{});
+  } else {
+    if (D <= 512) return call(eight{}, one{});
+    if (D <= 1024) return call(eight{}, two{});
+    return call(eight{}, four{});
+  }
+}
+
+template <typename T>
+void launch_rows(const EmbedArgs& a, hipStream_t st) {
+  by_columns<T>(a.embd, [&](auto vec, auto per) {
+    constexpr int VEC = decltype(vec)::value, PER = decltype(per)::value, EACH = VEC * PER >= 16 ? 2 : 4;
+    // Several tokens a wave where there are enough for the chip.
+    if (a.n >= 16384) {
+      const dim3 grid(cdiv(a.n, 4 * EACH));
+      if (a.norm) hipLaunchKernelGGL((embed_kernel<T, VEC, PER, EACH, true>), grid, dim3(256), 0, st, a);
+      else hipLaunchKernelGGL((embed_kernel<T, VEC, PER, EACH, false>), grid, dim3(256), 0, st, a);
+    } else {
+      const dim3 grid(cdiv(a.n, 4));
+      if (a.norm) hipLaunchKernelGGL((embed_kernel<T, VEC, PER, 1, true>), grid, dim3(256), 0, st, a);
+      else hipLaunchKernelGGL((embed_kernel<T, VEC, PER, 1, false>), grid, dim3(256), 0, st, a);
+    }
+  });
+}
+
+template <typename T>
+void launch_sums(const EmbedArgs& a, int64_t runs, hipStream_t st) {
+  by_columns<T>(a.embd, [&](auto vec, auto per) {
+    constexpr int VEC = decltype(vec)::value, PER = decltype(per)::value;
+    hipLaunchKernelGGL((embed_sums_kernel<T, VEC, PER>), dim3(cdiv(runs, 4)), dim3(256), 0, st, a);
+    if (runs > 1)
+      hipLaunchKernelGGL((embed_join_kernel<T, VEC, PER>), dim3((unsigned)runs), dim3(64 * kJoinWaves), 0, st, a);
+  });
 }
 
 }  // namespace
 
 bdh_status embed_tokens(const EmbedArgs& a, hipStream_t st) {
-  by_columns(a.embd, [&](auto per) {
-    constexpr int PER = decltype(per)::value;
-    const dim3 grid(cdiv(a.n, 4)), block(256);
-    if (a.bf16 && a.norm) hipLaunchKernelGGL((embed_kernel<bf16_t, PER, true>), grid, block, 0, st, a);
-    else if (a.bf16) hipLaunchKernelGGL((embed_kernel<bf16_t, PER, false>), grid, block, 0, st, a);
-    else if (a.norm) hipLaunchKernelGGL((embed_kernel<float, PER, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((embed_kernel<float, PER, false>), grid, block, 0, st, a);
-  });
+  if (a.bf16) launch_rows<bf16_t>(a, st);
+  else launch_rows<float>(a, st);
   BDH_HIP_TRY(hipGetLastError());
   return BDH_OK;
 }
@@ -366,8 +520,7 @@ bdh_status embed_tokens_vjp(EmbedArgs a, hipStream_t st, uint64_t* launches) {
   while (a.vocab >> bits) ++bits;  // of the keys 0 .. vocab
   const int passes = (bits + 8) / 9, per_pass = (bits + passes - 1) / passes;
   const int64_t blocks = cdiv(a.n, kItems);
-  // Fewer, longer runs of more tokens: their partial sums are joined one after the other.
-  a.run = a.n <= 16384 ? 16 : a.n <= 65536 ? 32 : 64;
+  a.run = a.n <= 32768 ? 16 : 32;
   const int64_t runs = cdiv(a.n, a.run);
   const int64_t words = 4 * a.n + (blocks << per_pass);
   void* buf = nullptr;
@@ -375,44 +528,48 @@ bdh_status embed_tokens_vjp(EmbedArgs a, hipStream_t st, uint64_t* launches) {
   if (s != BDH_OK) return s;
   uint32_t* keys[2] = {(uint32_t*)buf, (uint32_t*)buf + a.n};
   uint32_t* order[2] = {keys[1] + a.n, keys[1] + 2 * a.n};
+  a.part = (float*)buf + words;
   SortArgs q{};
   q.tokens = a.tokens;
   q.n = a.n;
   q.vocab = a.vocab;
   q.bins = 1 << per_pass;
+  q.passes = passes;
+  q.blocks = (int)blocks;
   q.counts = order[1] + a.n;
-  a.part = (float*)buf + words;
-  if (!a.accumulate) {
-    const int64_t halves = a.vocab * a.embd * (a.bf16 ? 1 : 2);
-    const int64_t grid = cdiv(halves / 2 + 1, 1024);
-    hipLaunchKernelGGL(zero_rows_kernel, dim3((unsigned)(grid < 4096 ? grid : 4096)), dim3(256), 0, st,
-                       (uint32_t*)a.out, halves / 2, (halves & 1) != 0);
-    *launches += 1;
-  }
-  for (int p = 0; p < passes; ++p) {
-    q.shift = p * per_pass;
-    q.keys_out = keys[p & 1];
-    q.order_out = order[p & 1];
-    hipLaunchKernelGGL(digit_counts_kernel, dim3((unsigned)blocks), dim3(256), 0, st, q);
-    hipLaunchKernelGGL(digit_scatter_kernel, dim3((unsigned)blocks), dim3(256), 0, st, q);
-    q.keys = q.keys_out;
-    q.order = q.order_out;
-    *launches += 2;
-  }
-  a.keys = q.keys;
-  a.order = q.order;
-  by_columns(a.embd, [&](auto per) {
-    constexpr int PER = decltype(per)::value;
-    const dim3 grid(cdiv(runs, 4)), join((unsigned)runs), block(256);
-    if (a.bf16) {
-      hipLaunchKernelGGL((embed_sums_kernel<bf16_t, PER>), grid, block, 0, st, a);
-      if (runs > 1) hipLaunchKernelGGL((embed_join_kernel<bf16_t, PER>), join, block, 0, st, a);
-    } else {
-      hipLaunchKernelGGL((embed_sums_kernel<float, PER>), grid, block, 0, st, a);
-      if (runs > 1) hipLaunchKernelGGL((embed_join_kernel<float, PER>), join, block, 0, st, a);
+  q.clear = (char*)a.out;
+  // Bytes to clear, an equal share a launch, by up to 1024 workgroups of 1024 threads.
+  const int64_t bytes = a.accumulate ? 0 : a.vocab * a.embd * (a.bf16 ? 2 : 4);
+  const int sorts = blocks == 1 ? 1 : 2 * passes;
+  int launch = 0;
+  const auto grid = [&] {
+    q.clear_from = bytes * launch / sorts / 16 * 16;
+    q.clear_to = launch + 1 == sorts ? bytes : bytes * (launch + 1) / sorts / 16 * 16;
+    ++launch;
+    const int64_t more = cdiv(q.clear_to - q.clear_from, 16384);
+    return dim3((unsigned)(q.blocks + (more < 1024 ? more : 1024)));
+  };
+  if (blocks == 1) {
+    q.shift = per_pass;
+    q.keys_out = keys[0];
+    q.order_out = order[0];
+    hipLaunchKernelGGL(sort_small_kernel, grid(), dim3(1024), 0, st, q);
+  } else {
+    for (int p = 0; p < passes; ++p) {
+      q.shift = p * per_pass;
+      q.keys_out = keys[p & 1];
+      q.order_out = order[p & 1];
+      hipLaunchKernelGGL(digit_counts_kernel, grid(), dim3(1024), 0, st, q);
+      hipLaunchKernelGGL(digit_scatter_kernel, grid(), dim3(1024), 0, st, q);
+      q.keys = q.keys_out;
+      q.order = q.order_out;
     }
-  });
-  *launches += runs > 1 ? 2 : 1;
+  }
+  a.keys = q.keys_out;
+  a.order = q.order_out;
+  if (a.bf16) launch_sums<bf16_t>(a, runs, st);
+  else launch_sums<float>(a, runs, st);
+  *launches += (uint64_t)sorts + (runs > 1 ? 2 : 1);
   BDH_HIP_TRY(hipGetLastError());
   return BDH_OK;
 }
