@@ -43,8 +43,15 @@ struct Row {
   __device__ __forceinline__ void clear() {
     each([](float& x, int) { x = 0.0f; });
   }
+  // (The lane is opaque at each row: else the comparisons with the row's end, one a column,
+  // are kept for the whole kernel, in more scalar registers than there are.)
+  static __device__ __forceinline__ int anew(int lane) {
+    asm volatile("" : "+v"(lane));
+    return lane;
+  }
   template <typename S>  // of T, or partial sums of f32
-  __device__ __forceinline__ void load(const S* row, int n, int lane) {
+  __device__ __forceinline__ void load(const S* row, int n, int lane_) {
+    const int lane = anew(lane_);
     constexpr int W = sizeof(S) == 4 ? 4 : VEC;
     typedef typename Vec<S, W>::type V;
 #pragma unroll
@@ -63,7 +70,8 @@ struct Row {
       }
   }
   template <typename S>
-  __device__ __forceinline__ void store(S* row, int n, int lane) const {
+  __device__ __forceinline__ void store(S* row, int n, int lane_) const {
+    const int lane = anew(lane_);
     constexpr int W = sizeof(S) == 4 ? 4 : VEC;
     typedef typename Vec<S, W>::type V;
 #pragma unroll
@@ -104,7 +112,8 @@ struct Row {
   // Less its mean, zeros past column n; returns 1 / sqrt(var + eps).  The mean is taken
   // twice: the first one's rounding is large beside the values of a row that lies far
   // from zero.
-  __device__ __forceinline__ float center(int n, int lane) {
+  __device__ __forceinline__ float center(int n, int lane_) {
+    const int lane = anew(lane_);
 #pragma unroll
     for (int pass = 0; pass < 2; ++pass) {
       const float mean = sum() / (float)n;
@@ -324,14 +333,25 @@ __global__ __launch_bounds__(1024) void sort_small_kernel(const SortArgs s) {
 }
 
 // --- the sums ---------------------------------------------------------------------------
+// The columns of a workgroup: with the norm all of a row, else a slice of it (blockIdx.y),
+// so that a wave holds few of each row, and many rows.
+struct Columns {
+  int row, first, n;
+};
+__device__ __forceinline__ Columns columns_of(const EmbedArgs& a, int width) {
+  const int D = (int)a.embd, first = (int)blockIdx.y * width;
+  return Columns{D, first, D - first < width ? D - first : width};
+}
+
 // The sum of id's rows, scaled and through the norm, to its row of the gradient.
 template <typename T, int VEC, int PER>
-__device__ __forceinline__ void write_row(const EmbedArgs& a, uint32_t id, Row<T, VEC, PER>& s, int lane) {
-  const int D = (int)a.embd;
+__device__ __forceinline__ void write_row(const EmbedArgs& a, const Columns& c, uint32_t id, Row<T, VEC, PER>& s,
+                                          int lane) {
+  const int D = c.n;
   s.each([&](float& x, int) { x *= a.scale; });
   if (a.norm) {
     Row<T, VEC, PER> x;
-    x.load((const T*)a.table + (int64_t)id * D, D, lane);
+    x.load((const T*)a.table + (int64_t)id * c.row, D, lane);
     const float r = x.center(D, lane);
     x.each([&](float& v, int) { v *= r; });
     const float mean = s.sum() / (float)D, along = s.dot(x) / (float)D;
@@ -340,7 +360,7 @@ __device__ __forceinline__ void write_row(const EmbedArgs& a, uint32_t id, Row<T
 #pragma unroll
       for (int j = 0; j < VEC; ++j) s.v[k][j] = (s.v[k][j] - mean - x.v[k][j] * along) * r;
   }
-  T* out = (T*)a.out + (int64_t)id * D;
+  T* out = (T*)a.out + (int64_t)id * c.row + c.first;
   if (a.accumulate) {
     Row<T, VEC, PER> old;
     old.load(out, D, lane);
@@ -365,7 +385,8 @@ __device__ __forceinline__ void add(Row<T, VEC, PER>& s, const Row<T, VEC, PER>&
 // of its last where it goes on after it; an id that does both is in the first.
 template <typename T, int VEC, int PER>
 __global__ __launch_bounds__(256) void embed_sums_kernel(const EmbedArgs a) {
-  const int run = (int)blockIdx.x * 4 + wave_id(), lane = threadIdx.x & 63, D = (int)a.embd;
+  const int run = (int)blockIdx.x * 4 + wave_id(), lane = threadIdx.x & 63;
+  const Columns c = columns_of(a, VEC * PER * 64);
   const int64_t p0 = (int64_t)run * a.run;
   if (p0 >= a.n) return;
   const int n = (int)(a.n - p0 < a.run ? a.n - p0 : a.run);
@@ -380,21 +401,21 @@ __global__ __launch_bounds__(256) void embed_sums_kernel(const EmbedArgs a) {
   bool begun = id_at(-1) == id;  // before this run
   Row<T, VEC, PER> s;
   s.clear();
-  const auto to_part = [&](int which) { s.store(a.part + ((int64_t)run * 2 + which) * D, D, lane); };
+  const auto to_part = [&](int which) { s.store(a.part + ((int64_t)run * 2 + which) * c.row + c.first, c.n, lane); };
   constexpr int AHEAD = 64 / (VEC * PER);  // rows asked for together
   for (int p = 0; p < n; p += AHEAD) {
     Row<T, VEC, PER> g[AHEAD];
 #pragma unroll
     for (int q = 0; q < AHEAD; ++q) {
       const uint32_t i = (uint32_t)__builtin_amdgcn_readlane((int)place, (p + q < n ? p + q : n - 1) + 1);
-      g[q].load((const T*)a.grad + (int64_t)i * D, D, lane);
+      g[q].load((const T*)a.grad + (int64_t)i * c.row + c.first, c.n, lane);
     }
 #pragma unroll
     for (int q = 0; q < AHEAD; ++q) {
       if (p + q >= n) break;
       if (id_at(p + q) != id) {
         if (begun) to_part(0);
-        else write_row(a, id, s, lane);
+        else write_row(a, c, id, s, lane);
         id = id_at(p + q);
         begun = false;
         if (id >= (uint32_t)a.vocab) return;
@@ -405,7 +426,7 @@ __global__ __launch_bounds__(256) void embed_sums_kernel(const EmbedArgs a) {
   }
   if (begun) to_part(0);
   else if (id_at(n) == id) to_part(1);
-  else write_row(a, id, s, lane);
+  else write_row(a, c, id, s, lane);
 }
 
 // A workgroup for each run: joins the id that begins in it and goes on past it.
@@ -413,7 +434,8 @@ constexpr int kJoinWaves = 8;
 template <typename T, int VEC, int PER>
 __global__ __launch_bounds__(64 * kJoinWaves) void embed_join_kernel(const EmbedArgs a) {
   __shared__ float sums[kJoinWaves][VEC * PER * 64];
-  const int run = (int)blockIdx.x, lane = threadIdx.x & 63, w = wave_id(), D = (int)a.embd;
+  const int run = (int)blockIdx.x, lane = threadIdx.x & 63, w = wave_id();
+  const Columns c = columns_of(a, VEC * PER * 64);
   const int64_t p0 = (int64_t)run * a.run, end = p0 + a.run;
   if (end >= a.n) return;
   const uint32_t id = a.keys[end], before = a.keys[end - 1], first = a.keys[p0], last = p0 > 0 ? a.keys[p0 - 1] : ~0u;
@@ -440,7 +462,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embed_join_kernel(const Embed
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) {
       const int r = q + k < q1 ? q + k : q1 - 1;
-      g[k].load(a.part + ((int64_t)(run + r) * 2 + (r == 0 ? 1 : 0)) * D, D, lane);
+      g[k].load(a.part + ((int64_t)(run + r) * 2 + (r == 0 ? 1 : 0)) * c.row + c.first, c.n, lane);
     }
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k)
@@ -454,7 +476,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embed_join_kernel(const Embed
     g.load(sums[q], VEC * PER * 64, lane);
     add(s, g);
   }
-  write_row(a, id, s, lane);
+  write_row(a, c, id, s, lane);
 }
 
 unsigned cdiv(int64_t a, int64_t b) { return (unsigned)((a + b - 1) / b); }
@@ -498,11 +520,14 @@ void launch_rows(const EmbedArgs& a, hipStream_t st) {
 
 template <typename T>
 void launch_sums(const EmbedArgs& a, int64_t runs, hipStream_t st) {
-  by_columns<T>(a.embd, [&](auto vec, auto per) {
+  const int64_t slice = sizeof(T) == 4 ? 256 : 512;
+  by_columns<T>(a.norm || a.embd < slice ? a.embd : slice, [&](auto vec, auto per) {
     constexpr int VEC = decltype(vec)::value, PER = decltype(per)::value;
-    hipLaunchKernelGGL((embed_sums_kernel<T, VEC, PER>), dim3(cdiv(runs, 4)), dim3(256), 0, st, a);
+    const unsigned slices = cdiv(a.embd, VEC * PER * 64);
+    hipLaunchKernelGGL((embed_sums_kernel<T, VEC, PER>), dim3(cdiv(runs, 4), slices), dim3(256), 0, st, a);
     if (runs > 1)
-      hipLaunchKernelGGL((embed_join_kernel<T, VEC, PER>), dim3((unsigned)runs), dim3(64 * kJoinWaves), 0, st, a);
+      hipLaunchKernelGGL((embed_join_kernel<T, VEC, PER>), dim3((unsigned)runs, slices), dim3(64 * kJoinWaves), 0, st,
+                         a);
   });
 }
 

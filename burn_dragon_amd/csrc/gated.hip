@@ -37,6 +37,15 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) {
 __device__ __forceinline__ void load_lds16(const char* p, uint32_t m0) {
   asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "{m0}"(m0) : "memory");
 }
+// The same from base (of the wave) + at.  (A scalar register that a vector instruction
+// wrote needs 5 wait states before the load.)
+__device__ __forceinline__ void load_lds16(const char* base, uint32_t at, uint32_t m0) {
+  const uint64_t b = (uint64_t)base;
+  const uint32_t low = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)b);
+  const uint32_t high = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32));
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(at), "s"(((uint64_t)high << 32) | low), "{m0}"(m0)
+               : "memory");
+}
 // At most n of this wave's loads are in flight and all its LDS accesses are done, in every wave.
 template <int N>
 __device__ __forceinline__ void wait_barrier() {
@@ -86,6 +95,18 @@ __device__ __forceinline__ void fill(char* lds, uint32_t tile, int w, int lane, 
   for (int j = 0; j < Tl::LOADS; ++j) {
     const uint32_t to = tile + (uint32_t)((w + Tl::WAVE_STEP * j) * 1024);
     if (whole || in(j)) load_lds16(at(j), lds_addr(lds) + to);
+    else *(u32x4*)(lds + to + 16 * lane) = u32x4{0, 0, 0, 0};
+  }
+}
+
+// The same from a base and per-lane places, which move with the lanes' own rows alone.
+template <class Tl, class In>
+__device__ __forceinline__ void fill(char* lds, uint32_t tile, int w, int lane, bool whole, const char* base,
+                                     const uint32_t (&at)[Tl::LOADS], In&& in) {
+#pragma unroll
+  for (int j = 0; j < Tl::LOADS; ++j) {
+    const uint32_t to = tile + (uint32_t)((w + Tl::WAVE_STEP * j) * 1024);
+    if (whole || in(j)) load_lds16(base, at[j], lds_addr(lds) + to);
     else *(u32x4*)(lds + to + 16 * lane) = u32x4{0, 0, 0, 0};
   }
 }
@@ -466,6 +487,174 @@ __global__ __launch_bounds__(256) void gated_grads_kernel(const GatedArgs a) {
   }
 }
 
+// --- few tokens -------------------------------------------------------------------------
+// Up to 64 tokens are bound by the weights, 4 D bytes a latent, each read once: a workgroup
+// has 16 VEC latents of a head and all tokens, its eight waves share the k's, and the
+// weights go from memory to registers.  A lane reads VEC neighbours of eight rows of k and
+// pairs the rows (one v_perm for two values), which leaves it with a fragment for each of
+// its latents: 16 lanes hold every VEC-th latent of the tile.
+constexpr int kFewTokens = 64, kFewWaves = 8;
+template <int VEC> struct Words;
+template <> struct Words<2> { typedef uint32_t type; };
+template <> struct Words<8> { typedef u32x4 type; };
+__device__ __forceinline__ uint32_t word_of(uint32_t v, int) { return v; }
+__device__ __forceinline__ uint32_t word_of(const u32x4& v, int i) { return v[i]; }
+
+template <int ACT, bool SAVED, bool CTX, int VEC, int MT>
+__global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const GatedArgs a) {
+  typedef typename Words<VEC>::type V;
+  constexpr int NT = 16 * VEC, PITCH = NT + 1;
+  __shared__ float sums[kFewWaves][2][16 * MT * PITCH];
+  const int lane = threadIdx.x & 63, w = wave_id(), i = lane & 15, g = lane >> 4;
+  const int D = (int)a.D, N = (int)a.N, M = (int)a.M;
+  // Neighbouring tiles on one XCD (every eighth workgroup): they share lines.
+  const int tiles = (N + NT - 1) / NT, all = tiles * a.H, per_xcd = (all + 7) / 8;
+  const int id = ((int)blockIdx.x & 7) * per_xcd + ((int)blockIdx.x >> 3);
+  if ((int)blockIdx.x >> 3 >= per_xcd || id >= all) return;
+  const int h = id / tiles, n0 = id % tiles * NT;
+  const int n = n0 + VEC * i < N ? n0 + VEC * i : N - VEC;
+  const bf16_t* const wp[2] = {a.up + (int64_t)h * D * N + n, a.gate + (int64_t)h * D * N + n};
+  const bf16_t *xp[MT], *cp[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    const uint32_t m = (uint32_t)(16 * t + i < M ? 16 * t + i : M - 1);
+    xp[t] = a.x + (int64_t)m * D;
+    cp[t] = CTX ? a.c + (int64_t)h * a.c_head + a.c_rows.at(m) : xp[t];
+  }
+  floatx4 acc[2][MT][VEC];
+#pragma unroll
+  for (int q = 0; q < 2; ++q)
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) acc[q][t][j] = zero4();
+  struct Step {
+    V rows[2][8];
+    bf16x8 x[MT], c[MT];
+  };
+  const int steps = (D + 31) / 32;
+  const auto load = [&](int s, Step& f) {
+    // (Past D: any row, and zeros below.)
+    const int k = 32 * s + 8 * g < D ? 32 * s + 8 * g : 0;
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+      for (int r = 0; r < 8; ++r) f.rows[q][r] = *(const V*)(wp[q] + (int64_t)(k + r) * N);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      f.x[t] = *(const bf16x8*)(xp[t] + k);
+      if (CTX) f.c[t] = *(const bf16x8*)(cp[t] + k);
+    }
+  };
+  const auto multiply = [&](int s, const Step& f) {
+    const bool in = 32 * s + 8 * g < D;
+    const bf16x8 none = {};
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        u32x4 v;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          v[r] = __builtin_amdgcn_perm(word_of(f.rows[q][2 * r + 1], j >> 1), word_of(f.rows[q][2 * r], j >> 1),
+                                       j & 1 ? 0x07060302u : 0x05040100u);
+        const bf16x8 wf = in ? __builtin_bit_cast(bf16x8, v) : none;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          const bf16x8 xf = CTX && q ? f.c[t] : f.x[t];
+          acc[q][t][j] = mfma16(wf, in ? xf : none, acc[q][t][j]);
+        }
+      }
+  };
+  // Wave w has every eighth step; the next one is asked for before a step is multiplied.
+  Step f[2];
+  if (w < steps) load(w, f[0]);
+  for (int s = w; s < steps; s += 2 * kFewWaves) {
+    if (s + kFewWaves < steps) load(s + kFewWaves, f[1]);
+    multiply(s, f[0]);
+    if (s + kFewWaves < steps) {
+      if (s + 2 * kFewWaves < steps) load(s + 2 * kFewWaves, f[0]);
+      multiply(s + kFewWaves, f[1]);
+    }
+  }
+  // A lane has token i of each 16, and of the tile latents VEC (4 g + r) + j.
+#pragma unroll
+  for (int q = 0; q < 2; ++q)
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sums[w][q][(16 * t + i) * PITCH + VEC * (4 * g + r) + j] = acc[q][t][j][r];
+  __syncthreads();
+  // Four (two) neighbours a thread: 32 latents lie in eight (sixteen) lanes.
+  constexpr int EACH = VEC == 8 ? 4 : 2;
+  for (int at = (int)threadIdx.x * EACH; at < M * NT; at += 64 * kFewWaves * EACH) {
+    const int m = at / NT, nt = at % NT, nn = n0 + nt;
+    const bool in = nn < N;
+    float p[EACH], q[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      p[e] = q[e] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kFewWaves; ++k) {
+        p[e] += sums[k][0][m * PITCH + nt + e];
+        q[e] += sums[k][1][m * PITCH + nt + e];
+      }
+      if (ACT == RELU) {
+        p[e] = relu(p[e] - a.th);
+        q[e] = relu(q[e] - a.th);
+      }
+    }
+    const int64_t row = (int64_t)m * a.H + h;
+    if (SAVED) {
+      const int nb = (N + kFp8Block - 1) / kFp8Block;
+      const auto keep = [&](float (&v)[EACH], uint8_t* codes, uint8_t* scales) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) top = in ? max(top, finite_bits(v[e])) : 0;
+#pragma unroll
+        for (int o = 1; o < kFp8Block / EACH; o <<= 1)
+          top = max(top, (uint32_t)__shfl_xor((int)top, o, kFp8Block / EACH));
+        const int scale = fp8_scale(top);
+        float f4[4] = {v[0], v[1], EACH == 4 ? v[EACH - 2] : 0.0f, EACH == 4 ? v[EACH - 1] : 0.0f};
+        fp8_keep_finite(f4, scale);
+        const uint32_t c = fp8_pack4(f4[0], f4[1], f4[2], f4[3], fp8_inverse(scale));
+        if (!in) return;
+        if (EACH == 4) *(uint32_t*)(codes + row * N + nn) = c;
+        else *(uint16_t*)(codes + row * N + nn) = (uint16_t)c;
+        if (nt % kFp8Block == 0) scales[row * nb + nn / kFp8Block] = (uint8_t)scale;
+      };
+      keep(p, a.up_codes, a.up_scales);
+      keep(q, a.gate_codes, a.gate_scales);
+    }
+    if (!in) continue;
+    float o[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      o[e] = value_of<ACT>(p[e], q[e]);
+      if (ACT == RELU && a.mask) o[e] *= a.mask[nn + e] * a.mask[nn + e];
+    }
+#pragma unroll
+    for (int e = 0; e < EACH; e += 2) *(uint32_t*)(a.out + row * N + nn + e) = pack_bf16x2(o[e], o[e + 1]);
+  }
+}
+
+template <int ACT, bool SAVED, bool CTX, int VEC, int MT>
+void launch_few_as(const GatedArgs& a, hipStream_t st) {
+  const int64_t tiles = (a.N + 16 * VEC - 1) / (16 * VEC) * a.H;
+  hipLaunchKernelGGL((few_kernel<ACT, SAVED, CTX, VEC, MT>), dim3((unsigned)((tiles + 7) / 8 * 8)),
+                     dim3(64 * kFewWaves), 0, st, a);
+}
+template <int ACT, bool SAVED, bool CTX>
+void launch_few(const GatedArgs& a, hipStream_t st) {
+  // Tiles of 128 latents (whole lines a row) where they fill the chip.
+  if (a.M <= 16 && a.H * a.N >= 32768) launch_few_as<ACT, SAVED, CTX, 8, 1>(a, st);
+  else if (a.M <= 16) launch_few_as<ACT, SAVED, CTX, 2, 1>(a, st);
+  else if (a.M <= 32) launch_few_as<ACT, SAVED, CTX, 2, 2>(a, st);
+  else launch_few_as<ACT, SAVED, CTX, 2, 4>(a, st);
+}
+
 // --- the four products of the backward pass -----------------------------------------------
 // A workgroup: 256 of the result's columns (first factor) by 128 of its rows, a wave
 // 128 by 64.  blockIdx.z: job and part of k.
@@ -660,22 +849,17 @@ __global__ __launch_bounds__(512, 1) void fused_kernel(const ProductArgs a, cons
   const int at0 = id % tiles * 128, part = id / tiles % a.parts, h = id / tiles / a.parts;
   const int K = IN ? N : M;
   const int nb = (N + kFp8Block - 1) / kFp8Block;
-  // The tiles' sources.
-  const int fc = F::chunk(w, lane) * 8;
-  const char* fp[2][F::LOADS];
+  // The tiles' sources: places in U_h, G_h or x (below 2^32, D being 256 at most); c's
+  // rows go by their tokens.
+  const int fc = F::chunk(w, lane) * 8, fd = fc < D ? fc : 0;
+  uint32_t f_place[F::LOADS];
 #pragma unroll
   for (int j = 0; j < F::LOADS; ++j) {
     const int r = F::row(j, w, lane);
-    if (IN) {
-      const int64_t off = ((int64_t)h * D + (r < D ? r : D - 1)) * N + fc;
-      fp[0][j] = (const char*)(a.up + off);
-      fp[1][j] = (const char*)(a.gate + off);
-    } else {
-      const int d = fc < D ? fc : 0;
-      fp[0][j] = (const char*)(a.x + (int64_t)r * D + d);
-      fp[1][j] = (const char*)(a.c + (int64_t)h * a.c_head + d);
-    }
+    f_place[j] = IN ? 2u * ((uint32_t)(r < D ? r : D - 1) * (uint32_t)N + (uint32_t)fc) : 2u * (uint32_t)(r * D + fd);
   }
+  const char* const f_base[2] = {(const char*)(IN ? a.up + (int64_t)h * D * N : a.x),
+                                 (const char*)(IN ? a.gate + (int64_t)h * D * N : a.c + (int64_t)h * a.c_head)};
   const bool two = IN || a.c;  // WEIGHTS without a context: x for both
   // Steps of this part: an even number before it.
   const int steps = (K + BK - 1) / BK, pairs = (steps + 1) / 2;
@@ -686,11 +870,13 @@ __global__ __launch_bounds__(512, 1) void fused_kernel(const ProductArgs a, cons
     const bool whole = decltype(inside)::value || (s < s1 && k0 + BK <= K);
     const uint32_t base = (uint32_t)(stage * TILES);
     const auto in = [&](int j) { return s < s1 && k0 + (IN ? fc : F::row(j, w, lane)) < K; };
-    fill<F>(lds, base, w, lane, whole, [&](int j) { return fp[0][j] + 2 * (IN ? (int64_t)k0 : (int64_t)k0 * D); }, in);
-    if (two)
+    const int64_t move = 2 * (IN ? (int64_t)k0 : (int64_t)k0 * D);
+    fill<F>(lds, base, w, lane, whole, f_base[0] + move, f_place, in);
+    if (IN)
+      fill<F>(lds, base + F::BYTES, w, lane, whole, f_base[1] + move, f_place, in);
+    else if (two)
       fill<F>(lds, base + F::BYTES, w, lane, whole,
-              [&](int j) { return fp[1][j] + 2 * (IN ? (int64_t)k0 : a.c_rows.at((uint32_t)(k0 + F::row(j, w, lane)))); },
-              in);
+              [&](int j) { return f_base[1] + 2 * (a.c_rows.at((uint32_t)(k0 + F::row(j, w, lane))) + fd); }, in);
   };
   // A thread's eight neighbours of step s (their k: where the step's begin, and theirs
   // beyond that).  odd: s & 1.  Where they lie: a base that moves with the step, and the
@@ -893,6 +1079,13 @@ TokenRows token_rows(int64_t time, int64_t batch_stride, int64_t step) {
 
 template <int ACT, int EPI>
 void launch_projections(const GatedArgs& a, hipStream_t st) {
+  if constexpr (EPI != BACK) {
+    if (a.M <= kFewTokens) {
+      if (a.c) launch_few<ACT, EPI == SAVE, true>(a, st);
+      else launch_few<ACT, EPI == SAVE, false>(a, st);
+      return;
+    }
+  }
   const dim3 grid(grid_of(a.order));
   if (a.c) hipLaunchKernelGGL((gated_kernel<ACT, EPI, true>), grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL((gated_kernel<ACT, EPI, false>), grid, dim3(256), 0, st, a);
