@@ -23,20 +23,26 @@ class ActivationCheckpoint(NamedTuple):
     scales: torch.Tensor    # [..., ceil(C / 32)] uint8: the power's exponent plus 127
 
 
+def _scales_shape(shape) -> tuple:
+    return (*shape[:-1], (shape[-1] + BLOCK - 1) // BLOCK)
+
+
 def new_checkpoint(shape, device: torch.device) -> ActivationCheckpoint:
     """Room for values of ``shape``."""
-    codes = torch.empty(shape, device=device, dtype=torch.uint8)
-    return ActivationCheckpoint(codes, torch.empty((*shape[:-1], -(-shape[-1] // BLOCK)), device=device,
-                                                   dtype=torch.uint8))
+    u8 = torch.uint8
+    return ActivationCheckpoint(torch.empty(shape, device=device, dtype=u8),
+                                torch.empty(_scales_shape(shape), device=device, dtype=u8))
 
 
 def check_checkpoint(c: ActivationCheckpoint, shape, device: torch.device, name: str) -> None:
     """Raises ValueError where c does not hold values of ``shape``."""
-    want = (tuple(shape), (*shape[:-1], -(-shape[-1] // BLOCK)))
-    for t, s in zip(c, want):
-        if tuple(t.shape) != s or t.dtype != torch.uint8 or t.device != device or not t.is_contiguous():
-            raise ValueError(f"{name} must hold contiguous uint8 tensors of {list(want[0])} and {list(want[1])} "
-                             "on the other tensors' device")
+    codes, scales = c
+    u8 = torch.uint8
+    if (codes.shape != shape or scales.shape != _scales_shape(shape) or codes.dtype is not u8 or scales.dtype is not u8
+            or codes.device != device or scales.device != device or not codes.is_contiguous()
+            or not scales.is_contiguous()):
+        raise ValueError(f"{name} must hold contiguous uint8 tensors of {list(shape)} and "
+                         f"{list(_scales_shape(shape))} on the other tensors' device")
 
 
 def checkpoint_activations(x: torch.Tensor, *, out: Optional[ActivationCheckpoint] = None
@@ -47,19 +53,20 @@ def checkpoint_activations(x: torch.Tensor, *, out: Optional[ActivationCheckpoin
     infinities and NaN are kept as NaN.  ``out``: a checkpoint to write over.
     None where the library does not support the input (no supported device,
     another dtype, an empty dimension)."""
-    dev = x.device
-    if not _supported(dev) or x.dim() == 0 or x.numel() == 0:
+    dev, shape, n = x.device, x.shape, x.numel()
+    if not _supported(dev) or not shape or n == 0:
         return None
     code = _dtype_code(x)
     if code is None:
         return None
-    if out is None:
-        out = new_checkpoint(x.shape, dev)
-    else:
-        check_checkpoint(out, x.shape, dev, "out")
     x = x.contiguous()
-    C = x.shape[-1]
-    st = _call_on(dev, _lib.load().bdh_activations_save, _ptr(x), code, x.numel() // C, C, _ptr(out.codes),
+    C = shape[-1]
+    if out is None:
+        u8 = torch.uint8
+        out = ActivationCheckpoint(torch.empty_like(x, dtype=u8), torch.empty(_scales_shape(shape), device=dev, dtype=u8))
+    else:
+        check_checkpoint(out, shape, dev, "out")
+    st = _call_on(dev, _lib.load().bdh_activations_save, _ptr(x), code, n // C, C, _ptr(out.codes),
                   _ptr(out.scales), _stream_ptr(dev))
     return out if _lib.check(st) else None
 
@@ -70,17 +77,18 @@ def restore_activations(saved: ActivationCheckpoint, *, dtype: torch.dtype = tor
     them exactly) or in ``out``.  None where the library does not support the
     input."""
     codes = saved.codes
-    dev = codes.device
+    dev, shape, n = codes.device, codes.shape, codes.numel()
     if out is not None:
         dtype = out.dtype
-    if not _supported(dev) or codes.dim() == 0 or codes.numel() == 0 or dtype not in (torch.float32, torch.bfloat16):
+    code = _lib.BDH_BF16 if dtype is torch.bfloat16 else _lib.BDH_F32 if dtype is torch.float32 else None
+    if not _supported(dev) or not shape or n == 0 or code is None:
         return None
-    check_checkpoint(saved, codes.shape, dev, "saved")
+    check_checkpoint(saved, shape, dev, "saved")
     if out is None:
-        out = torch.empty(codes.shape, device=dev, dtype=dtype)
-    elif out.shape != codes.shape or out.device != dev or not out.is_contiguous():
+        out = torch.empty(shape, device=dev, dtype=dtype)
+    elif out.shape != shape or out.device != dev or not out.is_contiguous():
         raise ValueError("out must be a contiguous tensor like the saved values")
-    C = codes.shape[-1]
-    st = _call_on(dev, _lib.load().bdh_activations_restore, _ptr(codes), _ptr(saved.scales), codes.numel() // C, C,
-                  _dtype_code(out), _ptr(out), _stream_ptr(dev))
+    C = shape[-1]
+    st = _call_on(dev, _lib.load().bdh_activations_restore, _ptr(codes), _ptr(saved.scales), n // C, C, code,
+                  _ptr(out), _stream_ptr(dev))
     return out if _lib.check(st) else None

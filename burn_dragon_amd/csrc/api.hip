@@ -979,7 +979,7 @@ static bdh_status gated_checks(const bdh_layer_plan* plan, const void* current, 
   if (p.latent % 8 != 0 || p.embd % 8 != 0) return fail(BDH_UNSUPPORTED, "latent and embd must be multiples of 8");
   const int64_t most = (int64_t)1 << 22;
   if (p.batch > most || p.time > most || p.batch * p.time > most || p.heads > 512 || p.latent > (int64_t)1 << 20 ||
-      p.embd > (int64_t)1 << 16 || p.batch * p.time > (((int64_t)1 << 35) - 1) / (p.heads * p.latent))
+      p.embd > (int64_t)1 << 16 || p.heads * p.latent > (int64_t)1 << 24 || p.batch * p.time > (((int64_t)1 << 35) - 1) / (p.heads * p.latent))
     return fail(BDH_UNSUPPORTED, "too large for one launch");
   bdh_gated_options o{BDH_RELU, 0.0f, nullptr};
   if (options) o = *options;

@@ -665,8 +665,8 @@ struct ProductArgs {
   int H;
   int64_t c_head;
   TokenRows c_rows;
-  int parts;                // of this launch's k
-  int fused_tiles;          // fused_kernel: tiles of 128 tokens or latents
+  int in_parts, w_parts;    // of k
+  int in_tiles, w_tiles;    // in all, parts counted
   int x_parts;              // sums that make up d_x
   int64_t x_size, c_size;   // elements of d_x, d_c
   bf16_t *d_x, *d_c, *d_up, *d_gate;
@@ -689,16 +689,16 @@ __device__ __forceinline__ void store_product(const ProductArgs& a, const floatx
     out_at = (int64_t)h * a.c_head;
     out = a.d_c;
     sums = a.c_sums + part * a.c_size;
-    direct = a.parts == 1;
+    direct = a.in_parts == 1;
   } else if (WHAT == INPUTS) {
     out = a.d_x;
-    sums = a.x_sums + ((int64_t)(which * a.H + h) * a.parts + part) * a.x_size;
+    sums = a.x_sums + ((int64_t)(which * a.H + h) * a.in_parts + part) * a.x_size;
     direct = a.x_parts == 1;
   } else {
     out_at = (int64_t)h * a.D * a.N;
     out = which ? a.d_gate : a.d_up;
     sums = a.w_sums + ((int64_t)part * 2 + which) * a.H * a.D * a.N;
-    direct = a.parts == 1;
+    direct = a.w_parts == 1;
   }
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
@@ -731,17 +731,29 @@ __device__ __forceinline__ void store_product(const ProductArgs& a, const floatx
   }
 }
 
+// Neighbouring ids on one XCD (every eighth workgroup): the id of workgroup b of n, -1: none.
+__device__ __forceinline__ int id_of(int b, int n) {
+  const int per_xcd = (n + 7) / 8, id = (b & 7) * per_xcd + (b >> 3);
+  return b >> 3 < per_xcd && id < n ? id : -1;
+}
+
+constexpr int PRODUCT_LDS = 3 * 64 * (256 + 128);
 template <int WHAT>
-__global__ __launch_bounds__(256, 2) void product_kernel(const ProductArgs a) {
+__device__ __forceinline__ void product_tile(const ProductArgs& a, char* lds, int id) {
   typedef Tile<WHAT == INPUTS ? KC : MC, 256> A;  // U, G rows d / dp, dq columns n
   typedef Tile<WHAT == INPUTS ? KC : MC, 128> B;  // dp, dq rows m / x, c columns d
   constexpr int STAGE = A::BYTES + B::BYTES, LOADS = A::LOADS + B::LOADS;
-  __shared__ __attribute__((aligned(16))) char lds[3 * STAGE];
+  static_assert(3 * STAGE == PRODUCT_LDS, "the ring");
   const int lane = threadIdx.x & 63, w = wave_id();
   const int D = (int)a.D, N = (int)a.N, M = (int)a.M;
-  const int part = (int)blockIdx.z % a.parts, job = (int)blockIdx.z / a.parts;
+  // The tiles along D, which share the larger operand, are neighbours.
+  const int d_tiles = (D + (WHAT == INPUTS ? 255 : 127)) / (WHAT == INPUTS ? 256 : 128);
+  const int other = WHAT == INPUTS ? (M + 127) / 128 : (N + 255) / 256;
+  const int parts = WHAT == INPUTS ? a.in_parts : a.w_parts;
+  const int di = id % d_tiles, oi = id / d_tiles % other, rest = id / d_tiles / other;
+  const int part = rest % parts, job = rest / parts;
   const int h = job % a.H, which = job / a.H;  // which: 0 up, 1 gate
-  const int a0 = (int)blockIdx.x * 256, b0 = (int)blockIdx.y * 128;
+  const int a0 = (WHAT == INPUTS ? di : oi) * 256, b0 = (WHAT == INPUTS ? oi : di) * 128;
   const int K = WHAT == INPUTS ? N : M;
   const bf16_t* dv = which ? a.dq : a.dp;        // [M, H, N]
   const int64_t d_row = (int64_t)a.H * N;
@@ -772,7 +784,7 @@ __global__ __launch_bounds__(256, 2) void product_kernel(const ProductArgs a) {
     }
   }
   const int steps = (K + BK - 1) / BK;
-  const int s0 = (int)((int64_t)steps * part / a.parts), s1 = (int)((int64_t)steps * (part + 1) / a.parts);
+  const int s0 = (int)((int64_t)steps * part / parts), s1 = (int)((int64_t)steps * (part + 1) / parts);
   const auto issue = [&](int s, int stage) {
     const int k0 = s * BK;
     const bool whole = k0 + BK <= K;
@@ -821,6 +833,16 @@ __global__ __launch_bounds__(256, 2) void product_kernel(const ProductArgs a) {
   store_product<WHAT>(a, acc, h, which, part, a0 + aw, b0 + bw, lane);
 }
 
+// The products of the inputs, then those of the weights.
+__global__ __launch_bounds__(256, 2) void product_kernel(const ProductArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[PRODUCT_LDS];
+  const int inputs = (a.in_tiles + 7) / 8 * 8, b = (int)blockIdx.x;
+  const int id = b < inputs ? id_of(b, a.in_tiles) : id_of(b - inputs, a.w_tiles);
+  if (id < 0) return;
+  if (b < inputs) product_tile<INPUTS>(a, lds, id);
+  else product_tile<WEIGHTS>(a, lds, id);
+}
+
 // Both products of a kind straight from what the forward saved, D up to 256: dp and dq are
 // made a step or two ahead, between memory and LDS, and never written.  A workgroup has
 // eight waves, four for each product: INPUTS  128 tokens of a head by all columns, dx by
@@ -842,11 +864,10 @@ __global__ __launch_bounds__(512, 1) void fused_kernel(const ProductArgs a, cons
   char* const grads = lds + 3 * TILES;
   const int lane = threadIdx.x & 63, w = wave_id(), which = w >> 2;
   const int D = (int)a.D, N = (int)a.N, M = (int)a.M;
-  // An XCD (every eighth workgroup) takes neighbours of a head, which share its tiles.
-  const int tiles = a.fused_tiles, per_xcd = (tiles * a.H * a.parts + 7) / 8;
-  const int id = ((int)blockIdx.x & 7) * per_xcd + ((int)blockIdx.x >> 3);
-  if ((int)blockIdx.x >> 3 >= per_xcd || id >= tiles * a.H * a.parts) return;
-  const int at0 = id % tiles * 128, part = id / tiles % a.parts, h = id / tiles / a.parts;
+  const int id = id_of((int)blockIdx.x, IN ? a.in_tiles : a.w_tiles);
+  if (id < 0) return;
+  const int tiles = ((IN ? M : N) + 127) / 128, parts = IN ? a.in_parts : a.w_parts;
+  const int at0 = id % tiles * 128, part = id / tiles % parts, h = id / tiles / parts;
   const int K = IN ? N : M;
   const int nb = (N + kFp8Block - 1) / kFp8Block;
   // The tiles' sources: places in U_h, G_h or x (below 2^32, D being 256 at most); c's
@@ -863,8 +884,8 @@ __global__ __launch_bounds__(512, 1) void fused_kernel(const ProductArgs a, cons
   const bool two = IN || a.c;  // WEIGHTS without a context: x for both
   // Steps of this part: an even number before it.
   const int steps = (K + BK - 1) / BK, pairs = (steps + 1) / 2;
-  const int s0 = 2 * (int)((int64_t)pairs * part / a.parts);
-  const int s1 = min(steps, 2 * (int)((int64_t)pairs * (part + 1) / a.parts));
+  const int s0 = 2 * (int)((int64_t)pairs * part / parts);
+  const int s1 = min(steps, 2 * (int)((int64_t)pairs * (part + 1) / parts));
   const auto issue = [&](auto inside, int s, int stage) {
     const int k0 = s * BK;
     const bool whole = decltype(inside)::value || (s < s1 && k0 + BK <= K);
@@ -1056,17 +1077,27 @@ __global__ __launch_bounds__(512, 1) void fused_kernel(const ProductArgs a, cons
   store_product<WHAT>(a, acc, h, which, part, (IN ? 0 : at0) + aw, (IN ? at0 : 0) + bw, lane);
 }
 
-// out[i] = the sum of n parts, in their order; eight neighbours a thread.
-__global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ sums, int n, int64_t stride,
-                                                   bf16_t* __restrict__ out, int64_t size) {
-  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; i < size; i += (int64_t)gridDim.x * 2048) {
-    floatx4 a = *(const floatx4*)(sums + i), b = *(const floatx4*)(sums + i + 4);
-    for (int k = 1; k < n; ++k) {
-      a += *(const floatx4*)(sums + k * stride + i);
-      b += *(const floatx4*)(sums + k * stride + i + 4);
+// out[i] = the sum of n parts, in their order; eight neighbours a thread.  Up to four
+// tensors (blockIdx.y).
+struct JoinArgs {
+  struct {
+    const float* sums;
+    int n;
+    int64_t stride, size;
+    bf16_t* out;
+  } of[4];
+};
+__global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
+  const auto& j = a.of[blockIdx.y];
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; i < j.size; i += (int64_t)gridDim.x * 2048) {
+    floatx4 x = *(const floatx4*)(j.sums + i), y = *(const floatx4*)(j.sums + i + 4);
+#pragma unroll 4
+    for (int k = 1; k < j.n; ++k) {
+      x += *(const floatx4*)(j.sums + k * j.stride + i);
+      y += *(const floatx4*)(j.sums + k * j.stride + i + 4);
     }
-    *(u32x4*)(out + i) = u32x4{pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(b[0], b[1]),
-                               pack_bf16x2(b[2], b[3])};
+    *(u32x4*)(j.out + i) =
+        u32x4{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
   }
 }
 
@@ -1098,9 +1129,8 @@ void launch_projections(const GatedArgs& a, int act, hipStream_t st) {
 }
 
 template <int WHAT>
-void launch_fused(ProductArgs p, const GatedArgs& a, int act, hipStream_t st) {
-  p.fused_tiles = (int)cdiv(WHAT == INPUTS ? p.M : p.N, 128);
-  const dim3 grid(cdiv((int64_t)p.fused_tiles * p.H * p.parts, 8) * 8);
+void launch_fused(const ProductArgs& p, const GatedArgs& a, int act, hipStream_t st) {
+  const dim3 grid(cdiv(WHAT == INPUTS ? p.in_tiles : p.w_tiles, 8) * 8);
   if (act == RELU && a.mask) hipLaunchKernelGGL((fused_kernel<WHAT, RELU, true>), grid, dim3(512), 0, st, p, a);
   else if (act == RELU) hipLaunchKernelGGL((fused_kernel<WHAT, RELU, false>), grid, dim3(512), 0, st, p, a);
   else if (act == SILU) hipLaunchKernelGGL((fused_kernel<WHAT, SILU, false>), grid, dim3(512), 0, st, p, a);
@@ -1145,8 +1175,11 @@ bdh_status gated_block(const GatedCall& g, hipStream_t st, uint64_t* launches) {
 bdh_status gated_block_vjp(const GatedCall& g, hipStream_t st, uint64_t* launches) {
   GatedArgs a = args_of(g);
   const int64_t M = a.M, H = g.H, N = g.N, D = g.D;
-  // (The fused kernels hold a step of 128 tokens' places in 32 bits.)
-  const bool fused = g.up_codes && D <= 256 && H * N <= (int64_t)1 << 23;
+  // From saved values without dp and dq in memory, where there are latents enough (us, fused /
+  // not, 4 heads, D 256: 385 tokens of 1000 latents 64 / 50, of 8192 101 / 116; 4096 of 1000
+  // 119 / 136, of 8192 475 / 606; 1 head of 8192: 1024 tokens 94 / 101; D 64: 70 / 70).  (A
+  // fused step of 128 tokens' places is held in 32 bits.)
+  const bool fused = g.up_codes && D <= 256 && M * H * N >= (int64_t)1 << 23 && H * N <= (int64_t)1 << 23;
   // Parts of k: enough workgroups to fill the chip.
   const int64_t cus = device_cus();
   const auto parts_of = [&](int64_t tiles, int64_t want, int64_t K) {
@@ -1155,18 +1188,24 @@ bdh_status gated_block_vjp(const GatedCall& g, hipStream_t st, uint64_t* launche
     p = p < most ? p : most;
     return (int)(p < 32 ? p : 32);
   };
-  const int in_parts = fused ? parts_of(cdiv(M, 128) * H, cus, N)
-                             : parts_of((int64_t)cdiv(D, 256) * cdiv(M, 128) * 2 * H, 2 * cus, N);
-  const int w_parts = fused ? parts_of(cdiv(N, 128) * H, cus, M)
-                            : parts_of((int64_t)cdiv(N, 256) * cdiv(D, 128) * 2 * H, 2 * cus, M);
+  const int64_t in_tiles = fused ? cdiv(M, 128) * H : (int64_t)cdiv(D, 256) * cdiv(M, 128) * 2 * H;
+  const int64_t w_tiles = fused ? cdiv(N, 128) * H : (int64_t)cdiv(N, 256) * cdiv(D, 128) * 2 * H;
   ProductArgs p{};
-  p.x_parts = (int)((g.c ? 1 : 2) * H * in_parts);
+  // (Both kinds run together where they are not fused.)
+  p.in_parts = parts_of(in_tiles, cus, N);
+  p.w_parts = parts_of(w_tiles, cus, M);
+  // (A launch has fewer than 2^32 threads.)
+  if (in_tiles * p.in_parts > (int64_t)1 << 22 || w_tiles * p.w_parts > (int64_t)1 << 22)
+    return fail(BDH_UNSUPPORTED, "too large for one launch");
+  p.in_tiles = (int)(in_tiles * p.in_parts);
+  p.w_tiles = (int)(w_tiles * p.w_parts);
+  p.x_parts = (int)((g.c ? 1 : 2) * H * p.in_parts);
   p.x_size = M * D;
   p.c_size = M * H * D;
   const int64_t w_size = H * D * N;
   const size_t x_bytes = p.x_parts > 1 ? (size_t)p.x_parts * p.x_size * 4 : 0;
-  const size_t c_bytes = g.c && in_parts > 1 ? (size_t)in_parts * p.c_size * 4 : 0;
-  const size_t w_bytes = w_parts > 1 ? (size_t)w_parts * 2 * w_size * 4 : 0;
+  const size_t c_bytes = g.c && p.in_parts > 1 ? (size_t)p.in_parts * p.c_size * 4 : 0;
+  const size_t w_bytes = p.w_parts > 1 ? (size_t)p.w_parts * 2 * w_size * 4 : 0;
   bdh_status s;
   if (!fused) {
     void* buf = nullptr;
@@ -1175,23 +1214,10 @@ bdh_status gated_block_vjp(const GatedCall& g, hipStream_t st, uint64_t* launche
     a.dp = (bf16_t*)buf;
     a.dq = a.dp + M * H * N;
   }
-  // (The inputs' sums are joined before the weights' are made.)
-  const size_t sums = x_bytes + c_bytes > w_bytes ? x_bytes + c_bytes : w_bytes;
-  void* part = nullptr;
-  if (sums > 0) {
-    s = scratch(st, SLOT_GATED_SUMS, sums, &part);
+  void* sums = nullptr;
+  if (x_bytes + c_bytes + w_bytes > 0) {
+    s = scratch(st, SLOT_GATED_SUMS, x_bytes + c_bytes + w_bytes, &sums);
     if (s != BDH_OK) return s;
-  }
-  if (!fused) {
-    if (g.up_codes) {
-      const dim3 grid((unsigned)capped(cdiv(M * H * (N / 8), 256)));
-      if (g.act == RELU) hipLaunchKernelGGL((gated_grads_kernel<RELU>), grid, dim3(256), 0, st, a);
-      else if (g.act == SILU) hipLaunchKernelGGL((gated_grads_kernel<SILU>), grid, dim3(256), 0, st, a);
-      else hipLaunchKernelGGL((gated_grads_kernel<GELU>), grid, dim3(256), 0, st, a);
-    } else {
-      launch_projections<BACK>(a, g.act, st);
-    }
-    *launches += 1;
   }
   p.dp = a.dp;
   p.dq = a.dq;
@@ -1209,30 +1235,40 @@ bdh_status gated_block_vjp(const GatedCall& g, hipStream_t st, uint64_t* launche
   p.d_c = g.d_c;
   p.d_up = g.d_up;
   p.d_gate = g.d_gate;
-  p.x_sums = (float*)part;
-  p.c_sums = (float*)((char*)part + x_bytes);
-  p.w_sums = (float*)part;
-  p.parts = in_parts;
-  if (fused) launch_fused<INPUTS>(p, a, g.act, st);
-  else
-    hipLaunchKernelGGL((product_kernel<INPUTS>), dim3(cdiv(D, 256), cdiv(M, 128), (unsigned)(2 * H * in_parts)),
-                       dim3(256), 0, st, p);
+  p.x_sums = (float*)sums;
+  p.c_sums = (float*)((char*)sums + x_bytes);
+  p.w_sums = (float*)((char*)sums + x_bytes + c_bytes);
+  if (fused) {
+    launch_fused<INPUTS>(p, a, g.act, st);
+    launch_fused<WEIGHTS>(p, a, g.act, st);
+  } else {
+    if (g.up_codes) {
+      const dim3 grid((unsigned)capped(cdiv(M * H * (N / 8), 256)));
+      if (g.act == RELU) hipLaunchKernelGGL((gated_grads_kernel<RELU>), grid, dim3(256), 0, st, a);
+      else if (g.act == SILU) hipLaunchKernelGGL((gated_grads_kernel<SILU>), grid, dim3(256), 0, st, a);
+      else hipLaunchKernelGGL((gated_grads_kernel<GELU>), grid, dim3(256), 0, st, a);
+    } else {
+      launch_projections<BACK>(a, g.act, st);
+    }
+    hipLaunchKernelGGL(product_kernel, dim3((cdiv(p.in_tiles, 8) + cdiv(p.w_tiles, 8)) * 8), dim3(256), 0, st, p);
+  }
+  *launches += 2;
+  JoinArgs j{};
+  int joins = 0;
+  int64_t most = 0;
   const auto join = [&](const float* from, int n, int64_t stride, bf16_t* out, int64_t size) {
-    hipLaunchKernelGGL(join_kernel, dim3((unsigned)capped(cdiv(size, 2048))), dim3(256), 0, st, from, n, stride, out,
-                       size);
-    *launches += 1;
+    j.of[joins++] = {from, n, stride, size, out};
+    most = size > most ? size : most;
   };
   if (x_bytes) join(p.x_sums, p.x_parts, p.x_size, g.d_x, p.x_size);
-  if (c_bytes) join(p.c_sums, in_parts, p.c_size, g.d_c, p.c_size);
-  p.parts = w_parts;
-  if (fused) launch_fused<WEIGHTS>(p, a, g.act, st);
-  else
-    hipLaunchKernelGGL((product_kernel<WEIGHTS>), dim3(cdiv(N, 256), cdiv(D, 128), (unsigned)(2 * H * w_parts)),
-                       dim3(256), 0, st, p);
-  *launches += 2;
+  if (c_bytes) join(p.c_sums, p.in_parts, p.c_size, g.d_c, p.c_size);
   if (w_bytes) {
-    join(p.w_sums, w_parts, 2 * w_size, g.d_up, w_size);
-    join(p.w_sums + w_size, w_parts, 2 * w_size, g.d_gate, w_size);
+    join(p.w_sums, p.w_parts, 2 * w_size, g.d_up, w_size);
+    join(p.w_sums + w_size, p.w_parts, 2 * w_size, g.d_gate, w_size);
+  }
+  if (joins) {
+    hipLaunchKernelGGL(join_kernel, dim3((unsigned)capped(cdiv(most, 2048)), (unsigned)joins), dim3(256), 0, st, j);
+    *launches += 1;
   }
   BDH_HIP_TRY(hipGetLastError());
   return BDH_OK;

@@ -14,16 +14,16 @@ from . import _lib
 from .recurrent import _call_on, _dtype_code, _ptr, _stream_ptr, _supported
 
 
-def _table(tokens: torch.Tensor, table: torch.Tensor) -> Optional[int]:
+def _table(tokens: torch.Tensor, table: torch.Tensor, device: torch.device) -> Optional[int]:
     """The table's dtype code; None where the library does not take it."""
-    if table.dim() != 2 or not _supported(table.device):
+    if len(table.shape) != 2 or not _supported(device):
         return None
     code = _dtype_code(table)
     if code is None or tokens.numel() == 0 or table.numel() == 0:
         return None
-    if tokens.dtype != torch.int32:
+    if tokens.dtype is not torch.int32:
         raise ValueError("tokens must be int32")
-    if tokens.device != table.device:
+    if tokens.device != device:
         raise ValueError("tokens and table must be on one device")
     return code
 
@@ -37,11 +37,12 @@ def embed_tokens(tokens: torch.Tensor, table: torch.Tensor, *, scale: float = 1.
     result.  None where the library does not support the input (no supported
     device, another dtype, an empty dimension, D above 2048, V or tokens
     above 2^24)."""
-    code = _table(tokens, table)
+    dev = table.device
+    code = _table(tokens, table, dev)
     if code is None:
         return None
     V, D = table.shape
-    shape, dev = (*tokens.shape, D), table.device
+    shape = (*tokens.shape, D)
     if out is None:
         out = torch.empty(shape, device=dev, dtype=table.dtype)
     elif tuple(out.shape) != shape or out.dtype != table.dtype or out.device != dev or not out.is_contiguous():
@@ -63,11 +64,11 @@ def embed_tokens_vjp(grad: torch.Tensor, tokens: torch.Tensor, table: torch.Tens
     the tokens sorted by id; rounded once.  None where the library does not
     support the input (as embed_tokens; a scratch that would have to grow
     under capture)."""
-    code = _table(tokens, table)
+    dev = table.device
+    code = _table(tokens, table, dev)
     if code is None:
         return None
     V, D = table.shape
-    dev = table.device
     if tuple(grad.shape) != (*tokens.shape, D) or grad.dtype != table.dtype or grad.device != dev:
         raise ValueError(f"grad must be {table.dtype} of {[*tokens.shape, D]} on the table's device")
     if accumulate and out is None:

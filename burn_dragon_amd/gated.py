@@ -15,6 +15,7 @@ forward kept of them in 8 bits.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import NamedTuple, Optional
 
 import torch
@@ -50,47 +51,68 @@ class GatedGrads(NamedTuple):
     gate: torch.Tensor                 # [H, D, N] bf16
 
 
-def _plan(current, weights, context, activation, relu_threshold, latent_mask):
-    """(plan, options, tensors) of a call; None where the library does not
-    support it, ValueError where the arguments do not fit together."""
-    if activation not in ACTIVATIONS:
+@functools.lru_cache(maxsize=1024)
+def _plan_of(B: int, H: int, T: int, N: int, D: int):
+    """The library's plan of a shape, by reference (it reads it only)."""
+    return ctypes.byref(_lib.BdhLayerPlan(B, H, T, N, D))
+
+
+@functools.lru_cache(maxsize=1024)
+def _options_of(activation: int, threshold: float):
+    return ctypes.byref(_lib.BdhGatedOptions(activation, threshold, None))
+
+
+def _call(current, weights, context, activation, relu_threshold, latent_mask):
+    """(device, (B, H, T, N, D), plan, options, tensors) of a call; None where
+    the library does not support it, ValueError where the arguments do not
+    fit together."""
+    kind = ACTIVATIONS.get(activation)
+    if kind is None:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}")
     up, gate = weights
-    dev = current.device
-    if not _supported(dev) or current.dim() != 3 or up.dim() != 3 or gate.dim() != 3:
+    dev, bf16 = current.device, torch.bfloat16
+    x_shape, w_shape = current.shape, up.shape
+    if not _supported(dev) or len(x_shape) != 3 or len(w_shape) != 3 or len(gate.shape) != 3:
         return None
-    tensors = [t for t in (current, up, gate, context) if t is not None]
-    if any(t.dtype != torch.bfloat16 for t in tensors):
+    if (current.dtype is not bf16 or up.dtype is not bf16 or gate.dtype is not bf16
+            or (context is not None and context.dtype is not bf16)):
         return None
-    B, T, D = current.shape
-    H, _, N = up.shape
-    if min(B, T, D, H, N) == 0:
+    B, T, D = x_shape
+    H, _, N = w_shape
+    if 0 in (B, T, D, H, N):
         return None
-    if tuple(up.shape) != (H, D, N) or tuple(gate.shape) != (H, D, N):
+    if w_shape[1] != D or gate.shape != w_shape:
         raise ValueError("up and gate must be [H, D, N] with current's D")
-    if context is not None and tuple(context.shape) != (B, H, T, D):
+    if context is not None and context.shape != (B, H, T, D):
         raise ValueError(f"context must be {[B, H, T, D]}")
     mask = None
     if latent_mask is not None:
         mask = latent_mask.reshape(-1)
-        if mask.numel() != N or mask.dtype != torch.float32:
+        if mask.numel() != N or mask.dtype is not torch.float32:
             raise ValueError(f"latent_mask must hold {N} f32 values")
-        tensors.append(mask)
-    if any(t.device != dev for t in tensors):
+    if (up.device != dev or gate.device != dev or (context is not None and context.device != dev)
+            or (mask is not None and mask.device != dev)):
         raise ValueError("the tensors must be on one device")
-    if activation != "relu" and (relu_threshold != 0.0 or mask is not None):
+    if kind != _lib.BDH_RELU and (relu_threshold != 0.0 or mask is not None):
         raise ValueError('relu_threshold and latent_mask go with activation="relu"')
-    current, up, gate, context, mask = (_aligned(t) for t in (current, up, gate, context, mask))
-    plan = _lib.BdhLayerPlan(B, H, T, N, D)
-    options = _lib.BdhGatedOptions(ACTIVATIONS[activation], float(relu_threshold), _ptr(mask))
-    return plan, options, (current, context, up, gate, mask)
+    if N % 8 or D % 8:
+        return None
+    tensors = [_aligned(current), _aligned(context), _aligned(up), _aligned(gate)]
+    if mask is None:
+        options = _options_of(kind, float(relu_threshold))
+    else:
+        mask = _aligned(mask)
+        tensors.append(mask)   # (held until the launch is enqueued)
+        options = ctypes.byref(_lib.BdhGatedOptions(kind, float(relu_threshold), _ptr(mask)))
+    return dev, (B, H, T, N, D), _plan_of(B, H, T, N, D), options, tensors
 
 
 def _aligned(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     """Contiguous, from a 16-byte boundary on."""
     if t is None:
         return None
-    t = t.contiguous()
+    if not t.is_contiguous():
+        t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
@@ -104,21 +126,17 @@ def gated_block(current: torch.Tensor, weights: GatedWeights, context: Optional[
     options, with "relu" alone.  None where the library does not support the
     input (no supported device, another dtype, an empty dimension, D or N not
     a multiple of 8 or too large)."""
-    call = _plan(current, weights, context, activation, relu_threshold, latent_mask)
+    call = _call(current, weights, context, activation, relu_threshold, latent_mask)
     if call is None:
         return None
-    plan, options, (current, context, up, gate, _mask) = call
-    B, H, T, N = plan.batch, plan.heads, plan.time, plan.latent
-    dev = current.device
-    if N % 8 or plan.embd % 8:
-        return None
+    dev, (B, H, T, N, D), plan, options, t = call
     out = torch.empty((B, T, H * N), device=dev, dtype=torch.bfloat16)
-    saved, parts = None, (None,) * 4
+    saved, parts = None, (None, None, None, None)
     if save:
         saved = GatedSaved(new_checkpoint((B, T, H, N), dev), new_checkpoint((B, T, H, N), dev))
-        parts = (*saved.up, *saved.gate)
-    st = _call_on(dev, _lib.load().bdh_gated_block_fwd, ctypes.byref(plan), _ptr(current), _ptr(context), _ptr(up),
-                  _ptr(gate), ctypes.byref(options), _ptr(out), *map(_ptr, parts), _stream_ptr(dev))
+        parts = [_ptr(p) for c in saved for p in c]
+    st = _call_on(dev, _lib.load().bdh_gated_block_fwd, plan, _ptr(t[0]), _ptr(t[1]), _ptr(t[2]), _ptr(t[3]), options,
+                  _ptr(out), *parts, _stream_ptr(dev))
     return GatedOutput(out, saved) if _lib.check(st) else None
 
 
@@ -132,25 +150,24 @@ def gated_block_vjp(grad: torch.Tensor, current: torch.Tensor, weights: GatedWei
     and the projections are not computed again.  Without a context current's
     gradient has both parts.  None where the library does not support the
     input (as gated_block; a scratch that would have to grow under capture)."""
-    call = _plan(current, weights, context, activation, relu_threshold, latent_mask)
-    if call is None:
+    call = _call(current, weights, context, activation, relu_threshold, latent_mask)
+    if call is None or grad.dtype is not torch.bfloat16:
         return None
-    plan, options, (current, context, up, gate, _mask) = call
-    B, H, T, N, D = plan.batch, plan.heads, plan.time, plan.latent, plan.embd
-    dev = current.device
-    if grad.dtype != torch.bfloat16 or N % 8 or D % 8:
-        return None
-    if tuple(grad.shape) != (B, T, H * N) or grad.device != dev:
+    dev, (B, H, T, N, D), plan, options, t = call
+    if grad.shape != (B, T, H * N) or grad.device != dev:
         raise ValueError(f"grad must be {[B, T, H * N]} on the other tensors' device")
-    parts = (None,) * 4
+    parts, kept = (None, None, None, None), None
     if saved is not None:
-        for c, name in zip(saved, ("saved.up", "saved.gate")):
-            check_checkpoint(c, (B, T, H, N), dev, name)
-        parts = tuple(_aligned(t) for t in (*saved.up, *saved.gate))
+        check_checkpoint(saved.up, (B, T, H, N), dev, "saved.up")
+        check_checkpoint(saved.gate, (B, T, H, N), dev, "saved.gate")
+        kept = [_aligned(saved.up.codes), saved.up.scales, _aligned(saved.gate.codes), saved.gate.scales]
+        parts = [_ptr(p) for p in kept]
     grad = _aligned(grad)
-    bf16 = lambda *shape: torch.empty(shape, device=dev, dtype=torch.bfloat16)  # noqa: E731
-    out = GatedGrads(bf16(B, T, D), None if context is None else bf16(B, H, T, D), bf16(H, D, N), bf16(H, D, N))
-    st = _call_on(dev, _lib.load().bdh_gated_block_vjp, ctypes.byref(plan), _ptr(current), _ptr(context), _ptr(up),
-                  _ptr(gate), ctypes.byref(options), _ptr(grad), *map(_ptr, parts), _ptr(out.current),
-                  _ptr(out.context), _ptr(out.up), _ptr(out.gate), _stream_ptr(dev))
-    return out if _lib.check(st) else None
+    bf16 = torch.bfloat16
+    d_current = torch.empty((B, T, D), device=dev, dtype=bf16)
+    d_context = None if context is None else torch.empty((B, H, T, D), device=dev, dtype=bf16)
+    d_up = torch.empty((H, D, N), device=dev, dtype=bf16)
+    d_gate = torch.empty((H, D, N), device=dev, dtype=bf16)
+    st = _call_on(dev, _lib.load().bdh_gated_block_vjp, plan, _ptr(t[0]), _ptr(t[1]), _ptr(t[2]), _ptr(t[3]), options,
+                  _ptr(grad), *parts, _ptr(d_current), _ptr(d_context), _ptr(d_up), _ptr(d_gate), _stream_ptr(dev))
+    return GatedGrads(d_current, d_context, d_up, d_gate) if _lib.check(st) else None

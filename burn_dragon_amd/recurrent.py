@@ -12,6 +12,7 @@ mismatch, plan mismatch) so that callers fall back exactly as
 from __future__ import annotations
 
 import ctypes
+import functools
 from dataclasses import dataclass
 from typing import NamedTuple, Optional
 
@@ -94,6 +95,7 @@ def _stream_ptr(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
+@functools.lru_cache(maxsize=None)
 def _supported(device: torch.device) -> bool:
     """supports_backend for a device tensor's call (torch is initialised)."""
     return device.type == "cuda" and bool(_call_on(device, _lib.load().bdh_supports_backend))

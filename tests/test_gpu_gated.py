@@ -134,6 +134,16 @@ def test_deep_and_wide():
     run(1, 5, 1, 40, 8200, "gelu", False)
 
 
+# The backward of saved values without the projections' gradients in memory begins at 2^23 of them.
+@pytest.mark.parametrize("B,T,H,D,N,act,context,masked", [
+    (3, 375, 1, 200, 7504, "relu", True, True), (1, 4097, 2, 72, 1032, "relu", True, False),
+    (5, 411, 2, 256, 2056, "silu", False, False), (1, 1025, 1, 256, 8192, "gelu", True, False),
+    (70, 61, 4, 8, 496, "relu", False, True), (2, 999, 3, 136, 1408, "silu", True, False)])
+def test_many_latents(B, T, H, D, N, act, context, masked):
+    assert B * T * H * N >= 1 << 23
+    run(B, T, H, D, N, act, context, 0.5 if masked else 0.0, masked)
+
+
 def test_differences():
     # <gradient, direction> against central differences of sum(g * out) in 64 bits.  The
     # gradients' bf16 (2^-7 of a term, twice) adds at random over thousands of terms, but is

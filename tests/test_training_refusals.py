@@ -107,6 +107,7 @@ BOTH = [
     (dict(heads=513), _lib.BDH_UNSUPPORTED, "large"),
     (dict(latent=(1 << 20) + 8), _lib.BDH_UNSUPPORTED, "large"),
     (dict(embd=(1 << 16) + 8), _lib.BDH_UNSUPPORTED, "large"),
+    (dict(heads=256, latent=(1 << 16) + 8), _lib.BDH_UNSUPPORTED, "large"),
     (dict(batch=1 << 10, time=1 << 10, heads=1, latent=1 << 15), _lib.BDH_UNSUPPORTED, "large"),
     (dict(activation=3), _lib.BDH_EINVAL, "activation"),
     (dict(threshold=math.inf), _lib.BDH_EINVAL, "finite"),
