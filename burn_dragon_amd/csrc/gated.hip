@@ -88,7 +88,22 @@ struct Tile {
   }
 };
 
-// Fills a tile from per-lane addresses; lanes that are not in write zeros.
+// Load j of a tile from per-lane addresses; lanes that are not in write zeros.
+template <class Tl>
+__device__ __forceinline__ void fill_one(char* lds, uint32_t tile, int w, int lane, int j, bool in, const char* from) {
+  const uint32_t to = tile + (uint32_t)((w + Tl::WAVE_STEP * j) * 1024);
+  if (in) load_lds16(from, lds_addr(lds) + to);
+  else *(u32x4*)(lds + to + 16 * lane) = u32x4{0, 0, 0, 0};
+}
+// The same from a base of the wave and the lane's place.
+template <class Tl, class Inside>
+__device__ __forceinline__ void fill_one(char* lds, uint32_t tile, int w, int lane, int j, Inside, bool in,
+                                         const char* base, uint32_t at) {
+  const uint32_t to = tile + (uint32_t)((w + Tl::WAVE_STEP * j) * 1024);
+  if (Inside::value || in) load_lds16(base, at, lds_addr(lds) + to);
+  else *(u32x4*)(lds + to + 16 * lane) = u32x4{0, 0, 0, 0};
+}
+// All of a tile's.
 template <class Tl, class At, class In>
 __device__ __forceinline__ void fill(char* lds, uint32_t tile, int w, int lane, bool whole, At&& at, In&& in) {
 #pragma unroll
@@ -109,6 +124,63 @@ __device__ __forceinline__ void fill(char* lds, uint32_t tile, int w, int lane, 
     if (whole || in(j)) load_lds16(base, at[j], lds_addr(lds) + to);
     else *(u32x4*)(lds + to + 16 * lane) = u32x4{0, 0, 0, 0};
   }
+}
+
+// The products of large calls: four waves, one a SIMD, of 256 f32 sums a lane; of a step of
+// 32 k's each takes 2 x 8 fragments and 2 x 16 products.  A ring of five stages of 32 KB;
+// at step s the barrier confirms stage s + 1, the loads of step s + 4 go into the stage of
+// step s - 1, and fragments are read half a step ahead of their products, a fragment for
+// every other product and a load for the ones between: so LDS, loads and the matrix cores
+// run side by side in one wave.  Against two workgroups a CU of half the sums, a step moves
+// 96 KB in LDS for the same products, not 144, and loads 32 KB, not 48.
+//   load(inside, s, stage, j) this wave's j-th of LOADS loads of step s; not inside: zeros
+//                             past k's end
+//   read(set, i, stage, kk)   fragment i of eight of half kk
+//   multiply(set, i)          product i of 16
+constexpr int BIG_STAGE = 32768, BIG_STAGES = 5, BIG_LOADS = 8;
+template <class Load, class Read, class Multiply>
+__device__ __forceinline__ void big_loop(int s0, int s1, int K, Load&& load, Read&& read, Multiply&& multiply) {
+  if (s0 >= s1) return;
+  const std::false_type no{};
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    if (s0 + q < s1) {
+#pragma unroll
+      for (int j = 0; j < BIG_LOADS; ++j) load(no, s0 + q, q, j);
+    }
+  wait_barrier<0>();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) read(0, i, 0, 0);
+  int stage = 0, s = s0;
+  const auto step = [&](auto inside) {
+    constexpr bool INSIDE = decltype(inside)::value;
+    // In flight: the steps s + 2 and s + 3, where they are whole.
+    if (INSIDE || (s + 3 < s1 && (s + 4) * BK <= K)) wait_barrier<2 * BIG_LOADS>();
+    else wait_barrier<0>();
+    const int next = stage == BIG_STAGES - 1 ? 0 : stage + 1, free = stage == 0 ? BIG_STAGES - 1 : stage - 1;
+    if (!INSIDE && s + 4 < s1) {
+#pragma unroll
+      for (int j = 0; j < BIG_LOADS; ++j) load(no, s + 4, free, j);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      multiply(0, i);
+      if (i % 2 == 0) read(1, i / 2, stage, 1);
+      else if (INSIDE) load(inside, s + 4, free, i / 2);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      multiply(1, i);
+      if (i % 2 == 0) read(0, i / 2, next, 0);  // (after the last step: any)
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    stage = next;
+  };
+  const int last = min(s1, K / BK) - 1;  // whole step
+  for (; s + 4 <= last; ++s) step(std::true_type{});
+  for (; s < s1; ++s) step(no);
 }
 
 // Rows of tokens: token i = (b, t) lies at b * batch + t * step elements.
@@ -208,6 +280,7 @@ struct GatedArgs {
   uint8_t *up_codes, *up_scales, *gate_codes, *gate_scales;
   bf16_t *dp, *dq;          // [M, H, N]
   TileOrder order;          // tiles of latents (of all heads) and of tokens
+  bool big;                 // gated_kernel's larger tiles
 };
 
 // --- both projections, and what is made of them ------------------------------------------
@@ -225,19 +298,22 @@ __device__ __forceinline__ u32x2 join_halves(uint32_t a, uint32_t b) {
 }
 
 // A workgroup: 128 latents (n) of a head by 128 tokens (m), a wave 64 by 64 of both
-// products.
-template <int ACT, int EPI, bool CTX>
-__global__ __launch_bounds__(256, 2) void gated_kernel(const GatedArgs a) {
+// products.  BIG (no context): by 256 tokens, a wave 64 by 128, in big_loop.
+template <int ACT, int EPI, bool CTX, bool BIG>
+__global__ __launch_bounds__(256, BIG ? 1 : 2) void gated_kernel(const GatedArgs a) {
+  static_assert(!(CTX && BIG), "a context's tiles do not fit");
+  constexpr int NJ = BIG ? 4 : 2;  // 32 tokens each of a wave
   typedef Tile<MC, 128> W;
-  typedef Tile<KC, 128> X;
-  constexpr int STAGE = 2 * W::BYTES + (CTX ? 2 : 1) * X::BYTES, STAGES = CTX ? 2 : 3;
+  typedef Tile<KC, 64 * NJ> X;
+  constexpr int STAGE = 2 * W::BYTES + (CTX ? 2 : 1) * X::BYTES, STAGES = BIG ? BIG_STAGES : CTX ? 2 : 3;
+  static_assert(!BIG || (STAGE == BIG_STAGE && 2 * W::LOADS + X::LOADS == BIG_LOADS), "big_loop's stages");
   __shared__ __attribute__((aligned(16))) char lds[STAGES * STAGE];
   const int lane = threadIdx.x & 63, w = wave_id();
   const int D = (int)a.D, N = (int)a.N, M = (int)a.M;
   int an, am;
   if (!a.order.at((int)blockIdx.x, an, am)) return;
   const int n_tiles = (N + 127) / 128;
-  const int n0 = an % n_tiles * 128, h = an / n_tiles, m0 = am * 128;
+  const int n0 = an % n_tiles * 128, h = an / n_tiles, m0 = am * 64 * NJ;
   const char* wp[2][2];
   {
     const int c = W::chunk(w, lane) * 8;
@@ -249,9 +325,9 @@ __global__ __launch_bounds__(256, 2) void gated_kernel(const GatedArgs a) {
       wp[1][j] = (const char*)(a.gate + off);
     }
   }
-  const char* xp[2][2];
+  const char* xp[2][X::LOADS];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
+  for (int j = 0; j < X::LOADS; ++j) {
     const int m = m0 + X::row(j, w, lane);
     const uint32_t i = (uint32_t)(m < M ? m : M - 1);
     xp[0][j] = (const char*)(a.x + (int64_t)i * D + X::chunk(w, lane) * 8);
@@ -271,12 +347,56 @@ __global__ __launch_bounds__(256, 2) void gated_kernel(const GatedArgs a) {
     if (CTX)
       fill<X>(lds, base + 2 * W::BYTES + X::BYTES, w, lane, whole, [&](int j) { return xp[1][j] + 2 * k0; }, x_ok);
   };
-  floatx16 p[2][2], q[2][2];
+  floatx16 p[2][NJ], q[2][NJ];
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) p[i][j] = q[i][j] = zero16();
-  const int nw = 64 * (w & 1), mw = 64 * (w >> 1);
+    for (int j = 0; j < NJ; ++j) p[i][j] = q[i][j] = zero16();
+  const int nw = 64 * (w & 1), mw = 32 * NJ * (w >> 1);
+  if constexpr (BIG) {
+    struct {
+      bf16x8 u[2], g[2], x[4];
+    } f[2];
+    const char* const w_base[2] = {(const char*)(a.up + (int64_t)h * D * N + n0),
+                                   (const char*)(a.gate + (int64_t)h * D * N + n0)};
+    const char* const x_base = (const char*)(a.x + (int64_t)m0 * D);
+    uint32_t w_at[2], x_at[X::LOADS];
+    {
+      const int c = W::chunk(w, lane) * 8;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) w_at[j] = 2u * (uint32_t)(W::row(j, w, lane) * N + (n0 + c < N ? c : 0));
+#pragma unroll
+      for (int j = 0; j < X::LOADS; ++j) {
+        const int m = X::row(j, w, lane);
+        x_at[j] = 2u * (uint32_t)((m0 + m < M ? m : M - 1 - m0) * D + X::chunk(w, lane) * 8);
+      }
+    }
+    big_loop(
+        0, steps, D,
+        [&](auto inside, int s, int stage, int j) {
+          const int k0 = s * BK;
+          const uint32_t base = (uint32_t)(stage * STAGE);
+          if (j < 4) {
+            const int r = j & 1, which = j >> 1;
+            fill_one<W>(lds, base + which * W::BYTES, w, lane, r, inside, k0 + W::row(r, w, lane) < D,
+                        w_base[which] + 2 * (int64_t)k0 * N, w_at[r]);
+          } else {
+            fill_one<X>(lds, base + 2 * W::BYTES, w, lane, j - 4, inside, k0 + X::chunk(w, lane) * 8 < D,
+                        x_base + 2 * k0, x_at[j - 4]);
+          }
+        },
+        [&](int set, int i, int stage, int kk) {
+          const char* t = lds + stage * STAGE;
+          if (i < 2) f[set].u[i] = W::frag(t, nw + 32 * i, kk, lane);
+          else if (i < 4) f[set].g[i - 2] = W::frag(t + W::BYTES, nw + 32 * (i - 2), kk, lane);
+          else f[set].x[i - 4] = X::frag(t + 2 * W::BYTES, mw + 32 * (i - 4), kk, lane);
+        },
+        [&](int set, int i) {
+          const int j = i / 4, e = i & 1;
+          if (i & 2) q[e][j] = mfma32(f[set].g[e], f[set].x[j], q[e][j]);
+          else p[e][j] = mfma32(f[set].u[e], f[set].x[j], p[e][j]);
+        });
+  } else {
   issue(0, 0);
   if (STAGES == 3 && steps > 1) issue(1, 1);
   for (int s = 0, stage = 0; s < steps; ++s) {
@@ -305,8 +425,9 @@ __global__ __launch_bounds__(256, 2) void gated_kernel(const GatedArgs a) {
         for (int j = 0; j < 2; ++j) q[i][j] = mfma32(g[i], c[j], q[i][j]);
     }
   }
+  }
   // A lane has token mw + 32 j + (lane & 31) and, of 32 latents, 8 r + 4 (lane >> 5)
-  // ..+3 for r of 0..3.  Half of the tile's tokens at a time (j) go through LDS, so that
+  // ..+3 for r of 0..3.  64 of the tile's tokens at a time (j) go through LDS, so that
   // memory sees whole rows of 128 latents, stored past the caches, which they would only
   // empty (16384 tokens, 4 heads of 8192, D 256, saved: 1400 -> 1200 us).
   constexpr int VP = 272, CP = 144;  // row pitches in bytes (bank spread)
@@ -315,12 +436,12 @@ __global__ __launch_bounds__(256, 2) void gated_kernel(const GatedArgs a) {
   char* const bytes = more + 128 * CP;
   static_assert(64 * VP + 128 * CP + 512 <= 2 * STAGE && 128 * VP <= 2 * STAGE, "the stages' memory");
   const int high = lane >> 5, nb = (N + kFp8Block - 1) / kFp8Block;
-  const int mine = 32 * (w >> 1) + (lane & 31);  // the lane's row of the half
-  // Row r of half j, and its place in [tokens, H].
-  const auto token = [&](int r, int j) { return m0 + 64 * (r >> 5) + 32 * j + (r & 31); };
+  const int mine = 32 * (w >> 1) + (lane & 31);  // the lane's row of the part
+  // Row r of part j, and its place in [tokens, H].
+  const auto token = [&](int r, int j) { return m0 + 32 * NJ * (r >> 5) + 32 * j + (r & 31); };
   const auto place = [&](int m) { return (int64_t)m * a.H + h; };
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
+  for (int j = 0; j < NJ; ++j) {
     wait_barrier<0>();
     if (EPI == BACK) {
 #pragma unroll
@@ -665,6 +786,7 @@ struct ProductArgs {
   int H;
   int64_t c_head;
   TokenRows c_rows;
+  bool c_apart;             // c's rows of a head do not follow one another
   int in_parts, w_parts;    // of k
   int in_tiles, w_tiles;    // in all, parts counted
   int x_parts;              // sums that make up d_x
@@ -737,76 +859,97 @@ __device__ __forceinline__ int id_of(int b, int n) {
   return b >> 3 < per_xcd && id < n ? id : -1;
 }
 
-constexpr int PRODUCT_LDS = 3 * 64 * (256 + 128);
-template <int WHAT>
+// BIG: 256 by 256, a wave 128 by 128, in big_loop.
+template <int WHAT, bool BIG>
 __device__ __forceinline__ void product_tile(const ProductArgs& a, char* lds, int id) {
   typedef Tile<WHAT == INPUTS ? KC : MC, 256> A;  // U, G rows d / dp, dq columns n
-  typedef Tile<WHAT == INPUTS ? KC : MC, 128> B;  // dp, dq rows m / x, c columns d
+  constexpr int NB = BIG ? 4 : 2;                 // 32 of the result's rows each of a wave
+  typedef Tile<WHAT == INPUTS ? KC : MC, 64 * NB> B;  // dp, dq rows m / x, c columns d
   constexpr int STAGE = A::BYTES + B::BYTES, LOADS = A::LOADS + B::LOADS;
-  static_assert(3 * STAGE == PRODUCT_LDS, "the ring");
+  static_assert(!BIG || (STAGE == BIG_STAGE && LOADS == BIG_LOADS), "big_loop's stages");
   const int lane = threadIdx.x & 63, w = wave_id();
   const int D = (int)a.D, N = (int)a.N, M = (int)a.M;
   // The tiles along D, which share the larger operand, are neighbours.
-  const int d_tiles = (D + (WHAT == INPUTS ? 255 : 127)) / (WHAT == INPUTS ? 256 : 128);
-  const int other = WHAT == INPUTS ? (M + 127) / 128 : (N + 255) / 256;
+  const int d_tiles = (D + (WHAT == INPUTS ? 256 : 64 * NB) - 1) / (WHAT == INPUTS ? 256 : 64 * NB);
+  const int other = WHAT == INPUTS ? (M + 64 * NB - 1) / (64 * NB) : (N + 255) / 256;
   const int parts = WHAT == INPUTS ? a.in_parts : a.w_parts;
   const int di = id % d_tiles, oi = id / d_tiles % other, rest = id / d_tiles / other;
   const int part = rest % parts, job = rest / parts;
   const int h = job % a.H, which = job / a.H;  // which: 0 up, 1 gate
-  const int a0 = (WHAT == INPUTS ? di : oi) * 256, b0 = (WHAT == INPUTS ? oi : di) * 128;
+  const int a0 = (WHAT == INPUTS ? di : oi) * 256, b0 = (WHAT == INPUTS ? oi : di) * 64 * NB;
   const int K = WHAT == INPUTS ? N : M;
   const bf16_t* dv = which ? a.dq : a.dp;        // [M, H, N]
   const int64_t d_row = (int64_t)a.H * N;
   const bool ctx = which && a.c;
-  const char* ap[A::LOADS];
-  const char* bp[B::LOADS];
+  // Bases of the workgroup, and the lanes' places (below 2^32 bytes: H N is 2^24 at most, of
+  // BIG 2^23).  apart: c's rows go by their tokens; else they follow one another, as x's.
+  const bool apart = !BIG && ctx && a.c_apart;
+  const char* a_base;
+  const char* b_base;
+  uint32_t a_at[A::LOADS], b_at[B::LOADS];
   const int ac = A::chunk(w, lane) * 8, bc = B::chunk(w, lane) * 8;
+  if (WHAT == INPUTS) {
+    a_base = (const char*)((which ? a.gate : a.up) + ((int64_t)h * D + a0) * N);
+    b_base = (const char*)(dv + b0 * d_row + (int64_t)h * N);
+  } else {
+    a_base = (const char*)(dv + (int64_t)h * N + a0);
+    b_base = (const char*)(ctx ? a.c + (int64_t)h * a.c_head : a.x);
+  }
 #pragma unroll
   for (int j = 0; j < A::LOADS; ++j) {
     const int r = A::row(j, w, lane);
-    if (WHAT == INPUTS) {
-      const int d = a0 + r < D ? a0 + r : D - 1;
-      ap[j] = (const char*)((which ? a.gate : a.up) + ((int64_t)h * D + d) * N + ac);
-    } else {
-      const int n = a0 + ac < N ? a0 + ac : 0;
-      ap[j] = (const char*)(dv + (int64_t)r * d_row + (int64_t)h * N + n);
-    }
+    a_at[j] = WHAT == INPUTS ? 2u * (uint32_t)((a0 + r < D ? r : D - 1 - a0) * N + ac)
+                             : 2u * ((uint32_t)r * (uint32_t)d_row + (uint32_t)(a0 + ac < N ? ac : 0));
   }
 #pragma unroll
   for (int j = 0; j < B::LOADS; ++j) {
-    const int r = B::row(j, w, lane);
-    if (WHAT == INPUTS) {
-      const int m = b0 + r < M ? b0 + r : M - 1;
-      bp[j] = (const char*)(dv + (int64_t)m * d_row + (int64_t)h * N + bc);
-    } else {
-      const int d = b0 + bc < D ? b0 + bc : 0;
-      bp[j] = (const char*)((ctx ? a.c + (int64_t)h * a.c_head : a.x + (int64_t)r * D) + d);
-    }
+    const int r = B::row(j, w, lane), d = b0 + bc < D ? b0 + bc : 0;
+    b_at[j] = WHAT == INPUTS ? 2u * ((uint32_t)(b0 + r < M ? r : M - 1 - b0) * (uint32_t)d_row + (uint32_t)bc)
+                             : 2u * (uint32_t)((apart ? 0 : r * D) + d);
   }
   const int steps = (K + BK - 1) / BK;
   const int s0 = (int)((int64_t)steps * part / parts), s1 = (int)((int64_t)steps * (part + 1) / parts);
-  const auto issue = [&](int s, int stage) {
+  const auto load = [&](auto inside, int s, int stage, int j) {
     const int k0 = s * BK;
-    const bool whole = k0 + BK <= K;
     const uint32_t base = (uint32_t)(stage * STAGE);
-    const auto a_in = [&](int j) { return k0 + (WHAT == INPUTS ? ac : A::row(j, w, lane)) < K; };
-    const auto b_in = [&](int j) { return k0 + (WHAT == INPUTS ? bc : B::row(j, w, lane)) < K; };
-    fill<A>(lds, base, w, lane, whole,
-            [&](int j) { return ap[j] + 2 * (WHAT == INPUTS ? (int64_t)k0 : k0 * d_row); }, a_in);
-    fill<B>(lds, base + A::BYTES, w, lane, whole,
-            [&](int j) {
-              if (WHAT == INPUTS) return bp[j] + 2 * (int64_t)k0;
-              if (ctx) return bp[j] + 2 * a.c_rows.at((uint32_t)(k0 + B::row(j, w, lane)));
-              return bp[j] + 2 * (int64_t)k0 * D;
-            },
-            b_in);
+    if (j < A::LOADS) {
+      fill_one<A>(lds, base, w, lane, j, inside, k0 + (WHAT == INPUTS ? ac : A::row(j, w, lane)) < K,
+                  a_base + 2 * (WHAT == INPUTS ? (int64_t)k0 : k0 * d_row), a_at[j]);
+    } else {
+      const int i = j - A::LOADS;
+      const bool in = decltype(inside)::value || k0 + (WHAT == INPUTS ? bc : B::row(i, w, lane)) < K;
+      if (WHAT == WEIGHTS && apart)
+        fill_one<B>(lds, base + A::BYTES, w, lane, i, in, b_base + 2 * a.c_rows.at((uint32_t)(k0 + B::row(i, w, lane))) + b_at[i]);
+      else
+        fill_one<B>(lds, base + A::BYTES, w, lane, i, inside, in,
+                    b_base + 2 * (WHAT == INPUTS ? (int64_t)k0 : (int64_t)k0 * D), b_at[i]);
+    }
   };
-  floatx16 acc[4][2];
+  const auto issue = [&](int s, int stage) {
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) load(std::false_type{}, s, stage, j);
+  };
+  floatx16 acc[4][NB];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) acc[i][j] = zero16();
-  const int aw = 128 * (w & 1), bw = 64 * (w >> 1);
+    for (int j = 0; j < NB; ++j) acc[i][j] = zero16();
+  const int aw = 128 * (w & 1), bw = 32 * NB * (w >> 1);
+  if constexpr (BIG) {
+    struct {
+      bf16x8 a[4], b[4];
+    } f[2];
+    big_loop(
+        s0, s1, K, load,
+        [&](int set, int i, int stage, int kk) {
+          const char* t = lds + stage * STAGE;
+          if (i < 4) f[set].a[i] = A::frag(t, aw + 32 * i, kk, lane);
+          else f[set].b[i - 4] = B::frag(t + A::BYTES, bw + 32 * (i - 4), kk, lane);
+        },
+        [&](int set, int i) { acc[i / 4][i % 4] = mfma32(f[set].a[i / 4], f[set].b[i % 4], acc[i / 4][i % 4]); });
+    store_product<WHAT>(a, acc, h, which, part, a0 + aw, b0 + bw, lane);
+    return;
+  }
   // Ring of three stages.  A step's loads may be in flight while the one before it is
   // multiplied, but only whole steps' are counted: a last one leaves out some.
   if (s0 < s1) issue(s0, 0);
@@ -819,28 +962,29 @@ __device__ __forceinline__ void product_tile(const ProductArgs& a, char* lds, in
     stage = stage == 2 ? 0 : stage + 1;
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
-      bf16x8 fa[4], fb[2];
+      bf16x8 fa[4], fb[NB];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) fb[j] = B::frag(t + A::BYTES, bw + 32 * j, kk, lane);
+      for (int j = 0; j < NB; ++j) fb[j] = B::frag(t + A::BYTES, bw + 32 * j, kk, lane);
 #pragma unroll
       for (int i = 0; i < 4; ++i) fa[i] = A::frag(t, aw + 32 * i, kk, lane);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = mfma32(fa[i], fb[j], acc[i][j]);
+        for (int j = 0; j < NB; ++j) acc[i][j] = mfma32(fa[i], fb[j], acc[i][j]);
     }
   }
   store_product<WHAT>(a, acc, h, which, part, a0 + aw, b0 + bw, lane);
 }
 
 // The products of the inputs, then those of the weights.
-__global__ __launch_bounds__(256, 2) void product_kernel(const ProductArgs a) {
-  __shared__ __attribute__((aligned(16))) char lds[PRODUCT_LDS];
+template <bool BIG>
+__global__ __launch_bounds__(256, BIG ? 1 : 2) void product_kernel(const ProductArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[BIG ? BIG_STAGES * BIG_STAGE : 3 * 64 * (256 + 128)];
   const int inputs = (a.in_tiles + 7) / 8 * 8, b = (int)blockIdx.x;
   const int id = b < inputs ? id_of(b, a.in_tiles) : id_of(b - inputs, a.w_tiles);
   if (id < 0) return;
-  if (b < inputs) product_tile<INPUTS>(a, lds, id);
-  else product_tile<WEIGHTS>(a, lds, id);
+  if (b < inputs) product_tile<INPUTS, BIG>(a, lds, id);
+  else product_tile<WEIGHTS, BIG>(a, lds, id);
 }
 
 // Both products of a kind straight from what the forward saved, D up to 256: dp and dq are
@@ -1117,9 +1261,15 @@ void launch_projections(const GatedArgs& a, hipStream_t st) {
       return;
     }
   }
+  if (a.big) {
+    GatedArgs b = a;
+    b.order = tile_order((int64_t)cdiv(a.N, 128) * a.H, cdiv(a.M, 256));
+    hipLaunchKernelGGL((gated_kernel<ACT, EPI, false, true>), dim3(grid_of(b.order)), dim3(256), 0, st, b);
+    return;
+  }
   const dim3 grid(grid_of(a.order));
-  if (a.c) hipLaunchKernelGGL((gated_kernel<ACT, EPI, true>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((gated_kernel<ACT, EPI, false>), grid, dim3(256), 0, st, a);
+  if (a.c) hipLaunchKernelGGL((gated_kernel<ACT, EPI, true, false>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((gated_kernel<ACT, EPI, false, false>), grid, dim3(256), 0, st, a);
 }
 template <int EPI>
 void launch_projections(const GatedArgs& a, int act, hipStream_t st) {
@@ -1158,6 +1308,7 @@ GatedArgs args_of(const GatedCall& g) {
   a.gate_codes = g.gate_codes;
   a.gate_scales = g.gate_scales;
   a.order = tile_order((int64_t)cdiv(g.N, 128) * g.H, cdiv(a.M, 128));
+  a.big = !g.c && (int64_t)cdiv(g.N, 128) * g.H * cdiv(a.M, 256) >= device_cus();
   return a;
 }
 
@@ -1188,12 +1339,14 @@ bdh_status gated_block_vjp(const GatedCall& g, hipStream_t st, uint64_t* launche
     p = p < most ? p : most;
     return (int)(p < 32 ? p : 32);
   };
-  const int64_t in_tiles = fused ? cdiv(M, 128) * H : (int64_t)cdiv(D, 256) * cdiv(M, 128) * 2 * H;
-  const int64_t w_tiles = fused ? cdiv(N, 128) * H : (int64_t)cdiv(N, 256) * cdiv(D, 128) * 2 * H;
+  const bool big = !fused && D > 128 && H * N <= (int64_t)1 << 23 && (!g.c || g.B == 1 || H == 1) &&
+                    (int64_t)cdiv(D, 256) * (cdiv(M, 256) + cdiv(N, 256)) * 2 * H >= cus / 2;
+  const int64_t in_tiles = fused ? cdiv(M, 128) * H : (int64_t)cdiv(D, 256) * cdiv(M, big ? 256 : 128) * 2 * H;
+  const int64_t w_tiles = fused ? cdiv(N, 128) * H : (int64_t)cdiv(N, 256) * cdiv(D, big ? 256 : 128) * 2 * H;
   ProductArgs p{};
   // (Both kinds run together where they are not fused.)
-  p.in_parts = parts_of(in_tiles, cus, N);
-  p.w_parts = parts_of(w_tiles, cus, M);
+  p.in_parts = parts_of(in_tiles, big ? cus / 2 : cus, N);
+  p.w_parts = parts_of(w_tiles, big ? cus / 2 : cus, M);
   // (A launch has fewer than 2^32 threads.)
   if (in_tiles * p.in_parts > (int64_t)1 << 22 || w_tiles * p.w_parts > (int64_t)1 << 22)
     return fail(BDH_UNSUPPORTED, "too large for one launch");
@@ -1231,6 +1384,7 @@ bdh_status gated_block_vjp(const GatedCall& g, hipStream_t st, uint64_t* launche
   p.H = (int)H;
   p.c_head = a.c_head;
   p.c_rows = a.c_rows;
+  p.c_apart = g.B > 1 && H > 1;
   p.d_x = g.d_x;
   p.d_c = g.d_c;
   p.d_up = g.d_up;
@@ -1250,7 +1404,9 @@ bdh_status gated_block_vjp(const GatedCall& g, hipStream_t st, uint64_t* launche
     } else {
       launch_projections<BACK>(a, g.act, st);
     }
-    hipLaunchKernelGGL(product_kernel, dim3((cdiv(p.in_tiles, 8) + cdiv(p.w_tiles, 8)) * 8), dim3(256), 0, st, p);
+    const dim3 grid((cdiv(p.in_tiles, 8) + cdiv(p.w_tiles, 8)) * 8);
+    if (big) hipLaunchKernelGGL(product_kernel<true>, grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL(product_kernel<false>, grid, dim3(256), 0, st, p);
   }
   *launches += 2;
   JoinArgs j{};
