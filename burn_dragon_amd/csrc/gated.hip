@@ -129,8 +129,8 @@ __device__ __forceinline__ void fill(char* lds, uint32_t tile, int w, int lane, 
 // The products of large calls: four waves, one a SIMD, of 256 f32 sums a lane; of a step of
 // 32 k's each takes 2 x 8 fragments and 2 x 16 products.  A ring of five stages of 32 KB;
 // at step s the barrier confirms stage s + 1, the loads of step s + 4 go into the stage of
-// step s - 1, and fragments are read half a step ahead of their products, a fragment for
-// every other product and a load for the ones between: so LDS, loads and the matrix cores
+// step s - 1, and fragments are read half a step ahead of their products, a fragment or
+// a load after each product: so LDS, loads and the matrix cores
 // run side by side in one wave.  Against two workgroups a CU of half the sums, a step moves
 // 96 KB in LDS for the same products, not 144, and loads 32 KB, not 48.
 //   load(inside, s, stage, j) this wave's j-th of LOADS loads of step s; not inside: zeros
@@ -152,6 +152,9 @@ __device__ __forceinline__ void big_loop(int s0, int s1, int K, Load&& load, Rea
 #pragma unroll
   for (int i = 0; i < 8; ++i) read(0, i, 0, 0);
   int stage = 0, s = s0;
+  // Fragments after the products 0, 1, 3, 4, 6, 7, 9, 10, so that the last of them has
+  // five products' time; loads after the others.
+  const auto is_read = [](int i) { return i % 3 != 2 && i < 11; };
   const auto step = [&](auto inside) {
     constexpr bool INSIDE = decltype(inside)::value;
     // In flight: the steps s + 2 and s + 3, where they are whole.
@@ -166,14 +169,14 @@ __device__ __forceinline__ void big_loop(int s0, int s1, int K, Load&& load, Rea
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       multiply(0, i);
-      if (i % 2 == 0) read(1, i / 2, stage, 1);
-      else if (INSIDE) load(inside, s + 4, free, i / 2);
+      if (is_read(i)) read(1, (2 * i + 1) / 3, stage, 1);
+      else if (INSIDE) load(inside, s + 4, free, i < 12 ? i / 3 : i - 8);
       __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       multiply(1, i);
-      if (i % 2 == 0) read(0, i / 2, next, 0);  // (after the last step: any)
+      if (is_read(i)) read(0, (2 * i + 1) / 3, next, 0);  // (after the last step: any)
       __builtin_amdgcn_sched_barrier(0);
     }
     stage = next;
@@ -280,7 +283,6 @@ struct GatedArgs {
   uint8_t *up_codes, *up_scales, *gate_codes, *gate_scales;
   bf16_t *dp, *dq;          // [M, H, N]
   TileOrder order;          // tiles of latents (of all heads) and of tokens
-  bool big;                 // gated_kernel's larger tiles
 };
 
 // --- both projections, and what is made of them ------------------------------------------
@@ -789,6 +791,7 @@ struct ProductArgs {
   bool c_apart;             // c's rows of a head do not follow one another
   int in_parts, w_parts;    // of k
   int in_tiles, w_tiles;    // in all, parts counted
+  bool weights_first;
   int x_parts;              // sums that make up d_x
   int64_t x_size, c_size;   // elements of d_x, d_c
   bf16_t *d_x, *d_c, *d_up, *d_gate;
@@ -976,15 +979,16 @@ __device__ __forceinline__ void product_tile(const ProductArgs& a, char* lds, in
   store_product<WHAT>(a, acc, h, which, part, a0 + aw, b0 + bw, lane);
 }
 
-// The products of the inputs, then those of the weights.
+// Both kinds of products, the one with the longer sums first.
 template <bool BIG>
 __global__ __launch_bounds__(256, BIG ? 1 : 2) void product_kernel(const ProductArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[BIG ? BIG_STAGES * BIG_STAGE : 3 * 64 * (256 + 128)];
-  const int inputs = (a.in_tiles + 7) / 8 * 8, b = (int)blockIdx.x;
-  const int id = b < inputs ? id_of(b, a.in_tiles) : id_of(b - inputs, a.w_tiles);
+  const int first = ((a.weights_first ? a.w_tiles : a.in_tiles) + 7) / 8 * 8, b = (int)blockIdx.x;
+  const bool weights = (b < first) == a.weights_first;
+  const int id = id_of(b < first ? b : b - first, weights ? a.w_tiles : a.in_tiles);
   if (id < 0) return;
-  if (b < inputs) product_tile<INPUTS, BIG>(a, lds, id);
-  else product_tile<WEIGHTS, BIG>(a, lds, id);
+  if (weights) product_tile<WEIGHTS, BIG>(a, lds, id);
+  else product_tile<INPUTS, BIG>(a, lds, id);
 }
 
 // Both products of a kind straight from what the forward saved, D up to 256: dp and dq are
@@ -1252,6 +1256,77 @@ TokenRows token_rows(int64_t time, int64_t batch_stride, int64_t step) {
   return TokenRows{batch_stride, step, (uint32_t)time, 1.0f / (float)time};
 }
 
+template <int WHAT>
+void launch_fused(const ProductArgs& p, const GatedArgs& a, int act, hipStream_t st) {
+  const dim3 grid(cdiv(WHAT == INPUTS ? p.in_tiles : p.w_tiles, 8) * 8);
+  if (act == RELU && a.mask) hipLaunchKernelGGL((fused_kernel<WHAT, RELU, true>), grid, dim3(512), 0, st, p, a);
+  else if (act == RELU) hipLaunchKernelGGL((fused_kernel<WHAT, RELU, false>), grid, dim3(512), 0, st, p, a);
+  else if (act == SILU) hipLaunchKernelGGL((fused_kernel<WHAT, SILU, false>), grid, dim3(512), 0, st, p, a);
+  else hipLaunchKernelGGL((fused_kernel<WHAT, GELU, false>), grid, dim3(512), 0, st, p, a);
+}
+
+// How long n1 tasks of length l1 and n2 of l2 <= l1 take on `slots`, the longer ones first.
+int64_t makespan(int64_t n1, int64_t l1, int64_t n2, int64_t l2, int64_t slots) {
+  const int64_t all = n1 / slots * l1, more = n1 % slots;  // every slot; and `more` of them one longer
+  int64_t low = all + (more ? l1 : 0), high = low + (n2 + slots - 1) / slots * l2;
+  while (low < high) {
+    const int64_t t = (low + high) / 2;
+    const int64_t room = (t >= all + l1 ? more * ((t - all - l1) / l2) : 0) + (slots - more) * ((t - all) / l2);
+    if (room >= n2 && t >= all + (more ? l1 : 0)) high = t;
+    else low = t + 1;
+  }
+  return low;
+}
+
+// Tiles and parts of k of the backward's products: what takes the least time by the steps of
+// the longest row of tiles on a slot and by the bytes of the partial sums.  Measured: a step of
+// 256 by 256 tiles (one a CU) 0.84 us, of 256 by 128 (two a CU) 1.11, a tile's ends about
+// six steps; sums 4.5 TB/s and a launch.  (3003 tokens of 4096 latents, D 1024: 160 -> 114 us.)
+struct ProductPlan {
+  int in_parts, w_parts;
+  double us;
+};
+ProductPlan plan_products(int64_t M, int64_t H, int64_t N, int64_t D, bool ctx, bool big) {
+  const int64_t slots = (int64_t)device_cus() * (big ? 1 : 2), b = big ? 256 : 128;
+  const int64_t in_tiles = (D + 255) / 256 * ((M + b - 1) / b) * 2 * H, w_tiles = (N + 255) / 256 * ((D + b - 1) / b) * 2 * H;
+  const int64_t in_steps = (N + BK - 1) / BK, w_steps = (M + BK - 1) / BK;
+  ProductPlan best{1, 1, 1e30};
+  for (const int pi : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+    if (pi > 1 && in_steps / pi < 8) break;
+    for (const int pw : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+      if (pw > 1 && w_steps / pw < 8) break;
+      const int64_t li = (in_steps + pi - 1) / pi + 6, lw = (w_steps + pw - 1) / pw + 6;
+      const int64_t ni = in_tiles * pi, nw = w_tiles * pw;
+      const int64_t steps = li >= lw ? makespan(ni, li, nw, lw, slots) : makespan(nw, lw, ni, li, slots);
+      const int64_t xp = (ctx ? 1 : 2) * H * pi;
+      const double bytes = 8.0 * ((xp > 1 ? (double)xp * M * D : 0.0) + (ctx && pi > 1 ? (double)pi * M * H * D : 0.0) +
+                                  (pw > 1 ? 2.0 * pw * H * D * N : 0.0));
+      const double us = (double)steps * (big ? 0.84 : 1.11) + bytes / 4.5e6 + (bytes > 0 ? 4.0 : 0.0);
+      if (us < best.us) best = ProductPlan{pi, pw, us};
+    }
+  }
+  return best;
+}
+
+// Whether the projections take the larger tiles: rounds of workgroups (between the whole
+// and the broken number of them) times steps and ends, us as measured (M 3003, 4096 and 8192,
+// N 4096 and 8192, D 256 to 2048).  The ends (activation, 8 bits, memory) run beside another
+// workgroup's products only in the smaller ones.
+template <int EPI>
+bool big_projections(const GatedArgs& a, int act) {
+  if (a.c) return false;
+  constexpr double ends[2][3][3] = {{{6.5, 6.2, 14.7}, {13.5, 12.7, 21.5}, {14.0, 13.8, 21.9}},
+                                    {{9.5, 8.3, 23.6}, {22.0, 23.0, 39.0}, {20.6, 20.0, 35.5}}};
+  double us[2];
+  for (int big = 0; big < 2; ++big) {
+    const int64_t slots = (int64_t)device_cus() * (big ? 1 : 2), m = big ? 256 : 128;
+    const int64_t tiles = (a.N + 127) / 128 * a.H * ((a.M + m - 1) / m);
+    const double rounds = 0.5 * ((double)((tiles + slots - 1) / slots) + (double)tiles / (double)slots);
+    us[big] = rounds * ((double)((a.D + BK - 1) / BK) * (big ? 0.82 : 1.07) + ends[big][EPI][act]);
+  }
+  return us[1] < us[0];
+}
+
 template <int ACT, int EPI>
 void launch_projections(const GatedArgs& a, hipStream_t st) {
   if constexpr (EPI != BACK) {
@@ -1261,7 +1336,7 @@ void launch_projections(const GatedArgs& a, hipStream_t st) {
       return;
     }
   }
-  if (a.big) {
+  if (big_projections<EPI>(a, ACT)) {
     GatedArgs b = a;
     b.order = tile_order((int64_t)cdiv(a.N, 128) * a.H, cdiv(a.M, 256));
     hipLaunchKernelGGL((gated_kernel<ACT, EPI, false, true>), dim3(grid_of(b.order)), dim3(256), 0, st, b);
@@ -1276,15 +1351,6 @@ void launch_projections(const GatedArgs& a, int act, hipStream_t st) {
   if (act == RELU) launch_projections<RELU, EPI>(a, st);
   else if (act == SILU) launch_projections<SILU, EPI>(a, st);
   else launch_projections<GELU, EPI>(a, st);
-}
-
-template <int WHAT>
-void launch_fused(const ProductArgs& p, const GatedArgs& a, int act, hipStream_t st) {
-  const dim3 grid(cdiv(WHAT == INPUTS ? p.in_tiles : p.w_tiles, 8) * 8);
-  if (act == RELU && a.mask) hipLaunchKernelGGL((fused_kernel<WHAT, RELU, true>), grid, dim3(512), 0, st, p, a);
-  else if (act == RELU) hipLaunchKernelGGL((fused_kernel<WHAT, RELU, false>), grid, dim3(512), 0, st, p, a);
-  else if (act == SILU) hipLaunchKernelGGL((fused_kernel<WHAT, SILU, false>), grid, dim3(512), 0, st, p, a);
-  else hipLaunchKernelGGL((fused_kernel<WHAT, GELU, false>), grid, dim3(512), 0, st, p, a);
 }
 
 GatedArgs args_of(const GatedCall& g) {
@@ -1308,7 +1374,6 @@ GatedArgs args_of(const GatedCall& g) {
   a.gate_codes = g.gate_codes;
   a.gate_scales = g.gate_scales;
   a.order = tile_order((int64_t)cdiv(g.N, 128) * g.H, cdiv(a.M, 128));
-  a.big = !g.c && (int64_t)cdiv(g.N, 128) * g.H * cdiv(a.M, 256) >= device_cus();
   return a;
 }
 
@@ -1331,22 +1396,38 @@ bdh_status gated_block_vjp(const GatedCall& g, hipStream_t st, uint64_t* launche
   // 119 / 136, of 8192 475 / 606; 1 head of 8192: 1024 tokens 94 / 101; D 64: 70 / 70).  (A
   // fused step of 128 tokens' places is held in 32 bits.)
   const bool fused = g.up_codes && D <= 256 && M * H * N >= (int64_t)1 << 23 && H * N <= (int64_t)1 << 23;
-  // Parts of k: enough workgroups to fill the chip.
   const int64_t cus = device_cus();
-  const auto parts_of = [&](int64_t tiles, int64_t want, int64_t K) {
-    int64_t p = (want + tiles - 1) / tiles;
-    const int64_t most = K / 256 > 1 ? K / 256 : 1;
-    p = p < most ? p : most;
-    return (int)(p < 32 ? p : 32);
-  };
-  const bool big = !fused && D > 128 && H * N <= (int64_t)1 << 23 && (!g.c || g.B == 1 || H == 1) &&
-                    (int64_t)cdiv(D, 256) * (cdiv(M, 256) + cdiv(N, 256)) * 2 * H >= cus / 2;
-  const int64_t in_tiles = fused ? cdiv(M, 128) * H : (int64_t)cdiv(D, 256) * cdiv(M, big ? 256 : 128) * 2 * H;
-  const int64_t w_tiles = fused ? cdiv(N, 128) * H : (int64_t)cdiv(N, 256) * cdiv(D, big ? 256 : 128) * 2 * H;
   ProductArgs p{};
-  // (Both kinds run together where they are not fused.)
-  p.in_parts = parts_of(in_tiles, big ? cus / 2 : cus, N);
-  p.w_parts = parts_of(w_tiles, big ? cus / 2 : cus, M);
+  bool big = false;
+  int64_t in_tiles, w_tiles;
+  if (fused) {
+    // Parts of k: enough workgroups to fill the chip.
+    const auto parts_of = [&](int64_t tiles, int64_t K) {
+      const int64_t want = (cus + tiles - 1) / tiles, most = K / 256 > 1 ? K / 256 : 1;
+      const int64_t parts = want < most ? want : most;
+      return (int)(parts < 32 ? parts : 32);
+    };
+    in_tiles = cdiv(M, 128) * H;
+    w_tiles = cdiv(N, 128) * H;
+    p.in_parts = parts_of(in_tiles, N);
+    p.w_parts = parts_of(w_tiles, M);
+  } else {
+    ProductPlan plan = plan_products(M, H, N, D, g.c != nullptr, false);
+    // (What the larger tiles' places in memory are held in takes H N up to 2^23, and rows
+    // of c that follow one another.)
+    if (H * N <= (int64_t)1 << 23 && (!g.c || g.B == 1 || H == 1)) {
+      const ProductPlan other = plan_products(M, H, N, D, g.c != nullptr, true);
+      if (other.us < plan.us) {
+        plan = other;
+        big = true;
+      }
+    }
+    in_tiles = (int64_t)cdiv(D, 256) * cdiv(M, big ? 256 : 128) * 2 * H;
+    w_tiles = (int64_t)cdiv(N, 256) * cdiv(D, big ? 256 : 128) * 2 * H;
+    p.in_parts = plan.in_parts;
+    p.w_parts = plan.w_parts;
+    p.weights_first = (M + p.w_parts - 1) / p.w_parts > (N + p.in_parts - 1) / p.in_parts;
+  }
   // (A launch has fewer than 2^32 threads.)
   if (in_tiles * p.in_parts > (int64_t)1 << 22 || w_tiles * p.w_parts > (int64_t)1 << 22)
     return fail(BDH_UNSUPPORTED, "too large for one launch");
