@@ -64,16 +64,14 @@ __global__ __launch_bounds__(256) void save_kernel(const T* __restrict__ x, uint
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = j < w.n ? (float)x[w.at + j] : 0.0f;
     }
-    uint32_t top = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, finite_bits(v[j]));
+    uint32_t top = finite_top<true, 8>(v);
     // (total is a multiple of 4: the lanes of a block are there or not together.)
     top = max(top, (uint32_t)__shfl_xor((int)top, 1, 4));
     top = max(top, (uint32_t)__shfl_xor((int)top, 2, 4));
     const int scale = fp8_scale(top);
-    const float inverse = fp8_inverse(scale);
+    const float power = fp8_power(scale);
     fp8_keep_finite(v, scale);
-    const u32x2_u c{fp8_pack4(v[0], v[1], v[2], v[3], inverse), fp8_pack4(v[4], v[5], v[6], v[7], inverse)};
+    const u32x2_u c{fp8_pack4(v[0], v[1], v[2], v[3], power), fp8_pack4(v[4], v[5], v[6], v[7], power)};
     if (w.n == 8) {
       *(u32x2_u*)(codes + w.at) = c;
     } else {

@@ -32,8 +32,24 @@ __device__ __forceinline__ int fp8_scale(uint32_t bits) {
   return e > kLeastExp + 127 ? e : kLeastExp + 127;
 }
 __device__ __forceinline__ float fp8_power(int scale) { return __uint_as_float((uint32_t)scale << 23); }
-__device__ __forceinline__ float fp8_inverse(int scale) { return __uint_as_float((uint32_t)(254 - scale) << 23); }
-
+// The largest of the finite magnitudes of a lane's values, as bits: one instruction for two
+// values (three where they are signed) unless a lane of the wave has an infinity or a NaN.
+template <bool SIGNED, int N, typename V>
+__device__ __forceinline__ uint32_t finite_top(const V& x) {
+  constexpr uint32_t magnitude = SIGNED ? 0x7fffffffu : 0xffffffffu;
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < N; j += 2) {
+    const uint32_t a = __float_as_uint(x[j]) & magnitude, b = __float_as_uint(x[j + 1]) & magnitude;
+    top = max(max(top, a), b);
+  }
+  if (__ballot(top >= 0x7f800000u) != 0) {
+    top = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) top = max(top, finite_bits(x[j]));
+  }
+  return top;
+}
 // Values of a block of the largest power stay finite.
 template <int N>
 __device__ __forceinline__ void fp8_keep_finite(float (&x)[N], int scale) {
@@ -42,13 +58,15 @@ __device__ __forceinline__ void fp8_keep_finite(float (&x)[N], int scale) {
   for (int j = 0; j < N; ++j)
     if (fabsf(x[j]) > 0x1.ep127f && fabsf(x[j]) < INFINITY) x[j] = copysignf(0x1.ep127f, x[j]);
 }
-// Four values of a block, first in the lowest byte.  (The conversion gives NaN past
-// 464, so an infinity too.)
-__device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d, float inverse) {
-  int w = __builtin_amdgcn_cvt_pk_fp8_f32(a * inverse, b * inverse, 0, false);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c * inverse, d * inverse, w, true);
+// Four values of a block, first in the lowest byte.  (The conversions take the power's
+// exponent, and give NaN past 464 times it, so for an infinity too.)
+__device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d, float power) {
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  s16x2 w = {0, 0};
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, a, b, power, false);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, c, d, power, true);
+  return __builtin_bit_cast(uint32_t, w);
 }
-// (The conversion takes the power's exponent.)
 __device__ __forceinline__ void fp8_unpack4(uint32_t w, float power, float (&x)[4]) {
   const floatx2 lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, power, false);
   const floatx2 hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, power, true);

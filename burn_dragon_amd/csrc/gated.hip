@@ -353,7 +353,9 @@ __global__ __launch_bounds__(256, BIG ? 1 : 2) void gated_kernel(const GatedArgs
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) p[i][j] = q[i][j] = zero16();
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) p[i][j][r] = q[i][j][r] = ACT == RELU ? -a.th : 0.0f;
   const int nw = 64 * (w & 1), mw = 32 * NJ * (w >> 1);
   if constexpr (BIG) {
     struct {
@@ -470,27 +472,30 @@ __global__ __launch_bounds__(256, BIG ? 1 : 2) void gated_kernel(const GatedArgs
       if (ACT == RELU) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          p[i][j][r] = relu(p[i][j][r] - a.th);
-          q[i][j][r] = relu(q[i][j][r] - a.th);
+          p[i][j][r] = relu(p[i][j][r]);
+          q[i][j][r] = relu(q[i][j][r]);
         }
       }
       if (EPI == SAVE) {
         // The same 32 latents in 8 bits (those past N do not count).
         const auto keep = [&](const floatx16& v, int which) {
-          uint32_t top = 0;
+          floatx16 x = v;
+          if (n0 + nt + 32 > N) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (n0 + nt + 8 * (r >> 2) < N) top = max(top, finite_bits(v[r]));
+            for (int r = 0; r < 16; ++r)
+              if (n0 + nt + 8 * (r >> 2) >= N) x[r] = 0.0f;
+          }
+          uint32_t top = finite_top<ACT != RELU, 16>(x);
           const auto both = __builtin_amdgcn_permlane32_swap(top, top, false, false);
           top = max((uint32_t)both[0], (uint32_t)both[1]);
           const int scale = fp8_scale(top);
-          const float inverse = fp8_inverse(scale);
+          const float power = fp8_power(scale);
           uint32_t c[4];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             float f[4] = {v[4 * r], v[4 * r + 1], v[4 * r + 2], v[4 * r + 3]};
             fp8_keep_finite(f, scale);
-            c[r] = fp8_pack4(f[0], f[1], f[2], f[3], inverse);
+            c[r] = fp8_pack4(f[0], f[1], f[2], f[3], power);
           }
 #pragma unroll
           for (int r = 0; r < 2; ++r)
@@ -742,7 +747,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const GatedArgs a) 
         const int scale = fp8_scale(top);
         float f4[4] = {v[0], v[1], EACH == 4 ? v[EACH - 2] : 0.0f, EACH == 4 ? v[EACH - 1] : 0.0f};
         fp8_keep_finite(f4, scale);
-        const uint32_t c = fp8_pack4(f4[0], f4[1], f4[2], f4[3], fp8_inverse(scale));
+        const uint32_t c = fp8_pack4(f4[0], f4[1], f4[2], f4[3], fp8_power(scale));
         if (!in) return;
         if (EACH == 4) *(uint32_t*)(codes + row * N + nn) = c;
         else *(uint16_t*)(codes + row * N + nn) = (uint16_t)c;
