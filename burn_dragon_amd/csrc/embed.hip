@@ -206,10 +206,11 @@ __device__ __forceinline__ void sort_step(SortMemory& mem, int shift, int bins, 
   __syncthreads();
   int64_t keys[kOwn / 64];
   uint32_t rank[kOwn / 64];
+#pragma unroll
+  for (int q = 0; q < kOwn / 64; ++q) keys[q] = key(64 * q + lane);
   // Each round's ranks within its digit; the digit's last lane moves the count on.
 #pragma unroll
   for (int q = 0; q < kOwn / 64; ++q) {
-    keys[q] = key(64 * q + lane);
     const int digit = (int)(keys[q] >> shift) & (bins - 1);
     uint64_t same = __ballot(keys[q] >= 0);
     for (int b = 1; b < bins; b <<= 1) {
@@ -279,6 +280,12 @@ __global__ __launch_bounds__(1024) void digit_scatter_kernel(const SortArgs s) {
       }
     }
   }
+  uint32_t from[kOwn / 64];
+#pragma unroll
+  for (int q = 0; q < kOwn / 64; ++q) {
+    const int64_t i = i0 + 64 * q + ((int)threadIdx.x & 63);
+    from[q] = s.order && i < s.n ? s.order[i] : (uint32_t)i;
+  }
   sort_step(
       mem, s.shift, s.bins, [&](int j) { return i0 + j < s.n ? (int64_t)key_of(s, i0 + j) : (int64_t)-1; },
       [&](SortMemory& m) {
@@ -295,7 +302,7 @@ __global__ __launch_bounds__(1024) void digit_scatter_kernel(const SortArgs s) {
       },
       [&](int j, uint32_t key, uint32_t place) {
         s.keys_out[place] = key;
-        s.order_out[place] = s.order ? s.order[i0 + j] : (uint32_t)(i0 + j);
+        s.order_out[place] = from[j >> 6];
       });
 }
 
