@@ -981,6 +981,9 @@ static bdh_status gated_checks(const bdh_layer_plan* plan, const void* current, 
   if (p.batch > most || p.time > most || p.batch * p.time > most || p.heads > 512 || p.latent > (int64_t)1 << 20 ||
       p.embd > (int64_t)1 << 16 || p.heads * p.latent > (int64_t)1 << 24 || p.batch * p.time > (((int64_t)1 << 35) - 1) / (p.heads * p.latent))
     return fail(BDH_UNSUPPORTED, "too large for one launch");
+  // (Short heads: tiles of 128 tokens by 128 of one head's latents.)
+  if ((p.batch * p.time + 127) / 128 * p.heads * ((p.latent + 127) / 128) > most)
+    return fail(BDH_UNSUPPORTED, "too large for one launch");
   bdh_gated_options o{BDH_RELU, 0.0f, nullptr};
   if (options) o = *options;
   if (o.activation != BDH_RELU && o.activation != BDH_SILU && o.activation != BDH_GELU)

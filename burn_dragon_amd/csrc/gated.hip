@@ -135,10 +135,11 @@ __device__ __forceinline__ void fill(char* lds, uint32_t tile, int w, int lane, 
 // 96 KB in LDS for the same products, not 144, and loads 32 KB, not 48.
 //   load(inside, s, stage, j) this wave's j-th of LOADS loads of step s; not inside: zeros
 //                             past k's end
-//   read(set, i, stage, kk)   fragment i of eight of half kk
-//   multiply(set, i)          product i of 16
+//   read(set, i, stage, kk)   fragment i of half kk (as many as loads)
+//   multiply(set, i)          product i of PRODUCTS
+// (12 products, 7 loads and fragments: tiles of three quarters, 28 KB a step.)
 constexpr int BIG_STAGE = 32768, BIG_STAGES = 5, BIG_LOADS = 8;
-template <class Load, class Read, class Multiply>
+template <int LOADS = BIG_LOADS, int PRODUCTS = 16, class Load, class Read, class Multiply>
 __device__ __forceinline__ void big_loop(int s0, int s1, int K, Load&& load, Read&& read, Multiply&& multiply) {
   if (s0 >= s1) return;
   const std::false_type no{};
@@ -146,37 +147,46 @@ __device__ __forceinline__ void big_loop(int s0, int s1, int K, Load&& load, Rea
   for (int q = 0; q < 4; ++q)
     if (s0 + q < s1) {
 #pragma unroll
-      for (int j = 0; j < BIG_LOADS; ++j) load(no, s0 + q, q, j);
+      for (int j = 0; j < LOADS; ++j) load(no, s0 + q, q, j);
     }
   wait_barrier<0>();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) read(0, i, 0, 0);
+  for (int i = 0; i < LOADS; ++i) read(0, i, 0, 0);
   int stage = 0, s = s0;
-  // Fragments after the products 0, 1, 3, 4, 6, 7, 9, 10, so that the last of them has
-  // five products' time; loads after the others.
-  const auto is_read = [](int i) { return i % 3 != 2 && i < 11; };
+  // Fragments after the products 0, 1, 3, 4, 6, 7, 9, 10 (0, 1, 2, 4, 5, 6, 8), so that the
+  // last of them has five (three) products' time; loads after the others.
+  static_assert((LOADS == 8 && PRODUCTS == 16) || (LOADS == 7 && PRODUCTS == 12), "the places of reads and loads");
+  constexpr int GROUP = LOADS == 8 ? 3 : 4, FREE = PRODUCTS - LOADS;
+  const auto is_read = [](int i) { return i % GROUP != GROUP - 1 && i < (LOADS == 8 ? 11 : 9); };
+  const auto read_of = [](int i) { return i - i / GROUP; };
+  const auto other_of = [](int i) {
+    int n = 0;
+    for (int k = 0; k < i; ++k) n += k % GROUP == GROUP - 1 || k >= (LOADS == 8 ? 11 : 9);
+    return n;
+  };
   const auto step = [&](auto inside) {
     constexpr bool INSIDE = decltype(inside)::value;
     // In flight: the steps s + 2 and s + 3, where they are whole.
-    if (INSIDE || (s + 3 < s1 && (s + 4) * BK <= K)) wait_barrier<2 * BIG_LOADS>();
+    if (INSIDE || (s + 3 < s1 && (s + 4) * BK <= K)) wait_barrier<2 * LOADS>();
     else wait_barrier<0>();
     const int next = stage == BIG_STAGES - 1 ? 0 : stage + 1, free = stage == 0 ? BIG_STAGES - 1 : stage - 1;
     if (!INSIDE && s + 4 < s1) {
 #pragma unroll
-      for (int j = 0; j < BIG_LOADS; ++j) load(no, s + 4, free, j);
+      for (int j = 0; j < LOADS; ++j) load(no, s + 4, free, j);
     }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < PRODUCTS; ++i) {
       multiply(0, i);
-      if (is_read(i)) read(1, (2 * i + 1) / 3, stage, 1);
-      else if (INSIDE) load(inside, s + 4, free, i < 12 ? i / 3 : i - 8);
+      if (is_read(i)) read(1, read_of(i), stage, 1);
+      else if (INSIDE) load(inside, s + 4, free, other_of(i));
       __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < PRODUCTS; ++i) {
       multiply(1, i);
-      if (is_read(i)) read(0, (2 * i + 1) / 3, next, 0);  // (after the last step: any)
+      if (is_read(i)) read(0, read_of(i), next, 0);  // (after the last step: any)
+      else if (INSIDE && FREE + other_of(i) < LOADS) load(inside, s + 4, free, FREE + other_of(i));
       __builtin_amdgcn_sched_barrier(0);
     }
     stage = next;
@@ -300,15 +310,15 @@ __device__ __forceinline__ u32x2 join_halves(uint32_t a, uint32_t b) {
 }
 
 // A workgroup: 128 latents (n) of a head by 128 tokens (m), a wave 64 by 64 of both
-// products.  BIG (no context): by 256 tokens, a wave 64 by 128, in big_loop.
-template <int ACT, int EPI, bool CTX, bool BIG>
-__global__ __launch_bounds__(256, BIG ? 1 : 2) void gated_kernel(const GatedArgs a) {
+// products.  NJ 3 and 4 (no context): by 192 and 256 tokens, a wave 64 by 96 and 128, in
+// big_loop.
+template <int ACT, int EPI, bool CTX, int NJ>  // NJ: 32 tokens each of a wave
+__global__ __launch_bounds__(256, NJ > 2 ? 1 : 2) void gated_kernel(const GatedArgs a) {
+  constexpr bool BIG = NJ > 2;
   static_assert(!(CTX && BIG), "a context's tiles do not fit");
-  constexpr int NJ = BIG ? 4 : 2;  // 32 tokens each of a wave
   typedef Tile<MC, 128> W;
   typedef Tile<KC, 64 * NJ> X;
   constexpr int STAGE = 2 * W::BYTES + (CTX ? 2 : 1) * X::BYTES, STAGES = BIG ? BIG_STAGES : CTX ? 2 : 3;
-  static_assert(!BIG || (STAGE == BIG_STAGE && 2 * W::LOADS + X::LOADS == BIG_LOADS), "big_loop's stages");
   __shared__ __attribute__((aligned(16))) char lds[STAGES * STAGE];
   const int lane = threadIdx.x & 63, w = wave_id();
   const int D = (int)a.D, N = (int)a.N, M = (int)a.M;
@@ -359,7 +369,7 @@ __global__ __launch_bounds__(256, BIG ? 1 : 2) void gated_kernel(const GatedArgs
   const int nw = 64 * (w & 1), mw = 32 * NJ * (w >> 1);
   if constexpr (BIG) {
     struct {
-      bf16x8 u[2], g[2], x[4];
+      bf16x8 u[2], g[2], x[NJ];
     } f[2];
     const char* const w_base[2] = {(const char*)(a.up + (int64_t)h * D * N + n0),
                                    (const char*)(a.gate + (int64_t)h * D * N + n0)};
@@ -375,7 +385,7 @@ __global__ __launch_bounds__(256, BIG ? 1 : 2) void gated_kernel(const GatedArgs
         x_at[j] = 2u * (uint32_t)((m0 + m < M ? m : M - 1 - m0) * D + X::chunk(w, lane) * 8);
       }
     }
-    big_loop(
+    big_loop<2 * W::LOADS + X::LOADS, 4 * NJ>(
         0, steps, D,
         [&](auto inside, int s, int stage, int j) {
           const int k0 = s * BK;
@@ -1313,23 +1323,33 @@ ProductPlan plan_products(int64_t M, int64_t H, int64_t N, int64_t D, bool ctx, 
   return best;
 }
 
-// Whether the projections take the larger tiles: rounds of workgroups (between the whole
-// and the broken number of them) times steps and ends, us as measured (M 3003, 4096 and 8192,
-// N 4096 and 8192, D 256 to 2048).  The ends (activation, 8 bits, memory) run beside another
-// workgroup's products only in the smaller ones.
+// The tokens of the projections' tiles: what takes the least time by rounds of workgroups
+// (between the whole and the broken number of them) times a step's and the ends' us, as
+// measured (M 1024 to 8192, N 4096 and 8192, D 256 to 2048).  The ends (activation, 8 bits,
+// memory) run beside another workgroup's products only in the smallest.  Over those 180 cases
+// 0.6 % off the fastest in the mean, 19 % at worst (3003 tokens of 4096, D 256: 33 us in 128
+// tokens, 40 in 192); without tiles of 192 2.9 % in the mean (D 1024: 69 us in 192, 76 in 128,
+// 79 in 256).
 template <int EPI>
-bool big_projections(const GatedArgs& a, int act) {
-  if (a.c) return false;
-  constexpr double ends[2][3][3] = {{{6.5, 6.2, 14.7}, {13.5, 12.7, 21.5}, {14.0, 13.8, 21.9}},
-                                    {{9.5, 8.3, 23.6}, {22.0, 23.0, 39.0}, {20.6, 20.0, 35.5}}};
-  double us[2];
-  for (int big = 0; big < 2; ++big) {
-    const int64_t slots = (int64_t)device_cus() * (big ? 1 : 2), m = big ? 256 : 128;
+int projection_tokens(const GatedArgs& a, int act) {
+  if (a.c) return 128;
+  constexpr double step[3] = {1.07, 0.63, 0.82};
+  constexpr double ends[3][3][3] = {{{6.3, 6.5, 13.5}, {11.6, 11.0, 18.5}, {14.5, 14.0, 21.0}},
+                                    {{8.0, 7.5, 18.3}, {13.5, 13.5, 26.5}, {15.0, 15.0, 26.8}},
+                                    {{9.8, 8.0, 22.2}, {17.8, 19.5, 36.9}, {20.0, 19.5, 35.5}}};
+  int best = 128;
+  double least = 1e30;
+  for (int k = 0; k < 3; ++k) {
+    const int64_t slots = (int64_t)device_cus() * (k == 0 ? 2 : 1), m = 128 + 64 * k;
     const int64_t tiles = (a.N + 127) / 128 * a.H * ((a.M + m - 1) / m);
     const double rounds = 0.5 * ((double)((tiles + slots - 1) / slots) + (double)tiles / (double)slots);
-    us[big] = rounds * ((double)((a.D + BK - 1) / BK) * (big ? 0.82 : 1.07) + ends[big][EPI][act]);
+    const double us = rounds * ((double)((a.D + BK - 1) / BK) * step[k] + ends[k][EPI][act]);
+    if (us < least) {
+      least = us;
+      best = (int)m;
+    }
   }
-  return us[1] < us[0];
+  return best;
 }
 
 template <int ACT, int EPI>
@@ -1341,15 +1361,19 @@ void launch_projections(const GatedArgs& a, hipStream_t st) {
       return;
     }
   }
-  if (big_projections<EPI>(a, ACT)) {
+  const int tokens = projection_tokens<EPI>(a, ACT);
+  if (tokens != 128) {
     GatedArgs b = a;
-    b.order = tile_order((int64_t)cdiv(a.N, 128) * a.H, cdiv(a.M, 256));
-    hipLaunchKernelGGL((gated_kernel<ACT, EPI, false, true>), dim3(grid_of(b.order)), dim3(256), 0, st, b);
+    b.order = tile_order((int64_t)cdiv(a.N, 128) * a.H, cdiv(a.M, tokens));
+    if (tokens == 256)
+      hipLaunchKernelGGL((gated_kernel<ACT, EPI, false, 4>), dim3(grid_of(b.order)), dim3(256), 0, st, b);
+    else
+      hipLaunchKernelGGL((gated_kernel<ACT, EPI, false, 3>), dim3(grid_of(b.order)), dim3(256), 0, st, b);
     return;
   }
   const dim3 grid(grid_of(a.order));
-  if (a.c) hipLaunchKernelGGL((gated_kernel<ACT, EPI, true, false>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((gated_kernel<ACT, EPI, false, false>), grid, dim3(256), 0, st, a);
+  if (a.c) hipLaunchKernelGGL((gated_kernel<ACT, EPI, true, 2>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((gated_kernel<ACT, EPI, false, 2>), grid, dim3(256), 0, st, a);
 }
 template <int EPI>
 void launch_projections(const GatedArgs& a, int act, hipStream_t st) {

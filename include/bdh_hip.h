@@ -419,7 +419,8 @@ bdh_status bdh_activations_restore(const void* codes, const void* scales, int64_
  * up_codes .. gate_scales (all four or none): p and q (with BDH_RELU after the ReLU, before
  * the mask) in 8 bits for the backward, as bdh_activations_save lays out [B*T*H, N].
  * D and N multiples of 8, up to 2^16 and 2^20; B*T up to 2^22, heads up to 512, H*N up to
- * 2^24, B*T*H*N below 2^35.  Tensors 16-byte aligned.  Outputs share no memory with inputs. */
+ * 2^24, B*T*H*N below 2^35; with N and B*T counted up to multiples of 128 up to 2^36.
+ * Tensors 16-byte aligned.  Outputs share no memory with inputs. */
 typedef enum { BDH_RELU = 0, BDH_SILU = 1, BDH_GELU = 2 } bdh_activation;
 typedef struct {
   int32_t activation;        /* bdh_activation */

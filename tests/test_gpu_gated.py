@@ -134,6 +134,13 @@ def test_deep_and_wide():
     run(1, 5, 1, 40, 8200, "gelu", False)
 
 
+# Without a context these calls go in tiles of 192 or 256 tokens (some kinds in 128).
+@pytest.mark.parametrize("T,D,N,act", [(1499, 520, 4088, "relu"), (1499, 1032, 4088, "gelu"), (1537, 2056, 4096, "silu"),
+                                       (1001, 1048, 8184, "relu"), (1023, 1040, 8192, "silu"), (1023, 1040, 8192, "gelu")])
+def test_larger_tiles(T, D, N, act):
+    run(1, T, 1, D, N, act, False, 0.25 if act == "relu" else 0.0, act == "relu")
+
+
 # The backward of saved values without the projections' gradients in memory begins at 2^23 of them.
 @pytest.mark.parametrize("B,T,H,D,N,act,context,masked", [
     (3, 375, 1, 200, 7504, "relu", True, True), (1, 4097, 2, 72, 1032, "relu", True, False),

@@ -141,6 +141,13 @@ def test_gated_block_vjp(kw, status, why):
     assert why in _lib.last_error()
 
 
+def test_more_tiles_than_a_launch_has():
+    kw = dict(batch=1 << 11, time=1 << 11, heads=512, latent=8)
+    for names, call in ((FWD, _lib.load().bdh_gated_block_fwd), (BWD, _lib.load().bdh_gated_block_vjp)):
+        assert _gated(dict(kw), names, call) == _lib.BDH_UNSUPPORTED
+        assert "large" in _lib.last_error()
+
+
 def test_python_surface_without_a_device():
     torch = pytest.importorskip("torch")
     if torch.cuda.is_available():
