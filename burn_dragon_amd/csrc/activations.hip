@@ -4,7 +4,8 @@
 //
 // Four lanes hold a block, eight neighbours each, so a block's largest magnitude
 // takes two exchanges and a wave reads and writes runs of 512 values.  Bound by the
-// bytes: 3 (5) of bf16 (f32) a value to save, 3 (5) to restore.
+// bytes: 3 (5) of bf16 (f32) a value to save, 3 (5) to restore (16384 rows of 8192 bf16: saved
+// in 74-86 us, 4.8-5.5 TB/s, restored in 65, 6.2 TB/s).
 #include "bdh_fp8.h"
 #include "bdh_internal.h"
 
@@ -112,6 +113,7 @@ __global__ __launch_bounds__(256) void restore_kernel(const uint8_t* __restrict_
   }
 }
 
+// (8192 workgroups are four rounds of the chip's; past that each goes on to further blocks.)
 unsigned grid_of(int64_t total) {
   const int64_t g = (total + 255) / 256;
   return (unsigned)(g < 8192 ? g : 8192);

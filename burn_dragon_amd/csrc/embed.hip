@@ -12,6 +12,12 @@
 // that lie within it.  An id that runs on into the next runs leaves partial sums,
 // which a second launch joins in their order.  The rows without a token are cleared
 // by the sort's launches beside their own work.
+//
+// Bound by the bytes (rows in, rows out) where there are many tokens, else by the chain of
+// dependent launches: 65536 tokens of 1024 bf16 columns of a table of 32000, 31 us (4.3 TB/s
+// of results); the gradient of 32768 such tokens to 131072 rows, two sort passes of 12 + 18
+// (they clear 268 MB), sums 32 (67 MB read in the order of the ids, the met rows written)
+// and join 11 us; of 16384 tokens to 256 rows of 256 f32 columns, 3 + 10 + 6 + 8 us.
 #include <type_traits>
 
 #include "bdh_internal.h"
@@ -123,8 +129,9 @@ struct Row {
   }
 };
 
-// A wave takes `each` neighbouring tokens, their rows asked for together: with one token a
-// wave, what counted was the wait for its id, then for its row (65536 tokens, D 1024, bf16).
+// A wave takes EACH neighbouring tokens, their rows asked for together: with one token a
+// wave, what counted was the wait for its id, then for its row (65536 tokens, D 1024, bf16:
+// 52 us a call, with two 41).
 template <typename T, int VEC, int PER, int EACH, bool NORM>
 __global__ __launch_bounds__(256) void embed_kernel(const EmbedArgs a) {
   const int64_t i0 = ((int64_t)blockIdx.x * 4 + wave_id()) * EACH;

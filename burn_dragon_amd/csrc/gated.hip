@@ -132,7 +132,8 @@ __device__ __forceinline__ void fill(char* lds, uint32_t tile, int w, int lane, 
 // step s - 1, and fragments are read half a step ahead of their products, a fragment or
 // a load after each product: so LDS, loads and the matrix cores
 // run side by side in one wave.  Against two workgroups a CU of half the sums, a step moves
-// 96 KB in LDS for the same products, not 144, and loads 32 KB, not 48.
+// 96 KB in LDS for the same products, not 144, and loads 32 KB, not 48 (4096 tokens of 8192
+// latents, D 2048: 279 -> 218-228 us, 1.2-1.26 PFLOP/s).
 //   load(inside, s, stage, j) this wave's j-th of LOADS loads of step s; not inside: zeros
 //                             past k's end
 //   read(set, i, stage, kk)   fragment i of half kk (as many as loads)
@@ -473,7 +474,9 @@ __global__ __launch_bounds__(256, NJ > 2 ? 1 : 2) void gated_kernel(const GatedA
   // A lane has token mw + 32 j + (lane & 31) and, of 32 latents, 8 r + 4 (lane >> 5)
   // ..+3 for r of 0..3.  64 of the tile's tokens at a time (j) go through LDS, so that
   // memory sees whole rows of 128 latents, stored past the caches, which they would only
-  // empty (16384 tokens, 4 heads of 8192, D 256, saved: 1400 -> 1200 us).
+  // empty (16384 tokens, 4 heads of 8192, D 256, saved: 1400 -> 1200 us; with the conversions
+  // of bdh_fp8.h 990-1040: 2.1 GB of results at 2.1 TB/s beside 0.55 PFLOP/s of products, which
+  // eight steps of k a tile leave waiting for their first loads and the ends).
   constexpr int VP = 272, CP = 144;  // row pitches in bytes (bank spread)
   char* const vals = lds;            // [64][VP]: out; the gradient, then dp
   char* const more = lds + 64 * VP;  // [64][VP]: dq; or [2][64][CP] codes, [2][64][4] scales
@@ -658,7 +661,8 @@ __global__ __launch_bounds__(256) void gated_grads_kernel(const GatedArgs a) {
 // --- few tokens -------------------------------------------------------------------------
 // Up to 64 tokens are bound by the weights, 4 D bytes a latent, each read once: a workgroup
 // has 16 VEC latents of a head and all tokens, its eight waves share the k's, and the
-// weights go from memory to registers.  A lane reads VEC neighbours of eight rows of k and
+// weights go from memory to registers (one token, 4 heads of 8192 latents, D 256: 5.8 us, 5.8
+// TB/s; 64 tokens of 8192, D 2048: 17 us, 3.9 TB/s).  A lane reads VEC neighbours of eight rows of k and
 // pairs the rows (one v_perm for two values), which leaves it with a fragment for each of
 // its latents: 16 lanes hold every VEC-th latent of the tile.
 constexpr int kFewTokens = 64, kFewWaves = 8;
@@ -816,7 +820,8 @@ void launch_few_as(const GatedArgs& a, hipStream_t st) {
 }
 template <int ACT, bool SAVED, bool CTX>
 void launch_few(const GatedArgs& a, hipStream_t st) {
-  // Tiles of 128 latents (whole lines a row) where they fill the chip.
+  // Tiles of 128 latents (whole lines a row) where they fill the chip; more tokens leave
+  // registers for two latents a lane.
   if (a.M <= 16 && a.H * a.N >= 32768) launch_few_as<ACT, SAVED, CTX, 8, 1>(a, st);
   else if (a.M <= 16) launch_few_as<ACT, SAVED, CTX, 2, 1>(a, st);
   else if (a.M <= 32) launch_few_as<ACT, SAVED, CTX, 2, 2>(a, st);
@@ -967,7 +972,8 @@ __device__ __forceinline__ void product_tile(const ProductArgs& a, char* lds, in
       const int i = j - A::LOADS;
       const bool in = decltype(inside)::value || k0 + (WHAT == INPUTS ? bc : B::row(i, w, lane)) < K;
       if (WHAT == WEIGHTS && apart)
-        fill_one<B>(lds, base + A::BYTES, w, lane, i, in, b_base + 2 * a.c_rows.at((uint32_t)(k0 + B::row(i, w, lane))) + b_at[i]);
+        fill_one<B>(lds, base + A::BYTES, w, lane, i, in,
+                    b_base + 2 * a.c_rows.at((uint32_t)(k0 + B::row(i, w, lane))) + b_at[i]);
       else
         fill_one<B>(lds, base + A::BYTES, w, lane, i, inside, in,
                     b_base + 2 * (WHAT == INPUTS ? (int64_t)k0 : (int64_t)k0 * D), b_at[i]);
@@ -1043,6 +1049,9 @@ __global__ __launch_bounds__(256, BIG ? 1 : 2) void product_kernel(const Product
 // the tiles' direct loads a thread asks for eight neighbours of the gradient and of both
 // codes a step, four steps ahead: WEIGHTS of 32 tokens by 128 latents; INPUTS of 64 tokens
 // by the 64 latents of two steps, so that memory sees 128 (64) bytes of a row.
+// 16384 tokens, 4 heads of 8192 latents, D 256: 990 and 690 us (0.55 and 0.8 PFLOP/s); a
+// step moves 146 KB in LDS, 1150 cycles beside 1024 of products, and INPUTS waits for the
+// gradients and codes besides, 64 bytes of a row at a time.
 template <int WHAT, int ACT, bool MASK>
 __global__ __launch_bounds__(512, 1) void fused_kernel(const ProductArgs a, const GatedArgs g) {
   constexpr bool IN = WHAT == INPUTS;
@@ -1326,14 +1335,15 @@ int64_t makespan(int64_t n1, int64_t l1, int64_t n2, int64_t l2, int64_t slots) 
 // Tiles and parts of k of the backward's products: what takes the least time by the steps of
 // the longest row of tiles on a slot and by the bytes of the partial sums.  Measured: a step of
 // 256 by 256 tiles (one a CU) 0.84 us, of 256 by 128 (two a CU) 1.11, a tile's ends about
-// six steps; sums 4.5 TB/s and a launch.  (3003 tokens of 4096 latents, D 1024: 160 -> 114 us.)
+// six steps; sums 4.5 TB/s and a launch.  (3003 tokens of 4096 latents, D 1024: 160 -> 109 us.)
 struct ProductPlan {
   int in_parts, w_parts;
   double us;
 };
 ProductPlan plan_products(int64_t M, int64_t H, int64_t N, int64_t D, bool ctx, bool big) {
   const int64_t slots = (int64_t)device_cus() * (big ? 1 : 2), b = big ? 256 : 128;
-  const int64_t in_tiles = (D + 255) / 256 * ((M + b - 1) / b) * 2 * H, w_tiles = (N + 255) / 256 * ((D + b - 1) / b) * 2 * H;
+  const int64_t in_tiles = (D + 255) / 256 * ((M + b - 1) / b) * 2 * H;
+  const int64_t w_tiles = (N + 255) / 256 * ((D + b - 1) / b) * 2 * H;
   const int64_t in_steps = (N + BK - 1) / BK, w_steps = (M + BK - 1) / BK;
   ProductPlan best{1, 1, 1e30};
   for (const int pi : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
