@@ -15,9 +15,9 @@
 //
 // Bound by the bytes (rows in, rows out) where there are many tokens, else by the chain of
 // dependent launches: 65536 tokens of 1024 bf16 columns of a table of 32000, 31 us (4.3 TB/s
-// of results); the gradient of 32768 such tokens to 131072 rows, two sort passes of 12 + 18
-// (they clear 268 MB), sums 32 (67 MB read in the order of the ids, the met rows written)
-// and join 11 us; of 16384 tokens to 256 rows of 256 f32 columns, 3 + 10 + 6 + 8 us.
+// of results); the gradient of 32768 such tokens to 131072 rows, 94 us: two sort passes, which
+// clear 268 MB, sums 32 (67 MB read in the order of the ids, the met rows written) and
+// join 11; of 16384 tokens to 256 rows of 256 f32 columns, 23 us in four launches.
 #include <type_traits>
 
 #include "bdh_internal.h"
@@ -159,7 +159,10 @@ __global__ __launch_bounds__(256) void embed_kernel(const EmbedArgs a) {
 
 // --- the order of the positions by id -----------------------------------------------
 constexpr int kMostBins = 512;                              // a pass's digits
-constexpr int kWaves = 16, kOwn = 256, kItems = kWaves * kOwn;  // a workgroup's positions, 256 a wave
+// A workgroup's positions: 16 waves have ROUNDS times 64 neighbours each.
+constexpr int kWaves = 16, kMostRounds = 4;
+constexpr int items(int rounds) { return 64 * rounds * kWaves; }
+constexpr int kSmall = items(kMostRounds);  // of the sort in one launch
 
 // The key of position i: its id, or vocab (past all ids) where it is none.
 __device__ __forceinline__ uint32_t key_of(const SortArgs& s, int64_t i) {
@@ -182,14 +185,15 @@ __device__ void clear_share(const SortArgs& s, int block, int blocks) {
 }
 
 // counts[workgroup][digit].
+template <int ROUNDS>
 __global__ __launch_bounds__(1024) void digit_counts_kernel(const SortArgs s) {
   if ((int)blockIdx.x >= s.blocks) return clear_share(s, (int)blockIdx.x - s.blocks, (int)gridDim.x - s.blocks);
   __shared__ uint32_t bins[kMostBins];
   for (int d = threadIdx.x; d < s.bins; d += 1024) bins[d] = 0;
   __syncthreads();
-  const int64_t i0 = (int64_t)blockIdx.x * kItems;
+  const int64_t i0 = (int64_t)blockIdx.x * items(ROUNDS);
 #pragma unroll
-  for (int j = 0; j < kItems; j += 1024) {
+  for (int j = 0; j < items(ROUNDS); j += 1024) {
     const int64_t i = i0 + j + threadIdx.x;
     if (i < s.n) atomicAdd(&bins[(key_of(s, i) >> s.shift) & (s.bins - 1)], 1u);
   }
@@ -197,27 +201,27 @@ __global__ __launch_bounds__(1024) void digit_counts_kernel(const SortArgs s) {
   for (int d = threadIdx.x; d < s.bins; d += 1024) s.counts[(int64_t)blockIdx.x * s.bins + d] = bins[d];
 }
 
-// The places of a workgroup's positions, stable: wave w has 256 neighbours, four rounds
-// of 64.  key(j), 0 <= j < 256 of the lane's wave: -1 where there is none.  first(digit):
+// The places of a workgroup's positions, stable: wave w has 64 ROUNDS neighbours.
+// key(j), 0 <= j < 64 ROUNDS of the lane's wave: -1 where there is none.  first(digit):
 // the place of the workgroup's first one.  put(j, key, place).
 struct SortMemory {
   uint32_t at[kWaves][kMostBins];  // counts, then next places
   uint32_t total[kMostBins];
   uint32_t sums[8];
 };
-template <typename Key, typename First, typename Put>
+template <int ROUNDS, typename Key, typename First, typename Put>
 __device__ __forceinline__ void sort_step(SortMemory& mem, int shift, int bins, const Key& key, const First& first,
                                           const Put& put) {
   const int lane = threadIdx.x & 63, w = wave_id();
   for (int d = threadIdx.x; d < kWaves * kMostBins; d += 1024) (&mem.at[0][0])[d] = 0;
   __syncthreads();
-  int64_t keys[kOwn / 64];
-  uint32_t rank[kOwn / 64];
+  int64_t keys[ROUNDS];
+  uint32_t rank[ROUNDS];
 #pragma unroll
-  for (int q = 0; q < kOwn / 64; ++q) keys[q] = key(64 * q + lane);
+  for (int q = 0; q < ROUNDS; ++q) keys[q] = key(64 * q + lane);
   // Each round's ranks within its digit; the digit's last lane moves the count on.
 #pragma unroll
-  for (int q = 0; q < kOwn / 64; ++q) {
+  for (int q = 0; q < ROUNDS; ++q) {
     const int digit = (int)(keys[q] >> shift) & (bins - 1);
     uint64_t same = __ballot(keys[q] >= 0);
     for (int b = 1; b < bins; b <<= 1) {
@@ -245,7 +249,7 @@ __device__ __forceinline__ void sort_step(SortMemory& mem, int shift, int bins, 
   }
   __syncthreads();
 #pragma unroll
-  for (int q = 0; q < kOwn / 64; ++q)
+  for (int q = 0; q < ROUNDS; ++q)
     if (keys[q] >= 0)
       put(64 * q + lane, (uint32_t)keys[q], mem.at[w][(int)(keys[q] >> shift) & (bins - 1)] + rank[q]);
   __syncthreads();
@@ -268,12 +272,13 @@ __device__ __forceinline__ void scan_digits(SortMemory& mem, uint32_t own, uint3
   __syncthreads();
 }
 
+template <int ROUNDS>
 __global__ __launch_bounds__(1024) void digit_scatter_kernel(const SortArgs s) {
   if ((int)blockIdx.x >= s.blocks) return clear_share(s, (int)blockIdx.x - s.blocks, (int)gridDim.x - s.blocks);
   __shared__ SortMemory mem;
   __shared__ uint32_t half[2][kMostBins];
   const int mine = (int)blockIdx.x;
-  const int64_t i0 = (int64_t)mine * kItems + wave_id() * kOwn;
+  const int64_t i0 = (int64_t)mine * items(ROUNDS) + wave_id() * 64 * ROUNDS;
   // Of a digit: all its positions, and those of earlier workgroups, by two threads.
   uint32_t total = 0, before = 0;
   {
@@ -287,13 +292,13 @@ __global__ __launch_bounds__(1024) void digit_scatter_kernel(const SortArgs s) {
       }
     }
   }
-  uint32_t from[kOwn / 64];
+  uint32_t from[ROUNDS];
 #pragma unroll
-  for (int q = 0; q < kOwn / 64; ++q) {
+  for (int q = 0; q < ROUNDS; ++q) {
     const int64_t i = i0 + 64 * q + ((int)threadIdx.x & 63);
     from[q] = s.order && i < s.n ? s.order[i] : (uint32_t)i;
   }
-  sort_step(
+  sort_step<ROUNDS>(
       mem, s.shift, s.bins, [&](int j) { return i0 + j < s.n ? (int64_t)key_of(s, i0 + j) : (int64_t)-1; },
       [&](SortMemory& m) {
         if (threadIdx.x >= kMostBins) {
@@ -317,17 +322,17 @@ __global__ __launch_bounds__(1024) void digit_scatter_kernel(const SortArgs s) {
 __global__ __launch_bounds__(1024) void sort_small_kernel(const SortArgs s) {
   if (blockIdx.x >= 1) return clear_share(s, (int)blockIdx.x - 1, (int)gridDim.x - 1);
   __shared__ SortMemory mem;
-  __shared__ uint32_t keys[kItems], order[kItems];
-  const int i0 = wave_id() * kOwn, n = (int)s.n;
+  __shared__ uint32_t keys[kSmall], order[kSmall];
+  const int i0 = wave_id() * 64 * kMostRounds, n = (int)s.n;
   for (int pass = 0; pass < s.passes; ++pass) {
     const bool last = pass + 1 == s.passes;
-    uint32_t from[kOwn / 64];
+    uint32_t from[kMostRounds];
 #pragma unroll
-    for (int q = 0; q < kOwn / 64; ++q) {
+    for (int q = 0; q < kMostRounds; ++q) {
       const int i = i0 + 64 * q + ((int)threadIdx.x & 63);
       from[q] = pass > 0 && i < n ? order[i] : (uint32_t)i;
     }
-    sort_step(
+    sort_step<kMostRounds>(
         mem, pass * s.shift, s.bins,
         [&](int j) {
           if (i0 + j >= n) return (int64_t)-1;
@@ -558,7 +563,11 @@ bdh_status embed_tokens_vjp(EmbedArgs a, hipStream_t st, uint64_t* launches) {
   int bits = 1;
   while (a.vocab >> bits) ++bits;  // of the keys 0 .. vocab
   const int passes = (bits + 8) / 9, per_pass = (bits + passes - 1) / passes;
-  const int64_t blocks = cdiv(a.n, kItems);
+  // Short sorts have one round a workgroup, since what counts is a workgroup's chain; many
+  // workgroups each read all counts (us a call, one round / four: 16384 tokens of 256 ids 20 / 24,
+  // of 131072 44 / 54; 262144 88 / 86 and 148 / 150; 1048576 418 / 346 and 580 / 421).
+  const int rounds = a.n <= kSmall || a.n > 131072 ? kMostRounds : 1;
+  const int64_t blocks = cdiv(a.n, items(rounds));
   a.run = a.n <= 32768 ? 16 : 32;
   const int64_t runs = cdiv(a.n, a.run);
   const int64_t words = 4 * a.n + (blocks << per_pass);
@@ -598,8 +607,13 @@ bdh_status embed_tokens_vjp(EmbedArgs a, hipStream_t st, uint64_t* launches) {
       q.shift = p * per_pass;
       q.keys_out = keys[p & 1];
       q.order_out = order[p & 1];
-      hipLaunchKernelGGL(digit_counts_kernel, grid(), dim3(1024), 0, st, q);
-      hipLaunchKernelGGL(digit_scatter_kernel, grid(), dim3(1024), 0, st, q);
+      if (rounds == 1) {
+        hipLaunchKernelGGL(digit_counts_kernel<1>, grid(), dim3(1024), 0, st, q);
+        hipLaunchKernelGGL(digit_scatter_kernel<1>, grid(), dim3(1024), 0, st, q);
+      } else {
+        hipLaunchKernelGGL(digit_counts_kernel<kMostRounds>, grid(), dim3(1024), 0, st, q);
+        hipLaunchKernelGGL(digit_scatter_kernel<kMostRounds>, grid(), dim3(1024), 0, st, q);
+      }
       q.keys = q.keys_out;
       q.order = q.order_out;
     }

@@ -210,3 +210,9 @@ def test_refusals():
             call()
     with pytest.raises(Exception, match="finite"):
         bd.embed_tokens(tokens, table, scale=float("inf"))
+
+
+# Tokens at the borders of a workgroup's share of the sort, in two passes.
+@pytest.mark.parametrize("n", [4096, 4097, 5119, 5120, 5121, 131072, 131073])
+def test_vjp_borders_of_the_sort(n):
+    run_vjp(n, 1000, 4, "float32", False, "uniform")
