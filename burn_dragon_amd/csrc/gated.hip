@@ -341,8 +341,8 @@ __device__ __forceinline__ u32x2 join_halves(uint32_t a, uint32_t b) {
 }
 
 // A workgroup: 128 latents (n) of a head by 128 tokens (m), a wave 64 by 64 of both
-// products.  NJ 3 and 4 (no context): by 192 and 256 tokens, a wave 64 by 96 and 128, in
-// big_loop.
+// products.  NJ 1: by 64 tokens, for calls of few tiles.  NJ 3 and 4 (no context): by 192
+// and 256 tokens, a wave 64 by 96 and 128, in big_loop.
 template <int ACT, int EPI, bool CTX, int NJ>  // NJ: 32 tokens each of a wave
 __global__ __launch_bounds__(256, NJ > 2 ? 1 : 2) void gated_kernel(const GatedArgs a) {
   constexpr bool BIG = NJ > 2;
@@ -445,29 +445,29 @@ __global__ __launch_bounds__(256, NJ > 2 ? 1 : 2) void gated_kernel(const GatedA
   issue(0, 0);
   if (STAGES == 3 && steps > 1) issue(1, 1);
   for (int s = 0, stage = 0; s < steps; ++s) {
-    if (STAGES == 3 && s + 1 < steps && (s + 2) * BK <= D) wait_barrier<6>();
+    if (STAGES == 3 && s + 1 < steps && (s + 2) * BK <= D) wait_barrier<2 * W::LOADS + X::LOADS>();
     else wait_barrier<0>();
     if (s + STAGES - 1 < steps) issue(s + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
     const char* t = lds + stage * STAGE;
     stage = stage == STAGES - 1 ? 0 : stage + 1;
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
-      bf16x8 u[2], g[2], x[2], c[2];
+      bf16x8 u[2], g[2], x[NJ], c[NJ];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         u[i] = W::frag(t, nw + 32 * i, kk, lane);
-        x[i] = X::frag(t + 2 * W::BYTES, mw + 32 * i, kk, lane);
+        if (i < NJ) x[i] = X::frag(t + 2 * W::BYTES, mw + 32 * i, kk, lane);
         g[i] = W::frag(t + W::BYTES, nw + 32 * i, kk, lane);
-        c[i] = CTX ? X::frag(t + 2 * W::BYTES + X::BYTES, mw + 32 * i, kk, lane) : x[i];
+        if (i < NJ) c[i] = CTX ? X::frag(t + 2 * W::BYTES + X::BYTES, mw + 32 * i, kk, lane) : x[i];
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) p[i][j] = mfma32(u[i], x[j], p[i][j]);
+        for (int j = 0; j < NJ; ++j) p[i][j] = mfma32(u[i], x[j], p[i][j]);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) q[i][j] = mfma32(g[i], c[j], q[i][j]);
+        for (int j = 0; j < NJ; ++j) q[i][j] = mfma32(g[i], c[j], q[i][j]);
     }
   }
   }
@@ -1372,6 +1372,10 @@ ProductPlan plan_products(int64_t M, int64_t H, int64_t N, int64_t D, bool ctx, 
 // 4096, D 1024: 72 us in 192, 79 in 128, 81 in 256).
 template <int EPI>
 int projection_tokens(const GatedArgs& a, int act) {
+  // Up to a tile a CU: half of it (us in 64 / 128 tokens, saved: 385 tokens of 3 x 1000, D 200
+  // 10.8 / 15.9, 1024 tokens of 4096, D 1024 33 / 40; 192 tokens of 4 x 8192, two tiles a CU,
+  // 20 / 18 at D 200).
+  if ((a.N + 127) / 128 * a.H * ((a.M + 127) / 128) <= device_cus()) return 64;
   if (a.c) return 128;
   constexpr double step[3] = {1.07, 0.63, 0.82};
   constexpr double ends[3][3][3] = {{{6.3, 6.5, 10.0}, {11.6, 11.0, 15.5}, {14.5, 14.0, 18.0}},
@@ -1405,10 +1409,15 @@ void launch_projections(const GatedArgs& a, hipStream_t st) {
   if (tokens != 128) {
     GatedArgs b = a;
     b.order = tile_order((int64_t)cdiv(a.N, 128) * a.H, cdiv(a.M, tokens));
-    if (tokens == 256)
-      hipLaunchKernelGGL((gated_kernel<ACT, EPI, false, 4>), dim3(grid_of(b.order)), dim3(256), 0, st, b);
+    const dim3 grid(grid_of(b.order));
+    if (tokens == 64 && a.c)
+      hipLaunchKernelGGL((gated_kernel<ACT, EPI, true, 1>), grid, dim3(256), 0, st, b);
+    else if (tokens == 64)
+      hipLaunchKernelGGL((gated_kernel<ACT, EPI, false, 1>), grid, dim3(256), 0, st, b);
+    else if (tokens == 256)
+      hipLaunchKernelGGL((gated_kernel<ACT, EPI, false, 4>), grid, dim3(256), 0, st, b);
     else
-      hipLaunchKernelGGL((gated_kernel<ACT, EPI, false, 3>), dim3(grid_of(b.order)), dim3(256), 0, st, b);
+      hipLaunchKernelGGL((gated_kernel<ACT, EPI, false, 3>), grid, dim3(256), 0, st, b);
     return;
   }
   const dim3 grid(grid_of(a.order));

@@ -141,6 +141,13 @@ def test_larger_tiles(T, D, N, act):
     run(1, T, 1, D, N, act, False, 0.25 if act == "relu" else 0.0, act == "relu")
 
 
+# More tiles of 128 by 128 than a chip has CUs, of few steps.
+@pytest.mark.parametrize("act", ["relu", "silu", "gelu"])
+@pytest.mark.parametrize("context", [False, True])
+def test_many_tiles(act, context):
+    run(1, 2055, 1, 72, 4104, act, context)
+
+
 # The backward of saved values without the projections' gradients in memory begins at 2^23 of them.
 @pytest.mark.parametrize("B,T,H,D,N,act,context,masked", [
     (3, 375, 1, 200, 7504, "relu", True, True), (1, 4097, 2, 72, 1032, "relu", True, False),
