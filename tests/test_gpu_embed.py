@@ -216,3 +216,29 @@ def test_refusals():
 @pytest.mark.parametrize("n", [4096, 4097, 5119, 5120, 5121, 131072, 131073])
 def test_vjp_borders_of_the_sort(n):
     run_vjp(n, 1000, 4, "float32", False, "uniform")
+
+
+def test_places_past_32_bits():
+    # Rows and table of more than 2^31 elements; the gradient is of the last 500 tokens alone.
+    torch = need_gpu()
+    import burn_dragon_amd as bd
+    n, D, last = (1 << 20) + 77, 2048, 500
+    V = n + 5
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    tokens = torch.randint(0, V, (n,), generator=gen, device="cuda", dtype=torch.int32)
+    tokens[-last::2] = torch.randint(V - 40, V, (last // 2,), generator=gen, device="cuda", dtype=torch.int32)
+    table = torch.empty(V, D, device="cuda", dtype=torch.bfloat16).normal_(generator=gen)
+    announce("embed past 2^31 elements")
+    out = bd.embed_tokens(tokens, table)
+    assert torch.equal(out[-last:], table[tokens[-last:].long()])
+    grad = out.zero_()
+    grad[-last:].normal_(generator=gen)
+    del table
+    announce("embed vjp past 2^31 elements")
+    got = bd.embed_tokens_vjp(grad, tokens, torch.empty(V, D, device="cuda", dtype=torch.bfloat16))
+    want = torch.zeros(V, D, device="cuda", dtype=torch.float32).index_add_(0, tokens[-last:].long(), grad[-last:].float())
+    # A rounding to bf16; f32 sums of up to 500 rows in another order.
+    rows = tokens[-last:].long().unique()
+    assert float((got[rows].float() - want[rows]).abs().max()) <= (2.0 ** -8 + 1e-4) * float(want[rows].abs().max())
+    got[rows] = 0
+    assert not got.any()

@@ -297,3 +297,32 @@ def test_refusals():
             call()
     with pytest.raises(Exception, match="finite"):
         bd.gated_block(t["x"], w, t["c"], relu_threshold=float("nan"))
+
+
+def test_places_past_32_bits():
+    # 2.15e9 latents; the gradient is of the last 300 tokens alone, so the calls on these
+    # alone give the same.  (Other tiles and parts: two roundings to bf16 of sums in another order.)
+    torch = need_gpu()
+    import burn_dragon_amd as bd
+    T, D, N, last = 131104, 8, 16400, 300
+    assert T * N > 1 << 31
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    rnd = lambda *s: torch.randn(*s, generator=gen, device="cuda").to(torch.bfloat16)  # noqa: E731
+    x, c = rnd(1, T, D), rnd(1, 1, T, D)
+    w = bd.GatedWeights(rnd(1, D, N), rnd(1, D, N))
+    g = torch.zeros(1, T, N, device="cuda", dtype=torch.bfloat16)
+    g[:, -last:] = rnd(1, last, N)
+    announce("gated past 2^31 latents")
+    o = bd.gated_block(x, w, c, save=True)
+    few = bd.gated_block(x[:, -last:], w, c[:, :, -last:], save=True)
+    assert torch.equal(o.out[:, -last:], few.out)
+    for a, b in zip(o.saved, few.saved):
+        assert torch.equal(a.codes[:, -last:], b.codes) and torch.equal(a.scales[:, -last:], b.scales)
+    for saved, few_saved in ((o.saved, few.saved), (None, None)):
+        announce("gated vjp past 2^31 latents", saved is not None)
+        d = bd.gated_block_vjp(g, x, w, c, saved=saved)
+        e = bd.gated_block_vjp(g[:, -last:], x[:, -last:], w, c[:, :, -last:], saved=few_saved)
+        assert not d.current[:, :-last].any() and not d.context[:, :, :-last].any()
+        for a, b in ((d.current[:, -last:], e.current), (d.context[:, :, -last:], e.context), (d.up, e.up), (d.gate, e.gate)):
+            a, b = a.double(), b.double()
+            assert float((a - b).norm()) <= 2.0 ** -7 * float(b.norm())
