@@ -8,7 +8,7 @@
 // The gradient goes by sorted tokens, without atomics on values, so a call repeats
 // bit for bit: the positions are sorted by id (a stable radix sort of up to 9 bits
 // a pass: one pass for up to 511 rows of E, two for 2^18 - 1; in one launch up to
-// 4096 tokens), then each wave sums the rows of a run of positions, and writes the ids
+// 4096 tokens; up to 64 need no sort), then each wave sums the rows of a run of positions, and writes the ids
 // that lie within it.  An id that runs on into the next runs leaves partial sums,
 // which a second launch joins in their order.  The rows without a token are cleared
 // by the sort's launches beside their own work.
@@ -498,6 +498,46 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embed_join_kernel(const Embed
   write_row(a, c, id, s, lane);
 }
 
+// Up to 64 tokens in one launch, their ids in the lanes of each wave: wave i < n sums the rows
+// of token i's id, if it is the id's first, in order; the waves after them clear the rows
+// without a token.
+template <typename T, int VEC, int PER>
+__global__ __launch_bounds__(256) void embed_few_kernel(const EmbedArgs a) {
+  const int lane = threadIdx.x & 63, n = (int)a.n, vocab = (int)a.vocab;
+  const int64_t wave = (int64_t)blockIdx.x * 4 + wave_id();
+  const Columns c = columns_of(a, VEC * PER * 64);
+  const int own = lane < n ? a.tokens[lane] : -1;
+  Row<T, VEC, PER> s;
+  s.clear();
+  if (wave < n) {
+    const int id = __builtin_amdgcn_readlane(own, (int)wave);
+    uint64_t same = __ballot(own == id);
+    if (id < 0 || id >= vocab || __builtin_ctzll(same) != (int)wave) return;
+    constexpr int AHEAD = 64 / (VEC * PER);  // rows asked for together
+    while (same != 0) {
+      Row<T, VEC, PER> g[AHEAD];
+      uint64_t rest = same;
+#pragma unroll
+      for (int q = 0; q < AHEAD; ++q) {
+        const int i = __builtin_ctzll(rest);
+        if ((rest & (rest - 1)) != 0) rest &= rest - 1;  // (past the last: the last again)
+        g[q].load((const T*)a.grad + (int64_t)i * c.row + c.first, c.n, lane);
+      }
+#pragma unroll
+      for (int q = 0; q < AHEAD; ++q) {
+        if (same != 0) add(s, g[q]);
+        same &= same - 1;
+      }
+    }
+    write_row(a, c, (uint32_t)id, s, lane);
+    return;
+  }
+  if (a.accumulate) return;
+  const int64_t waves = (int64_t)gridDim.x * 4 - n;
+  for (int64_t v = wave - n; v < vocab; v += waves)
+    if (__ballot(own == (int)v) == 0) s.store((T*)a.out + v * c.row + c.first, c.n, lane);
+}
+
 unsigned cdiv(int64_t a, int64_t b) { return (unsigned)((a + b - 1) / b); }
 
 // f(VEC, PER) for rows of D columns.
@@ -537,6 +577,22 @@ void launch_rows(const EmbedArgs& a, hipStream_t st) {
   });
 }
 
+// Whether embed_few_kernel takes a call (us, sorted / so: 64 tokens to 256 rows of 1024 f32
+// columns 13 / 4, of 256 with the norm 31 / 5, to 250000 rows of 512 bf16 columns 45 / 34; where
+// all 64 tokens have one id, 14 / 8, and 24 / 33 at 2048 f32 columns with the norm).
+template <typename T>
+bool launch_few(const EmbedArgs& a, hipStream_t st) {
+  if (a.n > 64) return false;
+  const int64_t slice = sizeof(T) == 4 ? 256 : 512;
+  by_columns<T>(a.norm || a.embd < slice ? a.embd : slice, [&](auto vec, auto per) {
+    constexpr int VEC = decltype(vec)::value, PER = decltype(per)::value;
+    const int64_t rows = a.accumulate ? 0 : (a.vocab < 8192 ? a.vocab : 8192);  // waves that clear
+    hipLaunchKernelGGL((embed_few_kernel<T, VEC, PER>), dim3(cdiv(a.n + rows, 4), cdiv(a.embd, VEC * PER * 64)),
+                       dim3(256), 0, st, a);
+  });
+  return true;
+}
+
 template <typename T>
 void launch_sums(const EmbedArgs& a, int64_t runs, hipStream_t st) {
   const int64_t slice = sizeof(T) == 4 ? 256 : 512;
@@ -560,6 +616,11 @@ bdh_status embed_tokens(const EmbedArgs& a, hipStream_t st) {
 }
 
 bdh_status embed_tokens_vjp(EmbedArgs a, hipStream_t st, uint64_t* launches) {
+  if (a.bf16 ? launch_few<bf16_t>(a, st) : launch_few<float>(a, st)) {
+    *launches += 1;
+    BDH_HIP_TRY(hipGetLastError());
+    return BDH_OK;
+  }
   int bits = 1;
   while (a.vocab >> bits) ++bits;  // of the keys 0 .. vocab
   const int passes = (bits + 8) / 9, per_pass = (bits + passes - 1) / passes;
@@ -568,7 +629,11 @@ bdh_status embed_tokens_vjp(EmbedArgs a, hipStream_t st, uint64_t* launches) {
   // of 131072 44 / 54; 262144 88 / 86 and 148 / 150; 1048576 418 / 346 and 580 / 421).
   const int rounds = a.n <= kSmall || a.n > 131072 ? kMostRounds : 1;
   const int64_t blocks = cdiv(a.n, items(rounds));
-  a.run = a.n <= 32768 ? 16 : 32;
+  // Short runs where there are few, and where most ids end in one, whose row's norm a wave
+  // takes in turn (us, runs of 4 / 8 / 16: 512 tokens to 32000 rows of 256 f32 columns with the
+  // norm 27 / 29 / 41, 4096 34 / 40 / 52, 16384 47 / 46 / 56, to 256 rows 25 / 23 / 21; of 1024
+  // columns without the norm 4096 tokens 38 / 35 / 35, 16384 85 / 68 / 59).
+  a.run = a.n <= 4096 ? 4 : a.n > 32768 ? 32 : a.norm && a.vocab > a.n / 8 ? 8 : 16;
   const int64_t runs = cdiv(a.n, a.run);
   const int64_t words = 4 * a.n + (blocks << per_pass);
   void* buf = nullptr;

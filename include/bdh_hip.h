@@ -384,7 +384,7 @@ bdh_status bdh_embed_tokens(const int32_t* tokens, int64_t n_tokens, const void*
  * accumulate added to what is there (rows without a token stay untouched).  Sums are
  * f32 over the tokens sorted by id, in an order that depends on the tokens alone:
  * the same call repeats bit for bit.  grad_table shares no memory with the inputs.
- * Uses the stream's scratch.  No counterpart in the reference, whose tensor library
+ * Past 64 tokens uses the stream's scratch.  No counterpart in the reference, whose tensor library
  * differentiates the lookup. */
 bdh_status bdh_embed_tokens_vjp(const int32_t* tokens, int64_t n_tokens, const void* table,
                                 int32_t dtype, int64_t vocab, int64_t embd, float scale,

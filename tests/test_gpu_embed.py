@@ -218,6 +218,16 @@ def test_vjp_borders_of_the_sort(n):
     run_vjp(n, 1000, 4, "float32", False, "uniform")
 
 
+# Few tokens, in one launch.
+@pytest.mark.parametrize("kind", ["uniform", "one", "none", "zipf"])
+@pytest.mark.parametrize("D,dtype,norm", [(2048, "float32", True), (2047, "bfloat16", True), (1001, "float32", False),
+                                          (513, "bfloat16", False), (3, "float32", True)])
+@pytest.mark.parametrize("n", [1, 31, 32, 33, 63, 64, 65])
+def test_vjp_few(n, D, dtype, norm, kind):
+    run_vjp(n, 90, D, dtype, norm, kind)
+    run_vjp(n, 40000 if D == 3 else 700, D, dtype, norm, kind, accumulate=n % 2 == 0)
+
+
 def test_places_past_32_bits():
     # Rows and table of more than 2^31 elements; the gradient is of the last 500 tokens alone.
     torch = need_gpu()
