@@ -12,7 +12,6 @@ mismatch, plan mismatch) so that callers fall back exactly as
 from __future__ import annotations
 
 import ctypes
-import functools
 from dataclasses import dataclass
 from typing import NamedTuple, Optional
 
@@ -95,10 +94,19 @@ def _stream_ptr(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
-@functools.lru_cache(maxsize=None)
+_supported_devices = set()
+
+
 def _supported(device: torch.device) -> bool:
-    """supports_backend for a device tensor's call (torch is initialised)."""
-    return device.type == "cuda" and bool(_call_on(device, _lib.load().bdh_supports_backend))
+    """supports_backend for a device tensor's call (torch is initialised).  Asked
+    once a device where the answer is yes; a no may be a query that failed, and
+    is asked for again."""
+    if device in _supported_devices:
+        return True
+    if device.type != "cuda" or not _call_on(device, _lib.load().bdh_supports_backend):
+        return False
+    _supported_devices.add(device)
+    return True
 
 
 def _call_on(device: torch.device, fn, *args):
