@@ -2,8 +2,9 @@
 (bdh_activations_save, bdh_activations_restore): e4m3 values with one power of
 two for 32 neighbours of a row, 33/32 bytes a value.
 
-A value is off by at most 2^-4 of its magnitude, or by 2^-19 of its block's
-largest where it is far below that.  ``gated_block(save=True)`` keeps its two
+A value is off by at most 2^-4 of its magnitude, or by 2^-17 of its block's
+largest where it is far below that (by 2^-127 in a block of which nothing passes
+2^-109).  ``gated_block(save=True)`` keeps its two
 projections so, and ``gated_block_vjp(saved=...)`` reads them.
 """
 from __future__ import annotations
