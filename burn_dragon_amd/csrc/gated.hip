@@ -261,10 +261,11 @@ __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf
 // The normal distribution at q, Phi(q), and exp(-q^2 / 2).  Of |q| the upper tail is
 // exp(-q^2 / 2) f(t), t = 1 / (1 + 0.265 |q|), with f a polynomial of degree 9 without a
 // constant, fitted here to the scaled complementary error function (least squares with
-// weights moved towards the largest error): 1.4e-8 of a tail to |q| = 14.5, past which the
-// exponential is 0; in f32 within 2e-7 of Phi, which is 2e-6 of a tail at |q| = 6.  The slope
-// takes the same exponential (the backward's projections of 3003 tokens of 4096, D 1024: 94 us
-// with the library's erf, 78 so; 8192 tokens of 8192 saved: 388 -> 366).
+// weights moved towards the largest error): with its constants in f32 1e-7 of a tail to
+// |q| = 14.5, past which the exponential is 0; in f32 steps within 2.1e-7 of Phi, which is
+// 2e-6 of a tail at |q| = 6.  The slope takes the same exponential (the backward's projections
+// of 3003 tokens of 4096, D 1024: 94 us with the library's erf, 78 so; 8192 tokens of 8192
+// saved: 388 -> 366).
 struct Normal {
   float cdf, bell;
 };
