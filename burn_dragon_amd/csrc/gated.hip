@@ -14,6 +14,7 @@
 // [H, D, N] serve the forward (MC) and dx, dc (KC) alike, dp and dq serve dx (KC) and
 // dU (MC).  The first factor of a product is the one whose rows lie along the
 // result's rows in memory: a lane's sums are then neighbours there.
+#include <algorithm>
 #include <type_traits>
 
 #include "bdh_fp8.h"
@@ -843,6 +844,8 @@ struct ProductArgs {
   int in_parts, w_parts;    // of k
   int in_tiles, w_tiles;    // in all, parts counted
   bool weights_first;
+  int x_units;              // products (up's or gate's of a head) that a workgroup sums for d_x
+  int x_jobs;               // such sums, of a part of k
   int x_parts;              // sums that make up d_x
   int64_t x_size, c_size;   // elements of d_x, d_c
   bf16_t *d_x, *d_c, *d_up, *d_gate;
@@ -850,10 +853,11 @@ struct ProductArgs {
 };
 
 // A wave's sums of a product, 32 NA of the result's columns from a0 by 32 NB of its rows
-// from b0: to the gradient in bf16, or as one of the parts that join_kernel adds.
+// from b0: to the gradient in bf16, or as one of the parts that join_kernel adds.  job: of
+// x_jobs, where they are d_x's.
 template <int WHAT, int NA, int NB>
 __device__ __forceinline__ void store_product(const ProductArgs& a, const floatx16 (&acc)[NA][NB], int h, int which,
-                                              int part, int a0, int b0, int lane) {
+                                              int part, int job, int a0, int b0, int lane) {
   const int high = lane >> 5;
   const bool ctx = which && a.c;
   const int a_end = (int)(WHAT == INPUTS ? a.D : a.N), b_end = (int)(WHAT == INPUTS ? a.M : a.D);
@@ -868,7 +872,7 @@ __device__ __forceinline__ void store_product(const ProductArgs& a, const floatx
     direct = a.in_parts == 1;
   } else if (WHAT == INPUTS) {
     out = a.d_x;
-    sums = a.x_sums + ((int64_t)(which * a.H + h) * a.in_parts + part) * a.x_size;
+    sums = a.x_sums + ((int64_t)job * a.in_parts + part) * a.x_size;
     direct = a.x_parts == 1;
   } else {
     out_at = (int64_t)h * a.D * a.N;
@@ -913,8 +917,9 @@ __device__ __forceinline__ int id_of(int b, int n) {
   return b >> 3 < per_xcd && id < n ? id : -1;
 }
 
-// BIG: 256 by 256, a wave 128 by 128, in big_loop.
-template <int WHAT, bool BIG>
+// BIG: 256 by 256, a wave 128 by 128, in big_loop.  MANY: d_x's sum goes on over x_units
+// products, up's of the heads in turn, then gate's (where that reads current too).
+template <int WHAT, bool BIG, bool MANY>
 __device__ __forceinline__ void product_tile(const ProductArgs& a, char* lds, int id) {
   typedef Tile<WHAT == INPUTS ? KC : MC, 256> A;  // U, G rows d / dp, dq columns n
   constexpr int NB = BIG ? 4 : 2;                 // 32 of the result's rows each of a wave
@@ -929,10 +934,13 @@ __device__ __forceinline__ void product_tile(const ProductArgs& a, char* lds, in
   const int parts = WHAT == INPUTS ? a.in_parts : a.w_parts;
   const int di = id % d_tiles, oi = id / d_tiles % other, rest = id / d_tiles / other;
   const int part = rest % parts, job = rest / parts;
-  const int h = job % a.H, which = job / a.H;  // which: 0 up, 1 gate
+  constexpr bool ALONG = WHAT == INPUTS && MANY;
+  // The products: d_x's jobs first, then d_c's heads.
+  const int first = !ALONG ? job : job < a.x_jobs ? job * a.x_units : a.H + job - a.x_jobs;
+  const int end = ALONG && job < a.x_jobs ? min(first + a.x_units, a.c ? a.H : 2 * a.H) : first + 1;
+  const int h = first % a.H, which = first / a.H;  // which: 0 up, 1 gate
   const int a0 = (WHAT == INPUTS ? di : oi) * 256, b0 = (WHAT == INPUTS ? oi : di) * 64 * NB;
   const int K = WHAT == INPUTS ? N : M;
-  const bf16_t* dv = which ? a.dq : a.dp;        // [M, H, N]
   const int64_t d_row = (int64_t)a.H * N;
   const bool ctx = which && a.c;
   // Bases of the workgroup, and the lanes' places (below 2^32 bytes: H N is 2^24 at most, of
@@ -942,11 +950,21 @@ __device__ __forceinline__ void product_tile(const ProductArgs& a, char* lds, in
   const char* b_base;
   uint32_t a_at[A::LOADS], b_at[B::LOADS];
   const int ac = A::chunk(w, lane) * 8, bc = B::chunk(w, lane) * 8;
-  if (WHAT == INPUTS) {
+  const auto inputs_of = [&](int h, int which) {
     a_base = (const char*)((which ? a.gate : a.up) + ((int64_t)h * D + a0) * N);
-    b_base = (const char*)(dv + b0 * d_row + (int64_t)h * N);
+    b_base = (const char*)((which ? a.dq : a.dp) + b0 * d_row + (int64_t)h * N);
+  };
+  // Goes on to product u, once every wave has read the last stages.  (Opaque: else the
+  // parts of its addresses are kept from the start on, in more scalar registers than there are.)
+  const auto next_of = [&](int& u) {
+    wait_barrier<0>();
+    asm volatile("" : "+s"(u));
+    inputs_of(u < a.H ? u : u - a.H, u >= a.H);
+  };
+  if (WHAT == INPUTS) {
+    inputs_of(h, which);
   } else {
-    a_base = (const char*)(dv + (int64_t)h * N + a0);
+    a_base = (const char*)((which ? a.dq : a.dp) + (int64_t)h * N + a0);
     b_base = (const char*)(ctx ? a.c + (int64_t)h * a.c_head : a.x);
   }
 #pragma unroll
@@ -994,53 +1012,61 @@ __device__ __forceinline__ void product_tile(const ProductArgs& a, char* lds, in
     struct {
       bf16x8 a[4], b[4];
     } f[2];
-    big_loop(
-        s0, s1, K, load,
-        [&](int set, int i, int stage, int kk) {
-          const char* t = lds + stage * STAGE;
-          if (i < 4) f[set].a[i] = A::frag(t, aw + 32 * i, kk, lane);
-          else f[set].b[i - 4] = B::frag(t + A::BYTES, bw + 32 * (i - 4), kk, lane);
-        },
-        [&](int set, int i) { acc[i / 4][i % 4] = mfma32(f[set].a[i / 4], f[set].b[i % 4], acc[i / 4][i % 4]); });
-    store_product<WHAT>(a, acc, h, which, part, a0 + aw, b0 + bw, lane);
+    for (int u = first;;) {
+      big_loop(
+          s0, s1, K, load,
+          [&](int set, int i, int stage, int kk) {
+            const char* t = lds + stage * STAGE;
+            if (i < 4) f[set].a[i] = A::frag(t, aw + 32 * i, kk, lane);
+            else f[set].b[i - 4] = B::frag(t + A::BYTES, bw + 32 * (i - 4), kk, lane);
+          },
+          [&](int set, int i) { acc[i / 4][i % 4] = mfma32(f[set].a[i / 4], f[set].b[i % 4], acc[i / 4][i % 4]); });
+      if (!ALONG || ++u == end) break;
+      next_of(u);
+    }
+    store_product<WHAT>(a, acc, h, which, part, job, a0 + aw, b0 + bw, lane);
     return;
   }
   // Ring of three stages.  A step's loads may be in flight while the one before it is
   // multiplied, but only whole steps' are counted: a last one leaves out some.
-  if (s0 < s1) issue(s0, 0);
-  if (s0 + 1 < s1) issue(s0 + 1, 1);
-  for (int s = s0, stage = 0; s < s1; ++s) {
-    if (s + 1 < s1 && (s + 2) * BK <= K) wait_barrier<LOADS>();
-    else wait_barrier<0>();
-    if (s + 2 < s1) issue(s + 2, stage == 0 ? 2 : stage - 1);
-    const char* t = lds + stage * STAGE;
-    stage = stage == 2 ? 0 : stage + 1;
+  for (int u = first;;) {
+    if (s0 < s1) issue(s0, 0);
+    if (s0 + 1 < s1) issue(s0 + 1, 1);
+    for (int s = s0, stage = 0; s < s1; ++s) {
+      if (s + 1 < s1 && (s + 2) * BK <= K) wait_barrier<LOADS>();
+      else wait_barrier<0>();
+      if (s + 2 < s1) issue(s + 2, stage == 0 ? 2 : stage - 1);
+      const char* t = lds + stage * STAGE;
+      stage = stage == 2 ? 0 : stage + 1;
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      bf16x8 fa[4], fb[NB];
+      for (int kk = 0; kk < 2; ++kk) {
+        bf16x8 fa[4], fb[NB];
 #pragma unroll
-      for (int j = 0; j < NB; ++j) fb[j] = B::frag(t + A::BYTES, bw + 32 * j, kk, lane);
+        for (int j = 0; j < NB; ++j) fb[j] = B::frag(t + A::BYTES, bw + 32 * j, kk, lane);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) fa[i] = A::frag(t, aw + 32 * i, kk, lane);
+        for (int i = 0; i < 4; ++i) fa[i] = A::frag(t, aw + 32 * i, kk, lane);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < NB; ++j) acc[i][j] = mfma32(fa[i], fb[j], acc[i][j]);
+          for (int j = 0; j < NB; ++j) acc[i][j] = mfma32(fa[i], fb[j], acc[i][j]);
+      }
     }
+    if (!ALONG || ++u == end) break;
+    next_of(u);
   }
-  store_product<WHAT>(a, acc, h, which, part, a0 + aw, b0 + bw, lane);
+  store_product<WHAT>(a, acc, h, which, part, job, a0 + aw, b0 + bw, lane);
 }
 
 // Both kinds of products, the one with the longer sums first.
-template <bool BIG>
+template <bool BIG, bool MANY>
 __global__ __launch_bounds__(256, BIG ? 1 : 2) void product_kernel(const ProductArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[BIG ? BIG_STAGES * BIG_STAGE : 3 * 64 * (256 + 128)];
   const int first = ((a.weights_first ? a.w_tiles : a.in_tiles) + 7) / 8 * 8, b = (int)blockIdx.x;
   const bool weights = (b < first) == a.weights_first;
   const int id = id_of(b < first ? b : b - first, weights ? a.w_tiles : a.in_tiles);
   if (id < 0) return;
-  if (weights) product_tile<WEIGHTS, BIG>(a, lds, id);
-  else product_tile<INPUTS, BIG>(a, lds, id);
+  if (weights) product_tile<WEIGHTS, BIG, MANY>(a, lds, id);
+  else product_tile<INPUTS, BIG, MANY>(a, lds, id);
 }
 
 // Both products of a kind straight from what the forward saved, D up to 256: dp and dq are
@@ -1277,7 +1303,7 @@ __global__ __launch_bounds__(512, 1) void fused_kernel(const ProductArgs a, cons
   if (s < s1) group(no);
   while (s + 10 <= last) group(std::true_type{});
   while (s < s1) group(no);
-  store_product<WHAT>(a, acc, h, which, part, (IN ? 0 : at0) + aw, (IN ? at0 : 0) + bw, lane);
+  store_product<WHAT>(a, acc, h, which, part, which * a.H + h, (IN ? 0 : at0) + aw, (IN ? at0 : 0) + bw, lane);
 }
 
 // out[i] = the sum of n parts, in their order; eight neighbours a thread.  Up to four
@@ -1467,18 +1493,27 @@ bdh_status gated_block(const GatedCall& g, hipStream_t st, uint64_t* launches) {
   return BDH_OK;
 }
 
+// Partial sums of d_x take no more than this, or the bytes of dp and dq: a sum for each product
+// of a head takes D / N of those (2 D / N without a context), past which a workgroup goes on
+// over several products (us, a sum for each / so: 8192 tokens, 64 heads of 256, D 4096 without a
+// context 13170 / 6220, its sums 17.2 GB / 0.5; 16384 tokens, 64 heads of 64, D 256, saved 1317 /
+// 464, with a context 1105 / 793; 8192 tokens, 8 heads of 512, D 2048 1240 / 842; 4096 tokens, 16
+// heads of 512, D 1024 704 / 525, with a context, at 2^28 bytes and ungrouped, 650).
+constexpr int64_t kMostSums = (int64_t)1 << 28;
+
 bdh_status gated_block_vjp(const GatedCall& g, hipStream_t st, uint64_t* launches) {
   GatedArgs a = args_of(g);
   const int64_t M = a.M, H = g.H, N = g.N, D = g.D;
+  const int64_t cus = device_cus(), all = (g.c ? 1 : 2) * H;  // products that d_x sums
+  const int64_t x_sum = M * D * 4, most_sums = std::max(kMostSums, 4 * M * H * N);
+  ProductArgs p{};
+  p.x_units = 1;
+  int64_t in_tiles = cdiv(M, 128) * H, w_tiles = cdiv(N, 128) * H;
   // From saved values without dp and dq in memory, where there are latents enough (us, fused /
   // not, 4 heads, D 256: 385 tokens of 1000 latents 64 / 50, of 8192 101 / 116; 4096 of 1000
   // 119 / 136, of 8192 475 / 606; 1 head of 8192: 1024 tokens 94 / 101; D 64: 70 / 70).  (A
   // fused step of 128 tokens' places is held in 32 bits.)
-  const bool fused = g.up_codes && D <= 256 && M * H * N >= (int64_t)1 << 23 && H * N <= (int64_t)1 << 23;
-  const int64_t cus = device_cus();
-  ProductArgs p{};
-  bool big = false;
-  int64_t in_tiles, w_tiles;
+  bool fused = g.up_codes && D <= 256 && M * H * N >= (int64_t)1 << 23 && H * N <= (int64_t)1 << 23;
   if (fused) {
     // Parts of k: enough workgroups to fill the chip.
     const auto parts_of = [&](int64_t tiles, int64_t K) {
@@ -1486,11 +1521,12 @@ bdh_status gated_block_vjp(const GatedCall& g, hipStream_t st, uint64_t* launche
       const int64_t parts = want < most ? want : most;
       return (int)(parts < 32 ? parts : 32);
     };
-    in_tiles = cdiv(M, 128) * H;
-    w_tiles = cdiv(N, 128) * H;
     p.in_parts = parts_of(in_tiles, N);
     p.w_parts = parts_of(w_tiles, M);
-  } else {
+    fused = all * p.in_parts == 1 || all * p.in_parts * x_sum <= most_sums;
+  }
+  bool big = false;
+  if (!fused) {
     ProductPlan plan = plan_products(M, H, N, D, g.c != nullptr, false);
     // (What the larger tiles' places in memory are held in takes H N up to 2^23, and rows
     // of c that follow one another.)
@@ -1501,18 +1537,23 @@ bdh_status gated_block_vjp(const GatedCall& g, hipStream_t st, uint64_t* launche
         big = true;
       }
     }
-    in_tiles = (int64_t)cdiv(D, 256) * cdiv(M, big ? 256 : 128) * 2 * H;
-    w_tiles = (int64_t)cdiv(N, 256) * cdiv(D, big ? 256 : 128) * 2 * H;
     p.in_parts = plan.in_parts;
     p.w_parts = plan.w_parts;
-    p.weights_first = (M + p.w_parts - 1) / p.w_parts > (N + p.in_parts - 1) / p.in_parts;
+    if (all * p.in_parts * x_sum > most_sums && all * p.in_parts > 1) {
+      p.in_parts = 1;
+      while (p.x_units < all && cdiv(all, p.x_units) * x_sum > most_sums) p.x_units *= 2;
+    }
+    p.x_jobs = (int)cdiv(all, p.x_units);
+    in_tiles = (int64_t)cdiv(D, 256) * cdiv(M, big ? 256 : 128) * (p.x_jobs + (g.c ? H : 0));
+    w_tiles = (int64_t)cdiv(N, 256) * cdiv(D, big ? 256 : 128) * 2 * H;
+    p.weights_first = (M + p.w_parts - 1) / p.w_parts > (N * p.x_units + p.in_parts - 1) / p.in_parts;
   }
   // (A launch has fewer than 2^32 threads.)
   if (in_tiles * p.in_parts > (int64_t)1 << 22 || w_tiles * p.w_parts > (int64_t)1 << 22)
     return fail(BDH_UNSUPPORTED, "too large for one launch");
   p.in_tiles = (int)(in_tiles * p.in_parts);
   p.w_tiles = (int)(w_tiles * p.w_parts);
-  p.x_parts = (int)((g.c ? 1 : 2) * H * p.in_parts);
+  p.x_parts = (int)(cdiv(all, p.x_units) * p.in_parts);
   p.x_size = M * D;
   p.c_size = M * H * D;
   const int64_t w_size = H * D * N;
@@ -1565,8 +1606,11 @@ bdh_status gated_block_vjp(const GatedCall& g, hipStream_t st, uint64_t* launche
       launch_projections<BACK>(a, g.act, st);
     }
     const dim3 grid((cdiv(p.in_tiles, 8) + cdiv(p.w_tiles, 8)) * 8);
-    if (big) hipLaunchKernelGGL(product_kernel<true>, grid, dim3(256), 0, st, p);
-    else hipLaunchKernelGGL(product_kernel<false>, grid, dim3(256), 0, st, p);
+    const bool many = p.x_units > 1;
+    if (big && many) hipLaunchKernelGGL((product_kernel<true, true>), grid, dim3(256), 0, st, p);
+    else if (big) hipLaunchKernelGGL((product_kernel<true, false>), grid, dim3(256), 0, st, p);
+    else if (many) hipLaunchKernelGGL((product_kernel<false, true>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((product_kernel<false, false>), grid, dim3(256), 0, st, p);
   }
   *launches += 2;
   JoinArgs j{};
