@@ -847,6 +847,7 @@ struct ProductArgs {
   int x_units;              // products (up's or gate's of a head) that a workgroup sums for d_x
   int x_jobs;               // such sums, of a part of k
   int x_parts;              // sums that make up d_x
+  bool w_kept, w_more;      // the weights' sums stay in f32 (and go on from those there)
   int64_t x_size, c_size;   // elements of d_x, d_c
   bf16_t *d_x, *d_c, *d_up, *d_gate;
   float *x_sums, *c_sums, *w_sums;
@@ -854,8 +855,8 @@ struct ProductArgs {
 
 // A wave's sums of a product, 32 NA of the result's columns from a0 by 32 NB of its rows
 // from b0: to the gradient in bf16, or as one of the parts that join_kernel adds.  job: of
-// x_jobs, where they are d_x's.
-template <int WHAT, int NA, int NB>
+// x_jobs, where they are d_x's.  KEEP: w_kept and w_more count.
+template <int WHAT, bool KEEP, int NA, int NB>
 __device__ __forceinline__ void store_product(const ProductArgs& a, const floatx16 (&acc)[NA][NB], int h, int which,
                                               int part, int job, int a0, int b0, int lane) {
   const int high = lane >> 5;
@@ -878,7 +879,7 @@ __device__ __forceinline__ void store_product(const ProductArgs& a, const floatx
     out_at = (int64_t)h * a.D * a.N;
     out = which ? a.d_gate : a.d_up;
     sums = a.w_sums + ((int64_t)part * 2 + which) * a.H * a.D * a.N;
-    direct = a.w_parts == 1;
+    direct = a.w_parts == 1 && !(KEEP && a.w_kept);
   }
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
@@ -903,6 +904,10 @@ __device__ __forceinline__ void store_product(const ProductArgs& a, const floatx
           *(u32x4*)(out + row + at) = u32x4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
                                             pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
         } else {
+          if (WHAT == WEIGHTS && KEEP && a.w_more) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += sums[row + at + e];
+          }
           *(floatx4*)(sums + row + at) = floatx4{v[0], v[1], v[2], v[3]};
           *(floatx4*)(sums + row + at + 4) = floatx4{v[4], v[5], v[6], v[7]};
         }
@@ -918,7 +923,8 @@ __device__ __forceinline__ int id_of(int b, int n) {
 }
 
 // BIG: 256 by 256, a wave 128 by 128, in big_loop.  MANY: d_x's sum goes on over x_units
-// products, up's of the heads in turn, then gate's (where that reads current too).
+// products, up's of the heads in turn, then gate's (where that reads current too), and the
+// weights' sums over several launches.
 template <int WHAT, bool BIG, bool MANY>
 __device__ __forceinline__ void product_tile(const ProductArgs& a, char* lds, int id) {
   typedef Tile<WHAT == INPUTS ? KC : MC, 256> A;  // U, G rows d / dp, dq columns n
@@ -1024,7 +1030,7 @@ __device__ __forceinline__ void product_tile(const ProductArgs& a, char* lds, in
       if (!ALONG || ++u == end) break;
       next_of(u);
     }
-    store_product<WHAT>(a, acc, h, which, part, job, a0 + aw, b0 + bw, lane);
+    store_product<WHAT, MANY>(a, acc, h, which, part, ALONG ? job : which * a.H + h, a0 + aw, b0 + bw, lane);
     return;
   }
   // Ring of three stages.  A step's loads may be in flight while the one before it is
@@ -1054,7 +1060,7 @@ __device__ __forceinline__ void product_tile(const ProductArgs& a, char* lds, in
     if (!ALONG || ++u == end) break;
     next_of(u);
   }
-  store_product<WHAT>(a, acc, h, which, part, job, a0 + aw, b0 + bw, lane);
+  store_product<WHAT, MANY>(a, acc, h, which, part, ALONG ? job : which * a.H + h, a0 + aw, b0 + bw, lane);
 }
 
 // Both kinds of products, the one with the longer sums first.
@@ -1303,7 +1309,7 @@ __global__ __launch_bounds__(512, 1) void fused_kernel(const ProductArgs a, cons
   if (s < s1) group(no);
   while (s + 10 <= last) group(std::true_type{});
   while (s < s1) group(no);
-  store_product<WHAT>(a, acc, h, which, part, which * a.H + h, (IN ? 0 : at0) + aw, (IN ? at0 : 0) + bw, lane);
+  store_product<WHAT, false>(a, acc, h, which, part, which * a.H + h, (IN ? 0 : at0) + aw, (IN ? at0 : 0) + bw, lane);
 }
 
 // out[i] = the sum of n parts, in their order; eight neighbours a thread.  Up to four
@@ -1501,32 +1507,53 @@ bdh_status gated_block(const GatedCall& g, hipStream_t st, uint64_t* launches) {
 // heads of 512, D 1024 704 / 525, with a context, at 2^28 bytes and ungrouped, 650).
 constexpr int64_t kMostSums = (int64_t)1 << 28;
 
-bdh_status gated_block_vjp(const GatedCall& g, hipStream_t st, uint64_t* launches) {
-  GatedArgs a = args_of(g);
-  const int64_t M = a.M, H = g.H, N = g.N, D = g.D;
+namespace {
+
+// How a backward call goes, and the scratch that it takes.
+struct VjpPlan {
+  bool fused, big;
+  int64_t group;   // tokens at a time
+  ProductArgs p;   // (the counts of a whole call)
+  size_t grads, x_bytes, c_bytes, w_bytes;
+};
+// The tiles of d_x and d_c of M tokens, parts counted.
+int64_t in_tiles_of(const GatedCall& g, const VjpPlan& v, int64_t M) {
+  if (v.fused) return cdiv(M, 128) * g.H * v.p.in_parts;
+  return (int64_t)cdiv(g.D, 256) * cdiv(M, v.big ? 256 : 128) * (v.p.x_jobs + (g.c ? g.H : 0)) * v.p.in_parts;
+}
+// less: 0 what is fastest; where there is no memory for that, 1 without parts of k, 2 without
+// any partial sums, 3 on with the tokens in 2, 4, .. groups, whose weights' sums add up in f32.
+bdh_status plan_vjp(const GatedCall& g, int less, VjpPlan* out) {
+  VjpPlan v{};
+  ProductArgs& p = v.p;
+  const int64_t M = g.B * g.T, H = g.H, N = g.N, D = g.D;
   const int64_t cus = device_cus(), all = (g.c ? 1 : 2) * H;  // products that d_x sums
   const int64_t x_sum = M * D * 4, most_sums = std::max(kMostSums, 4 * M * H * N);
-  ProductArgs p{};
   p.x_units = 1;
-  int64_t in_tiles = cdiv(M, 128) * H, w_tiles = cdiv(N, 128) * H;
+  v.group = M;
   // From saved values without dp and dq in memory, where there are latents enough (us, fused /
   // not, 4 heads, D 256: 385 tokens of 1000 latents 64 / 50, of 8192 101 / 116; 4096 of 1000
   // 119 / 136, of 8192 475 / 606; 1 head of 8192: 1024 tokens 94 / 101; D 64: 70 / 70).  (A
   // fused step of 128 tokens' places is held in 32 bits.)
-  bool fused = g.up_codes && D <= 256 && M * H * N >= (int64_t)1 << 23 && H * N <= (int64_t)1 << 23;
-  if (fused) {
+  v.fused = less < 2 && g.up_codes && D <= 256 && M * H * N >= (int64_t)1 << 23 && H * N <= (int64_t)1 << 23;
+  if (v.fused) {
     // Parts of k: enough workgroups to fill the chip.
     const auto parts_of = [&](int64_t tiles, int64_t K) {
+      if (less) return 1;
       const int64_t want = (cus + tiles - 1) / tiles, most = K / 256 > 1 ? K / 256 : 1;
       const int64_t parts = want < most ? want : most;
       return (int)(parts < 32 ? parts : 32);
     };
-    p.in_parts = parts_of(in_tiles, N);
-    p.w_parts = parts_of(w_tiles, M);
-    fused = all * p.in_parts == 1 || all * p.in_parts * x_sum <= most_sums;
+    p.in_parts = parts_of(cdiv(M, 128) * H, N);
+    p.w_parts = parts_of(cdiv(N, 128) * H, M);
+    v.fused = all * p.in_parts == 1 || all * p.in_parts * x_sum <= most_sums;
   }
-  bool big = false;
-  if (!fused) {
+  if (!v.fused && less) {
+    p.in_parts = p.w_parts = 1;
+    while (p.x_units < all) p.x_units *= 2;
+    for (int n = 2; n < less; ++n) v.group = (v.group + 1) / 2;
+    p.w_kept = v.group < M;
+  } else if (!v.fused) {
     ProductPlan plan = plan_products(M, H, N, D, g.c != nullptr, false);
     // (What the larger tiles' places in memory are held in takes H N up to 2^23, and rows
     // of c that follow one another.)
@@ -1534,7 +1561,7 @@ bdh_status gated_block_vjp(const GatedCall& g, hipStream_t st, uint64_t* launche
       const ProductPlan other = plan_products(M, H, N, D, g.c != nullptr, true);
       if (other.us < plan.us) {
         plan = other;
-        big = true;
+        v.big = true;
       }
     }
     p.in_parts = plan.in_parts;
@@ -1543,76 +1570,130 @@ bdh_status gated_block_vjp(const GatedCall& g, hipStream_t st, uint64_t* launche
       p.in_parts = 1;
       while (p.x_units < all && cdiv(all, p.x_units) * x_sum > most_sums) p.x_units *= 2;
     }
-    p.x_jobs = (int)cdiv(all, p.x_units);
-    in_tiles = (int64_t)cdiv(D, 256) * cdiv(M, big ? 256 : 128) * (p.x_jobs + (g.c ? H : 0));
-    w_tiles = (int64_t)cdiv(N, 256) * cdiv(D, big ? 256 : 128) * 2 * H;
-    p.weights_first = (M + p.w_parts - 1) / p.w_parts > (N * p.x_units + p.in_parts - 1) / p.in_parts;
   }
+  p.x_jobs = (int)cdiv(all, p.x_units);
+  p.x_parts = p.x_jobs * p.in_parts;
+  p.weights_first = !v.fused && (M + p.w_parts - 1) / p.w_parts > (N * p.x_units + p.in_parts - 1) / p.in_parts;
+  const int64_t w_tiles = (v.fused ? cdiv(N, 128) * H : (int64_t)cdiv(N, 256) * cdiv(D, v.big ? 256 : 128) * 2 * H) * p.w_parts;
   // (A launch has fewer than 2^32 threads.)
-  if (in_tiles * p.in_parts > (int64_t)1 << 22 || w_tiles * p.w_parts > (int64_t)1 << 22)
+  if (in_tiles_of(g, v, v.group) > (int64_t)1 << 22 || w_tiles > (int64_t)1 << 22)
     return fail(BDH_UNSUPPORTED, "too large for one launch");
-  p.in_tiles = (int)(in_tiles * p.in_parts);
-  p.w_tiles = (int)(w_tiles * p.w_parts);
-  p.x_parts = (int)(cdiv(all, p.x_units) * p.in_parts);
-  p.x_size = M * D;
-  p.c_size = M * H * D;
-  const int64_t w_size = H * D * N;
-  const size_t x_bytes = p.x_parts > 1 ? (size_t)p.x_parts * p.x_size * 4 : 0;
-  const size_t c_bytes = g.c && p.in_parts > 1 ? (size_t)p.in_parts * p.c_size * 4 : 0;
-  const size_t w_bytes = p.w_parts > 1 ? (size_t)p.w_parts * 2 * w_size * 4 : 0;
-  bdh_status s;
-  if (!fused) {
-    void* buf = nullptr;
-    s = scratch(st, SLOT_GATED_GRADS, (size_t)(2 * M * H * N) * sizeof(bf16_t), &buf);
-    if (s != BDH_OK) return s;
-    a.dp = (bf16_t*)buf;
-    a.dq = a.dp + M * H * N;
+  p.w_tiles = (int)w_tiles;
+  v.grads = v.fused ? 0 : (size_t)(2 * v.group * H * N) * sizeof(bf16_t);
+  v.x_bytes = p.x_parts > 1 ? (size_t)(p.x_parts * x_sum) : 0;
+  v.c_bytes = g.c && p.in_parts > 1 ? (size_t)(p.in_parts * H * x_sum) : 0;
+  v.w_bytes = p.w_parts > 1 || p.w_kept ? (size_t)p.w_parts * 2 * H * D * N * 4 : 0;
+  *out = v;
+  return BDH_OK;
+}
+
+// The sequences b .. b + nb - 1 of a call, tokens t .. t + nt - 1 of each (all, where nb > 1).
+struct TokenGroup {
+  int64_t b, nb, t, nt;
+};
+GatedArgs args_of(const GatedCall& g, const TokenGroup& k) {
+  GatedArgs a = args_of(g);
+  const int64_t i = k.b * g.T + k.t;
+  if (k.nb == g.B && k.nt == g.T) return a;
+  a.M = k.nb * k.nt;
+  a.x += i * g.D;
+  if (a.c) a.c += k.b * g.H * g.T * g.D + k.t * g.D;
+  a.c_rows = token_rows(k.nt, g.H * g.T * g.D, g.D);
+  a.g += i * g.H * g.N;
+  if (a.up_codes) {
+    const int64_t blocks = i * g.H * ((g.N + kFp8Block - 1) / kFp8Block);
+    a.up_codes += i * g.H * g.N;
+    a.gate_codes += i * g.H * g.N;
+    a.up_scales += blocks;
+    a.gate_scales += blocks;
   }
-  void* sums = nullptr;
-  if (x_bytes + c_bytes + w_bytes > 0) {
-    s = scratch(st, SLOT_GATED_SUMS, x_bytes + c_bytes + w_bytes, &sums);
+  a.order = tile_order((int64_t)cdiv(g.N, 128) * g.H, cdiv(a.M, 128));
+  return a;
+}
+
+}  // namespace
+
+bdh_status gated_block_vjp(const GatedCall& g, hipStream_t st, uint64_t* launches) {
+  const int64_t H = g.H, N = g.N, D = g.D, w_size = H * D * N;
+  VjpPlan v;
+  void *grads = nullptr, *sums = nullptr;
+  bool dropped = false;
+  for (int less = 0;;) {
+    bdh_status s = plan_vjp(g, less, &v);
     if (s != BDH_OK) return s;
+    if (v.grads) s = scratch(st, SLOT_GATED_GRADS, v.grads, &grads);
+    const size_t bytes = v.x_bytes + v.c_bytes + v.w_bytes;
+    if (s == BDH_OK && bytes) s = scratch(st, SLOT_GATED_SUMS, bytes, &sums);
+    if (s == BDH_OK) break;
+    if (!scratch_no_memory() || (less > 1 && v.group <= 256)) return s;
+    // Once more without what earlier calls have left, then with less.
+    const bdh_status d = scratch_drop(st, {SLOT_GATED_GRADS, SLOT_GATED_SUMS});
+    if (d != BDH_OK) return d;
+    less += dropped;
+    dropped = true;
   }
-  p.dp = a.dp;
-  p.dq = a.dq;
-  p.x = a.x;
-  p.c = a.c;
-  p.up = a.up;
-  p.gate = a.gate;
-  p.M = M;
+  ProductArgs p = v.p;
+  p.up = g.up;
+  p.gate = g.gate;
   p.N = N;
   p.D = D;
   p.H = (int)H;
-  p.c_head = a.c_head;
-  p.c_rows = a.c_rows;
-  p.c_apart = g.B > 1 && H > 1;
-  p.d_x = g.d_x;
-  p.d_c = g.d_c;
   p.d_up = g.d_up;
   p.d_gate = g.d_gate;
   p.x_sums = (float*)sums;
-  p.c_sums = (float*)((char*)sums + x_bytes);
-  p.w_sums = (float*)((char*)sums + x_bytes + c_bytes);
-  if (fused) {
-    launch_fused<INPUTS>(p, a, g.act, st);
-    launch_fused<WEIGHTS>(p, a, g.act, st);
-  } else {
-    if (g.up_codes) {
-      const dim3 grid((unsigned)capped(cdiv(M * H * (N / 8), 256)));
-      if (g.act == RELU) hipLaunchKernelGGL((gated_grads_kernel<RELU>), grid, dim3(256), 0, st, a);
-      else if (g.act == SILU) hipLaunchKernelGGL((gated_grads_kernel<SILU>), grid, dim3(256), 0, st, a);
-      else hipLaunchKernelGGL((gated_grads_kernel<GELU>), grid, dim3(256), 0, st, a);
+  p.c_sums = (float*)((char*)sums + v.x_bytes);
+  p.w_sums = (float*)((char*)sums + v.x_bytes + v.c_bytes);
+  TokenGroup k{0, g.B, 0, g.T};
+  if (v.group < g.T) k = TokenGroup{0, 1, 0, v.group};
+  else if (v.group < g.B * g.T) k.nb = v.group / g.T;
+  while (k.b < g.B) {
+    TokenGroup now = k;
+    now.nb = std::min(k.nb, g.B - k.b);
+    now.nt = std::min(k.nt, g.T - k.t);
+    GatedArgs a = args_of(g, now);
+    const int64_t M = a.M;
+    a.dp = (bf16_t*)grads;
+    a.dq = a.dp + M * H * N;
+    p.dp = a.dp;
+    p.dq = a.dq;
+    p.x = a.x;
+    p.c = a.c;
+    p.M = M;
+    p.c_head = a.c_head;
+    p.c_rows = a.c_rows;
+    p.c_apart = now.nb > 1 && H > 1;
+    p.x_size = M * D;
+    p.c_size = M * H * D;
+    p.d_x = g.d_x + (a.x - g.x);
+    p.d_c = g.d_c ? g.d_c + (a.c - g.c) : nullptr;
+    p.in_tiles = (int)in_tiles_of(g, v, M);
+    if (v.fused) {
+      launch_fused<INPUTS>(p, a, g.act, st);
+      launch_fused<WEIGHTS>(p, a, g.act, st);
     } else {
-      launch_projections<BACK>(a, g.act, st);
+      if (g.up_codes) {
+        const dim3 grid((unsigned)capped(cdiv(M * H * (N / 8), 256)));
+        if (g.act == RELU) hipLaunchKernelGGL((gated_grads_kernel<RELU>), grid, dim3(256), 0, st, a);
+        else if (g.act == SILU) hipLaunchKernelGGL((gated_grads_kernel<SILU>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((gated_grads_kernel<GELU>), grid, dim3(256), 0, st, a);
+      } else {
+        launch_projections<BACK>(a, g.act, st);
+      }
+      const dim3 grid((cdiv(p.in_tiles, 8) + cdiv(p.w_tiles, 8)) * 8);
+      const bool many = p.x_units > 1 || p.w_kept;
+      if (v.big && many) hipLaunchKernelGGL((product_kernel<true, true>), grid, dim3(256), 0, st, p);
+      else if (v.big) hipLaunchKernelGGL((product_kernel<true, false>), grid, dim3(256), 0, st, p);
+      else if (many) hipLaunchKernelGGL((product_kernel<false, true>), grid, dim3(256), 0, st, p);
+      else hipLaunchKernelGGL((product_kernel<false, false>), grid, dim3(256), 0, st, p);
     }
-    const dim3 grid((cdiv(p.in_tiles, 8) + cdiv(p.w_tiles, 8)) * 8);
-    const bool many = p.x_units > 1;
-    if (big && many) hipLaunchKernelGGL((product_kernel<true, true>), grid, dim3(256), 0, st, p);
-    else if (big) hipLaunchKernelGGL((product_kernel<true, false>), grid, dim3(256), 0, st, p);
-    else if (many) hipLaunchKernelGGL((product_kernel<false, true>), grid, dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((product_kernel<false, false>), grid, dim3(256), 0, st, p);
+    *launches += 2;
+    p.w_more = true;
+    k.t += now.nt;
+    if (k.t == g.T) {
+      k.t = 0;
+      k.b += now.nb;
+    }
   }
-  *launches += 2;
   JoinArgs j{};
   int joins = 0;
   int64_t most = 0;
@@ -1620,9 +1701,10 @@ bdh_status gated_block_vjp(const GatedCall& g, hipStream_t st, uint64_t* launche
     j.of[joins++] = {from, n, stride, size, out};
     most = size > most ? size : most;
   };
-  if (x_bytes) join(p.x_sums, p.x_parts, p.x_size, g.d_x, p.x_size);
-  if (c_bytes) join(p.c_sums, p.in_parts, p.c_size, g.d_c, p.c_size);
-  if (w_bytes) {
+  // (Partial sums of d_x and d_c are a whole call's.)
+  if (v.x_bytes) join(p.x_sums, p.x_parts, p.x_size, g.d_x, p.x_size);
+  if (v.c_bytes) join(p.c_sums, p.in_parts, p.c_size, g.d_c, p.c_size);
+  if (v.w_bytes) {
     join(p.w_sums, p.w_parts, 2 * w_size, g.d_up, w_size);
     join(p.w_sums + w_size, p.w_parts, 2 * w_size, g.d_gate, w_size);
   }

@@ -440,7 +440,9 @@ bdh_status bdh_gated_block_fwd(const bdh_layer_plan* plan, const void* current, 
  * parts.  The gradients of p and q are rounded to bf16 once before the four products
  * over them, which sum in f32 (heads and parts of a sum in a fixed order: a call
  * repeats bit for bit) and round once.  Uses the stream's scratch: 4 bytes for each of
- * the B*T*H*N latents, and partial sums (grad_current's: at most as many bytes, or 256 MB). */
+ * the B*T*H*N latents, and partial sums (grad_current's: at most as many bytes, or 256 MB).
+ * Where there is no memory for that a call goes without partial sums, then with its tokens
+ * in groups (8 bytes for each weight, and 4 for a group's latents). */
 bdh_status bdh_gated_block_vjp(const bdh_layer_plan* plan, const void* current, const void* context,
                                const void* up, const void* gate, const bdh_gated_options* options,
                                const void* grad_out, const void* up_codes, const void* up_scales,

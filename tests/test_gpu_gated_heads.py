@@ -97,3 +97,60 @@ def test_scratch_of_many_heads(context):
     assert d is not None
     bd.release_stream_scratch(st)
     assert took <= 1.25 * (SUMS + 4 * B * T * H * N) + (64 << 20)
+
+
+def with_little_memory(torch, left, call):
+    """call() with about `left` bytes of the device's memory free, its outputs' room kept."""
+    import burn_dragon_amd as bd
+    torch.cuda.synchronize()
+    bd.release_stream_scratch()
+    torch.cuda.empty_cache()
+    hold = []
+    try:
+        free = torch.cuda.mem_get_info()[0]
+        while free > left + (16 << 20):
+            hold.append(torch.empty(min(free - left, 32 << 30), dtype=torch.uint8, device="cuda"))
+            free = torch.cuda.mem_get_info()[0]
+        assert free > left - (16 << 20)
+        out = call()
+        torch.cuda.synchronize()
+    finally:
+        del hold
+        bd.release_stream_scratch()
+        torch.cuda.empty_cache()
+    return out
+
+
+# What is planned does not fit in `left` MiB: 8 of dp and dq with 64 of partial sums; 66 with 139;
+# 128 to 131 of dp and dq alone, which go in groups of tokens, of whole sequences (three, or
+# one) or pieces of one; from saved values 128 of partial sums, of which 8 are left without
+# parts; 98, then 64, where dp and dq take 33.
+@pytest.mark.parametrize("B,T,H,D,N,act,context,saved,left", [
+    (1, 4096, 1, 1024, 512, "silu", False, False, 40), (2, 1000, 33, 1024, 264, "relu", True, True, 88),
+    (1, 8192, 1, 64, 4096, "silu", False, False, 64), (3, 1400, 2, 64, 4096, "gelu", True, False, 64),
+    (3, 1400, 2, 64, 4096, "relu", True, False, 36), (7, 600, 2, 320, 4096, "silu", False, True, 108),
+    (7, 600, 2, 64, 4096, "silu", True, False, 108), (1, 4096, 1, 256, 8192, "relu", False, True, 64),
+    (2, 8192, 2, 256, 264, "relu", False, True, 56)])
+def test_little_memory(B, T, H, D, N, act, context, saved, left):
+    torch = need_gpu()
+    import burn_dragon_amd as bd
+    t = make(torch, B, T, H, D, N, context)
+    w = bd.GatedWeights(t["up"], t["gate"])
+    kept = bd.gated_block(t["x"], w, t["c"], activation=act, save=True).saved if saved else None
+    call = lambda: bd.gated_block_vjp(t["g"], t["x"], w, t["c"], saved=kept, activation=act)  # noqa: E731
+    announce("gated vjp, memory short", B, T, H, D, N, act, context, saved, left)
+    room = [torch.empty_like(v) for v in (t["x"], t["up"], t["gate"], t["c"]) if v is not None]
+
+    def short():
+        room.clear()  # (to the caching allocator)
+        return call()
+    d = with_little_memory(torch, left << 20, short)
+    x, c, wu, wg, _, _ = plain(t)
+    if saved:
+        p, q = (heads(bd.restore_activations(k, dtype=torch.float32), H) for k in kept)
+        op = oq = np.zeros_like(p)
+    else:
+        p, q, op, oq = R.project(x, c, wu, wg, 0.0)
+    check_grads(d, reference(act, t, p, q, op, oq), t)
+    # With the memory there again the call goes as planned.
+    check_grads(call(), reference(act, t, p, q, op, oq), t)
