@@ -444,34 +444,34 @@ __global__ __launch_bounds__(256, NJ > 2 ? 1 : 2) void gated_kernel(const GatedA
           else p[e][j] = mfma32(f[set].u[e], f[set].x[j], p[e][j]);
         });
   } else {
-  issue(0, 0);
-  if (STAGES == 3 && steps > 1) issue(1, 1);
-  for (int s = 0, stage = 0; s < steps; ++s) {
-    if (STAGES == 3 && s + 1 < steps && (s + 2) * BK <= D) wait_barrier<2 * W::LOADS + X::LOADS>();
-    else wait_barrier<0>();
-    if (s + STAGES - 1 < steps) issue(s + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
-    const char* t = lds + stage * STAGE;
-    stage = stage == STAGES - 1 ? 0 : stage + 1;
+    issue(0, 0);
+    if (STAGES == 3 && steps > 1) issue(1, 1);
+    for (int s = 0, stage = 0; s < steps; ++s) {
+      if (STAGES == 3 && s + 1 < steps && (s + 2) * BK <= D) wait_barrier<2 * W::LOADS + X::LOADS>();
+      else wait_barrier<0>();
+      if (s + STAGES - 1 < steps) issue(s + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
+      const char* t = lds + stage * STAGE;
+      stage = stage == STAGES - 1 ? 0 : stage + 1;
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      bf16x8 u[2], g[2], x[NJ], c[NJ];
+      for (int kk = 0; kk < 2; ++kk) {
+        bf16x8 u[2], g[2], x[NJ], c[NJ];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        u[i] = W::frag(t, nw + 32 * i, kk, lane);
-        if (i < NJ) x[i] = X::frag(t + 2 * W::BYTES, mw + 32 * i, kk, lane);
-        g[i] = W::frag(t + W::BYTES, nw + 32 * i, kk, lane);
-        if (i < NJ) c[i] = CTX ? X::frag(t + 2 * W::BYTES + X::BYTES, mw + 32 * i, kk, lane) : x[i];
+        for (int i = 0; i < 2; ++i) {
+          u[i] = W::frag(t, nw + 32 * i, kk, lane);
+          if (i < NJ) x[i] = X::frag(t + 2 * W::BYTES, mw + 32 * i, kk, lane);
+          g[i] = W::frag(t + W::BYTES, nw + 32 * i, kk, lane);
+          if (i < NJ) c[i] = CTX ? X::frag(t + 2 * W::BYTES + X::BYTES, mw + 32 * i, kk, lane) : x[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) p[i][j] = mfma32(u[i], x[j], p[i][j]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) q[i][j] = mfma32(g[i], c[j], q[i][j]);
       }
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) p[i][j] = mfma32(u[i], x[j], p[i][j]);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) q[i][j] = mfma32(g[i], c[j], q[i][j]);
     }
-  }
   }
   // A lane has token mw + 32 j + (lane & 31) and, of 32 latents, 8 r + 4 (lane >> 5)
   // ..+3 for r of 0..3.  64 of the tile's tokens at a time (j) go through LDS, so that
@@ -1574,7 +1574,8 @@ bdh_status plan_vjp(const GatedCall& g, int less, VjpPlan* out) {
   p.x_jobs = (int)cdiv(all, p.x_units);
   p.x_parts = p.x_jobs * p.in_parts;
   p.weights_first = !v.fused && (M + p.w_parts - 1) / p.w_parts > (N * p.x_units + p.in_parts - 1) / p.in_parts;
-  const int64_t w_tiles = (v.fused ? cdiv(N, 128) * H : (int64_t)cdiv(N, 256) * cdiv(D, v.big ? 256 : 128) * 2 * H) * p.w_parts;
+  const int64_t w_tiles =
+      (v.fused ? cdiv(N, 128) * H : (int64_t)cdiv(N, 256) * cdiv(D, v.big ? 256 : 128) * 2 * H) * p.w_parts;
   // (A launch has fewer than 2^32 threads.)
   if (in_tiles_of(g, v, v.group) > (int64_t)1 << 22 || w_tiles > (int64_t)1 << 22)
     return fail(BDH_UNSUPPORTED, "too large for one launch");
