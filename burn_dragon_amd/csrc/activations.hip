@@ -5,7 +5,7 @@
 // Four lanes hold a block, eight neighbours each, so a block's largest magnitude
 // takes two exchanges and a wave reads and writes runs of 512 values.  Bound by the
 // bytes: 3 (5) of bf16 (f32) a value to save, 3 (5) to restore (16384 rows of 8192 bf16: saved
-// in 74-86 us, 4.8-5.5 TB/s, restored in 65, 6.2 TB/s).
+// in 77-93 us, 4.4-5.3 TB/s, restored in 64-69, 5.9-6.3 TB/s).
 #include "bdh_fp8.h"
 #include "bdh_internal.h"
 

@@ -14,8 +14,8 @@
 // by the sort's launches beside their own work.
 //
 // Bound by the bytes (rows in, rows out) where there are many tokens, else by the chain of
-// dependent launches: 65536 tokens of 1024 bf16 columns of a table of 32000, 31 us (4.3 TB/s
-// of results); the gradient of 32768 such tokens to 131072 rows, 94 us: two sort passes, which
+// dependent launches: 65536 tokens of 1024 bf16 columns of a table of 32000, 40 us (3.3 TB/s
+// of results, 4.0 with the rows); the gradient of 32768 such tokens to 131072 rows, 94 us: two sort passes, which
 // clear 268 MB, sums 32 (67 MB read in the order of the ids, the met rows written) and
 // join 11; of 16384 tokens to 256 rows of 256 f32 columns, 23 us in four launches.
 #include <type_traits>

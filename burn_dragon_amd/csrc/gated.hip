@@ -265,7 +265,7 @@ __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf
 // weights moved towards the largest error): with its constants in f32 1e-7 of a tail to
 // |q| = 14.5, past which the exponential is 0; in f32 steps within 2.1e-7 of Phi, which is
 // 2e-6 of a tail at |q| = 6.  The slope takes the same exponential (the backward's projections
-// of 3003 tokens of 4096, D 1024: 94 us with the library's erf, 78 so; 8192 tokens of 8192
+// of 3003 tokens of 4096, D 1024: 94 us with the library's erf, 78-83 so; 8192 tokens of 8192
 // saved: 388 -> 366).
 struct Normal {
   float cdf, bell;
@@ -324,7 +324,9 @@ struct GatedArgs {
   bf16_t* out;              // [M, H, N]
   const bf16_t* g;          // [M, H, N]
   uint8_t *up_codes, *up_scales, *gate_codes, *gate_scales;
-  bf16_t *dp, *dq;          // [M, H, N]
+  // [M, H, N].  Rounded to bf16, as the products' operands have to be: 0.0017 of them in the
+  // mean square, as the gradients' own rounding (f32 operands would cost three products for one).
+  bf16_t *dp, *dq;
   TileOrder order;          // tiles of latents (of all heads) and of tokens
 };
 
@@ -477,8 +479,9 @@ __global__ __launch_bounds__(256, NJ > 2 ? 1 : 2) void gated_kernel(const GatedA
   // ..+3 for r of 0..3.  64 of the tile's tokens at a time (j) go through LDS, so that
   // memory sees whole rows of 128 latents, stored past the caches, which they would only
   // empty (16384 tokens, 4 heads of 8192, D 256, saved: 1400 -> 1200 us; with the conversions
-  // of bdh_fp8.h 990-1040: 2.1 GB of results at 2.1 TB/s beside 0.55 PFLOP/s of products, which
-  // eight steps of k a tile leave waiting for their first loads and the ends).
+  // of bdh_fp8.h 1000-1100: 2.1 GB of results at 2 TB/s beside 0.52 PFLOP/s of products, which
+  // eight steps of k a tile, each waited for in full with a context, leave waiting for loads
+  // and the ends; without saving 783).
   constexpr int VP = 272, CP = 144;  // row pitches in bytes (bank spread)
   char* const vals = lds;            // [64][VP]: out; the gradient, then dp
   char* const more = lds + 64 * VP;  // [64][VP]: dq; or [2][64][CP] codes, [2][64][4] scales
@@ -663,8 +666,9 @@ __global__ __launch_bounds__(256) void gated_grads_kernel(const GatedArgs a) {
 // --- few tokens -------------------------------------------------------------------------
 // Up to 64 tokens are bound by the weights, 4 D bytes a latent, each read once: a workgroup
 // has 16 VEC latents of a head and all tokens, its eight waves share the k's, and the
-// weights go from memory to registers (one token, 4 heads of 8192 latents, D 256: 5.8 us, 5.8
-// TB/s; 64 tokens of 8192, D 2048: 17 us, 3.9 TB/s).  A lane reads VEC neighbours of eight rows of k and
+// weights go from memory to registers (one token, 4 heads of 8192 latents, D 256: 8.2 us a call,
+// 4.1 TB/s, 5.2 a launch of many in a graph, which find the weights in the caches; 64 tokens of
+// 8192, D 2048: 17.4 us, 3.9 TB/s).  A lane reads VEC neighbours of eight rows of k and
 // pairs the rows (one v_perm for two values), which leaves it with a fragment for each of
 // its latents: 16 lanes hold every VEC-th latent of the tile.
 constexpr int kFewTokens = 64, kFewWaves = 8;
@@ -1081,10 +1085,13 @@ __global__ __launch_bounds__(256, BIG ? 1 : 2) void product_kernel(const Product
 // four waves and dc by four; WEIGHTS  128 latents by all columns of dU and of dG.  Beside
 // the tiles' direct loads a thread asks for eight neighbours of the gradient and of both
 // codes a step, four steps ahead: WEIGHTS of 32 tokens by 128 latents; INPUTS of 64 tokens
-// by the 64 latents of two steps, so that memory sees 128 (64) bytes of a row.
-// 16384 tokens, 4 heads of 8192 latents, D 256: 990 and 690 us (0.55 and 0.8 PFLOP/s); a
-// step moves 146 KB in LDS, 1150 cycles beside 1024 of products, and INPUTS waits for the
-// gradients and codes besides, 64 bytes of a row at a time.
+// by the 64 latents of two steps, so that memory sees 128 (64) bytes of a row.  (The barriers'
+// counts leave two steps' of them in flight.)
+// 16384 tokens, 4 heads of 8192 latents, D 256: 937 and 726 us (0.59 and 0.76 PFLOP/s), 1.8
+// and 1.4 a step.  A step's 146 KB in LDS are 1150 cycles and its products 1024, half a
+// microsecond each: the rest is waiting for loads.  One step in four waits for all that are in
+// flight (vmcnt 0), since the compiler converts the powers of all four sets of raw values
+// there, the last asked for a step ago.
 template <int WHAT, int ACT, bool MASK>
 __global__ __launch_bounds__(512, 1) void fused_kernel(const ProductArgs a, const GatedArgs g) {
   constexpr bool IN = WHAT == INPUTS;
@@ -1368,7 +1375,8 @@ int64_t makespan(int64_t n1, int64_t l1, int64_t n2, int64_t l2, int64_t slots) 
 // Tiles and parts of k of the backward's products: what takes the least time by the steps of
 // the longest row of tiles on a slot and by the bytes of the partial sums.  Measured: a step of
 // 256 by 256 tiles (one a CU) 0.84 us, of 256 by 128 (two a CU) 1.11, a tile's ends about
-// six steps; sums 4.5 TB/s and a launch.  (3003 tokens of 4096 latents, D 1024: 160 -> 109 us.)
+// six steps; sums 4.5 TB/s and a launch.  (3003 tokens of 4096 latents, D 1024: 160 -> 109-121
+// us.  A single workgroup on a CU is priced as one of two: few tiles are not told apart well.)
 struct ProductPlan {
   int in_parts, w_parts;
   double us;
