@@ -198,6 +198,13 @@ __device__ __forceinline__ void big_loop(int s0, int s1, int K, Load&& load, Rea
   for (; s < s1; ++s) step(no);
 }
 
+// Sums of the large tiles stay where the matrix cores have them until they are taken: else all
+// 256 a lane move to the other registers at once where the loop ends, which pushes what is there
+// to memory.  (Memory of its own, which the runtime has to find at a launch, makes a kernel end
+// the process where the device has none left.  The products' 440 bytes a lane took 15 us a launch
+// besides: the backward of 64 tokens of 8192, D 2048, saved 61 -> 45 us.)
+__device__ __forceinline__ void until_here(floatx16& sums) { asm volatile("" : "+a"(sums)); }
+
 // Rows of tokens: token i = (b, t) lies at b * batch + t * step elements.
 struct TokenRows {
   int64_t batch, step;
@@ -360,7 +367,10 @@ __global__ __launch_bounds__(256, NJ > 2 ? 1 : 2) void gated_kernel(const GatedA
   int an, am;
   if (!a.order.at((int)blockIdx.x, an, am)) return;
   const int n_tiles = (N + 127) / 128;
-  const int n0 = an % n_tiles * 128, h = an / n_tiles, m0 = am * 64 * NJ;
+  // (With the largest tiles all vector registers are taken: the divisions' results, which are
+  // the vector unit's, go to scalar ones.)
+  const auto scalar = [](int v) { return NJ == 4 ? __builtin_amdgcn_readfirstlane(v) : v; };
+  const int n0 = scalar(an % n_tiles) * 128, h = scalar(an / n_tiles), m0 = scalar(am) * 64 * NJ;
   const char* wp[2][2];
   {
     const int c = W::chunk(w, lane) * 8;
@@ -487,8 +497,11 @@ __global__ __launch_bounds__(256, NJ > 2 ? 1 : 2) void gated_kernel(const GatedA
   char* const more = lds + 64 * VP;  // [64][VP]: dq; or [2][64][CP] codes, [2][64][4] scales
   char* const bytes = more + 128 * CP;
   static_assert(64 * VP + 128 * CP + 512 <= 2 * STAGE && 128 * VP <= 2 * STAGE, "the stages' memory");
-  const int high = lane >> 5, nb = (N + kFp8Block - 1) / kFp8Block;
-  const int mine = 32 * (w >> 1) + (lane & 31);  // the lane's row of the part
+  // (The thread opaque: else places computed from it before the products are kept through them.)
+  int tid = (int)threadIdx.x;
+  if (NJ == 4) asm volatile("" : "+v"(tid));
+  const int high = (NJ == 4 ? tid & 63 : lane) >> 5, nb = (N + kFp8Block - 1) / kFp8Block;
+  const int mine = 32 * (w >> 1) + ((NJ == 4 ? tid : lane) & 31);  // the lane's row of the part
   // Row r of part j, and its place in [tokens, H].
   const auto token = [&](int r, int j) { return m0 + 32 * NJ * (r >> 5) + 32 * j + (r & 31); };
   const auto place = [&](int m) { return (int64_t)m * a.H + h; };
@@ -498,7 +511,7 @@ __global__ __launch_bounds__(256, NJ > 2 ? 1 : 2) void gated_kernel(const GatedA
     if (EPI == BACK) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int r = (int)threadIdx.x / 16 + 16 * e, c = (int)threadIdx.x % 16, m = token(r, j);
+        const int r = tid / 16 + 16 * e, c = tid % 16, m = token(r, j);
         u32x4 g = {0, 0, 0, 0};
         if (m < M && n0 + 8 * c < N) g = *(const u32x4*)(a.g + place(m) * N + n0 + 8 * c);
         *(u32x4*)(vals + r * VP + 16 * c) = g;
@@ -508,6 +521,10 @@ __global__ __launch_bounds__(256, NJ > 2 ? 1 : 2) void gated_kernel(const GatedA
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int nt = nw + 32 * i;  // in the tile
+      if (NJ == 4 && ACT != RELU) {
+        until_here(p[i][j]);
+        until_here(q[i][j]);
+      }
       floatx4 mask[4];
       if (ACT == RELU && a.mask) {
 #pragma unroll
@@ -590,7 +607,7 @@ __global__ __launch_bounds__(256, NJ > 2 ? 1 : 2) void gated_kernel(const GatedA
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int r = (int)threadIdx.x / 16 + 16 * e, c = (int)threadIdx.x % 16, m = token(r, j);
+      const int r = tid / 16 + 16 * e, c = tid % 16, m = token(r, j);
       if (m >= M || n0 + 8 * c >= N) continue;
       const int64_t to = place(m) * N + n0 + 8 * c;
       const u32x4 v = *(const u32x4*)(vals + r * VP + 16 * c);
@@ -600,18 +617,18 @@ __global__ __launch_bounds__(256, NJ > 2 ? 1 : 2) void gated_kernel(const GatedA
     if (EPI == SAVE) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int which = e >> 1, r = (int)threadIdx.x / 8 + 32 * (e & 1), c = (int)threadIdx.x % 8, m = token(r, j);
+        const int which = e >> 1, r = tid / 8 + 32 * (e & 1), c = tid % 8, m = token(r, j);
         if (m >= M || n0 + 16 * c >= N) continue;
         uint8_t* to = (which ? a.gate_codes : a.up_codes) + place(m) * N + n0 + 16 * c;
         const u32x4 v = *(const u32x4*)(more + (64 * which + r) * CP + 16 * c);
         if (n0 + 16 * c + 16 <= N) __builtin_nontemporal_store(v, (u32x4_8*)to);
         else *(u32x2*)to = u32x2{v[0], v[1]};
       }
-      if (threadIdx.x < 128) {
-        const int which = (int)threadIdx.x >> 6, r = (int)threadIdx.x & 63, m = token(r, j);
+      if (tid < 128) {
+        const int which = tid >> 6, r = tid & 63, m = token(r, j);
         if (m < M) {
           uint8_t* to = (which ? a.gate_scales : a.up_scales) + place(m) * nb + n0 / kFp8Block;
-          const uint32_t v = *(const uint32_t*)(bytes + threadIdx.x * 4);
+          const uint32_t v = *(const uint32_t*)(bytes + tid * 4);
           if (n0 + 96 < N) {
             *(u32_1*)to = v;
           } else {
@@ -861,7 +878,7 @@ struct ProductArgs {
 // from b0: to the gradient in bf16, or as one of the parts that join_kernel adds.  job: of
 // x_jobs, where they are d_x's.  KEEP: w_kept and w_more count.
 template <int WHAT, bool KEEP, int NA, int NB>
-__device__ __forceinline__ void store_product(const ProductArgs& a, const floatx16 (&acc)[NA][NB], int h, int which,
+__device__ __forceinline__ void store_product(const ProductArgs& a, floatx16 (&acc)[NA][NB], int h, int which,
                                               int part, int job, int a0, int b0, int lane) {
   const int high = lane >> 5;
   const bool ctx = which && a.c;
@@ -892,6 +909,7 @@ __device__ __forceinline__ void store_product(const ProductArgs& a, const floatx
     const int64_t row = out_at + (WHAT == WEIGHTS ? b * a.N : ctx ? a.c_rows.at((uint32_t)b) : b * a.D);
 #pragma unroll
     for (int i = 0; i < NA; ++i) {
+      if (NA * NB == 16) until_here(acc[i][j]);
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         float v[8];
@@ -1084,17 +1102,22 @@ __global__ __launch_bounds__(256, BIG ? 1 : 2) void product_kernel(const Product
 // eight waves, four for each product: INPUTS  128 tokens of a head by all columns, dx by
 // four waves and dc by four; WEIGHTS  128 latents by all columns of dU and of dG.  Beside
 // the tiles' direct loads a thread asks for eight neighbours of the gradient and of both
-// codes a step, four steps ahead: WEIGHTS of 32 tokens by 128 latents; INPUTS of 64 tokens
+// codes a step, SETS steps ahead: WEIGHTS of 32 tokens by 128 latents; INPUTS of 64 tokens
 // by the 64 latents of two steps, so that memory sees 128 (64) bytes of a row.  (The barriers'
 // counts leave two steps' of them in flight.)
 // 16384 tokens, 4 heads of 8192 latents, D 256: 937 and 726 us (0.59 and 0.76 PFLOP/s), 1.8
 // and 1.4 a step.  A step's 146 KB in LDS are 1150 cycles and its products 1024, half a
 // microsecond each: the rest is waiting for loads.  One step in four waits for all that are in
 // flight (vmcnt 0), since the compiler converts the powers of all four sets of raw values
-// there, the last asked for a step ago.
+// there, the last asked for a step ago (not so where LEAN).
 template <int WHAT, int ACT, bool MASK>
 __global__ __launch_bounds__(512, 1) void fused_kernel(const ProductArgs a, const GatedArgs g) {
   constexpr bool IN = WHAT == INPUTS;
+  // An activation's or the mask's own values leave registers for two steps' raw values, not
+  // four (SiLU: for four), and none for what can be computed again (4096 tokens as above, us with
+  // spilled registers / so: GELU 619 / 545, mask 552 / 535, SiLU 493 / 490, with two sets 524).
+  constexpr bool LEAN = IN ? ACT != RELU : ACT == GELU || MASK;
+  constexpr int SETS = LEAN && ACT != SILU ? 2 : 4;
   typedef Tile<IN ? KC : MC, 256, 8> F;  // U, G rows d / x, c columns d
   typedef Tile<MC, 128, 8> P;            // WEIGHTS: dp, dq columns n
   constexpr int TILES = 2 * F::BYTES, LOADS = 2 * F::LOADS;
@@ -1149,14 +1172,15 @@ __global__ __launch_bounds__(512, 1) void fused_kernel(const ProductArgs a, cons
   const int64_t d_base = (int64_t)h * N + (IN ? at0 * d_row : 0), b_base = (int64_t)h * nb + (IN ? at0 * b_row : 0);
   const auto k_of = [&](int s) { return IN ? (s >> 1) * 2 * BK + col : s * BK + row; };
   const auto place = [&](int odd, uint32_t& d, uint32_t& b) {
-    const int r = IN ? row + 64 * odd : row;
+    int r = IN ? row + 64 * odd : row;
+    if (LEAN && IN) asm volatile("" : "+v"(r));  // (at each step anew)
     const int m = IN && at0 + r >= M ? M - 1 - at0 : r, n = IN ? col : (at0 + col < N ? at0 + col : N - 8);
     d = (uint32_t)(m * d_row + n);
     b = (uint32_t)(m * b_row + n / kFp8Block);
   };
-  uint32_t d_own[2], b_own[2];
-  place(0, d_own[0], b_own[0]);
-  place(1, d_own[1], b_own[1]);
+  uint32_t d_kept[2], b_kept[2];
+  place(0, d_kept[0], b_kept[0]);
+  place(1, d_kept[1], b_kept[1]);
   struct Raw {
     u32x4 g;
     u32x2 p, q;
@@ -1173,20 +1197,22 @@ __global__ __launch_bounds__(512, 1) void fused_kernel(const ProductArgs a, cons
   };
   // inside: all of a step's k lies within K.
   const auto load = [&](auto inside, int s, int odd, Raw& r) {
+    uint32_t d_own = d_kept[odd], b_own = b_kept[odd];
+    if (LEAN && IN) place(odd, d_own, b_own);
     const auto d_at = [&](int s) { return d_base + (IN ? (int64_t)(s >> 1) * 2 * BK : s * BK * d_row); };
     const auto b_at = [&](int s) { return b_base + (IN ? (int64_t)(s >> 1) * 2 : s * BK * b_row); };
     if constexpr (decltype(inside)::value) {
-      load_at(d_at(s), b_at(s), d_own[odd], b_own[odd], r);
+      load_at(d_at(s), b_at(s), d_own, b_own, r);
       return;
     }
     // Past the end: INPUTS the last eight latents, WEIGHTS the last token.
     const int k = k_of(s), last = IN ? K - 8 : K - 1;
     if (k <= last) {
-      load_at(d_at(s), b_at(s), d_own[odd], b_own[odd], r);
+      load_at(d_at(s), b_at(s), d_own, b_own, r);
     } else if (IN) {
-      load_at(d_base + last - col, b_base + last / kFp8Block - col / kFp8Block, d_own[odd], b_own[odd], r);
+      load_at(d_base + last - col, b_base + last / kFp8Block - col / kFp8Block, d_own, b_own, r);
     } else {
-      load_at(d_base + (last - row) * d_row, b_base + (last - row) * b_row, d_own[odd], b_own[odd], r);
+      load_at(d_base + (last - row) * d_row, b_base + (last - row) * b_row, d_own, b_own, r);
     }
   };
   // MASK: relu's mask, squared, of the thread's latents.
@@ -1202,7 +1228,9 @@ __global__ __launch_bounds__(512, 1) void fused_kernel(const ProductArgs a, cons
   if (MASK && !IN) mask_of(at0 + col, m2);
   u32x4 dp, dq;
   const auto make = [&](auto inside, int s, const Raw& r) {
-    const float sp = fp8_power(r.sp), sq = fp8_power(r.sq);
+    int up = r.sp, gate = r.sq;
+    if (LEAN) asm volatile("" : "+v"(up), "+v"(gate));  // (not before)
+    const float sp = fp8_power(up), sq = fp8_power(gate);
     const bf16x8 gv = __builtin_bit_cast(bf16x8, r.g);
     if (MASK && IN) mask_of(k_of(s), m2);
 #pragma unroll
@@ -1262,22 +1290,22 @@ __global__ __launch_bounds__(512, 1) void fused_kernel(const ProductArgs a, cons
     acc[i / NB][i % NB] = mfma32(f.a[i / NB], f.b[i % NB], acc[i / NB][i % NB]);
   };
   // Step s: the tile of step s + 2 is asked for, the gradients of step s + AHEAD are made
-  // from what was asked for four steps ago, step s is multiplied.  (INPUTS: a pair's
+  // from what was asked for SETS steps ago, step s is multiplied.  (INPUTS: a pair's
   // gradients are made while the pair before it is multiplied.)  Groups of four steps, in
   // which the raw values keep their registers; inside: all that a group asks for lies
   // within k, and nothing in it branches.  The last groups end with steps of zeros.
   constexpr int AHEAD = IN ? 2 : 1;
   const std::false_type no{};
-  Raw raw[4];
+  Raw raw[SETS];
 #pragma unroll
-  for (int u = 0; u < 4; ++u) load(no, s0 + u, u & 1, raw[u]);
+  for (int u = 0; u < SETS; ++u) load(no, s0 + u, u & 1, raw[u]);
   issue(no, s0, 0);
   issue(no, s0 + 1, 1);
 #pragma unroll
   for (int u = 0; u < AHEAD; ++u) {
     make(no, s0 + u, raw[u]);
     put(0, u);
-    load(no, s0 + 4 + u, u, raw[u]);
+    load(no, s0 + SETS + u, u, raw[u]);
   }
   int stage = 0, s = s0;
   const auto group = [&](auto inside) {
@@ -1295,7 +1323,7 @@ __global__ __launch_bounds__(512, 1) void fused_kernel(const ProductArgs a, cons
       const char* t = lds + stage * TILES;
       const char* d = grads + (IN ? u >> 1 : stage) * 2 * GRAD;
       const int to_buffer = IN ? (u >> 1) ^ 1 : next;
-      Raw& r = raw[(u + AHEAD) & 3];
+      Raw& r = raw[(u + AHEAD) % SETS];
       issue(inside, s + 2, after);
       Frags f;
 #pragma unroll
@@ -1308,7 +1336,7 @@ __global__ __launch_bounds__(512, 1) void fused_kernel(const ProductArgs a, cons
 #pragma unroll
       for (int i = 0; i < 8; ++i) product(f, i);
       put(to_buffer, u & 1);
-      load(inside, s + AHEAD + 4, (u + AHEAD) & 1, r);
+      load(inside, s + AHEAD + SETS, (u + AHEAD) & 1, r);
       stage = next;
     }
   };
