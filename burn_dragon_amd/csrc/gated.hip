@@ -489,9 +489,9 @@ __global__ __launch_bounds__(256, NJ > 2 ? 1 : 2) void gated_kernel(const GatedA
   // ..+3 for r of 0..3.  64 of the tile's tokens at a time (j) go through LDS, so that
   // memory sees whole rows of 128 latents, stored past the caches, which they would only
   // empty (16384 tokens, 4 heads of 8192, D 256, saved: 1400 -> 1200 us; with the conversions
-  // of bdh_fp8.h 1000-1100: 2.1 GB of results at 2 TB/s beside 0.52 PFLOP/s of products, which
+  // of bdh_fp8.h 1000-1130: 2.1 GB of results at 2 TB/s beside 0.52 PFLOP/s of products, which
   // eight steps of k a tile, each waited for in full with a context, leave waiting for loads
-  // and the ends; without saving 783).
+  // and the ends; without saving 790).
   constexpr int VP = 272, CP = 144;  // row pitches in bytes (bank spread)
   char* const vals = lds;            // [64][VP]: out; the gradient, then dp
   char* const more = lds + 64 * VP;  // [64][VP]: dq; or [2][64][CP] codes, [2][64][4] scales
@@ -1105,7 +1105,7 @@ __global__ __launch_bounds__(256, BIG ? 1 : 2) void product_kernel(const Product
 // codes a step, SETS steps ahead: WEIGHTS of 32 tokens by 128 latents; INPUTS of 64 tokens
 // by the 64 latents of two steps, so that memory sees 128 (64) bytes of a row.  (The barriers'
 // counts leave two steps' of them in flight.)
-// 16384 tokens, 4 heads of 8192 latents, D 256: 937 and 726 us (0.59 and 0.76 PFLOP/s), 1.8
+// 16384 tokens, 4 heads of 8192 latents, D 256: 938 and 730 us (0.59 and 0.75 PFLOP/s), 1.8
 // and 1.4 a step.  A step's 146 KB in LDS are 1150 cycles and its products 1024, half a
 // microsecond each: the rest is waiting for loads.  One step in four waits for all that are in
 // flight (vmcnt 0), since the compiler converts the powers of all four sets of raw values
