@@ -1434,8 +1434,8 @@ ProductPlan plan_products(int64_t M, int64_t H, int64_t N, int64_t D, bool ctx, 
 
 // The tokens of the projections' tiles: what takes the least time by rounds of workgroups
 // (between the whole and the broken number of them) times a step's and the ends' us, as
-// measured (M 1024 to 8192, N 4096 and 8192, D 256 to 2048).  The ends (activation, 8 bits,
-// memory) run beside another workgroup's products only in the smallest.  Over those 180 cases
+// measured (M 1024 to 8192, N 4096 and 8192, D 256 to 2048; taken for other sizes too).  The
+// ends (activation, 8 bits, memory) run beside another workgroup's products only in the smallest.  Over those 180 cases
 // 0.8 % off the fastest in the mean, 18 % at worst (1024 tokens of 8192, D 256: 15 us in 128
 // tokens, 18 in 256); without tiles of 192 2.9 % in the mean (the backward's at 3003 tokens of
 // 4096, D 1024: 72 us in 192, 79 in 128, 81 in 256).

@@ -149,7 +149,8 @@ def gated_block_vjp(grad: torch.Tensor, current: torch.Tensor, weights: GatedWei
     what the forward kept: the gradient is then the block's at those values,
     and the projections are not computed again.  Without a context current's
     gradient has both parts.  None where the library does not support the
-    input (as gated_block; a scratch that would have to grow under capture)."""
+    input (as gated_block; a scratch that would have to grow under capture).
+    Where the device has no memory for the scratch, the tokens go in groups."""
     call = _call(current, weights, context, activation, relu_threshold, latent_mask)
     if call is None or grad.dtype is not torch.bfloat16:
         return None
